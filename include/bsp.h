@@ -486,6 +486,41 @@ int bsp_attention_f32_bwd(const bsp_attention_f32_call *call, const float *d_o, 
                           float *neg_delta, const int32_t *d_items, int n_items, float *partial, int n_slots, const int32_t *d_split,
                           int n_split, void *stream);
 
+/* Block-sparse attention with score rules: o = softmax(y) . v and its gradients without any sparse tensor, with
+ *     y_ij = cap * tanh(scale * q_i . k_j / cap) - slope_h * |i - j|      (softcap 0: scale * q_i . k_j - ...)
+ * over the keys j that row i sees: block (h, i / block, j / block) is in the layout; documents[z][i] = documents[z][j] >= 0
+ * (where documents is not NULL); and, with causal, j <= i or j < prefix[z] (prefix NULL: none).  A row that sees no key gets zeros
+ * in o and dq.  Positions with a negative document number reach nothing, whatever q, k, v and d_o hold there.  Query head h
+ * uses head h / (H / kv_heads) of k and v; their gradients are the sums over the query heads that share them.
+ * dtype: any; D = 64 or 128.  length: positions of q, k, v and o, 1 .. 2^24 - 1, any number up to 64 lines.
+ * strides: of batch, head and row, in elements, three per tensor: q, k, v, o, d_o, dq, dk, dv (those that a call does not use: 0);
+ * multiples of 8 elements (fp32: 4), unit inner stride, 16-byte aligned pointers, rows of a head within 4 GiB.
+ * d_rows, lines: the table of the lines of bsp_attention_tables_build (blocks of 16, 32, 64; larger ones are given as blocks of 64).
+ * stats: [Z][H][2][64 lines] floats, written by fwd (NULL: no backward pass to follow) and read by bwd.  ranges: with documents,
+ * [Z][ceil(length / 16)][2] ints, written by fwd and read by bwd.
+ * bwd: neg_delta: [Z][H][64 lines] floats of scratch.  dk and dv: both or neither.  d_items .. n_split: the columns of
+ * bsp_attention_tables_build for the layout [kv_heads, lines of the H / kv_heads query heads, columns], the positions in their
+ * entries split into 2^24 * (query head of the key head) + position in it; partial: [Z][n_slots][2][64][D] floats.  No atomics: the
+ * same call gives the same bits. */
+typedef struct {
+  int dtype, Z, H, kv_heads, lines, D;
+  int64_t length;
+  int64_t strides[24];
+  float scale, softcap;
+  int causal;
+  const float *slopes;             /* [H] or NULL */
+  const int32_t *documents;        /* element (z, i) at documents[z * documents_stride + i], or NULL */
+  int64_t documents_stride;
+  const int32_t *prefix;           /* [Z] or NULL; only with causal */
+  int32_t *ranges;
+  const int32_t *d_rows;
+  float *stats;
+} bsp_attention_rules_call;
+int bsp_attention_rules_fwd(const bsp_attention_rules_call *call, const void *q, const void *k, const void *v, void *o, void *stream);
+int bsp_attention_rules_bwd(const bsp_attention_rules_call *call, const void *d_o, const void *q, const void *k, const void *v, const void *o,
+                            void *dq, void *dk, void *dv, float *neg_delta, const int32_t *d_items, int n_items, float *partial, int n_slots,
+                            const int32_t *d_split, int n_split, void *stream);
+
 /* ---------------------------------------------------------------------------------------------------
  * Dense utility ops of the reference package.
  * ReLU: replaces the relu_y / relu_dxdsdbdres kernels and their launches (relu.py:8-91).  All tensors hold n

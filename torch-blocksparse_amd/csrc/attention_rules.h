@@ -1,0 +1,392 @@
+// Shared pieces of the attention kernels with score rules (attention_rules_fwd.hip, attention_rules_bwd.hip): block-sparse
+// attention whose logits are
+//     y_ij = cap * tanh(scale * q_i . k_j / cap) - slope_h * |i - j|        (no cap: scale * q_i . k_j - ...)
+// over the keys j that row i sees: block (h, i / block, j / block) is in the layout, both positions carry the same document
+// number and it is not negative, and without `causal` any j, with it j <= i or j < prefix of the batch.  q has G heads for each
+// head of k and v.  The length need not fill the last block.  A row that sees no key gets zeros, in the result and as gradient.
+//
+// The tiles, the work split and the LDS ring are those of attention_quad.h: a workgroup of two wavefronts has the 64 rows of a line
+// (keys of a column) and walks the line's (column's) tiles in halves of 32 columns (rows).  What the rules add:
+//   * a walk (Walk): 64 halves at a time, one a lane, are held against the rules by their positions and the range of document numbers
+//     in each group of sixteen positions; three lane masks say which halves any row sees, which every row sees whole, and
+//     which hold positions without document or past the end.  The loop visits the first kind only, and looks at single scores
+//     in those of them that are not of the second.
+//   * a score is seen or not by a bit of a sixteen-bit word per lane.  What the position rules leave of a lane's two runs of
+//     eight consecutive keys is a run itself, so the word is two shifts; documents are compared one by one.
+//   * positions without document (padding) and past the end may hold anything, NaN included: their rows of a stage are set to zero
+//     before the products (0 * NaN would reach every row of the tile).
+// fp32: the same kernels on the fp32 matrix units (32x32x2), which take their operands as they lie in a row: no transposing reads.
+#ifndef BSP_ATTENTION_RULES_H
+#define BSP_ATTENTION_RULES_H
+#include "attention_quad.h"
+
+namespace bsp {
+
+struct RuleArgs {
+  const void *q, *k, *v;
+  const void *d_o, *o_in;          // backward: do, and the forward result (row kernel)
+  void *o, *o2;                    // forward: o; row kernel: dq; column kernel: dk and dv
+  float *ref, *delta;              // ref: [Z][H][2][rows]: p = exp2(y - ref) * factor, y in the log2 domain; delta: [Z][H][rows], -sum_d do . o
+  int64_t rows;                    // 64 * lines
+  int64_t q_sz, q_sh, q_ld, k_sz, k_sh, k_ld, v_sz, v_sh, v_ld, do_sz, do_sh, do_ld, oin_sz, oin_sh, oin_ld;
+  int64_t o_sz, o_sh, o_ld, o2_sz, o2_sh, o2_ld;
+  float in, out;                   // y = out * tanh(in * s / 2) with a cap, s * out without (see logit_args)
+  float scale;                     // of the sums dq and dk
+  const float *slopes;
+  const int32_t *docs; int64_t docs_sz;
+  const int32_t *prefix;
+  const int32_t *ranges; int groups;   // per batch and group of sixteen positions the least and the greatest document number (least: -1 if any is negative)
+  int causal, capped;
+  const int32_t *lut;
+  float *partial;                  // column kernel: slots of the parts of long columns, [Z][n_slots][dk, dv][64][D]
+  const int32_t *split_lut;
+  int n_slots, n_split;
+  int Z, H, G, R, L;               // G: query heads a key head; R: lines of the table per head, 64 R >= L (column kernel: work items)
+};
+
+namespace {
+
+template <typename T, int D> struct Geo {
+  static constexpr int ESZ = sizeof(T), RB = D * ESZ, CPR = RB / 16, NF = RB / 32, VEC = 16 / ESZ;   // bytes and 16-byte chunks of a row; operand fragments; elements a chunk
+  static constexpr int PIECE = 32 * RB, STAGE = 2 * PIECE, RING = 2 * STAGE;
+  static constexpr int EXTRA = 768;                      // bytes behind each stage's pieces: documents, statistics
+};
+template <typename T> struct RuleOperand { typedef typename Mma<T, 32>::frag_t type; };
+template <> struct RuleOperand<float> { typedef f32x4 type; };
+template <typename T, int D> using held_t = typename RuleOperand<T>::type[Geo<T, D>::NF];
+
+template <typename T, int D> __device__ __forceinline__ int rule_swz(int r) {
+  if constexpr (sizeof(T) == 4) return r & 15;
+  else return quad_swz<D>(r);
+}
+
+// The lane's row of an operand that stays in registers: chunk 2 s + lane / 32 of it, or zeros
+template <typename T, int D> __device__ __forceinline__ void hold_operand(held_t<T, D> &f, const T *row, int half, bool dead) {
+#pragma unroll
+  for (int s = 0; s < Geo<T, D>::NF; s++) {
+    const u32x4 raw = *reinterpret_cast<const u32x4 *>(row + Geo<T, D>::VEC * (2 * s + half));
+    f[s] = __builtin_bit_cast(typename RuleOperand<T>::type, dead ? u32x4{0, 0, 0, 0} : raw);
+  }
+}
+
+// Sixteen consecutive rows, global -> LDS.  Rows behind the last are fetched as that one (and not used).
+template <typename T, int D, bool LEAN> struct RowsLoad {
+  typedef Geo<T, D> Q;
+  static constexpr int RPL = 64 / Q::CPR, LW = 16 / RPL;
+  uint32_t off[LEAN ? 1 : LW];
+  uint32_t chunk;
+  __device__ __forceinline__ void init(int64_t ld, int lane) {
+    chunk = (uint32_t)((lane % Q::CPR) ^ rule_swz<T, D>(lane / Q::CPR));
+#pragma unroll
+    for (int i = 0; i < (LEAN ? 1 : LW); i++)
+      off[i] = (uint32_t)((i * RPL + lane / Q::CPR) * ld) * Q::ESZ + (LEAN ? 0u : (chunk ^ (uint32_t)rule_swz<T, D>(i * RPL)) << 4);
+  }
+  __device__ __forceinline__ void issue(const char *base, int pos, uint32_t row_bytes, uint32_t lds, int L, int lane) const {
+    if (pos + 16 <= L) {
+      uint32_t c = chunk;
+      if constexpr (LEAN) asm volatile("" : "+v"(c));
+#pragma unroll
+      for (int i = 0; i < LW; i++)
+        if constexpr (LEAN) load_to_lds<16>(base, off[0] + ((c ^ (uint32_t)rule_swz<T, D>(i * RPL)) << 4), (uint32_t)(pos + i * RPL) * row_bytes, lds + i * 1024);
+        else load_to_lds<16>(base, off[i], (uint32_t)pos * row_bytes, lds + i * 1024);
+    } else {
+#pragma unroll
+      for (int i = 0; i < LW; i++) {
+        const int r = pos + i * RPL + lane / Q::CPR;
+        load_to_lds<16>(base, (uint32_t)(r < L ? r : L - 1) * row_bytes + ((chunk ^ (uint32_t)rule_swz<T, D>(i * RPL)) << 4), 0, lds + i * 1024);
+      }
+    }
+  }
+};
+
+// Row `row` of a piece (0 .. 31) to zeros: the lane's chunk of it
+template <typename T, int D> __device__ __forceinline__ void clear_rows(unsigned char *piece, int row0, const int32_t *docs_of_stage, bool docs, int pos, int L, int lane) {
+  typedef Geo<T, D> Q;
+  constexpr int RPL = 64 / Q::CPR;
+#pragma unroll 1
+  for (int i = 0; i < 16 / RPL; i++) {
+    const int r = i * RPL + lane / Q::CPR;
+    if (pos + r >= L || (docs && docs_of_stage[row0 + r] < 0)) {
+      u32x4 *at = reinterpret_cast<u32x4 *>(piece + (row0 + r) * Q::RB + (lane % Q::CPR) * 16);
+      *at = u32x4{0, 0, 0, 0};
+      at[Q::PIECE / 16] = u32x4{0, 0, 0, 0};
+    }
+  }
+}
+
+// The operand reads of a piece, along its rows and transposed
+template <typename T, int D, bool LEAN> struct PieceReads {
+  RowReads<D, LEAN> rows;
+  TrReads<D, LEAN> tr;
+  __device__ __forceinline__ void init(const unsigned char *smem, int lane) {
+    rows.init(0, lane);
+    tr.init(lds_address(smem), 0, lane);
+  }
+};
+template <int D, bool LEAN> struct PieceReads<float, D, LEAN> {
+  uint32_t row, tr;                // the others are an exclusive-or of constants away
+  __device__ __forceinline__ void init(const unsigned char *, int lane) {
+    const int half = lane >> 5, l32 = lane & 31, r = deal_row(l32);
+    row = (uint32_t)(r * Geo<float, D>::RB + ((half ^ rule_swz<float, D>(r)) << 4));
+    tr = (uint32_t)(8 * half * Geo<float, D>::RB + (((l32 >> 2) ^ (8 * half)) << 4) + ((l32 & 3) << 2));
+  }
+};
+
+// acc + (32 rows of a piece, dealt by deal_row) . b: value i = row 16 (i / 8) + 8 (lane / 32) + i % 8 of the piece, column lane % 32
+template <typename T, int D, int OFF, bool LEAN>
+__device__ __forceinline__ f32x16 rows_times(const unsigned char *smem, const PieceReads<T, D, LEAN> &reads, const held_t<T, D> &b, f32x16 acc) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int s = 0; s < Geo<T, D>::NF; s++) {
+      const f32x4 f = *reinterpret_cast<const f32x4 *>(smem + OFF + (reads.row ^ (uint32_t)(s << 5)));
+#pragma unroll
+      for (int j = 0; j < 4; j++) acc = Mma<float, 32>::run(f[j], b[s][j], acc);
+    }
+    return acc;
+  } else {
+    return row_product<T, D, OFF, LEAN>(smem, reads.rows, b, acc);
+  }
+}
+__device__ __forceinline__ f32x16 zeros16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; i++) z[i] = 0.f;
+  return z;
+}
+
+// Sixteen values a lane, one per row of a piece as rows_times deals them, as the operand of columns_times: rounded to the
+// operands' type (the products take no other), in fp32 as they are
+template <typename T> struct Shares {
+  typename Mma<T, 32>::frag_t f[2];
+  __device__ __forceinline__ void set(const float (&e)[16]) {
+#pragma unroll
+    for (int ks = 0; ks < 2; ks++) f[ks] = pack8<T>(reinterpret_cast<const float (&)[8]>(e[8 * ks]));
+  }
+};
+template <> struct Shares<float> {
+  float e[16];
+  __device__ __forceinline__ void set(const float (&v)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; i++) e[i] = v[i];
+  }
+};
+
+// acc[mt] += (32 rows of a piece, transposed)[column 32 mt ..][row] . b[row]
+template <typename T, int D, int OFF, bool LEAN>
+__device__ __forceinline__ void columns_times(f32x16 (&acc)[D / 32], const unsigned char *smem, const PieceReads<T, D, LEAN> &reads, const Shares<T> &b) {
+  if constexpr (sizeof(T) == 4) {
+    constexpr int RB = Geo<T, D>::RB;
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+#pragma unroll
+      for (int mt = 0; mt < D / 32; mt++) {
+        const float x = *reinterpret_cast<const float *>(smem + OFF + (16 * (i / 8) + i % 8) * RB + (reads.tr ^ (uint32_t)((8 * mt ^ (i & 7)) << 4)));
+        acc[mt] = Mma<float, 32>::run(x, b.e[i], acc[mt]);
+      }
+  } else {
+    tr_product<T, D, OFF, LEAN>(acc, reads.tr, b.f);
+  }
+}
+
+// tanh(x) for x = in * s / 2 and s -> logit.  1 - 2 / (exp(2 x) + 1) is off by 2^-23 at most, which cap * log2 e takes to the logit: little
+// beside what 16-bit operands leave of it.  In fp32 small x (in trained models most) take the series, which keeps their relative precision:
+// up to x = 0.45 its next term is below 2^-27 of the sum.
+template <typename T> __device__ __forceinline__ float tanh_of(float s, float in) {
+  const float t = fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * (in * kLog2e)) + 1.f), 1.f);
+  if constexpr (sizeof(T) == 4) {
+    const float x = 0.5f * in * s, z = x * x;
+    float p = fmaf(z, 21844.f / 6081075.f, -1382.f / 155925.f);
+    p = fmaf(z, p, 62.f / 2835.f);
+    p = fmaf(z, p, -17.f / 315.f);
+    p = fmaf(z, p, 2.f / 15.f);
+    p = fmaf(z, p, -1.f / 3.f);
+    return z < 0.2025f ? fmaf(x * z, p, x) : t;
+  }
+  return t;
+}
+inline void logit_args(RuleArgs &a, float scale, float cap) {
+  a.scale = scale;
+  a.capped = cap > 0.f;
+  a.in = cap > 0.f ? 2.f * scale / cap : 0.f;
+  a.out = (cap > 0.f ? cap : scale) * kLog2e;
+}
+
+// the least and greatest document number of a group of sixteen positions: everything if there are no documents
+struct Range { int lo, hi; };
+__device__ __forceinline__ Range range_of(const RuleArgs &a, int z, int pos) {
+  const int g = pos >> 4;
+  const int32_t *r = a.ranges + 2 * ((int64_t)z * a.groups + (g < a.groups ? g : a.groups - 1));
+  return Range{r[0], r[1]};
+}
+
+// The halves of a line's (column's) tiles that are worth a visit, 64 looked at together, one a lane
+struct Half { int n, lo, hi, bits; bool full, pad; };
+struct Walk {
+  const int32_t *core;
+  int steps, base;
+  uint64_t live, full, pad;
+  int v_lo, v_hi, v_bits;
+  __device__ __forceinline__ void init(const int32_t *entries, int halves) {
+    core = entries;
+    steps = halves;
+    base = -64;
+    live = 0;
+  }
+  // look(lo, hi, bits of the half's pieces, &full, &pad) -> does any row see anything of it
+  template <class F> __device__ __forceinline__ Half next(int lane, F &&look) {
+    while (live == 0) {
+      base += 64;
+      if (base >= steps) return Half{-1, 0, 0, 0, false, false};
+      const int n = base + lane, at = n < steps ? n : steps - 1;
+      const int32_t *e = core + kEntry * (at >> 1);
+      v_lo = e[2 * (at & 1)];
+      v_hi = e[2 * (at & 1) + 1];
+      v_bits = e[4];
+      bool f = false, p = false;
+      const bool l = look(v_lo, v_hi, v_bits, at & 1, f, p);
+      live = __builtin_amdgcn_ballot_w64(l && n < steps);
+      full = __builtin_amdgcn_ballot_w64(f);
+      pad = __builtin_amdgcn_ballot_w64(p);
+    }
+    const int j = __builtin_ctzll(live);
+    live &= live - 1;
+    return Half{base + j, __builtin_amdgcn_readlane(v_lo, j), __builtin_amdgcn_readlane(v_hi, j), __builtin_amdgcn_readlane(v_bits, j),
+                (bool)((full >> j) & 1), (bool)((pad >> j) & 1)};
+  }
+};
+
+// The rules as the row kernels (a line of 64 rows; the lane has row `row`) apply them
+struct LineRules {
+  int most, least;                 // the keys below `most` are seen by a row of the line, those below `least` by all, as far as positions go
+  int limit;                       // ... the keys below it by the lane's row
+  int doc;                         // the lane's document
+  Range range;                     // of the line
+  __device__ __forceinline__ void init(const RuleArgs &a, int z, int line, int row, bool &dead) {
+    const int prefix = a.causal && a.prefix ? as_table(a.prefix)[z] : 0, first = line * 64, r = row < a.L ? row : a.L - 1;
+    doc = 0;
+    range = Range{0, 0};
+    if (a.docs) {
+      doc = a.docs[z * a.docs_sz + r];
+      const int lane = threadIdx.x & 3;
+      const Range g = range_of(a, z, first + 16 * lane < a.L ? first + 16 * lane : first);
+      int lo = g.lo, hi = g.hi;
+#pragma unroll
+      for (int d = 1; d < 4; d <<= 1) {
+        const int ol = __shfl_xor(lo, d), oh = __shfl_xor(hi, d);
+        lo = ol < lo ? ol : lo;
+        hi = oh > hi ? oh : hi;
+      }
+      range = Range{__builtin_amdgcn_readfirstlane(lo), __builtin_amdgcn_readfirstlane(hi)};
+    }
+    dead = row >= a.L || doc < 0;
+    auto below = [&](int i) { const int n = a.causal ? (i + 1 > prefix ? i + 1 : prefix) : a.L; return n < a.L ? n : a.L; };
+    most = below(first + 63);
+    least = below(first);
+    limit = dead ? 0 : below(row);
+  }
+  __device__ __forceinline__ bool look(const RuleArgs &a, int z, int lo, int hi, int bits, int half, bool &full, bool &pad) const {
+    bits >>= 2 * half;
+    bool see_lo = (bits & 0x1111) && lo < most, see_hi = (bits & 0x2222) && hi < most;
+    full = (bits & 0x3333) == 0x3333 && lo + 15 < least && hi + 15 < least;
+    pad = lo + 15 >= a.L || hi + 15 >= a.L;
+    if (a.docs) {
+      const Range x = range_of(a, z, lo), y = range_of(a, z, hi);
+      const int from = range.lo < 0 ? 0 : range.lo;
+      see_lo = see_lo && x.hi >= from && x.lo <= range.hi;
+      see_hi = see_hi && y.hi >= from && y.lo <= range.hi;
+      full = full && range.lo == range.hi && x.lo == range.lo && x.hi == range.lo && y.lo == range.lo && y.hi == range.lo;
+      pad = pad || x.lo < 0 || y.lo < 0;
+    }
+    return see_lo || see_hi;
+  }
+};
+
+// the lowest n of eight bits, n any number
+__device__ __forceinline__ uint32_t first_bits(int n) { return (1u << (n < 0 ? 0 : n > 8 ? 8 : n)) - 1u; }
+// value i where bit i of the word is set, else zero (whatever the value: NaN too)
+__device__ __forceinline__ float keep_bit(float v, uint32_t word, int i) {
+  return __builtin_bit_cast(float, __builtin_bit_cast(int, v) & ((int)(word << (31 - i)) >> 31));
+}
+// the bits of the word whose documents (eight and eight consecutive ones) are not the lane's taken out
+__device__ __forceinline__ uint32_t same_document(uint32_t word, const int32_t *docs, int doc) {
+  typedef int i32x4v __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (int g = 0; g < 4; g++) {
+    const i32x4v d = *reinterpret_cast<const i32x4v *>(docs + 16 * (g >> 1) + 4 * (g & 1));
+#pragma unroll
+    for (int i = 0; i < 4; i++) word &= d[i] == doc ? ~0u : ~(1u << (4 * g + i));
+  }
+  return word;
+}
+
+// the documents of a half's 32 positions to LDS, twice (64 lanes)
+__device__ __forceinline__ void load_documents(const int32_t *docs, int lo, int hi, int L, int lane, uint32_t dst) {
+  const int p = (lane & 16 ? hi : lo) + (lane & 15);
+  load_to_lds<4>(reinterpret_cast<const char *>(docs), (uint32_t)(p < L ? p : L - 1) * 4u, 0, dst);
+}
+
+// acc[mt][4g + e] = out[row][32 mt + 8 g + 4 (lane / 32) + e], row = lane % 32 of 32 rows: those of lo (16, of which the first n_lo
+// exist) and hi, through the wavefront's piece of LDS to stores of whole rows
+template <typename T, int D> __device__ __forceinline__ void store_some_rows(unsigned char *piece, T *lo, int n_lo, T *hi, int n_hi, int64_t ld, const f32x16 (&acc)[D / 32], int lane) {
+  typedef Geo<T, D> Q;
+  T *stage = reinterpret_cast<T *>(piece);
+  constexpr int LDS = D + Q::VEC;
+#pragma unroll
+  for (int mt = 0; mt < D / 32; mt++)
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      T *at = stage + (lane & 31) * LDS + 32 * mt + 8 * g + 4 * (lane >> 5);
+      if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<f32x4 *>(at) = f32x4{acc[mt][4 * g], acc[mt][4 * g + 1], acc[mt][4 * g + 2], acc[mt][4 * g + 3]};
+      } else {
+        union { u32x2 raw; T e[4]; } pk;
+#pragma unroll
+        for (int e = 0; e < 4; e++) pk.e[e] = from_float<T>(acc[mt][4 * g + e]);
+        *reinterpret_cast<u32x2 *>(at) = pk.raw;
+      }
+    }
+  __builtin_amdgcn_wave_barrier();   // LDS operations of one wavefront complete in order; this only pins the code order
+  constexpr int RPS = 64 / Q::CPR;   // rows per store
+#pragma unroll
+  for (int i = 0; i < 32 / RPS; i++) {
+    const int r = i * RPS + lane / Q::CPR, ch = lane % Q::CPR;
+    const bool low = i * RPS < 16;
+    if ((low ? r < n_lo : r - 16 < n_hi)) {
+      T *dst = (low ? lo + (int64_t)r * ld : hi + (int64_t)(r - 16) * ld) + Q::VEC * ch;
+      __builtin_nontemporal_store(*reinterpret_cast<const u32x4 *>(stage + r * LDS + Q::VEC * ch), reinterpret_cast<u32x4 *>(dst));
+    }
+  }
+  __builtin_amdgcn_wave_barrier();
+}
+template <typename T, int D> constexpr int rules_lds() {
+  constexpr int ring = Geo<T, D>::RING + 2 * Geo<T, D>::EXTRA, out = 64 * (D + Geo<T, D>::VEC) * Geo<T, D>::ESZ;
+  return ring > out ? ring : out;
+}
+
+// line and (batch, head) of a workgroup, as line_of
+__device__ __forceinline__ void rules_line_of(int64_t wg, const RuleArgs &a, int &line, int &zh) {
+  const int per = kHeadsTogether * a.R, first = (int)(wg / per) * kHeadsTogether, j = (int)(wg % per);
+  const int heads = a.Z * a.H - first < kHeadsTogether ? a.Z * a.H - first : kHeadsTogether;
+  line = a.R - 1 - j / heads;
+  zh = first + j % heads;
+}
+
+// everybody's LDS operations are done
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+template <typename K> int rules_launch(K kernel, int64_t n_wg, int lds, std::atomic<uint64_t> &done, const RuleArgs &a, hipStream_t st) {
+  if (lds > 65536 && !raise_lds_limit(reinterpret_cast<const void *>(kernel), lds, done)) return BSP_ERR_HIP;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)n_wg), dim3(128), lds, st, a);
+  return BSP_OK;
+}
+
+}  // namespace
+
+// call -> kernel arguments, checked (attention_rules_fwd.hip)
+int rules_args(const bsp_attention_rules_call *c, RuleArgs &a);
+}  // namespace bsp
+#endif

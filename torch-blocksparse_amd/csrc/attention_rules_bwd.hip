@@ -1,0 +1,425 @@
+// Backward pass of attention with score rules (attention_rules.h), p = exp2(y - ref) * factor computed again:
+//     dv = p^T . do,   e = p * (dp - delta) * (1 - t^2)  (t the tanh of a capped score),   dq = scale * e . k,   dk = scale * e^T . q
+// with dp = do . v^T and delta = sum_d do_d o_d.
+//   row kernel    : a line of tiles per workgroup -> dq and -delta
+//   column kernel : a column of tiles (or a part of a long one) of a key head per workgroup -> dk and dv; the column's tiles are
+//                   those of all the query heads that share the key head, one after the other, so their sum needs no memory
+#include "attention_rules.h"
+
+namespace bsp {
+namespace {
+
+template <typename T, int D, bool CAP> constexpr int row_waves() { return sizeof(T) == 4 ? (D == 64 ? 2 : 1) : D == 64 ? (CAP ? 2 : 3) : 2; }
+template <typename T, int D, bool CAP> constexpr int col_waves() { return sizeof(T) == 4 ? 1 : D == 64 ? 2 : 1; }
+
+template <typename T, int D, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(128, (row_waves<T, D, CAP>())) k_rules_bwd_rows(RuleArgs a) {
+  typedef Geo<T, D> Q;
+  constexpr int MT = D / 32;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  unsigned char *extra = smem + Q::RING;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, half = lane >> 5;
+  const int64_t wg = xcd_remap(blockIdx.x, (int64_t)a.Z * a.H * a.R);
+  int line, zh;
+  rules_line_of(wg, a, line, zh);
+  const int h = zh % a.H, z = zh / a.H, hk = h / a.G;
+  const table_ptr lut = as_table(a.lut);
+  const int row = line * 64 + 32 * wave + l32, row_in = row < a.L ? row : a.L - 1;
+  bool dead;
+  LineRules rules;
+  rules.init(a, z, line, row, dead);
+  f32x16 dq[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; mt++) dq[mt] = zeros16();
+
+  held_t<T, D> xo;
+  hold_operand<T, D>(xo, reinterpret_cast<const T *>(a.d_o) + z * a.do_sz + h * a.do_sh + row_in * a.do_ld, half, dead);
+  float delta = 0.f;
+  {
+    held_t<T, D> of;
+    hold_operand<T, D>(of, reinterpret_cast<const T *>(a.o_in) + z * a.oin_sz + h * a.oin_sh + row_in * a.oin_ld, half, dead);
+#pragma unroll
+    for (int s = 0; s < Q::NF; s++)
+#pragma unroll
+      for (int i = 0; i < Q::VEC; i++) delta = fmaf(to_float(xo[s][i]), to_float(of[s][i]), delta);
+    delta += swap32(delta);
+  }
+  if (half == 0) a.delta[((int64_t)z * a.H + h) * a.rows + row] = -delta;   // (its negative: where the column kernel's dp starts from)
+
+  Walk walk;
+  walk.init(a.lut + lut[2 * (h * a.R + line) + 1], line * 64 < a.L ? lut[2 * (h * a.R + line)] * 2 : 0);
+  auto next = [&]() {
+    return walk.next(lane, [&](int lo, int hi, int bits, int hf, bool &full, bool &pad) { return rules.look(a, z, lo, hi, bits, hf, full, pad); });
+  };
+  const float *stats = a.ref + ((int64_t)z * a.H + h) * 2 * a.rows + row;
+  const float ref = stats[0], factor = stats[a.rows];
+  Half cur = next();
+  if (cur.n >= 0) {
+    held_t<T, D> xq;
+    hold_operand<T, D>(xq, reinterpret_cast<const T *>(a.q) + z * a.q_sz + h * a.q_sh + row_in * a.q_ld, half, dead);
+    const float slope = BIAS ? a.slopes[h] * kLog2e : 0.f;
+    const char *pk = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.k) + z * a.k_sz + hk * a.k_sh);
+    const char *pv = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.v) + z * a.v_sz + hk * a.v_sh);
+    const int32_t *docs = a.docs ? a.docs + z * a.docs_sz : nullptr;
+    const uint32_t k_row = (uint32_t)a.k_ld * Q::ESZ, v_row = (uint32_t)a.v_ld * Q::ESZ;
+    RowsLoad<T, D, sizeof(T) == 4> gk, gv;
+    gk.init(a.k_ld, lane);
+    gv.init(a.v_ld, lane);
+    auto issue = [&](int stage_no, const Half &x) {
+      const uint32_t st = lds_address(smem) + stage_no * Q::STAGE + wave * (16 * Q::RB);
+      const int pos = wave ? x.hi : x.lo;
+      gk.issue(pk, pos, k_row, st, a.L, lane);
+      gv.issue(pv, pos, v_row, st + Q::PIECE, a.L, lane);
+      if (docs && wave == 0) load_documents(docs, x.lo, x.hi, a.L, lane, lds_address(extra) + stage_no * Q::EXTRA);
+    };
+    issue(0, cur);
+    PieceReads<T, D, false> reads;                      // the same for the k and the v piece
+    reads.init(smem, lane);
+
+    auto step = [&](auto stage_no) {
+      constexpr int S = decltype(stage_no)::value;
+      const Half nxt = next();
+      quad_barrier();
+      const int32_t *kd = reinterpret_cast<const int32_t *>(extra + S * Q::EXTRA);
+      if (cur.pad) {
+        clear_rows<T, D>(smem + S * Q::STAGE, 16 * wave, kd, docs != nullptr, wave ? cur.hi : cur.lo, a.L, lane);
+        lds_barrier();
+      }
+      if (nxt.n >= 0) issue(1 - S, nxt);
+      uint32_t seen = 0xffffu;                          // as in the forward kernel
+      if (!cur.full) {
+        const int mine = cur.bits >> (2 * (cur.n & 1) + 8 * wave + 4 * ((lane >> 4) & 1));
+        seen = (mine & 1 ? first_bits(rules.limit - cur.lo - 8 * half) : 0u) | (mine & 2 ? first_bits(rules.limit - cur.hi - 8 * half) << 8 : 0u);
+        if (docs) seen = same_document(seen, kd + 8 * half, rules.doc);
+      }
+      const bool some = __builtin_amdgcn_ballot_w64(seen != 0) != 0, whole = __builtin_amdgcn_ballot_w64(seen != 0xffffu) == 0;
+      if (some) {
+        f32x16 s = rows_times<T, D, S * Q::STAGE, false>(smem, reads, xq, zeros16());
+        const f32x16 dp = rows_times<T, D, S * Q::STAGE + Q::PIECE, false>(smem, reads, xo, zeros16());
+        const float near[2] = {BIAS ? (float)(row - cur.lo - 8 * half) : 0.f, BIAS ? (float)(row - cur.hi - 8 * half) : 0.f};
+        float e[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          float through = 1.f, x = s[i];
+          if constexpr (CAP) {
+            x = tanh_of<T>(x, a.in);
+            through = fmaf(-x, x, 1.f);
+          }
+          const float p = __builtin_amdgcn_exp2f(fmaf(x, a.out, BIAS ? fmaf(fabsf(near[i >> 3] - (float)(i & 7)), -slope, -ref) : -ref));
+          e[i] = p * (dp[i] - delta);
+          if constexpr (CAP) e[i] *= through;
+        }
+        if (!whole)
+#pragma unroll
+          for (int i = 0; i < 16; i++) e[i] = keep_bit(e[i], seen, i);
+        Shares<T> ds;
+        ds.set(e);
+        columns_times<T, D, S * Q::STAGE, false>(dq, smem, reads, ds);
+      }
+      cur = nxt;
+      return cur.n >= 0;
+    };
+    while (step(Const<0>{}) && step(Const<1>{})) {}
+  }
+  const float last = a.scale * factor;
+#pragma unroll
+  for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) dq[mt][i] *= last;
+  quad_barrier();                                       // the ring is free
+  T *po = reinterpret_cast<T *>(a.o) + z * a.o_sz + h * a.o_sh;
+  const int first = line * 64 + 32 * wave;
+  store_some_rows<T, D>(smem + wave * (32 * (D + Q::VEC) * Q::ESZ), po + (int64_t)first * a.o_ld, a.L - first, po + (int64_t)(first + 16) * a.o_ld, a.L - first - 16, a.o_ld, dq, lane);
+}
+
+// Columns.  A work item is a column of tiles (64 keys: four groups of sixteen) of a key head or a part of a long one: twelve
+// ints (tiles, offset of their entries, key head, column, slot of its partial sums or -1, ., ., ., the positions of the four groups
+// of keys); an entry names the four groups of rows, each by its query head among those of the key head, times 2^24, plus its
+// position.  A wavefront owns 32 of the keys; its k and v rows stay in registers.
+constexpr int kHeadShift = 24, kPosition = (1 << kHeadShift) - 1;
+
+template <typename T, int D, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(128, (col_waves<T, D, CAP>())) k_rules_bwd_cols(RuleArgs a) {
+  typedef Geo<T, D> Q;
+  constexpr int MT = D / 32;
+  constexpr bool LEAN = D == 128 || sizeof(T) == 4;     // dk, dv, k and v alone take 192 registers there
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  unsigned char *extra = smem + Q::RING;                // per stage: ref of its 32 rows, their factors, their -delta (twice), their documents (twice)
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, half = lane >> 5;
+  const int64_t wg = xcd_remap(blockIdx.x, (int64_t)a.Z * a.R);
+  const int item = (int)(wg % a.R), z = (int)(wg / a.R);
+  const table_ptr head = as_table(a.lut) + 12 * item;
+  const int hk = head[2], slot = head[4];
+  const int key_lo = head[8 + 2 * wave], key_hi = head[8 + 2 * wave + 1];
+  const int key = (l32 < 16 ? key_lo : key_hi) + (l32 & 15), key_in = key < a.L ? key : a.L - 1;
+  const int32_t *docs = a.docs ? a.docs + z * a.docs_sz : nullptr;
+  const int doc = docs ? docs[key_in] : 0;
+  const bool dead = key >= a.L || doc < 0;
+  const int prefix = a.causal && a.prefix ? as_table(a.prefix)[z] : 0;
+  // the lane's key is seen by the rows from this one on
+  const int from = dead ? kPosition : a.causal && key >= prefix ? key : 0;
+  int key_min = head[8], key_max = head[8];
+#pragma unroll
+  for (int g = 1; g < 4; g++) {
+    const int p = head[8 + g];
+    key_min = p < key_min ? p : key_min;
+    key_max = p > key_max ? p : key_max;
+  }
+  key_max += 15;
+  const int most = a.causal && key_max >= prefix ? key_max : 0, least = a.causal && key_min >= prefix ? key_min : 0;   // rows from `most` on see all of the column's keys, those below `least` none
+  Range range{0, 0};
+  if (docs) {
+    range = range_of(a, z, head[8]);
+#pragma unroll
+    for (int g = 1; g < 4; g++) {
+      const Range r = range_of(a, z, head[8 + g]);
+      range.lo = r.lo < range.lo ? r.lo : range.lo;
+      range.hi = r.hi > range.hi ? r.hi : range.hi;
+    }
+  }
+  f32x16 dk[MT], dv[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; mt++) dk[mt] = dv[mt] = zeros16();
+
+  Walk walk;
+  walk.init(a.lut + head[1], key_min < a.L ? head[0] * 2 : 0);
+  auto next = [&]() {
+    return walk.next(lane, [&](int lo, int hi, int bits, int hf, bool &full, bool &pad) {
+      bits >>= 8 * hf;
+      lo &= kPosition;
+      hi &= kPosition;
+      bool see_lo = (bits & 0x0f) && lo < a.L && lo + 15 >= least, see_hi = (bits & 0xf0) && hi < a.L && hi + 15 >= least;
+      full = (bits & 0xff) == 0xff && lo >= most && hi >= most;
+      pad = lo + 15 >= a.L || hi + 15 >= a.L;
+      if (docs) {
+        const Range x = range_of(a, z, lo), y = range_of(a, z, hi);
+        const int low = range.lo < 0 ? 0 : range.lo;
+        see_lo = see_lo && x.hi >= low && x.lo <= range.hi;
+        see_hi = see_hi && y.hi >= low && y.lo <= range.hi;
+        full = full && range.lo == range.hi && x.lo == range.lo && x.hi == range.lo && y.lo == range.lo && y.hi == range.lo;
+        pad = pad || x.lo < 0 || y.lo < 0;
+      }
+      return see_lo || see_hi;
+    });
+  };
+  Half cur = next();
+  if (cur.n >= 0) {
+    held_t<T, D> xk, xv;
+    hold_operand<T, D>(xk, reinterpret_cast<const T *>(a.k) + z * a.k_sz + hk * a.k_sh + key_in * a.k_ld, half, dead);
+    hold_operand<T, D>(xv, reinterpret_cast<const T *>(a.v) + z * a.v_sz + hk * a.v_sh + key_in * a.v_ld, half, dead);
+    const int first_head = hk * a.G;
+    const char *pq = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.q) + z * a.q_sz + first_head * a.q_sh);
+    const char *pdo = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.d_o) + z * a.do_sz + first_head * a.do_sh);
+    const char *pstat = reinterpret_cast<const char *>(wave == 0 ? a.ref + ((int64_t)z * a.H + first_head) * 2 * a.rows : a.delta + ((int64_t)z * a.H + first_head) * a.rows);
+    const uint32_t q_row = (uint32_t)a.q_ld * Q::ESZ, do_row = (uint32_t)a.do_ld * Q::ESZ;
+    RowsLoad<T, D, LEAN> gq, gdo;
+    gq.init(a.q_ld, lane);
+    gdo.init(a.do_ld, lane);
+    auto issue = [&](int stage_no, const Half &x) {
+      const uint32_t st = lds_address(smem) + stage_no * Q::STAGE + wave * (16 * Q::RB), ex = lds_address(extra) + stage_no * Q::EXTRA;
+      const int pos = wave ? x.hi : x.lo, hq = pos >> kHeadShift, lo = x.lo & kPosition, hi = x.hi & kPosition;
+      gq.issue(pq + hq * a.q_sh * Q::ESZ, pos & kPosition, q_row, st, a.L, lane);
+      gdo.issue(pdo + hq * a.do_sh * Q::ESZ, pos & kPosition, do_row, st + Q::PIECE, a.L, lane);
+      const int per = (int)a.rows << (1 - wave), at_lo = (x.lo >> kHeadShift) * per + lo, at_hi = (x.hi >> kHeadShift) * per + hi;
+      load_to_lds<4>(pstat, (uint32_t)((lane & 16 ? at_hi : at_lo) + (lane & 15) + (wave == 0 && half ? (int)a.rows : 0)) * 4u, 0, ex + wave * 256);
+      if (docs && wave == 1) load_documents(docs, lo, hi, a.L, lane, ex + 512);
+    };
+    issue(0, cur);
+    PieceReads<T, D, LEAN> reads;                       // the same for the q and the do piece
+    reads.init(smem, lane);
+
+    auto step = [&](auto stage_no) {
+      constexpr int S = decltype(stage_no)::value, Q0 = S * Q::STAGE, O0 = Q0 + Q::PIECE;
+      const Half nxt = next();
+      quad_barrier();
+      const int lo = cur.lo & kPosition, hi = cur.hi & kPosition;
+      const float *stat = reinterpret_cast<const float *>(extra + S * Q::EXTRA);
+      const int32_t *rd = reinterpret_cast<const int32_t *>(extra + S * Q::EXTRA + 512);
+      if (cur.pad) {
+        clear_rows<T, D>(smem + Q0, 16 * wave, rd, docs != nullptr, wave ? hi : lo, a.L, lane);
+        lds_barrier();
+      }
+      if (nxt.n >= 0) issue(1 - S, nxt);
+      uint32_t seen = 0xffffu;                          // bit i: the lane's key is seen by row i of the lane's sixteen
+      if (!cur.full) {
+        const int mine = cur.bits >> (8 * (cur.n & 1) + 2 * wave + ((lane >> 4) & 1));
+        seen = (mine & 1 ? 0xffu & ~first_bits(from - lo - 8 * half) : 0u) | (mine & 16 ? (0xffu & ~first_bits(from - hi - 8 * half)) << 8 : 0u);
+        if (docs) seen = same_document(seen, rd + 8 * half, doc);
+      }
+      const bool some = __builtin_amdgcn_ballot_w64(seen != 0) != 0, whole = __builtin_amdgcn_ballot_w64(seen != 0xffffu) == 0;
+      if (some) {
+        const bool factors = __builtin_amdgcn_ballot_w64(stat[32 + l32] != 1.f) != 0;
+        f32x16 s = rows_times<T, D, Q0, LEAN>(smem, reads, xk, zeros16());
+        const float near[2] = {BIAS ? (float)(lo + 8 * half - key) : 0.f, BIAS ? (float)(hi + 8 * half - key) : 0.f};
+        float slope[2] = {0.f, 0.f};
+        if constexpr (BIAS) {
+          slope[0] = a.slopes[first_head + (cur.lo >> kHeadShift)] * kLog2e;
+          slope[1] = a.slopes[first_head + (cur.hi >> kHeadShift)] * kLog2e;
+        }
+        if constexpr (CAP)
+#pragma unroll
+          for (int i = 0; i < 16; i++) s[i] = tanh_of<T>(s[i], a.in);
+        // the rows' values, in the lane's order: 8 half .., 16 + 8 half ..
+        const float *st = stat + 8 * half;
+        float p[16], e[16];
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+          const f32x4 ref = *reinterpret_cast<const f32x4 *>(st + 16 * (g >> 1) + 4 * (g & 1));
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const int i = 4 * g + j;
+            p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.out, BIAS ? fmaf(fabsf(near[i >> 3] + (float)(i & 7)), -slope[i >> 3], -ref[j]) : -ref[j]));
+          }
+        }
+        if (factors)
+#pragma unroll
+          for (int g = 0; g < 4; g++) {
+            const f32x4 f = *reinterpret_cast<const f32x4 *>(st + 32 + 16 * (g >> 1) + 4 * (g & 1));
+#pragma unroll
+            for (int j = 0; j < 4; j++) p[4 * g + j] *= f[j];
+          }
+        if (!whole)
+#pragma unroll
+          for (int i = 0; i < 16; i++) p[i] = keep_bit(p[i], seen, i);
+        Shares<T> share;
+        share.set(p);
+        columns_times<T, D, O0, LEAN>(dv, smem, reads, share);
+        f32x16 dp;
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+          const f32x4 nd = *reinterpret_cast<const f32x4 *>(st + 64 + 16 * (g >> 1) + 4 * (g & 1));
+#pragma unroll
+          for (int j = 0; j < 4; j++) dp[4 * g + j] = nd[j];
+        }
+        dp = rows_times<T, D, O0, LEAN>(smem, reads, xv, dp);
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          e[i] = p[i] * dp[i];
+          if constexpr (CAP) e[i] *= fmaf(-s[i], s[i], 1.f);
+        }
+        if (!whole)
+#pragma unroll
+          for (int i = 0; i < 16; i++) e[i] = keep_bit(e[i], seen, i);
+        share.set(e);
+        columns_times<T, D, Q0, LEAN>(dk, smem, reads, share);
+      }
+      cur = nxt;
+      return cur.n >= 0;
+    };
+    while (step(Const<0>{}) && step(Const<1>{})) {}
+  }
+#pragma unroll
+  for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) dk[mt][i] *= a.scale;
+  if (slot >= 0) {                                      // a part of a long column: fp32 sums to its slot [dk, dv][64 keys][D]
+    float *ws = a.partial + ((int64_t)z * a.n_slots + slot) * (2 * 64 * D) + (32 * wave + l32) * D + 4 * half;
+#pragma unroll
+    for (int j = 0; j < MT; j++)
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        *reinterpret_cast<f32x4 *>(ws + 32 * j + 8 * g) = f32x4{dk[j][4 * g], dk[j][4 * g + 1], dk[j][4 * g + 2], dk[j][4 * g + 3]};
+        *reinterpret_cast<f32x4 *>(ws + 64 * D + 32 * j + 8 * g) = f32x4{dv[j][4 * g], dv[j][4 * g + 1], dv[j][4 * g + 2], dv[j][4 * g + 3]};
+      }
+    return;
+  }
+  quad_barrier();                                       // the ring is free
+  unsigned char *stage = smem + wave * (32 * (D + Q::VEC) * Q::ESZ);
+  T *pdk = reinterpret_cast<T *>(a.o) + z * a.o_sz + hk * a.o_sh, *pdv = reinterpret_cast<T *>(a.o2) + z * a.o2_sz + hk * a.o2_sh;
+  store_some_rows<T, D>(stage, pdk + (int64_t)key_lo * a.o_ld, a.L - key_lo, pdk + (int64_t)key_hi * a.o_ld, a.L - key_hi, a.o_ld, dk, lane);
+  store_some_rows<T, D>(stage, pdv + (int64_t)key_lo * a.o2_ld, a.L - key_lo, pdv + (int64_t)key_hi * a.o2_ld, a.L - key_hi, a.o2_ld, dv, lane);
+}
+
+// dk and dv of the columns computed in parts: the sum of the parts' slots in order.  split_lut: per such column eight ints
+// (key head, column, first slot, parts, the positions of its four groups of keys).
+template <typename T, int D> __global__ void __launch_bounds__(256) k_rules_bwd_cols_sum(RuleArgs a) {
+  constexpr int PER = 64 * D / 4, WGS = 2 * PER / 256;   // four values a thread
+  const int piece = blockIdx.x % WGS, col = (blockIdx.x / WGS) % a.n_split, z = (blockIdx.x / WGS) / a.n_split;
+  const table_ptr lut = as_table(a.split_lut) + 8 * col;
+  const int hk = lut[0], first = lut[2], parts = lut[3];
+  const float *ws = a.partial + ((int64_t)z * a.n_slots + first) * (2 * 64 * D);
+  const int g = piece * 256 + threadIdx.x, which = g / PER, rem = g % PER, key = rem / (D / 4), d4 = rem % (D / 4);
+  const int pos = (key < 32 ? (key < 16 ? lut[4] : lut[5]) : (key < 48 ? lut[6] : lut[7])) + (key & 15);
+  if (pos >= a.L) return;
+  f32x4 sum = *reinterpret_cast<const f32x4 *>(ws + 4 * g);
+  for (int part = 1; part < parts; part++) {
+    const f32x4 v = *reinterpret_cast<const f32x4 *>(ws + (int64_t)part * (2 * 64 * D) + 4 * g);
+#pragma unroll
+    for (int e = 0; e < 4; e++) sum[e] += v[e];
+  }
+  T *dst = (which ? reinterpret_cast<T *>(a.o2) + z * a.o2_sz + hk * a.o2_sh + (int64_t)pos * a.o2_ld
+                  : reinterpret_cast<T *>(a.o) + z * a.o_sz + hk * a.o_sh + (int64_t)pos * a.o_ld) + 4 * d4;
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<f32x4 *>(dst) = sum;
+  } else {
+    union { u32x2 raw; T e[4]; } pk;
+#pragma unroll
+    for (int e = 0; e < 4; e++) pk.e[e] = from_float<T>(sum[e]);
+    *reinterpret_cast<u32x2 *>(dst) = pk.raw;
+  }
+}
+
+template <typename T, int D, bool CAP, bool BIAS> int launch_rules_bwd(const RuleArgs &a, bool cols, hipStream_t st) {
+  if (!cols) {
+    static std::atomic<uint64_t> done{0};
+    return rules_launch(k_rules_bwd_rows<T, D, CAP, BIAS>, (int64_t)a.Z * a.H * a.R, rules_lds<T, D>(), done, a, st);
+  }
+  static std::atomic<uint64_t> done{0};
+  const int rc = rules_launch(k_rules_bwd_cols<T, D, CAP, BIAS>, (int64_t)a.Z * a.R, rules_lds<T, D>(), done, a, st);
+  if (rc != BSP_OK) return rc;
+  if (a.n_split > 0)
+    hipLaunchKernelGGL((k_rules_bwd_cols_sum<T, D>), dim3((unsigned)((int64_t)a.Z * a.n_split * (2 * 64 * D / 4 / 256))), dim3(256), 0, st, a);
+  return BSP_OK;
+}
+template <typename T, int D> int launch_rules_bwd(const RuleArgs &a, bool cols, hipStream_t st) {
+  if (a.capped) return a.slopes ? launch_rules_bwd<T, D, true, true>(a, cols, st) : launch_rules_bwd<T, D, true, false>(a, cols, st);
+  return a.slopes ? launch_rules_bwd<T, D, false, true>(a, cols, st) : launch_rules_bwd<T, D, false, false>(a, cols, st);
+}
+int launch_rules_bwd(int dtype, int D, const RuleArgs &a, bool cols, hipStream_t st) {
+  if (dtype == BSP_F16) return D == 64 ? launch_rules_bwd<f16, 64>(a, cols, st) : launch_rules_bwd<f16, 128>(a, cols, st);
+  if (dtype == BSP_BF16) return D == 64 ? launch_rules_bwd<bf16, 64>(a, cols, st) : launch_rules_bwd<bf16, 128>(a, cols, st);
+  return D == 64 ? launch_rules_bwd<float, 64>(a, cols, st) : launch_rules_bwd<float, 128>(a, cols, st);
+}
+
+}  // namespace
+}  // namespace bsp
+
+using namespace bsp;
+
+static inline bool off16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+
+extern "C" int bsp_attention_rules_bwd(const bsp_attention_rules_call *call, const void *d_o, const void *q, const void *k, const void *v, const void *o,
+                                       void *dq, void *dk, void *dv, float *neg_delta, const int32_t *d_items, int n_items, float *partial, int n_slots,
+                                       const int32_t *d_split, int n_split, void *stream) {
+  RuleArgs a;
+  const int rc = rules_args(call, a);
+  if (rc != BSP_OK) return rc;
+  const int64_t *s = call->strides;
+  if (!d_o || !q || !k || !v || !o || !dq || !neg_delta || !call->stats || (dk != nullptr) != (dv != nullptr)) return BSP_ERR_ARG;
+  const void *ptrs[] = {d_o, q, k, v, o, dq, dk, dv, partial};
+  for (const void *p : ptrs)
+    if (off16(p)) return BSP_ERR_ARG;
+  for (int i = 2; i < 24; i += 3)
+    if (!s[i] && (dk || i < 18)) return BSP_ERR_ARG;
+  if (dk && (!d_items || n_items <= 0 || n_slots < 0 || n_split < 0 || (n_slots > 0) != (n_split > 0) || (n_slots > 0 && (!partial || !d_split)))) return BSP_ERR_ARG;
+  if (dk && ((int64_t)a.Z * n_items >= ((int64_t)1 << 31) || (int64_t)a.Z * n_split * 16 >= ((int64_t)1 << 31) || a.rows * 2 * a.G >= ((int64_t)1 << 30))) return BSP_ERR_UNSUPPORTED;
+  a.q = q; a.k = k; a.v = v; a.d_o = d_o; a.o_in = o; a.delta = neg_delta;
+  a.oin_sz = s[9]; a.oin_sh = s[10]; a.oin_ld = s[11];
+  a.do_sz = s[12]; a.do_sh = s[13]; a.do_ld = s[14];
+  a.o = dq; a.o_sz = s[15]; a.o_sh = s[16]; a.o_ld = s[17];
+  const hipStream_t st = as_stream(stream);
+  int rl = launch_rules_bwd(call->dtype, call->D, a, false, st);
+  if (rl != BSP_OK) return rl;
+  if (dk) {
+    a.o = dk; a.o_sz = s[18]; a.o_sh = s[19]; a.o_ld = s[20];
+    a.o2 = dv; a.o2_sz = s[21]; a.o2_sh = s[22]; a.o2_ld = s[23];
+    a.lut = d_items; a.R = n_items;
+    a.partial = partial; a.n_slots = n_slots; a.split_lut = d_split; a.n_split = n_split;
+    rl = launch_rules_bwd(call->dtype, call->D, a, true, st);
+    if (rl != BSP_OK) return rl;
+  }
+  BSP_LAUNCH_CHECK();
+  return BSP_OK;
+}

@@ -94,6 +94,8 @@ SIGNATURES = {
     'bsp_attention_f32_slots': (_i64, [_i, _i]),
     'bsp_attention_f32_fwd': (_i, [_vp] * 6),
     'bsp_attention_f32_bwd': (_i, [_vp] * 9 + [_i, _vp, _i, _vp, _i, _vp]),
+    'bsp_attention_rules_fwd': (_i, [_vp] * 6),
+    'bsp_attention_rules_bwd': (_i, [_vp] * 11 + [_i, _vp, _i, _vp, _i, _vp]),
     'bsp_layout_fixed': (_i, [_vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp]),
     'bsp_layout_sparse_transformer': (_i, [_vp, _i, _i, _i, _i, _i, _vp]),
     'bsp_layout_bigbird': (_i, [_vp, _i, _i, _i, _i, _i, _vp, _i, _vp]),
@@ -158,6 +160,22 @@ def check(code, what):
 
 def stream_ptr(device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+class _Nothing:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_nothing = _Nothing()
+
+
+def on_device(device):
+    """a context in which `device` is the current one (launches go to it); costs nothing where it is already"""
+    return _nothing if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def ptr(t):

@@ -1,0 +1,260 @@
+"""Block-sparse attention whose scores follow rules: a cap, a bias by distance, documents, a causal order with a prefix.
+
+`Attention(layout, block)(q, k, v, ...)` is the chain scores -> softmax -> context of the attention modules for models whose masks
+and biases are functions of the positions.  The modules take those as tensors of every pair (`rpe`, `attn_mask`); here they are a few
+numbers per row or head and no pair of positions costs memory:
+
+    y_ij = softcap * tanh(scale * q_i . k_j / softcap) - slopes[h] * |i - j|        (softcap 0: scale * q_i . k_j - ...)
+    o_i  = sum_j softmax_j(y_ij) v_j   over the keys j that row i sees
+
+Row i sees key j if block (h, i // block, j // block) is in the layout, if documents[z, i] == documents[z, j] >= 0 (where documents
+are given) and, with causal, if j <= i or j < prefix[z].  A row that sees no key gets zeros, as result and as gradient.  Positions
+with a negative document number (padding) see nothing and are seen by nothing: what q, k, v and the incoming gradient hold there
+reaches no result, NaN included.  At positions that some rows see, a NaN or an infinity in v (in the backward pass, in any operand) can make
+rows NaN that do not see it, as 0 * NaN does in a product with a masked softmax.
+
+One kernel forward, two backward (rows: dq; columns: dk and dv), none of which stores a sparse tensor (bsp_attention_rules_fwd,
+bsp_attention_rules_bwd).  The results of a call are the same bits every time.
+"""
+import ctypes
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+
+class _Call(ctypes.Structure):             # bsp_attention_rules_call
+    _fields_ = ([(n, ctypes.c_int) for n in ('dtype', 'Z', 'H', 'kv_heads', 'lines', 'D')] + [('length', ctypes.c_int64), ('strides', ctypes.c_int64 * 24)]
+                + [(n, ctypes.c_float) for n in ('scale', 'softcap')] + [('causal', ctypes.c_int), ('slopes', ctypes.c_void_p), ('documents', ctypes.c_void_p),
+                   ('documents_stride', ctypes.c_int64), ('prefix', ctypes.c_void_p), ('ranges', ctypes.c_void_p), ('d_rows', ctypes.c_void_p), ('stats', ctypes.c_void_p)])
+
+
+def _strides(t):
+    """batch, head and row stride; those that no address depends on as the kernels want them"""
+    z, h, row, _ = t.stride()
+    return (z if t.size(0) > 1 else 0, h if t.size(1) > 1 else 0, row if t.size(2) > 1 else t.size(3))
+
+
+def _addressable(t):
+    """t, or a copy of it where the kernels could not address t: unit inner stride, 16-byte vectors, rows that do not overlap and lie
+    within 4 GiB of a head's first"""
+    z, h, row = _strides(t)
+    unit = 16 // t.element_size()
+    if (t.stride(3) == 1 and not (z | h | row) % unit and row >= t.size(3) and not t.data_ptr() % 16
+            and row * (t.size(2) + 64) * t.element_size() < 2 ** 32):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+class _Tables:
+    """The tables of a layout on one device: the lines of 64 rows, and per number of query heads that share a key head the columns of
+    64 keys (bsp_attention_tables_build)."""
+
+    def __init__(self, layout, block, device):
+        lay = (layout != 0).cpu()
+        if block > 64:                     # larger blocks are read as blocks of 64
+            lay = lay.repeat_interleave(block // 64, 1).repeat_interleave(block // 64, 2)
+        self.block, self.device = min(block, 64), device
+        S = 64 // self.block
+        self.layout = torch.nn.functional.pad(lay.to(torch.uint8), (0, -lay.size(2) % S, 0, -lay.size(1) % S)).contiguous()
+        host, info = self._build(self.layout)
+        self.lines = info.lines
+        self.rows = host[:info.items_offset].to(device)
+        self._columns = dict()
+
+    def _build(self, lay):
+        H, R, C = lay.shape
+        info = _lib.AttentionTables()
+        cap = 32 * H * (R + C) + 16 * int(torch.count_nonzero(lay)) + 64
+        host = torch.empty(cap, dtype=torch.int32)
+        _lib.check(_lib.load().bsp_attention_tables_build(_lib.ptr(lay), H, R, C, self.block, _lib.ptr(host), cap, ctypes.byref(info)), 'bsp_attention_tables_build')
+        return host, info
+
+    # Work items of the columns for a launch over `batches` sequences: a column of many tiles is cut into parts, so that the longest do not
+    # outlast the launch (twice the average, as in the tables of the other kernels) and a small launch still has some
+    # WANTED items for its 256 compute units; every part costs a slot of 512 D bytes written and read.
+    WANTED = 1024
+
+    def columns(self, kv_heads, batches):
+        """(items, number of items, splits, number of splits, slots), tensors on the device"""
+        H, R, C = self.layout.shape
+        tiles = self._columns.get(kv_heads)
+        if tiles is None:
+            host, info = self._build(self.layout.view(kv_heads, H // kv_heads * R, C))
+            items = host[info.items_offset:info.split_offset]
+            heads = items[:12 * info.n_items].view(-1, 12).clone()
+            begin = -(-12 * info.n_items // 8) * 8                   # (entries start at a multiple of eight ints)
+            entries = items[begin:].view(-1, 8).clone()
+            if kv_heads != H:              # positions of the stacked query heads -> query head and position in it
+                length = R * self.block
+                entries[:, :4] = (entries[:, :4] // length << 24) + entries[:, :4] % length
+            # the builder's own parts of a column are joined again: by key head and column, in the order of their entries
+            column = heads[:, 2].long() * info.columns + heads[:, 3]
+            order = torch.argsort(column * (len(entries) + 1) + (heads[:, 1] - begin) // 8)
+            heads, column = heads[order], column[order]
+            first = (heads[:, 1].long() - begin) // 8
+            whole = torch.ones(info.n_items, dtype=torch.bool)
+            whole[1:] = column[1:] != column[:-1]
+            group = whole.cumsum(0) - 1
+            count = torch.zeros(int(group[-1]) + 1, dtype=torch.long).index_add_(0, group, heads[:, 0].long())
+            tiles = self._columns[kv_heads] = (heads[whole], first[whole], count, entries, dict())
+        heads, first, count, entries, made = tiles
+        total, n = int(count.sum()), count.numel()
+        part = max(16, -(-2 * total // n))
+        while part > 4 and batches * int(((count + part - 1) // part).clamp(min=1).sum()) < self.WANTED:
+            part //= 2
+        if part not in made:
+            made[part] = self._cut(heads, first, count, entries, part)
+        return made[part]
+
+    def _cut(self, heads, first, count, entries, part):
+        parts = ((count + part - 1) // part).clamp(min=1)
+        of = torch.repeat_interleave(torch.arange(count.numel()), parts)
+        k = torch.arange(of.numel()) - (parts.cumsum(0) - parts)[of]
+        base, rest = (count // parts)[of], (count % parts)[of]
+        items = heads[of].clone()
+        items[:, 0] = (base + (k < rest)).int()
+        items[:, 1] = (12 * of.numel() + 8 * (first[of] + k * base + torch.minimum(k, rest))).int()
+        split = parts[of] > 1
+        items[:, 4] = torch.where(split, split.long().cumsum(0) - 1, -1).int()
+        slots = int(split.sum())
+        cut = parts > 1
+        splits = torch.stack([heads[cut, 2], heads[cut, 3], (parts[cut].cumsum(0) - parts[cut]).int(), parts[cut].int()] + [heads[cut, 8 + g] for g in range(4)], 1)
+        # the key heads of about four query heads at a time, their longest items first: q and do of those stay in L2 and no long item starts last
+        near = items[:, 2].long() // max(1, 4 * int(heads[:, 2].max() + 1) // self.layout.size(0))
+        order = torch.argsort(near * (1 << 32) - items[:, 0], stable=True)
+        dev = torch.cat([items[order].flatten(), entries.flatten()]).to(self.device)
+        return dev, of.numel(), splits.contiguous().to(self.device) if slots else None, splits.size(0), slots
+
+
+class _rules(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, q, k, v, tables, scale, softcap, slopes, causal, documents, prefix, grad_enabled):
+        lib = _lib.load()
+        q, k, v = _addressable(q), _addressable(k), _addressable(v)
+        Z, H, L, D = q.shape
+        keep = grad_enabled and any(ctx.needs_input_grad[:3])
+        o = torch.empty((Z, H, L, D), dtype=q.dtype, device=q.device)
+        stats = torch.empty((Z, H, 2, 64 * tables.lines), dtype=torch.float32, device=q.device) if keep else None
+        ranges = torch.empty((Z, (L + 15) // 16, 2), dtype=torch.int32, device=q.device) if documents is not None else None
+        call = _rules.call(q, k, v, o, tables, scale, softcap, slopes, causal, documents, prefix, ranges, stats)
+        _lib.check(lib.bsp_attention_rules_fwd(ctypes.byref(call), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _lib.stream_ptr(q.device)), 'bsp_attention_rules_fwd')
+        if keep:
+            ctx.save_for_backward(q, k, v, o, stats, ranges, slopes, documents, prefix)
+            ctx.tables, ctx.numbers = tables, (scale, softcap, causal)
+        return o
+
+    @staticmethod
+    def call(q, k, v, o, tables, scale, softcap, slopes, causal, documents, prefix, ranges, stats, grads=()):
+        Z, H, L, D = q.shape
+        strides = [s for t in (q, k, v, o) + tuple(grads) for s in (_strides(t) if t is not None else (0, 0, 0))]
+        p = lambda t: None if t is None else t.data_ptr()   # noqa: E731
+        return _Call(_lib.DTYPES[q.dtype], Z, H, k.size(1), tables.lines, D, L, (ctypes.c_int64 * 24)(*strides), scale, softcap, int(causal), p(slopes), p(documents),
+                     documents.stride(0) if documents is not None and Z > 1 else 0, p(prefix), p(ranges), tables.rows.data_ptr(), p(stats))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        q, k, v, o, stats, ranges, slopes, documents, prefix = ctx.saved_tensors
+        tables, (scale, softcap, causal) = ctx.tables, ctx.numbers
+        need_q, need_k, need_v = ctx.needs_input_grad[:3]
+        with _lib.on_device(q.device):
+            do = _addressable(do)
+            Z, H, L, D = q.shape
+            new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)   # noqa: E731
+            dq, dk, dv = new(q), None, None
+            delta = torch.empty((Z, H, 64 * tables.lines), dtype=torch.float32, device=q.device)
+            items, n_items, splits, n_splits, slots, partial = None, 0, None, 0, 0, None
+            if need_k or need_v:
+                dk, dv = new(k), new(v)
+                items, n_items, splits, n_splits, slots = tables.columns(k.size(1), Z)
+                partial = torch.empty((Z, slots, 2, 64, D), dtype=torch.float32, device=q.device) if slots else None
+            call = _rules.call(q, k, v, o, tables, scale, softcap, slopes, causal, documents, prefix, ranges, stats, (do, dq, dk, dv))
+            p = _lib.ptr
+            _lib.check(_lib.load().bsp_attention_rules_bwd(ctypes.byref(call), p(do), p(q), p(k), p(v), p(o), p(dq), p(dk), p(dv), p(delta), p(items), n_items,
+                                                           p(partial), slots, p(splits), n_splits, _lib.stream_ptr(q.device)), 'bsp_attention_rules_bwd')
+        return (dq if need_q else None, dk if need_k else None, dv if need_v else None) + (None,) * 8
+
+
+class Attention:
+    """Attention over a block-sparse layout [heads, blocks, blocks] (block 16, 32, 64 or 128) with score rules.
+
+    Called with q [batch, heads, length, dim] and k, v [batch, key heads, length, dim]: dim 64 or 128, float16, bfloat16 or float32, the
+    number of heads a multiple of that of the key heads (query head h uses key head h // (heads / key heads)), any length that ends in the
+    layout's last block.
+
+    scale     factor of the scores
+    softcap   0 for none, else the scores are softcap * tanh(scale * q . k / softcap)
+    slopes    None, or [heads] float32: slopes[h] * |i - j| is taken off the scores (constants: no gradient)
+    causal    row i sees the keys up to i only
+    documents None, or [batch, length] int32: a row sees keys of its own document only; negative: padding
+    prefix    None, or [batch] int32, with causal: keys before prefix[z] are seen by every row
+
+    Differentiable in q, k and v, once.  Tables are made at the first call on a device (for a backward pass, at the first
+    one), so a call that is captured into a graph needs one like it before."""
+
+    def __init__(self, layout, block):
+        if layout.dim() != 3 or layout.size(1) != layout.size(2):
+            raise ValueError('layout must have shape [heads, blocks, blocks]')
+        if block not in (16, 32, 64, 128):
+            raise ValueError('block must be 16, 32, 64 or 128 (got %s)' % (block,))
+        if layout.size(0) > 0 and layout.size(1) * block >= 1 << 24:
+            raise ValueError('the layout covers %d positions, more than 2^24' % (layout.size(1) * block))
+        self.layout, self.block = layout, block
+        self._tables = dict()
+
+    def tables(self, device):
+        made = self._tables.get(device)
+        if made is None:
+            made = self._tables[device] = _Tables(self.layout, self.block, device)
+        return made
+
+    def __getstate__(self):
+        return dict(self.__dict__, _tables=dict())
+
+    def _check(self, q, k, v, softcap, scale, slopes, causal, documents, prefix):
+        for name, t in (('q', q), ('k', k), ('v', v)):
+            _lib.require_gpu_tensor(t, name)
+            if t.dim() != 4:
+                raise ValueError('%s must have shape [batch, heads, length, dim]' % name)
+            if t.dtype != q.dtype or t.device != q.device:
+                raise ValueError('q, k and v must be of one type and on one device')
+        if q.dtype not in _lib.DTYPES:
+            raise ValueError('Attention supports float16, bfloat16 and float32 (got %s)' % q.dtype)
+        Z, H, L, D = q.shape
+        kv = k.size(1)
+        if D not in (64, 128):
+            raise ValueError('head dimensions are 64 and 128 (got %d)' % D)
+        if k.shape != v.shape or tuple(k.shape) != (Z, kv, L, D) or kv == 0 or H % kv:
+            raise ValueError('q %s, k %s and v %s do not fit together' % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+        if H // kv > 127:
+            raise ValueError('at most 127 query heads share a key head (got %d)' % (H // kv))
+        heads, blocks = self.layout.shape[:2]
+        if H != heads or -(-L // self.block) != blocks:
+            raise ValueError('q %s does not fit a layout of %d heads and %d blocks of %d' % (tuple(q.shape), heads, blocks, self.block))
+        if not (softcap >= 0 and math.isfinite(softcap) and math.isfinite(scale)):
+            raise ValueError('softcap must be finite and not negative, scale finite (got %s and %s)' % (softcap, scale))
+        if prefix is not None and not causal:
+            raise ValueError('a prefix needs causal=True')
+        for name, t, shape, dtype in (('slopes', slopes, (H,), torch.float32), ('documents', documents, (Z, L), torch.int32), ('prefix', prefix, (Z,), torch.int32)):
+            if t is not None and (tuple(t.shape) != shape or t.dtype != dtype or t.device != q.device):
+                raise ValueError('%s must be %s %s on %s (got %s %s on %s)' % (name, dtype, list(shape), q.device, t.dtype, list(t.shape), t.device))
+        if slopes is not None and slopes.requires_grad:
+            raise ValueError('slopes are constants: they get no gradient')
+
+    def __call__(self, q, k, v, scale=1., softcap=0., slopes=None, causal=False, documents=None, prefix=None):
+        scale, softcap = float(scale), float(softcap or 0.)
+        self._check(q, k, v, softcap, scale, slopes, causal, documents, prefix)
+        if q.size(0) == 0:
+            return torch.empty_like(q) + 0 * (q.sum() + k.sum() + v.sum())
+        if slopes is not None:
+            slopes = slopes.contiguous()
+        if prefix is not None:
+            prefix = prefix.contiguous()
+        if documents is not None and documents.size(1) > 1 and documents.stride(1) != 1:
+            documents = documents.contiguous()
+        with _lib.on_device(q.device):
+            return _rules.apply(q, k, v, self.tables(q.device), scale, softcap, slopes, bool(causal), documents, prefix, torch.is_grad_enabled())
