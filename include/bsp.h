@@ -521,6 +521,37 @@ int bsp_attention_rules_bwd(const bsp_attention_rules_call *call, const void *d_
                             void *dq, void *dk, void *dv, float *neg_delta, const int32_t *d_items, int n_items, float *partial, int n_slots,
                             const int32_t *d_split, int n_split, void *stream);
 
+/* A quantised cache of keys and values.  A page holds `block` (16, 32, 64, 128) consecutive positions of a sequence for `heads` key
+ * heads of D = 64 or 128 elements in `bits` = 4 or 8: bsp_cache_page_bytes bytes, pages back to back at a 16-byte aligned address.
+ * Position `at` of page p is slot p * block + at.  Of 32 neighbouring elements, taken into [-65504, 65504], least = fp16(min), step =
+ * fp16((max - least) / (2^bits - 1)), code = (x - least) / step to the nearest integer, ties to even, in 0 .. 2^bits - 1 (0 where step is 0),
+ * all in exact arithmetic; the element then is least + code * step.  A group with a NaN becomes NaN.  How they lie in a page: csrc/cache.h.
+ * write: k, v: element (t, head, d) at t * stride_t + head * stride_h + d, 16-byte aligned, strides multiples of 8 elements (fp32: 4);
+ *   slots: [T]; those outside the cache (negative ones) are left out; of positions with one slot the last is written.  owner: [n_pages *
+ *   block] ints, zero before the first call (each call leaves them so).
+ * read: k, v: [T, heads, D], contiguous; slots outside the cache give zeros. */
+int64_t bsp_cache_page_bytes(int block, int heads, int D, int bits);
+int bsp_cache_write(int dtype, void *pages, int n_pages, int block, int heads, int D, int bits, const void *k, int64_t k_stride_t, int64_t k_stride_h,
+                    const void *v, int64_t v_stride_t, int64_t v_stride_h, const int32_t *slots, int T, int32_t *owner, void *stream);
+int bsp_cache_read(int dtype, const void *pages, int n_pages, int block, int heads, int D, int bits, void *k, void *v, const int32_t *slots, int T,
+                   void *stream);
+
+/* Attention of one position a sequence over such a cache: o = softmax(y) . v, y_j = softcap * tanh(scale * q . k_j / softcap) - slope_h *
+ * (n - 1 - j) (softcap 0: no cap), over the positions j < n = lengths[b] of the sequence: position j is in page table[b * table_stride
+ * + j / block] (numbers outside 0 .. n_pages - 1: not held, not seen).  A length of at most 0 gives zeros, one past width * block (n_rows *
+ * block) counts as that.  q, o: [B, H, D] in fp16 or bf16, q 16-byte aligned with strides that are multiples of 8; query head h uses key head
+ * h / (H / kv_heads).  rows: NULL, or what is seen beside that: the query heads of a key head form units of at most 16 (ceil(G / ceil(G / 16)) heads of G each,
+ * the last may have fewer); per unit n_rows + 1 ints, from rows[0] on: the place in `rows` of the first entry of each block-row of the unit's
+ * layout and the end of the last one's; an entry: block-column << 16 | a bit for each of the unit's heads that sees it.  The row is (n - 1) /
+ * block.  splits: workgroups that a sequence's positions are split among (bsp_cache_attention_splits gives a good number for
+ * rows of `blocks` blocks at most); workspace: bsp_cache_attention_workspace_bytes bytes, 16-byte aligned, or NULL where that is 0. */
+int bsp_cache_attention_splits(int B, int H, int kv_heads, int block, int64_t blocks);
+int64_t bsp_cache_attention_workspace_bytes(int B, int H, int kv_heads, int D, int splits);
+int bsp_cache_attention(int dtype, const void *q, int64_t q_stride_b, int64_t q_stride_h, void *o, int64_t o_stride_b, int64_t o_stride_h, int B, int H,
+                        const void *pages, int n_pages, int block, int kv_heads, int D, int bits, const int32_t *table, int64_t table_stride, int width,
+                        const int32_t *lengths, const int32_t *rows, int n_rows, float scale, float softcap, const float *slopes, void *workspace,
+                        int64_t workspace_bytes, int splits, void *stream);
+
 /* ---------------------------------------------------------------------------------------------------
  * Dense utility ops of the reference package.
  * ReLU: replaces the relu_y / relu_dxdsdbdres kernels and their launches (relu.py:8-91).  All tensors hold n

@@ -5,10 +5,11 @@ from .matmul import MatMul, Linear
 from .attention import MultiheadAttention, make_layout, replace_mha
 from .deepspeedsparseselfattention import DeepSpeedSparseSelfAttention, SparseSelfAttention, SparsityConfig
 from .rules import Attention
+from .cache import KeyValueCache, CacheAttention
 from .layouts import fixed_layout, bigbird_layout, sparse_transformer_layout
 from .permute import _permute, Permute
 from .relu import ReLU
 
 __all__ = ['Softmax', 'MatMul', 'Linear', 'MultiheadAttention', 'make_layout', 'replace_mha',
            'DeepSpeedSparseSelfAttention', 'SparseSelfAttention', 'SparsityConfig', 'fixed_layout', 'bigbird_layout', 'sparse_transformer_layout',
-           'Permute', 'ReLU', 'Attention']
+           'Permute', 'ReLU', 'Attention', 'KeyValueCache', 'CacheAttention']
