@@ -500,7 +500,8 @@ int bsp_attention_f32_bwd(const bsp_attention_f32_call *call, const float *d_o, 
  * [Z][ceil(length / 16)][2] ints, written by fwd and read by bwd.
  * bwd: neg_delta: [Z][H][64 lines] floats of scratch.  dk and dv: both or neither.  d_items .. n_split: the columns of
  * bsp_attention_tables_build for the layout [kv_heads, lines of the H / kv_heads query heads, columns], the positions in their
- * entries split into 2^24 * (query head of the key head) + position in it; partial: [Z][n_slots][2][64][D] floats.  No atomics: the
+ * entries split into 2^24 * (query head of the key head) + position in it; n_items work items for each key head, by key head, the longest
+ * first, those past a head's own with column -1; partial: [Z][n_slots][2][64][D] floats.  No atomics: the
  * same call gives the same bits. */
 typedef struct {
   int dtype, Z, H, kv_heads, lines, D;

@@ -43,9 +43,14 @@ def test_tables_hold_every_block_once(shape, block, kv, density):
     for batches in (1, 3, 1000):
         items, n_items, splits, n_splits, slots = t.columns(kv, batches)
         got = torch.zeros_like(want, dtype=torch.int32)
-        heads, used, keys = items[:12 * n_items].view(-1, 12), [], dict()
-        for i in heads.tolist():
-            assert i[1] >= 12 * n_items and (i[1] - 12 * n_items) % 8 == 0 and i[1] + 8 * i[0] <= items.numel()
+        heads, used, keys = items[:12 * kv * n_items].view(kv, n_items, 12), [], dict()
+        assert bool((heads[:, 1:, 0] <= heads[:, :-1, 0]).all())
+        for at, i in enumerate(heads.flatten(0, 1).tolist()):
+            assert i[1] >= 12 * kv * n_items and (i[1] - 12 * kv * n_items) % 8 == 0 and i[1] + 8 * i[0] <= items.numel()
+            if i[3] < 0:
+                assert i[0] == 0 and i[4] == -1
+                continue
+            assert i[2] == at // n_items
             used += [i[4]] if i[4] >= 0 else []
             keys.setdefault((i[2], i[3]), []).append(i)
             for e in items[i[1]:i[1] + 8 * i[0]].view(-1, 8):
@@ -61,6 +66,27 @@ def test_tables_hold_every_block_once(shape, block, kv, density):
         for s in ([] if splits is None else splits.tolist()):
             parts = cut[s[0], s[1]]
             assert sorted(i[4] for i in parts) == list(range(s[2], s[2] + s[3])) and s[4:] == parts[0][8:]
+
+
+def test_every_item_has_one_workgroup():
+    # the order of workgroups in the kernels (rules_place): each item of each head once, and the XCDs (every eighth workgroup) get equal shares of them
+    for units in (1, 2, 7, 8, 9, 12, 16, 40, 100):
+        for n in (1, 3, 8, 65):
+            rest, spread = units % 8, (units % 8 * n + 7) // 8 * 8
+            got, share = set(), [0] * 8
+            for wg in range(spread + units // 8 * 8 * n):
+                if wg < spread:
+                    unit, item = (units // 8 * 8 + wg % rest if wg // rest < n else -1), wg // rest
+                else:
+                    per, x, i = units // 8, wg - spread & 7, wg - spread >> 3
+                    first = i // (4 * n) * 4
+                    heads = min(4, per - first)
+                    unit, item = x * per + first + i % (4 * n) % heads, i % (4 * n) // heads
+                if unit >= 0:
+                    assert 0 <= unit < units and 0 <= item < n and (unit, item) not in got
+                    got.add((unit, item))
+                    share[wg % 8] += 1
+            assert len(got) == units * n and max(share) - min(share) <= 1
 
 
 def test_refusals_of_the_constructor():

@@ -9,12 +9,13 @@
 // (keys of a column) and walks the line's (column's) tiles in halves of 32 columns (rows).  What the rules add:
 //   * a walk (Walk): 64 halves at a time, one a lane, are held against the rules by their positions and the range of document numbers
 //     in each group of sixteen positions; three lane masks say which halves any row sees, which every row sees whole, and
-//     which hold positions without document or past the end.  The loop visits the first kind only, and looks at single scores
+//     which hold positions without document.  The loop visits the first kind only, and looks at single scores
 //     in those of them that are not of the second.
 //   * a score is seen or not by a bit of a sixteen-bit word per lane.  What the position rules leave of a lane's two runs of
 //     eight consecutive keys is a run itself, so the word is two shifts; documents are compared one by one.
-//   * positions without document (padding) and past the end may hold anything, NaN included: their rows of a stage are set to zero
-//     before the products (0 * NaN would reach every row of the tile).
+//   * positions without document (padding) may hold anything, NaN included: their rows of a stage are set to zero before the
+//     products (0 * NaN would reach every row of the tile).  Positions past the end are loaded as zeros: operands are fetched
+//     through buffer descriptors that end with the head's last row.
 // fp32: the same kernels on the fp32 matrix units (32x32x2), which take their operands as they lie in a row: no transposing reads.
 #ifndef BSP_ATTENTION_RULES_H
 #define BSP_ATTENTION_RULES_H
@@ -30,7 +31,7 @@ struct RuleArgs {
   int64_t rows;                    // 64 * lines
   int64_t q_sz, q_sh, q_ld, k_sz, k_sh, k_ld, v_sz, v_sh, v_ld, do_sz, do_sh, do_ld, oin_sz, oin_sh, oin_ld;
   int64_t o_sz, o_sh, o_ld, o2_sz, o2_sh, o2_ld;
-  float in, out;                   // y = out * tanh(in * s / 2) with a cap, s * out without (see logit_args)
+  float in, out;                   // y = out * tanh(in * s / 2) with a cap, s * out without
   float scale;                     // of the sums dq and dk
   const float *slopes;
   const int32_t *docs; int64_t docs_sz;
@@ -41,7 +42,7 @@ struct RuleArgs {
   float *partial;                  // column kernel: slots of the parts of long columns, [Z][n_slots][dk, dv][64][D]
   const int32_t *split_lut;
   int n_slots, n_split;
-  int Z, H, G, R, L;               // G: query heads a key head; R: lines of the table per head, 64 R >= L (column kernel: work items)
+  int Z, H, G, R, L;               // G: query heads a key head; R: lines of the table per head, 64 R >= L (column kernel: work items of a key head)
 };
 
 namespace {
@@ -69,7 +70,22 @@ template <typename T, int D> __device__ __forceinline__ void hold_operand(held_t
   }
 }
 
-// Sixteen consecutive rows, global -> LDS.  Rows behind the last are fetched as that one (and not used).
+// `bytes` bytes from p on as a buffer: loads from behind it give zeros
+typedef int i32x4r __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ i32x4r buffer_of(const void *p, int64_t bytes) {
+  const uint64_t at = reinterpret_cast<uint64_t>(p);
+  return i32x4r{(int)(uint32_t)at, (int)(uint32_t)(at >> 32) & 0xffff, (int)(uint32_t)bytes, 0x00020000};
+}
+// the rows of a head: row stride ld and `length` rows of D elements
+template <typename T, int D> __device__ __forceinline__ i32x4r rows_buffer(const T *p, int64_t ld, int length) { return buffer_of(p, ((length - 1) * ld + D) * (int64_t)sizeof(T)); }
+// load_to_lds from a buffer
+template <int BYTES> __device__ __forceinline__ void buffer_to_lds(const i32x4r &rsrc, uint32_t off, uint32_t add, uint32_t dst) {
+  uint32_t at;                                            // (the addition also is the instruction that must lie between m0 and its use)
+  if constexpr (BYTES == 16) asm volatile("s_mov_b32 m0, %4\n\tv_add_u32 %0, %2, %1\n\tbuffer_load_dwordx4 %0, %3, 0 offen lds" : "=&v"(at) : "v"(off), "s"(add), "s"(rsrc), "s"(dst) : "memory");
+  else asm volatile("s_mov_b32 m0, %4\n\tv_add_u32 %0, %2, %1\n\tbuffer_load_dword %0, %3, 0 offen lds" : "=&v"(at) : "v"(off), "s"(add), "s"(rsrc), "s"(dst) : "memory");
+}
+
+// Sixteen consecutive rows, global -> LDS.  Rows behind the last one come as zeros.
 template <typename T, int D, bool LEAN> struct RowsLoad {
   typedef Geo<T, D> Q;
   static constexpr int RPL = 64 / Q::CPR, LW = 16 / RPL;
@@ -81,33 +97,25 @@ template <typename T, int D, bool LEAN> struct RowsLoad {
     for (int i = 0; i < (LEAN ? 1 : LW); i++)
       off[i] = (uint32_t)((i * RPL + lane / Q::CPR) * ld) * Q::ESZ + (LEAN ? 0u : (chunk ^ (uint32_t)rule_swz<T, D>(i * RPL)) << 4);
   }
-  __device__ __forceinline__ void issue(const char *base, int pos, uint32_t row_bytes, uint32_t lds, int L, int lane) const {
-    if (pos + 16 <= L) {
-      uint32_t c = chunk;
-      if constexpr (LEAN) asm volatile("" : "+v"(c));
+  __device__ __forceinline__ void issue(const i32x4r &rows, int pos, uint32_t row_bytes, uint32_t lds) const {
+    uint32_t c = chunk;
+    if constexpr (LEAN) asm volatile("" : "+v"(c));
 #pragma unroll
-      for (int i = 0; i < LW; i++)
-        if constexpr (LEAN) load_to_lds<16>(base, off[0] + ((c ^ (uint32_t)rule_swz<T, D>(i * RPL)) << 4), (uint32_t)(pos + i * RPL) * row_bytes, lds + i * 1024);
-        else load_to_lds<16>(base, off[i], (uint32_t)pos * row_bytes, lds + i * 1024);
-    } else {
-#pragma unroll
-      for (int i = 0; i < LW; i++) {
-        const int r = pos + i * RPL + lane / Q::CPR;
-        load_to_lds<16>(base, (uint32_t)(r < L ? r : L - 1) * row_bytes + ((chunk ^ (uint32_t)rule_swz<T, D>(i * RPL)) << 4), 0, lds + i * 1024);
-      }
-    }
+    for (int i = 0; i < LW; i++)
+      if constexpr (LEAN) buffer_to_lds<16>(rows, off[0] + ((c ^ (uint32_t)rule_swz<T, D>(i * RPL)) << 4), (uint32_t)(pos + i * RPL) * row_bytes, lds + i * 1024);
+      else buffer_to_lds<16>(rows, off[i], (uint32_t)pos * row_bytes, lds + i * 1024);
   }
 };
 
-// Row `row` of a piece (0 .. 31) to zeros: the lane's chunk of it
-template <typename T, int D> __device__ __forceinline__ void clear_rows(unsigned char *piece, int row0, const int32_t *docs_of_stage, bool docs, int pos, int L, int lane) {
+// Those of sixteen rows (from row0 on) of a stage's two pieces whose positions carry no document: zeros
+template <typename T, int D> __device__ __forceinline__ void clear_rows(unsigned char *piece, int row0, const int32_t *docs_of_stage, int lane) {
   typedef Geo<T, D> Q;
   constexpr int RPL = 64 / Q::CPR;
 #pragma unroll 1
   for (int i = 0; i < 16 / RPL; i++) {
-    const int r = i * RPL + lane / Q::CPR;
-    if (pos + r >= L || (docs && docs_of_stage[row0 + r] < 0)) {
-      u32x4 *at = reinterpret_cast<u32x4 *>(piece + (row0 + r) * Q::RB + (lane % Q::CPR) * 16);
+    const int r = row0 + i * RPL + lane / Q::CPR;
+    if (docs_of_stage[r] < 0) {
+      u32x4 *at = reinterpret_cast<u32x4 *>(piece + r * Q::RB + (lane % Q::CPR) * 16);
       *at = u32x4{0, 0, 0, 0};
       at[Q::PIECE / 16] = u32x4{0, 0, 0, 0};
     }
@@ -188,11 +196,12 @@ __device__ __forceinline__ void columns_times(f32x16 (&acc)[D / 32], const unsig
   }
 }
 
-// tanh(x) for x = in * s / 2 and s -> logit.  1 - 2 / (exp(2 x) + 1) is off by 2^-23 at most, which cap * log2 e takes to the logit: little
-// beside what 16-bit operands leave of it.  In fp32 small x (in trained models most) take the series, which keeps their relative precision:
-// up to x = 0.45 its next term is below 2^-27 of the sum.
-template <typename T> __device__ __forceinline__ float tanh_of(float s, float in) {
-  const float t = fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * (in * kLog2e)) + 1.f), 1.f);
+// Capped scores.  With x = scale * s / cap, tanh(x) = 1 - 2 r and 1 - tanh(x)^2 = 4 (r - r^2), r = 1 / (exp(2 x) + 1): the kernels for 16-bit
+// types keep r, whose error of 2^-24 cap * log2 e takes to the logit: little beside what the operands' rounding leaves of it.  In fp32 they keep
+// the tanh, from its series where x is small (in trained models nearly everywhere) with its relative precision: up to x = 0.45 the
+// next term is below 2^-27 of the sum.
+template <typename T> __device__ __forceinline__ float cap_score(float s, float in) {
+  const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * (in * kLog2e)) + 1.f);
   if constexpr (sizeof(T) == 4) {
     const float x = 0.5f * in * s, z = x * x;
     float p = fmaf(z, 21844.f / 6081075.f, -1382.f / 155925.f);
@@ -200,10 +209,19 @@ template <typename T> __device__ __forceinline__ float tanh_of(float s, float in
     p = fmaf(z, p, -17.f / 315.f);
     p = fmaf(z, p, 2.f / 15.f);
     p = fmaf(z, p, -1.f / 3.f);
-    return z < 0.2025f ? fmaf(x * z, p, x) : t;
+    return z < 0.2025f ? fmaf(x * z, p, x) : fmaf(-2.f, r, 1.f);
   }
-  return t;
+  return r;
 }
+// 1 - tanh^2 of what cap_score gives, or (QUARTER, 16-bit types) a quarter of it, which is one operation less
+template <typename T, bool QUARTER> __device__ __forceinline__ float cap_through(float c) {
+  if constexpr (sizeof(T) == 4) return fmaf(-c, c, 1.f);
+  else if constexpr (QUARTER) return fmaf(-c, c, c);
+  else return fmaf(-4.f * c, c, 4.f * c);
+}
+// the logit of a score s (or of what cap_score gives) is s * factor + shift
+template <typename T, bool CAP> __device__ __forceinline__ float logit_factor(float out) { return CAP && sizeof(T) != 4 ? -2.f * out : out; }
+template <typename T, bool CAP> __device__ __forceinline__ float logit_shift(float out) { return CAP && sizeof(T) != 4 ? out : 0.f; }
 inline void logit_args(RuleArgs &a, float scale, float cap) {
   a.scale = scale;
   a.capped = cap > 0.f;
@@ -219,54 +237,56 @@ __device__ __forceinline__ Range range_of(const RuleArgs &a, int z, int pos) {
   return Range{r[0], r[1]};
 }
 
-// The halves of a line's (column's) tiles that are worth a visit, 64 looked at together, one a lane
+// The halves of a line's (column's) tiles that are worth a visit, 64 looked at together, one a lane.  From the last to the first: in a
+// causal layout the nearest keys come first then, whose logits a bias by distance makes the largest, so that the running maximum is found at
+// once (from the first on it moves in two steps of three: 221 us for the forward pass of fp16 8 x 16 x 4096 over the layout of blocks of
+// 16 with stride 64).
 struct Half { int n, lo, hi, bits; bool full, pad; };
-struct Walk {
+template <bool DOCS> struct Walk {
   const int32_t *core;
-  int steps, base;
+  int base;
   uint64_t live, full, pad;
   int v_lo, v_hi, v_bits;
   __device__ __forceinline__ void init(const int32_t *entries, int halves) {
     core = entries;
-    steps = halves;
-    base = -64;
+    base = halves;                 // halves at and above it are done
     live = 0;
   }
-  // look(lo, hi, bits of the half's pieces, &full, &pad) -> does any row see anything of it
+  // look(lo, hi, bits of the half's pieces, which half of its tile, &full, &pad) -> does any row see anything of it
   template <class F> __device__ __forceinline__ Half next(int lane, F &&look) {
     while (live == 0) {
-      base += 64;
-      if (base >= steps) return Half{-1, 0, 0, 0, false, false};
-      const int n = base + lane, at = n < steps ? n : steps - 1;
+      if (base <= 0) return Half{-1, 0, 0, 0, false, false};
+      const int end = base;
+      base = base > 64 ? base - 64 : 0;
+      const int n = base + lane, at = n < end ? n : end - 1;
       const int32_t *e = core + kEntry * (at >> 1);
       v_lo = e[2 * (at & 1)];
       v_hi = e[2 * (at & 1) + 1];
       v_bits = e[4];
       bool f = false, p = false;
       const bool l = look(v_lo, v_hi, v_bits, at & 1, f, p);
-      live = __builtin_amdgcn_ballot_w64(l && n < steps);
+      live = __builtin_amdgcn_ballot_w64(l && n < end);
       full = __builtin_amdgcn_ballot_w64(f);
-      pad = __builtin_amdgcn_ballot_w64(p);
+      if constexpr (DOCS) pad = __builtin_amdgcn_ballot_w64(p);
     }
-    const int j = __builtin_ctzll(live);
-    live &= live - 1;
+    const int j = 63 - __builtin_clzll(live);
+    live &= ~((uint64_t)1 << j);
     return Half{base + j, __builtin_amdgcn_readlane(v_lo, j), __builtin_amdgcn_readlane(v_hi, j), __builtin_amdgcn_readlane(v_bits, j),
-                (bool)((full >> j) & 1), (bool)((pad >> j) & 1)};
+                (bool)((full >> j) & 1), DOCS && (bool)((pad >> j) & 1)};
   }
 };
 
 // The rules as the row kernels (a line of 64 rows; the lane has row `row`) apply them
-struct LineRules {
+template <bool DOCS> struct LineRules {
   int most, least;                 // the keys below `most` are seen by a row of the line, those below `least` by all, as far as positions go
   int limit;                       // ... the keys below it by the lane's row
   int doc;                         // the lane's document
   Range range;                     // of the line
   __device__ __forceinline__ void init(const RuleArgs &a, int z, int line, int row, bool &dead) {
-    const int prefix = a.causal && a.prefix ? as_table(a.prefix)[z] : 0, first = line * 64, r = row < a.L ? row : a.L - 1;
+    const int prefix = a.causal && a.prefix ? as_table(a.prefix)[z] : 0, first = line * 64;
     doc = 0;
-    range = Range{0, 0};
-    if (a.docs) {
-      doc = a.docs[z * a.docs_sz + r];
+    if constexpr (DOCS) {
+      doc = a.docs[z * a.docs_sz + (row < a.L ? row : a.L - 1)];
       const int lane = threadIdx.x & 3;
       const Range g = range_of(a, z, first + 16 * lane < a.L ? first + 16 * lane : first);
       int lo = g.lo, hi = g.hi;
@@ -288,16 +308,57 @@ struct LineRules {
     bits >>= 2 * half;
     bool see_lo = (bits & 0x1111) && lo < most, see_hi = (bits & 0x2222) && hi < most;
     full = (bits & 0x3333) == 0x3333 && lo + 15 < least && hi + 15 < least;
-    pad = lo + 15 >= a.L || hi + 15 >= a.L;
-    if (a.docs) {
+    if constexpr (DOCS) {
       const Range x = range_of(a, z, lo), y = range_of(a, z, hi);
       const int from = range.lo < 0 ? 0 : range.lo;
       see_lo = see_lo && x.hi >= from && x.lo <= range.hi;
       see_hi = see_hi && y.hi >= from && y.lo <= range.hi;
       full = full && range.lo == range.hi && x.lo == range.lo && x.hi == range.lo && y.lo == range.lo && y.hi == range.lo;
-      pad = pad || x.lo < 0 || y.lo < 0;
+      pad = x.lo < 0 || y.lo < 0;
     }
     return see_lo || see_hi;
+  }
+};
+
+// floats that are the same in all lanes, read as table_ptr reads tables
+typedef const float __attribute__((address_space(4))) *floats_ptr;
+__device__ __forceinline__ floats_ptr as_floats(const float *p) { return (floats_ptr)p; }
+
+// Logits of the lane's sixteen scores less `minus`: s * out - slope * distance - minus, the scores of run g at distances |at_g - i|, i = 0 .. 7.
+// Where a wavefront's scores all lie on one side of the diagonal (nearly everywhere) the distances are at_g - i or its negative, and
+// one multiply-add more than without a bias is enough.
+template <bool BIAS> struct Logits {
+  float base[2], slope[2];
+  bool straight;
+  __device__ __forceinline__ Logits(int at_lo, int at_hi, float s) : Logits(at_lo, at_hi, s, s) {}
+  __device__ __forceinline__ Logits(int at_lo, int at_hi, float s_lo, float s_hi) {
+    if constexpr (BIAS) {
+      const int least = at_lo < at_hi ? at_lo : at_hi, most = at_lo < at_hi ? at_hi : at_lo;
+      const bool past = __builtin_amdgcn_ballot_w64(least < 7) == 0;        // every distance is at - i
+      straight = past || __builtin_amdgcn_ballot_w64(most > 0) == 0;
+      base[0] = (float)at_lo;
+      base[1] = (float)at_hi;
+      slope[0] = s_lo;
+      slope[1] = s_hi;
+      if (straight) {
+        const float sign = past ? 1.f : -1.f;
+#pragma unroll
+        for (int g = 0; g < 2; g++) slope[g] *= sign, base[g] *= -slope[g];
+      }
+    }
+  }
+  // y(i) for i = 0 .. 15, minus(i) a value per score (a constant, usually)
+  template <class S, class M> __device__ __forceinline__ void get(float (&y)[16], const S &s, float out, M &&minus) const {
+    if constexpr (!BIAS) {
+#pragma unroll
+      for (int i = 0; i < 16; i++) y[i] = fmaf(s[i], out, -minus(i));
+    } else if (straight) {
+#pragma unroll
+      for (int i = 0; i < 16; i++) y[i] = fmaf(s[i], out, fmaf(slope[i >> 3], (float)(i & 7), base[i >> 3] - minus(i)));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; i++) y[i] = fmaf(s[i], out, fmaf(-slope[i >> 3], fabsf(base[i >> 3] - (float)(i & 7)), -minus(i)));
+    }
   }
 };
 
@@ -305,7 +366,7 @@ struct LineRules {
 __device__ __forceinline__ uint32_t first_bits(int n) { return (1u << (n < 0 ? 0 : n > 8 ? 8 : n)) - 1u; }
 // value i where bit i of the word is set, else zero (whatever the value: NaN too)
 __device__ __forceinline__ float keep_bit(float v, uint32_t word, int i) {
-  return __builtin_bit_cast(float, __builtin_bit_cast(int, v) & ((int)(word << (31 - i)) >> 31));
+  return __builtin_bit_cast(float, __builtin_bit_cast(int, v) & __builtin_amdgcn_sbfe((int)word, (uint32_t)i, 1u));
 }
 // the bits of the word whose documents (eight and eight consecutive ones) are not the lane's taken out
 __device__ __forceinline__ uint32_t same_document(uint32_t word, const int32_t *docs, int doc) {
@@ -320,9 +381,8 @@ __device__ __forceinline__ uint32_t same_document(uint32_t word, const int32_t *
 }
 
 // the documents of a half's 32 positions to LDS, twice (64 lanes)
-__device__ __forceinline__ void load_documents(const int32_t *docs, int lo, int hi, int L, int lane, uint32_t dst) {
-  const int p = (lane & 16 ? hi : lo) + (lane & 15);
-  load_to_lds<4>(reinterpret_cast<const char *>(docs), (uint32_t)(p < L ? p : L - 1) * 4u, 0, dst);
+__device__ __forceinline__ void load_documents(const i32x4r &docs, int lo, int hi, int lane, uint32_t dst) {
+  buffer_to_lds<4>(docs, (uint32_t)((lane & 16 ? hi : lo) + (lane & 15)) * 4u, 0, dst);
 }
 
 // acc[mt][4g + e] = out[row][32 mt + 8 g + 4 (lane / 32) + e], row = lane % 32 of 32 rows: those of lo (16, of which the first n_lo
@@ -363,13 +423,38 @@ template <typename T, int D> constexpr int rules_lds() {
   return ring > out ? ring : out;
 }
 
-// line and (batch, head) of a workgroup, as line_of
-__device__ __forceinline__ void rules_line_of(int64_t wg, const RuleArgs &a, int &line, int &zh) {
-  const int per = kHeadsTogether * a.R, first = (int)(wg / per) * kHeadsTogether, j = (int)(wg % per);
-  const int heads = a.Z * a.H - first < kHeadsTogether ? a.Z * a.H - first : kHeadsTogether;
-  line = a.R - 1 - j / heads;
-  zh = first + j % heads;
+// Which of n work items of which of `units` heads (all of equal cost, item 0 the longest) a workgroup does.  Workgroups go round the eight
+// XCDs, each with an L2 of its own: the heads are dealt to the XCDs whole, so that a head's k and v are fetched into one L2, four heads at a
+// time, their longest items first.  Heads past a multiple of eight go first, an item here, an item there: every XCD gets the same
+// share of the long ones.  (One run of heads and lines cut in eight pieces gives the XCDs unequal work: the first half of a causal head's lines is three
+// times the second.  Full causal attention over 8192 positions in 16 heads of 128: 595 us that way.)
+struct Place { int unit, item; };
+__host__ __device__ __forceinline__ int64_t rules_grid(int64_t units, int64_t n) { return (units % 8 * n + 7) / 8 * 8 + units / 8 * 8 * n; }
+__device__ __forceinline__ Place rules_place(uint32_t wg, int units, int n) {
+  const uint32_t rest = units & 7, spread = (rest * n + 7) & ~7u;
+  if (wg < spread) {
+    const Quotient p(wg, rest);
+    return Place{p.q < (uint32_t)n ? (int)((units & ~7) + p.r) : -1, (int)p.q};
+  }
+  wg -= spread;
+  const uint32_t per = units >> 3, x = wg & 7, i = wg >> 3;      // heads per XCD
+  const Quotient g(i, kHeadsTogether * n);
+  const uint32_t first = g.q * kHeadsTogether, heads = per - first < kHeadsTogether ? per - first : kHeadsTogether;
+  const Quotient p(g.r, heads);
+  return Place{(int)(x * per + first + p.r), (int)p.q};
 }
+
+// The query head and batch of a unit: the heads that share a key head next to each other, then the batches (their documents, and with them
+// the cost of a head, may differ: an XCD gets some of each)
+struct HeadOf {
+  int h, hk, z;
+  __device__ __forceinline__ HeadOf(int unit, int Z, int G) {
+    const Quotient g(unit, G), b(g.q, Z);
+    z = b.r;
+    hk = b.q;
+    h = hk * G + g.r;
+  }
+};
 
 // everybody's LDS operations are done
 __device__ __forceinline__ void lds_barrier() {

@@ -12,7 +12,7 @@ namespace {
 template <typename T, int D, bool CAP> constexpr int row_waves() { return sizeof(T) == 4 ? (D == 64 ? 2 : 1) : D == 64 ? (CAP ? 2 : 3) : 2; }
 template <typename T, int D, bool CAP> constexpr int col_waves() { return sizeof(T) == 4 ? 1 : D == 64 ? 2 : 1; }
 
-template <typename T, int D, bool CAP, bool BIAS>
+template <typename T, int D, bool CAP, bool BIAS, bool DOCS>
 __global__ void __launch_bounds__(128, (row_waves<T, D, CAP>())) k_rules_bwd_rows(RuleArgs a) {
   typedef Geo<T, D> Q;
   constexpr int MT = D / 32;
@@ -20,14 +20,15 @@ __global__ void __launch_bounds__(128, (row_waves<T, D, CAP>())) k_rules_bwd_row
   unsigned char *extra = smem + Q::RING;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, half = lane >> 5;
-  const int64_t wg = xcd_remap(blockIdx.x, (int64_t)a.Z * a.H * a.R);
-  int line, zh;
-  rules_line_of(wg, a, line, zh);
-  const int h = zh % a.H, z = zh / a.H, hk = h / a.G;
+  const Place place = rules_place(blockIdx.x, a.Z * a.H, a.R);
+  if (place.unit < 0) return;
+  const int line = a.R - 1 - place.item;                // (the last lines first, which in a causal layout are the longest)
+  const HeadOf head(place.unit, a.Z, a.G);
+  const int h = head.h, z = head.z, hk = head.hk;
   const table_ptr lut = as_table(a.lut);
   const int row = line * 64 + 32 * wave + l32, row_in = row < a.L ? row : a.L - 1;
   bool dead;
-  LineRules rules;
+  LineRules<DOCS> rules;
   rules.init(a, z, line, row, dead);
   f32x16 dq[MT];
 #pragma unroll
@@ -47,7 +48,7 @@ __global__ void __launch_bounds__(128, (row_waves<T, D, CAP>())) k_rules_bwd_row
   }
   if (half == 0) a.delta[((int64_t)z * a.H + h) * a.rows + row] = -delta;   // (its negative: where the column kernel's dp starts from)
 
-  Walk walk;
+  Walk<DOCS> walk;
   walk.init(a.lut + lut[2 * (h * a.R + line) + 1], line * 64 < a.L ? lut[2 * (h * a.R + line)] * 2 : 0);
   auto next = [&]() {
     return walk.next(lane, [&](int lo, int hi, int bits, int hf, bool &full, bool &pad) { return rules.look(a, z, lo, hi, bits, hf, full, pad); });
@@ -58,20 +59,21 @@ __global__ void __launch_bounds__(128, (row_waves<T, D, CAP>())) k_rules_bwd_row
   if (cur.n >= 0) {
     held_t<T, D> xq;
     hold_operand<T, D>(xq, reinterpret_cast<const T *>(a.q) + z * a.q_sz + h * a.q_sh + row_in * a.q_ld, half, dead);
-    const float slope = BIAS ? a.slopes[h] * kLog2e : 0.f;
-    const char *pk = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.k) + z * a.k_sz + hk * a.k_sh);
-    const char *pv = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.v) + z * a.v_sz + hk * a.v_sh);
-    const int32_t *docs = a.docs ? a.docs + z * a.docs_sz : nullptr;
+    const float slope = BIAS ? as_floats(a.slopes)[h] * kLog2e : 0.f, out = logit_factor<T, CAP>(a.out), minus = ref - logit_shift<T, CAP>(a.out) - (CAP && sizeof(T) != 4 ? 2.f : 0.f);   // (e^y times four: see cap_through)
+    const i32x4r pk = rows_buffer<T, D>(reinterpret_cast<const T *>(a.k) + z * a.k_sz + hk * a.k_sh, a.k_ld, a.L);
+    const i32x4r pv = rows_buffer<T, D>(reinterpret_cast<const T *>(a.v) + z * a.v_sz + hk * a.v_sh, a.v_ld, a.L);
+    const i32x4r docs = buffer_of(DOCS ? a.docs + z * a.docs_sz : nullptr, (int64_t)a.L * 4);
     const uint32_t k_row = (uint32_t)a.k_ld * Q::ESZ, v_row = (uint32_t)a.v_ld * Q::ESZ;
     RowsLoad<T, D, sizeof(T) == 4> gk, gv;
     gk.init(a.k_ld, lane);
     gv.init(a.v_ld, lane);
+    // each wavefront loads one of the two groups of sixteen rows of each piece
     auto issue = [&](int stage_no, const Half &x) {
       const uint32_t st = lds_address(smem) + stage_no * Q::STAGE + wave * (16 * Q::RB);
       const int pos = wave ? x.hi : x.lo;
-      gk.issue(pk, pos, k_row, st, a.L, lane);
-      gv.issue(pv, pos, v_row, st + Q::PIECE, a.L, lane);
-      if (docs && wave == 0) load_documents(docs, x.lo, x.hi, a.L, lane, lds_address(extra) + stage_no * Q::EXTRA);
+      gk.issue(pk, pos, k_row, st);
+      gv.issue(pv, pos, v_row, st + Q::PIECE);
+      if (DOCS && wave == 0) load_documents(docs, x.lo, x.hi, lane, lds_address(extra) + stage_no * Q::EXTRA);
     };
     issue(0, cur);
     PieceReads<T, D, false> reads;                      // the same for the k and the v piece
@@ -82,33 +84,33 @@ __global__ void __launch_bounds__(128, (row_waves<T, D, CAP>())) k_rules_bwd_row
       const Half nxt = next();
       quad_barrier();
       const int32_t *kd = reinterpret_cast<const int32_t *>(extra + S * Q::EXTRA);
-      if (cur.pad) {
-        clear_rows<T, D>(smem + S * Q::STAGE, 16 * wave, kd, docs != nullptr, wave ? cur.hi : cur.lo, a.L, lane);
+      if (DOCS && cur.pad) {
+        clear_rows<T, D>(smem + S * Q::STAGE, 16 * wave, kd, lane);
         lds_barrier();
       }
       if (nxt.n >= 0) issue(1 - S, nxt);
       uint32_t seen = 0xffffu;                          // as in the forward kernel
+      bool some = true, whole = true;
       if (!cur.full) {
         const int mine = cur.bits >> (2 * (cur.n & 1) + 8 * wave + 4 * ((lane >> 4) & 1));
         seen = (mine & 1 ? first_bits(rules.limit - cur.lo - 8 * half) : 0u) | (mine & 2 ? first_bits(rules.limit - cur.hi - 8 * half) << 8 : 0u);
-        if (docs) seen = same_document(seen, kd + 8 * half, rules.doc);
+        if constexpr (DOCS) seen = same_document(seen, kd + 8 * half, rules.doc);
+        some = __builtin_amdgcn_ballot_w64(seen != 0) != 0;
+        whole = __builtin_amdgcn_ballot_w64(seen != 0xffffu) == 0;
       }
-      const bool some = __builtin_amdgcn_ballot_w64(seen != 0) != 0, whole = __builtin_amdgcn_ballot_w64(seen != 0xffffu) == 0;
       if (some) {
         f32x16 s = rows_times<T, D, S * Q::STAGE, false>(smem, reads, xq, zeros16());
         const f32x16 dp = rows_times<T, D, S * Q::STAGE + Q::PIECE, false>(smem, reads, xo, zeros16());
-        const float near[2] = {BIAS ? (float)(row - cur.lo - 8 * half) : 0.f, BIAS ? (float)(row - cur.hi - 8 * half) : 0.f};
+        const Logits<BIAS> logits(row - cur.lo - 8 * half, row - cur.hi - 8 * half, slope);
+        if constexpr (CAP)
+#pragma unroll
+          for (int i = 0; i < 16; i++) s[i] = cap_score<T>(s[i], a.in);
         float e[16];
+        logits.get(e, s, out, [&](int) { return minus; });
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-          float through = 1.f, x = s[i];
-          if constexpr (CAP) {
-            x = tanh_of<T>(x, a.in);
-            through = fmaf(-x, x, 1.f);
-          }
-          const float p = __builtin_amdgcn_exp2f(fmaf(x, a.out, BIAS ? fmaf(fabsf(near[i >> 3] - (float)(i & 7)), -slope, -ref) : -ref));
-          e[i] = p * (dp[i] - delta);
-          if constexpr (CAP) e[i] *= through;
+          e[i] = __builtin_amdgcn_exp2f(e[i]) * (dp[i] - delta);
+          if constexpr (CAP) e[i] *= cap_through<T, true>(s[i]);
         }
         if (!whole)
 #pragma unroll
@@ -134,12 +136,12 @@ __global__ void __launch_bounds__(128, (row_waves<T, D, CAP>())) k_rules_bwd_row
 }
 
 // Columns.  A work item is a column of tiles (64 keys: four groups of sixteen) of a key head or a part of a long one: twelve
-// ints (tiles, offset of their entries, key head, column, slot of its partial sums or -1, ., ., ., the positions of the four groups
+// ints (tiles, offset of their entries, key head, column or -1: nothing to do, slot of its partial sums or -1, ., ., ., the positions of the four groups
 // of keys); an entry names the four groups of rows, each by its query head among those of the key head, times 2^24, plus its
 // position.  A wavefront owns 32 of the keys; its k and v rows stay in registers.
 constexpr int kHeadShift = 24, kPosition = (1 << kHeadShift) - 1;
 
-template <typename T, int D, bool CAP, bool BIAS>
+template <typename T, int D, bool CAP, bool BIAS, bool DOCS>
 __global__ void __launch_bounds__(128, (col_waves<T, D, CAP>())) k_rules_bwd_cols(RuleArgs a) {
   typedef Geo<T, D> Q;
   constexpr int MT = D / 32;
@@ -148,14 +150,17 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, CAP>())) k_rules_bwd_col
   unsigned char *extra = smem + Q::RING;                // per stage: ref of its 32 rows, their factors, their -delta (twice), their documents (twice)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, half = lane >> 5;
-  const int64_t wg = xcd_remap(blockIdx.x, (int64_t)a.Z * a.R);
-  const int item = (int)(wg % a.R), z = (int)(wg / a.R);
-  const table_ptr head = as_table(a.lut) + 12 * item;
-  const int hk = head[2], slot = head[4];
+  const int kv_heads = (int)Quotient(a.H, a.G).q;
+  const Place place = rules_place(blockIdx.x, a.Z * kv_heads, a.R);
+  if (place.unit < 0) return;
+  const HeadOf of(place.unit, a.Z, 1);
+  const int z = of.z, hk = of.hk;
+  const table_ptr head = as_table(a.lut) + 12 * (hk * a.R + place.item);
+  if (head[3] < 0) return;                              // (the key heads' lists are filled up to one length)
+  const int slot = head[4];
   const int key_lo = head[8 + 2 * wave], key_hi = head[8 + 2 * wave + 1];
   const int key = (l32 < 16 ? key_lo : key_hi) + (l32 & 15), key_in = key < a.L ? key : a.L - 1;
-  const int32_t *docs = a.docs ? a.docs + z * a.docs_sz : nullptr;
-  const int doc = docs ? docs[key_in] : 0;
+  const int doc = DOCS ? a.docs[z * a.docs_sz + key_in] : 0;
   const bool dead = key >= a.L || doc < 0;
   const int prefix = a.causal && a.prefix ? as_table(a.prefix)[z] : 0;
   // the lane's key is seen by the rows from this one on
@@ -170,7 +175,7 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, CAP>())) k_rules_bwd_col
   key_max += 15;
   const int most = a.causal && key_max >= prefix ? key_max : 0, least = a.causal && key_min >= prefix ? key_min : 0;   // rows from `most` on see all of the column's keys, those below `least` none
   Range range{0, 0};
-  if (docs) {
+  if constexpr (DOCS) {
     range = range_of(a, z, head[8]);
 #pragma unroll
     for (int g = 1; g < 4; g++) {
@@ -183,7 +188,7 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, CAP>())) k_rules_bwd_col
 #pragma unroll
   for (int mt = 0; mt < MT; mt++) dk[mt] = dv[mt] = zeros16();
 
-  Walk walk;
+  Walk<DOCS> walk;
   walk.init(a.lut + head[1], key_min < a.L ? head[0] * 2 : 0);
   auto next = [&]() {
     return walk.next(lane, [&](int lo, int hi, int bits, int hf, bool &full, bool &pad) {
@@ -192,14 +197,13 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, CAP>())) k_rules_bwd_col
       hi &= kPosition;
       bool see_lo = (bits & 0x0f) && lo < a.L && lo + 15 >= least, see_hi = (bits & 0xf0) && hi < a.L && hi + 15 >= least;
       full = (bits & 0xff) == 0xff && lo >= most && hi >= most;
-      pad = lo + 15 >= a.L || hi + 15 >= a.L;
-      if (docs) {
+      if constexpr (DOCS) {
         const Range x = range_of(a, z, lo), y = range_of(a, z, hi);
         const int low = range.lo < 0 ? 0 : range.lo;
         see_lo = see_lo && x.hi >= low && x.lo <= range.hi;
         see_hi = see_hi && y.hi >= low && y.lo <= range.hi;
         full = full && range.lo == range.hi && x.lo == range.lo && x.hi == range.lo && y.lo == range.lo && y.hi == range.lo;
-        pad = pad || x.lo < 0 || y.lo < 0;
+        pad = x.lo < 0 || y.lo < 0;
       }
       return see_lo || see_hi;
     });
@@ -210,9 +214,9 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, CAP>())) k_rules_bwd_col
     hold_operand<T, D>(xk, reinterpret_cast<const T *>(a.k) + z * a.k_sz + hk * a.k_sh + key_in * a.k_ld, half, dead);
     hold_operand<T, D>(xv, reinterpret_cast<const T *>(a.v) + z * a.v_sz + hk * a.v_sh + key_in * a.v_ld, half, dead);
     const int first_head = hk * a.G;
-    const char *pq = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.q) + z * a.q_sz + first_head * a.q_sh);
-    const char *pdo = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.d_o) + z * a.do_sz + first_head * a.do_sh);
-    const char *pstat = reinterpret_cast<const char *>(wave == 0 ? a.ref + ((int64_t)z * a.H + first_head) * 2 * a.rows : a.delta + ((int64_t)z * a.H + first_head) * a.rows);
+    const T *pq = reinterpret_cast<const T *>(a.q) + z * a.q_sz + first_head * a.q_sh, *pdo = reinterpret_cast<const T *>(a.d_o) + z * a.do_sz + first_head * a.do_sh;
+    const i32x4r docs = buffer_of(DOCS ? a.docs + z * a.docs_sz : nullptr, (int64_t)a.L * 4);
+    const i32x4r stats = wave == 0 ? buffer_of(a.ref + ((int64_t)z * a.H + first_head) * 2 * a.rows, a.G * a.rows * 8) : buffer_of(a.delta + ((int64_t)z * a.H + first_head) * a.rows, a.G * a.rows * 4);
     const uint32_t q_row = (uint32_t)a.q_ld * Q::ESZ, do_row = (uint32_t)a.do_ld * Q::ESZ;
     RowsLoad<T, D, LEAN> gq, gdo;
     gq.init(a.q_ld, lane);
@@ -220,11 +224,11 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, CAP>())) k_rules_bwd_col
     auto issue = [&](int stage_no, const Half &x) {
       const uint32_t st = lds_address(smem) + stage_no * Q::STAGE + wave * (16 * Q::RB), ex = lds_address(extra) + stage_no * Q::EXTRA;
       const int pos = wave ? x.hi : x.lo, hq = pos >> kHeadShift, lo = x.lo & kPosition, hi = x.hi & kPosition;
-      gq.issue(pq + hq * a.q_sh * Q::ESZ, pos & kPosition, q_row, st, a.L, lane);
-      gdo.issue(pdo + hq * a.do_sh * Q::ESZ, pos & kPosition, do_row, st + Q::PIECE, a.L, lane);
+      gq.issue(rows_buffer<T, D>(pq + hq * a.q_sh, a.q_ld, a.L), pos & kPosition, q_row, st);
+      gdo.issue(rows_buffer<T, D>(pdo + hq * a.do_sh, a.do_ld, a.L), pos & kPosition, do_row, st + Q::PIECE);
       const int per = (int)a.rows << (1 - wave), at_lo = (x.lo >> kHeadShift) * per + lo, at_hi = (x.hi >> kHeadShift) * per + hi;
-      load_to_lds<4>(pstat, (uint32_t)((lane & 16 ? at_hi : at_lo) + (lane & 15) + (wave == 0 && half ? (int)a.rows : 0)) * 4u, 0, ex + wave * 256);
-      if (docs && wave == 1) load_documents(docs, lo, hi, a.L, lane, ex + 512);
+      buffer_to_lds<4>(stats, (uint32_t)((lane & 16 ? at_hi : at_lo) + (lane & 15) + (wave == 0 && half ? (int)a.rows : 0)) * 4u, 0, ex + wave * 256);
+      if (DOCS && wave == 1) load_documents(docs, lo, hi, lane, ex + 512);
     };
     issue(0, cur);
     PieceReads<T, D, LEAN> reads;                       // the same for the q and the do piece
@@ -237,42 +241,43 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, CAP>())) k_rules_bwd_col
       const int lo = cur.lo & kPosition, hi = cur.hi & kPosition;
       const float *stat = reinterpret_cast<const float *>(extra + S * Q::EXTRA);
       const int32_t *rd = reinterpret_cast<const int32_t *>(extra + S * Q::EXTRA + 512);
-      if (cur.pad) {
-        clear_rows<T, D>(smem + Q0, 16 * wave, rd, docs != nullptr, wave ? hi : lo, a.L, lane);
+      if (DOCS && cur.pad) {
+        clear_rows<T, D>(smem + Q0, 16 * wave, rd, lane);
         lds_barrier();
       }
       if (nxt.n >= 0) issue(1 - S, nxt);
       uint32_t seen = 0xffffu;                          // bit i: the lane's key is seen by row i of the lane's sixteen
+      bool some = true, whole = true;
       if (!cur.full) {
         const int mine = cur.bits >> (8 * (cur.n & 1) + 2 * wave + ((lane >> 4) & 1));
         seen = (mine & 1 ? 0xffu & ~first_bits(from - lo - 8 * half) : 0u) | (mine & 16 ? (0xffu & ~first_bits(from - hi - 8 * half)) << 8 : 0u);
-        if (docs) seen = same_document(seen, rd + 8 * half, doc);
+        if constexpr (DOCS) seen = same_document(seen, rd + 8 * half, doc);
+        some = __builtin_amdgcn_ballot_w64(seen != 0) != 0;
+        whole = __builtin_amdgcn_ballot_w64(seen != 0xffffu) == 0;
       }
-      const bool some = __builtin_amdgcn_ballot_w64(seen != 0) != 0, whole = __builtin_amdgcn_ballot_w64(seen != 0xffffu) == 0;
       if (some) {
         const bool factors = __builtin_amdgcn_ballot_w64(stat[32 + l32] != 1.f) != 0;
         f32x16 s = rows_times<T, D, Q0, LEAN>(smem, reads, xk, zeros16());
-        const float near[2] = {BIAS ? (float)(lo + 8 * half - key) : 0.f, BIAS ? (float)(hi + 8 * half - key) : 0.f};
-        float slope[2] = {0.f, 0.f};
+        float slope_lo = 0.f, slope_hi = 0.f;
         if constexpr (BIAS) {
-          slope[0] = a.slopes[first_head + (cur.lo >> kHeadShift)] * kLog2e;
-          slope[1] = a.slopes[first_head + (cur.hi >> kHeadShift)] * kLog2e;
+          slope_lo = as_floats(a.slopes)[first_head + (cur.lo >> kHeadShift)] * kLog2e;
+          slope_hi = as_floats(a.slopes)[first_head + (cur.hi >> kHeadShift)] * kLog2e;
         }
+        const Logits<BIAS> logits(key - lo - 8 * half, key - hi - 8 * half, slope_lo, slope_hi);
         if constexpr (CAP)
 #pragma unroll
-          for (int i = 0; i < 16; i++) s[i] = tanh_of<T>(s[i], a.in);
+          for (int i = 0; i < 16; i++) s[i] = cap_score<T>(s[i], a.in);
         // the rows' values, in the lane's order: 8 half .., 16 + 8 half ..
         const float *st = stat + 8 * half;
         float p[16], e[16];
+        {
+          f32x4 ref[4];
 #pragma unroll
-        for (int g = 0; g < 4; g++) {
-          const f32x4 ref = *reinterpret_cast<const f32x4 *>(st + 16 * (g >> 1) + 4 * (g & 1));
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const int i = 4 * g + j;
-            p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.out, BIAS ? fmaf(fabsf(near[i >> 3] + (float)(i & 7)), -slope[i >> 3], -ref[j]) : -ref[j]));
-          }
+          for (int g = 0; g < 4; g++) ref[g] = *reinterpret_cast<const f32x4 *>(st + 16 * (g >> 1) + 4 * (g & 1));
+          logits.get(p, s, logit_factor<T, CAP>(a.out), [&](int i) { return ref[i >> 2][i & 3] - logit_shift<T, CAP>(a.out); });
         }
+#pragma unroll
+        for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f(p[i]);
         if (factors)
 #pragma unroll
           for (int g = 0; g < 4; g++) {
@@ -297,7 +302,7 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, CAP>())) k_rules_bwd_col
 #pragma unroll
         for (int i = 0; i < 16; i++) {
           e[i] = p[i] * dp[i];
-          if constexpr (CAP) e[i] *= fmaf(-s[i], s[i], 1.f);
+          if constexpr (CAP) e[i] *= cap_through<T, __is_same(T, bf16)>(s[i]);   // (fp16 keeps the factor: what is rounded next should be no smaller than it is)
         }
         if (!whole)
 #pragma unroll
@@ -313,7 +318,7 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, CAP>())) k_rules_bwd_col
 #pragma unroll
   for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-    for (int i = 0; i < 16; i++) dk[mt][i] *= a.scale;
+    for (int i = 0; i < 16; i++) dk[mt][i] *= a.scale * (CAP && __is_same(T, bf16) ? 4.f : 1.f);
   if (slot >= 0) {                                      // a part of a long column: fp32 sums to its slot [dk, dv][64 keys][D]
     float *ws = a.partial + ((int64_t)z * a.n_slots + slot) * (2 * 64 * D) + (32 * wave + l32) * D + 4 * half;
 #pragma unroll
@@ -361,17 +366,20 @@ template <typename T, int D> __global__ void __launch_bounds__(256) k_rules_bwd_
   }
 }
 
-template <typename T, int D, bool CAP, bool BIAS> int launch_rules_bwd(const RuleArgs &a, bool cols, hipStream_t st) {
+template <typename T, int D, bool CAP, bool BIAS, bool DOCS> int launch_rules_bwd(const RuleArgs &a, bool cols, hipStream_t st) {
   if (!cols) {
     static std::atomic<uint64_t> done{0};
-    return rules_launch(k_rules_bwd_rows<T, D, CAP, BIAS>, (int64_t)a.Z * a.H * a.R, rules_lds<T, D>(), done, a, st);
+    return rules_launch(k_rules_bwd_rows<T, D, CAP, BIAS, DOCS>, rules_grid((int64_t)a.Z * a.H, a.R), rules_lds<T, D>(), done, a, st);
   }
   static std::atomic<uint64_t> done{0};
-  const int rc = rules_launch(k_rules_bwd_cols<T, D, CAP, BIAS>, (int64_t)a.Z * a.R, rules_lds<T, D>(), done, a, st);
+  const int rc = rules_launch(k_rules_bwd_cols<T, D, CAP, BIAS, DOCS>, rules_grid((int64_t)a.Z * (a.H / a.G), a.R), rules_lds<T, D>(), done, a, st);
   if (rc != BSP_OK) return rc;
   if (a.n_split > 0)
     hipLaunchKernelGGL((k_rules_bwd_cols_sum<T, D>), dim3((unsigned)((int64_t)a.Z * a.n_split * (2 * 64 * D / 4 / 256))), dim3(256), 0, st, a);
   return BSP_OK;
+}
+template <typename T, int D, bool CAP, bool BIAS> int launch_rules_bwd(const RuleArgs &a, bool cols, hipStream_t st) {
+  return a.docs ? launch_rules_bwd<T, D, CAP, BIAS, true>(a, cols, st) : launch_rules_bwd<T, D, CAP, BIAS, false>(a, cols, st);
 }
 template <typename T, int D> int launch_rules_bwd(const RuleArgs &a, bool cols, hipStream_t st) {
   if (a.capped) return a.slopes ? launch_rules_bwd<T, D, true, true>(a, cols, st) : launch_rules_bwd<T, D, true, false>(a, cols, st);
@@ -404,7 +412,7 @@ extern "C" int bsp_attention_rules_bwd(const bsp_attention_rules_call *call, con
   for (int i = 2; i < 24; i += 3)
     if (!s[i] && (dk || i < 18)) return BSP_ERR_ARG;
   if (dk && (!d_items || n_items <= 0 || n_slots < 0 || n_split < 0 || (n_slots > 0) != (n_split > 0) || (n_slots > 0 && (!partial || !d_split)))) return BSP_ERR_ARG;
-  if (dk && ((int64_t)a.Z * n_items >= ((int64_t)1 << 31) || (int64_t)a.Z * n_split * 16 >= ((int64_t)1 << 31) || a.rows * 2 * a.G >= ((int64_t)1 << 30))) return BSP_ERR_UNSUPPORTED;
+  if (dk && ((int64_t)a.Z * call->kv_heads * n_items >= ((int64_t)1 << 31) - 64 || (int64_t)a.Z * n_split * 16 >= ((int64_t)1 << 31) || a.rows * 2 * a.G >= ((int64_t)1 << 30))) return BSP_ERR_UNSUPPORTED;
   a.q = q; a.k = k; a.v = v; a.d_o = d_o; a.o_in = o; a.delta = neg_delta;
   a.oin_sz = s[9]; a.oin_sh = s[10]; a.oin_ld = s[11];
   a.do_sz = s[12]; a.do_sh = s[13]; a.do_ld = s[14];

@@ -7,31 +7,33 @@
 namespace bsp {
 namespace {
 
-template <typename T, int D> constexpr int fwd_waves() { return sizeof(T) == 4 ? (D == 64 ? 2 : 1) : D == 64 ? 3 : 2; }
+// (four wavefronts a SIMD leave 128 registers, which a bias or documents overrun)
+template <typename T, int D, bool BIAS, bool DOCS> constexpr int fwd_waves() { return sizeof(T) == 4 ? (D == 64 ? 2 : 1) : D == 64 ? (BIAS || DOCS ? 3 : 4) : 2; }
 
-template <typename T, int D, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(128, (fwd_waves<T, D>())) k_rules_fwd(RuleArgs a) {
+template <typename T, int D, bool CAP, bool BIAS, bool DOCS>
+__global__ void __launch_bounds__(128, (fwd_waves<T, D, BIAS, DOCS>())) k_rules_fwd(RuleArgs a) {
   typedef Geo<T, D> Q;
   constexpr int MT = D / 32;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   unsigned char *extra = smem + Q::RING;                // per stage: the documents of its 32 keys, twice
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, half = lane >> 5;
-  const int64_t wg = xcd_remap(blockIdx.x, (int64_t)a.Z * a.H * a.R);
-  int line, zh;
-  rules_line_of(wg, a, line, zh);
-  const int h = zh % a.H, z = zh / a.H, hk = h / a.G;
+  const Place place = rules_place(blockIdx.x, a.Z * a.H, a.R);
+  if (place.unit < 0) return;
+  const int line = a.R - 1 - place.item;                // (the last lines first, which in a causal layout are the longest)
+  const HeadOf head(place.unit, a.Z, a.G);
+  const int h = head.h, z = head.z, hk = head.hk;
   const table_ptr lut = as_table(a.lut);
   const int row = line * 64 + 32 * wave + l32, row_in = row < a.L ? row : a.L - 1;
   bool dead;
-  LineRules rules;
+  LineRules<DOCS> rules;
   rules.init(a, z, line, row, dead);
   f32x16 o[MT];
 #pragma unroll
   for (int mt = 0; mt < MT; mt++) o[mt] = zeros16();
   float m = dead ? 0.f : -INFINITY, l = 0.f;
 
-  Walk walk;
+  Walk<DOCS> walk;
   walk.init(a.lut + lut[2 * (h * a.R + line) + 1], line * 64 < a.L ? lut[2 * (h * a.R + line)] * 2 : 0);
   auto next = [&]() {
     return walk.next(lane, [&](int lo, int hi, int bits, int hf, bool &full, bool &pad) { return rules.look(a, z, lo, hi, bits, hf, full, pad); });
@@ -40,10 +42,10 @@ __global__ void __launch_bounds__(128, (fwd_waves<T, D>())) k_rules_fwd(RuleArgs
   if (cur.n >= 0) {
     held_t<T, D> xq;
     hold_operand<T, D>(xq, reinterpret_cast<const T *>(a.q) + z * a.q_sz + h * a.q_sh + row_in * a.q_ld, half, dead);
-    const float slope = BIAS ? a.slopes[h] * kLog2e : 0.f;
-    const char *pk = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.k) + z * a.k_sz + hk * a.k_sh);
-    const char *pv = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.v) + z * a.v_sz + hk * a.v_sh);
-    const int32_t *docs = a.docs ? a.docs + z * a.docs_sz : nullptr;
+    const float slope = BIAS ? as_floats(a.slopes)[h] * kLog2e : 0.f, factor = logit_factor<T, CAP>(a.out), shift = logit_shift<T, CAP>(a.out);
+    const i32x4r pk = rows_buffer<T, D>(reinterpret_cast<const T *>(a.k) + z * a.k_sz + hk * a.k_sh, a.k_ld, a.L);
+    const i32x4r pv = rows_buffer<T, D>(reinterpret_cast<const T *>(a.v) + z * a.v_sz + hk * a.v_sh, a.v_ld, a.L);
+    const i32x4r docs = buffer_of(DOCS ? a.docs + z * a.docs_sz : nullptr, (int64_t)a.L * 4);
     const uint32_t k_row = (uint32_t)a.k_ld * Q::ESZ, v_row = (uint32_t)a.v_ld * Q::ESZ;
     RowsLoad<T, D, sizeof(T) == 4> gk, gv;
     gk.init(a.k_ld, lane);
@@ -52,9 +54,9 @@ __global__ void __launch_bounds__(128, (fwd_waves<T, D>())) k_rules_fwd(RuleArgs
     auto issue = [&](int stage_no, const Half &x) {
       const uint32_t st = lds_address(smem) + stage_no * Q::STAGE + wave * (16 * Q::RB);
       const int pos = wave ? x.hi : x.lo;
-      gk.issue(pk, pos, k_row, st, a.L, lane);
-      gv.issue(pv, pos, v_row, st + Q::PIECE, a.L, lane);
-      if (docs && wave == 0) load_documents(docs, x.lo, x.hi, a.L, lane, lds_address(extra) + stage_no * Q::EXTRA);
+      gk.issue(pk, pos, k_row, st);
+      gv.issue(pv, pos, v_row, st + Q::PIECE);
+      if (DOCS && wave == 0) load_documents(docs, x.lo, x.hi, lane, lds_address(extra) + stage_no * Q::EXTRA);
     };
     issue(0, cur);
     PieceReads<T, D, false> reads;
@@ -66,45 +68,43 @@ __global__ void __launch_bounds__(128, (fwd_waves<T, D>())) k_rules_fwd(RuleArgs
       const Half nxt = next();
       quad_barrier();
       const int32_t *kd = reinterpret_cast<const int32_t *>(extra + S * Q::EXTRA);
-      if (cur.pad) {
-        clear_rows<T, D>(smem + S * Q::STAGE, 16 * wave, kd, docs != nullptr, wave ? cur.hi : cur.lo, a.L, lane);
+      if (DOCS && cur.pad) {
+        clear_rows<T, D>(smem + S * Q::STAGE, 16 * wave, kd, lane);
         lds_barrier();
       }
       if (nxt.n >= 0) issue(1 - S, nxt);
       uint32_t seen = 0xffffu;                          // bit i: the lane's row sees its key i
+      bool some = true, whole = true;
       if (!cur.full) {
         const int mine = cur.bits >> (2 * (cur.n & 1) + 8 * wave + 4 * ((lane >> 4) & 1));
         seen = (mine & 1 ? first_bits(rules.limit - cur.lo - 8 * half) : 0u) | (mine & 2 ? first_bits(rules.limit - cur.hi - 8 * half) << 8 : 0u);
-        if (docs) seen = same_document(seen, kd + 8 * half, rules.doc);
+        if constexpr (DOCS) seen = same_document(seen, kd + 8 * half, rules.doc);
+        some = __builtin_amdgcn_ballot_w64(seen != 0) != 0;
+        whole = __builtin_amdgcn_ballot_w64(seen != 0xffffu) == 0;
       }
-      const bool some = __builtin_amdgcn_ballot_w64(seen != 0) != 0, whole = __builtin_amdgcn_ballot_w64(seen != 0xffffu) == 0;
       if (some) {
         f32x16 s = rows_times<T, D, S * Q::STAGE, false>(smem, reads, xq, zeros16());
         if constexpr (CAP)
 #pragma unroll
-          for (int i = 0; i < 16; i++) s[i] = tanh_of<T>(s[i], a.in);
-        // distances of the row to its keys: |near[g] - i| for keys i of run g
-        const float near[2] = {BIAS ? (float)(row - cur.lo - 8 * half) : 0.f, BIAS ? (float)(row - cur.hi - 8 * half) : 0.f};
+          for (int i = 0; i < 16; i++) s[i] = cap_score<T>(s[i], a.in);
+        const Logits<BIAS> logits(row - cur.lo - 8 * half, row - cur.hi - 8 * half, slope);
         float e[16], sum;
-        auto logit = [&](int i, float minus) {
-          return fmaf(s[i], a.out, BIAS ? fmaf(fabsf(near[i >> 3] - (float)(i & 7)), -slope, -minus) : -minus);
-        };
-        auto exponentials = [&]() {
+        for (bool moved = false;; moved = true) {
           const float ms = m == -INFINITY ? 0.f : m;
+          logits.get(e, s, factor, [&](int) { return ms - shift; });
           sum = 0.f;
 #pragma unroll
-          for (int i = 0; i < 16; i++) e[i] = __builtin_amdgcn_exp2f(logit(i, ms));
+          for (int i = 0; i < 16; i++) e[i] = __builtin_amdgcn_exp2f(e[i]);
           if (!whole)
 #pragma unroll
             for (int i = 0; i < 16; i++) e[i] = keep_bit(e[i], seen, i);
 #pragma unroll
           for (int i = 0; i < 16; i++) sum += e[i];
-        };
-        exponentials();
-        if (__builtin_amdgcn_ballot_w64(sum > 8192.f || (m == -INFINITY && seen != 0))) {
-          float top = -INFINITY;
+          if (moved || !__builtin_amdgcn_ballot_w64(sum > 8192.f || (m == -INFINITY && seen != 0))) break;
+          float y[16], top = -INFINITY;
+          logits.get(y, s, factor, [&](int) { return -shift; });
 #pragma unroll
-          for (int i = 0; i < 16; i++) top = fmaxf(top, (seen >> i) & 1 ? logit(i, 0.f) : -INFINITY);
+          for (int i = 0; i < 16; i++) top = fmaxf(top, (seen >> i) & 1 ? y[i] : -INFINITY);
           const float mn = fmaxf(m, fmaxf(top, swap32(top)));
           const float f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
           l *= f;
@@ -113,7 +113,6 @@ __global__ void __launch_bounds__(128, (fwd_waves<T, D>())) k_rules_fwd(RuleArgs
 #pragma unroll
             for (int i = 0; i < 16; i++) o[mt][i] *= f;
           m = mn;
-          exponentials();
         }
         l += sum;
         Shares<T> p;
@@ -163,9 +162,12 @@ __global__ void __launch_bounds__(256) k_rules_ranges(const int32_t *docs, int64
   out[2 * at + 1] = hi < 0 ? -1 : hi;
 }
 
-template <typename T, int D, bool CAP, bool BIAS> int launch_rules_fwd(const RuleArgs &a, hipStream_t st) {
+template <typename T, int D, bool CAP, bool BIAS, bool DOCS> int launch_rules_fwd(const RuleArgs &a, hipStream_t st) {
   static std::atomic<uint64_t> done{0};
-  return rules_launch(k_rules_fwd<T, D, CAP, BIAS>, (int64_t)a.Z * a.H * a.R, rules_lds<T, D>(), done, a, st);
+  return rules_launch(k_rules_fwd<T, D, CAP, BIAS, DOCS>, rules_grid((int64_t)a.Z * a.H, a.R), rules_lds<T, D>(), done, a, st);
+}
+template <typename T, int D, bool CAP, bool BIAS> int launch_rules_fwd(const RuleArgs &a, hipStream_t st) {
+  return a.docs ? launch_rules_fwd<T, D, CAP, BIAS, true>(a, st) : launch_rules_fwd<T, D, CAP, BIAS, false>(a, st);
 }
 template <typename T, int D> int launch_rules_fwd(const RuleArgs &a, hipStream_t st) {
   if (a.capped) return a.slopes ? launch_rules_fwd<T, D, true, true>(a, st) : launch_rules_fwd<T, D, true, false>(a, st);
@@ -182,7 +184,7 @@ int rules_args(const bsp_attention_rules_call *c, RuleArgs &a) {
   if ((c->documents != nullptr) != (c->ranges != nullptr) || (c->prefix && !c->causal)) return BSP_ERR_ARG;
   const int64_t lines = c->lines, unit = c->dtype == BSP_F32 ? 4 : 8, size = c->dtype == BSP_F32 ? 4 : 2;
   if (lines < (c->length + 63) / 64 || lines > (1 << 18)) return BSP_ERR_ARG;
-  if ((int64_t)c->Z * c->H * lines >= ((int64_t)1 << 31)) return BSP_ERR_UNSUPPORTED;
+  if ((int64_t)c->Z * c->H * lines >= ((int64_t)1 << 31) - 64) return BSP_ERR_UNSUPPORTED;
   for (int i = 0; i < 24; i++)
     if (c->strides[i] % unit) return BSP_ERR_ARG;
   // the rows of q, k, v and do are fetched by byte offsets of 32 bits from a head's first

@@ -78,7 +78,7 @@ class _Tables:
     WANTED = 1024
 
     def columns(self, kv_heads, batches):
-        """(items, number of items, splits, number of splits, slots), tensors on the device"""
+        """(items, their number per key head, splits, number of splits, slots), tensors on the device"""
         H, R, C = self.layout.shape
         tiles = self._columns.get(kv_heads)
         if tiles is None:
@@ -116,17 +116,25 @@ class _Tables:
         base, rest = (count // parts)[of], (count % parts)[of]
         items = heads[of].clone()
         items[:, 0] = (base + (k < rest)).int()
-        items[:, 1] = (12 * of.numel() + 8 * (first[of] + k * base + torch.minimum(k, rest))).int()
+        items[:, 1] = (8 * (first[of] + k * base + torch.minimum(k, rest))).int()
         split = parts[of] > 1
         items[:, 4] = torch.where(split, split.long().cumsum(0) - 1, -1).int()
         slots = int(split.sum())
         cut = parts > 1
         splits = torch.stack([heads[cut, 2], heads[cut, 3], (parts[cut].cumsum(0) - parts[cut]).int(), parts[cut].int()] + [heads[cut, 8 + g] for g in range(4)], 1)
-        # the key heads of about four query heads at a time, their longest items first: q and do of those stay in L2 and no long item starts last
-        near = items[:, 2].long() // max(1, 4 * int(heads[:, 2].max() + 1) // self.layout.size(0))
-        order = torch.argsort(near * (1 << 32) - items[:, 0], stable=True)
-        dev = torch.cat([items[order].flatten(), entries.flatten()]).to(self.device)
-        return dev, of.numel(), splits.contiguous().to(self.device) if slots else None, splits.size(0), slots
+        # by key head, the longest first, every key head's list filled up to the longest of them
+        kv_heads = int(heads[:, 2].max()) + 1
+        order = torch.argsort(items[:, 2].long() * (1 << 32) - items[:, 0], stable=True)
+        items, number = items[order], torch.bincount(items[:, 2].long(), minlength=kv_heads)
+        n_items = int(number.max())
+        rank = torch.arange(of.numel()) - (number.cumsum(0) - number)[items[:, 2].long()]
+        begin = 12 * kv_heads * n_items
+        lists = torch.zeros((kv_heads, n_items, 12), dtype=torch.int32)
+        lists[:, :, 1], lists[:, :, 3], lists[:, :, 4] = begin, -1, -1
+        lists[items[:, 2].long(), rank] = items
+        lists[:, :, 1] += begin * (lists[:, :, 3] >= 0)
+        dev = torch.cat([lists.flatten(), entries.flatten()]).to(self.device)
+        return dev, n_items, splits.contiguous().to(self.device) if slots else None, splits.size(0), slots
 
 
 class _rules(torch.autograd.Function):
