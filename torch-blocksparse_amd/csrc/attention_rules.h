@@ -78,6 +78,8 @@ __device__ __forceinline__ i32x4r buffer_of(const void *p, int64_t bytes) {
 }
 // the rows of a head: row stride ld and `length` rows of D elements
 template <typename T, int D> __device__ __forceinline__ i32x4r rows_buffer(const T *p, int64_t ld, int length) { return buffer_of(p, ((length - 1) * ld + D) * (int64_t)sizeof(T)); }
+// the same length from another place
+__device__ __forceinline__ i32x4r move_buffer(const i32x4r &b, const char *p) { return i32x4r{(int)(uint32_t)reinterpret_cast<uint64_t>(p), (int)(uint32_t)(reinterpret_cast<uint64_t>(p) >> 32) & 0xffff, b[2], b[3]}; }
 // load_to_lds from a buffer
 template <int BYTES> __device__ __forceinline__ void buffer_to_lds(const i32x4r &rsrc, uint32_t off, uint32_t add, uint32_t dst) {
   uint32_t at;                                            // (the addition also is the instruction that must lie between m0 and its use)
@@ -229,13 +231,38 @@ inline void logit_args(RuleArgs &a, float scale, float cap) {
   a.out = (cap > 0.f ? cap : scale) * kLog2e;
 }
 
-// the least and greatest document number of a group of sixteen positions: everything if there are no documents
-struct Range { int lo, hi; };
-__device__ __forceinline__ Range range_of(const RuleArgs &a, int z, int pos) {
-  const int g = pos >> 4;
-  const int32_t *r = a.ranges + 2 * ((int64_t)z * a.groups + (g < a.groups ? g : a.groups - 1));
-  return Range{r[0], r[1]};
+// A value that is the same in all lanes, in scalar registers of its own.  Arguments are loaded sixteen dwords at a time, and as long as one
+// of them is used in a loop all sixteen are kept, spilled to lanes of vector registers and read back there: thirty of the instructions of a step.
+template <typename V> __device__ __forceinline__ V apart(V v) {
+  constexpr int N = sizeof(V) / 4;
+  struct Words { int w[N]; };
+  Words x = __builtin_bit_cast(Words, v);
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    int w;
+    // (the unit waits for neither side by itself: the lane's value may have been written by the instruction before, and any unit may read
+    // the scalar register next)
+    asm volatile("s_nop 1\n\tv_readfirstlane_b32 %0, %1\n\ts_nop 4" : "=s"(w) : "v"(x.w[i]));
+    x.w[i] = w;
+  }
+  return __builtin_bit_cast(V, x);
 }
+
+// The least and greatest document number of a group of sixteen positions
+struct Range { int lo, hi; };
+struct Ranges {
+  const int32_t *of_batch;
+  int last;
+  __device__ __forceinline__ void init(const RuleArgs &a, int z) {
+    of_batch = apart(a.ranges + 2 * (int64_t)z * a.groups);
+    last = apart(a.groups - 1);
+  }
+  __device__ __forceinline__ Range at(int pos) const {
+    const int g = pos >> 4;
+    const int32_t *r = of_batch + 2 * (g < last ? g : last);
+    return Range{r[0], r[1]};
+  }
+};
 
 // The halves of a line's (column's) tiles that are worth a visit, 64 looked at together, one a lane.  From the last to the first: in a
 // causal layout the nearest keys come first then, whose logits a bias by distance makes the largest, so that the running maximum is found at
@@ -282,13 +309,15 @@ template <bool DOCS> struct LineRules {
   int limit;                       // ... the keys below it by the lane's row
   int doc;                         // the lane's document
   Range range;                     // of the line
+  Ranges ranges;
   __device__ __forceinline__ void init(const RuleArgs &a, int z, int line, int row, bool &dead) {
     const int prefix = a.causal && a.prefix ? as_table(a.prefix)[z] : 0, first = line * 64;
     doc = 0;
     if constexpr (DOCS) {
+      ranges.init(a, z);
       doc = a.docs[z * a.docs_sz + (row < a.L ? row : a.L - 1)];
       const int lane = threadIdx.x & 3;
-      const Range g = range_of(a, z, first + 16 * lane < a.L ? first + 16 * lane : first);
+      const Range g = ranges.at(first + 16 * lane < a.L ? first + 16 * lane : first);
       int lo = g.lo, hi = g.hi;
 #pragma unroll
       for (int d = 1; d < 4; d <<= 1) {
@@ -300,16 +329,16 @@ template <bool DOCS> struct LineRules {
     }
     dead = row >= a.L || doc < 0;
     auto below = [&](int i) { const int n = a.causal ? (i + 1 > prefix ? i + 1 : prefix) : a.L; return n < a.L ? n : a.L; };
-    most = below(first + 63);
-    least = below(first);
+    most = apart(below(first + 63));
+    least = apart(below(first));
     limit = dead ? 0 : below(row);
   }
-  __device__ __forceinline__ bool look(const RuleArgs &a, int z, int lo, int hi, int bits, int half, bool &full, bool &pad) const {
+  __device__ __forceinline__ bool look(int lo, int hi, int bits, int half, bool &full, bool &pad) const {
     bits >>= 2 * half;
     bool see_lo = (bits & 0x1111) && lo < most, see_hi = (bits & 0x2222) && hi < most;
     full = (bits & 0x3333) == 0x3333 && lo + 15 < least && hi + 15 < least;
     if constexpr (DOCS) {
-      const Range x = range_of(a, z, lo), y = range_of(a, z, hi);
+      const Range x = ranges.at(lo), y = ranges.at(hi);
       const int from = range.lo < 0 ? 0 : range.lo;
       see_lo = see_lo && x.hi >= from && x.lo <= range.hi;
       see_hi = see_hi && y.hi >= from && y.lo <= range.hi;
@@ -364,10 +393,14 @@ template <bool BIAS> struct Logits {
 
 // the lowest n of eight bits, n any number
 __device__ __forceinline__ uint32_t first_bits(int n) { return (1u << (n < 0 ? 0 : n > 8 ? 8 : n)) - 1u; }
-// value i where bit i of the word is set, else zero (whatever the value: NaN too)
-__device__ __forceinline__ float keep_bit(float v, uint32_t word, int i) {
-  return __builtin_bit_cast(float, __builtin_bit_cast(int, v) & __builtin_amdgcn_sbfe((int)word, (uint32_t)i, 1u));
+// all ones where bit i of the word is set, else zero; what is `and`ed with it is kept or becomes zero, whatever it is, NaN too.  (As assembly: the
+// compiler makes a test and a selection of it, three operations and a wait.)
+template <int I> __device__ __forceinline__ uint32_t bit_mask(uint32_t word) {
+  uint32_t m;
+  asm("v_bfe_i32 %0, %1, %2, 1" : "=v"(m) : "v"(word), "n"(I));
+  return m;
 }
+__device__ __forceinline__ float keep(float v, uint32_t mask) { return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & mask); }
 // the bits of the word whose documents (eight and eight consecutive ones) are not the lane's taken out
 __device__ __forceinline__ uint32_t same_document(uint32_t word, const int32_t *docs, int doc) {
   typedef int i32x4v __attribute__((ext_vector_type(4)));
@@ -434,14 +467,14 @@ __device__ __forceinline__ Place rules_place(uint32_t wg, int units, int n) {
   const uint32_t rest = units & 7, spread = (rest * n + 7) & ~7u;
   if (wg < spread) {
     const Quotient p(wg, rest);
-    return Place{p.q < (uint32_t)n ? (int)((units & ~7) + p.r) : -1, (int)p.q};
+    return Place{__builtin_amdgcn_readfirstlane(p.q < (uint32_t)n ? (int)((units & ~7) + p.r) : -1), __builtin_amdgcn_readfirstlane((int)p.q)};
   }
   wg -= spread;
   const uint32_t per = units >> 3, x = wg & 7, i = wg >> 3;      // heads per XCD
   const Quotient g(i, kHeadsTogether * n);
   const uint32_t first = g.q * kHeadsTogether, heads = per - first < kHeadsTogether ? per - first : kHeadsTogether;
   const Quotient p(g.r, heads);
-  return Place{(int)(x * per + first + p.r), (int)p.q};
+  return Place{__builtin_amdgcn_readfirstlane((int)(x * per + first + p.r)), __builtin_amdgcn_readfirstlane((int)p.q)};
 }
 
 // The query head and batch of a unit: the heads that share a key head next to each other, then the batches (their documents, and with them
@@ -450,9 +483,9 @@ struct HeadOf {
   int h, hk, z;
   __device__ __forceinline__ HeadOf(int unit, int Z, int G) {
     const Quotient g(unit, G), b(g.q, Z);
-    z = b.r;
-    hk = b.q;
-    h = hk * G + g.r;
+    z = __builtin_amdgcn_readfirstlane(b.r);            // (a division's result is in a vector register, and what follows from it would be)
+    hk = __builtin_amdgcn_readfirstlane(b.q);
+    h = __builtin_amdgcn_readfirstlane(hk * G + g.r);
   }
 };
 

@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(128, (row_waves<T, D, CAP>())) k_rules_bwd_row
   Walk<DOCS> walk;
   walk.init(a.lut + lut[2 * (h * a.R + line) + 1], line * 64 < a.L ? lut[2 * (h * a.R + line)] * 2 : 0);
   auto next = [&]() {
-    return walk.next(lane, [&](int lo, int hi, int bits, int hf, bool &full, bool &pad) { return rules.look(a, z, lo, hi, bits, hf, full, pad); });
+    return walk.next(lane, [&](int lo, int hi, int bits, int hf, bool &full, bool &pad) { return rules.look(lo, hi, bits, hf, full, pad); });
   };
   const float *stats = a.ref + ((int64_t)z * a.H + h) * 2 * a.rows + row;
   const float ref = stats[0], factor = stats[a.rows];
@@ -59,11 +59,11 @@ __global__ void __launch_bounds__(128, (row_waves<T, D, CAP>())) k_rules_bwd_row
   if (cur.n >= 0) {
     held_t<T, D> xq;
     hold_operand<T, D>(xq, reinterpret_cast<const T *>(a.q) + z * a.q_sz + h * a.q_sh + row_in * a.q_ld, half, dead);
-    const float slope = BIAS ? as_floats(a.slopes)[h] * kLog2e : 0.f, out = logit_factor<T, CAP>(a.out), minus = ref - logit_shift<T, CAP>(a.out) - (CAP && sizeof(T) != 4 ? 2.f : 0.f);   // (e^y times four: see cap_through)
+    const float slope = BIAS ? as_floats(a.slopes)[h] * kLog2e : 0.f, out = apart(logit_factor<T, CAP>(a.out)), in = apart(a.in), minus = ref - logit_shift<T, CAP>(a.out) - (CAP && sizeof(T) != 4 ? 2.f : 0.f);   // (e^y times four: see cap_through)
     const i32x4r pk = rows_buffer<T, D>(reinterpret_cast<const T *>(a.k) + z * a.k_sz + hk * a.k_sh, a.k_ld, a.L);
     const i32x4r pv = rows_buffer<T, D>(reinterpret_cast<const T *>(a.v) + z * a.v_sz + hk * a.v_sh, a.v_ld, a.L);
     const i32x4r docs = buffer_of(DOCS ? a.docs + z * a.docs_sz : nullptr, (int64_t)a.L * 4);
-    const uint32_t k_row = (uint32_t)a.k_ld * Q::ESZ, v_row = (uint32_t)a.v_ld * Q::ESZ;
+    const uint32_t k_row = apart((uint32_t)a.k_ld * Q::ESZ), v_row = apart((uint32_t)a.v_ld * Q::ESZ);
     RowsLoad<T, D, sizeof(T) == 4> gk, gv;
     gk.init(a.k_ld, lane);
     gv.init(a.v_ld, lane);
@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(128, (row_waves<T, D, CAP>())) k_rules_bwd_row
         const Logits<BIAS> logits(row - cur.lo - 8 * half, row - cur.hi - 8 * half, slope);
         if constexpr (CAP)
 #pragma unroll
-          for (int i = 0; i < 16; i++) s[i] = cap_score<T>(s[i], a.in);
+          for (int i = 0; i < 16; i++) s[i] = cap_score<T>(s[i], in);
         float e[16];
         logits.get(e, s, out, [&](int) { return minus; });
 #pragma unroll
@@ -113,8 +113,7 @@ __global__ void __launch_bounds__(128, (row_waves<T, D, CAP>())) k_rules_bwd_row
           if constexpr (CAP) e[i] *= cap_through<T, true>(s[i]);
         }
         if (!whole)
-#pragma unroll
-          for (int i = 0; i < 16; i++) e[i] = keep_bit(e[i], seen, i);
+          for_16<0>([&](auto ic) { e[decltype(ic)::value] = keep(e[decltype(ic)::value], bit_mask<decltype(ic)::value>(seen)); });
         Shares<T> ds;
         ds.set(e);
         columns_times<T, D, S * Q::STAGE, false>(dq, smem, reads, ds);
@@ -173,13 +172,15 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, CAP>())) k_rules_bwd_col
     key_max = p > key_max ? p : key_max;
   }
   key_max += 15;
-  const int most = a.causal && key_max >= prefix ? key_max : 0, least = a.causal && key_min >= prefix ? key_min : 0;   // rows from `most` on see all of the column's keys, those below `least` none
+  const int L = apart(a.L), most = apart(a.causal && key_max >= prefix ? key_max : 0), least = apart(a.causal && key_min >= prefix ? key_min : 0);   // rows from `most` on see all of the column's keys, those below `least` none
   Range range{0, 0};
+  Ranges ranges;
   if constexpr (DOCS) {
-    range = range_of(a, z, head[8]);
+    ranges.init(a, z);
+    range = ranges.at(head[8]);
 #pragma unroll
     for (int g = 1; g < 4; g++) {
-      const Range r = range_of(a, z, head[8 + g]);
+      const Range r = ranges.at(head[8 + g]);
       range.lo = r.lo < range.lo ? r.lo : range.lo;
       range.hi = r.hi > range.hi ? r.hi : range.hi;
     }
@@ -195,10 +196,10 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, CAP>())) k_rules_bwd_col
       bits >>= 8 * hf;
       lo &= kPosition;
       hi &= kPosition;
-      bool see_lo = (bits & 0x0f) && lo < a.L && lo + 15 >= least, see_hi = (bits & 0xf0) && hi < a.L && hi + 15 >= least;
+      bool see_lo = (bits & 0x0f) && lo < L && lo + 15 >= least, see_hi = (bits & 0xf0) && hi < L && hi + 15 >= least;
       full = (bits & 0xff) == 0xff && lo >= most && hi >= most;
       if constexpr (DOCS) {
-        const Range x = range_of(a, z, lo), y = range_of(a, z, hi);
+        const Range x = ranges.at(lo), y = ranges.at(hi);
         const int low = range.lo < 0 ? 0 : range.lo;
         see_lo = see_lo && x.hi >= low && x.lo <= range.hi;
         see_hi = see_hi && y.hi >= low && y.lo <= range.hi;
@@ -214,20 +215,32 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, CAP>())) k_rules_bwd_col
     hold_operand<T, D>(xk, reinterpret_cast<const T *>(a.k) + z * a.k_sz + hk * a.k_sh + key_in * a.k_ld, half, dead);
     hold_operand<T, D>(xv, reinterpret_cast<const T *>(a.v) + z * a.v_sz + hk * a.v_sh + key_in * a.v_ld, half, dead);
     const int first_head = hk * a.G;
-    const T *pq = reinterpret_cast<const T *>(a.q) + z * a.q_sz + first_head * a.q_sh, *pdo = reinterpret_cast<const T *>(a.d_o) + z * a.do_sz + first_head * a.do_sh;
+    const char *pq = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.q) + z * a.q_sz + first_head * a.q_sh);
+    const char *pdo = reinterpret_cast<const char *>(reinterpret_cast<const T *>(a.d_o) + z * a.do_sz + first_head * a.do_sh);
+    const int64_t q_head = apart(a.q_sh * Q::ESZ), do_head = apart(a.do_sh * Q::ESZ);
+    const uint32_t q_row = apart((uint32_t)a.q_ld * Q::ESZ), do_row = apart((uint32_t)a.do_ld * Q::ESZ);
+    i32x4r q_rows = rows_buffer<T, D>(reinterpret_cast<const T *>(pq), a.q_ld, a.L), do_rows = rows_buffer<T, D>(reinterpret_cast<const T *>(pdo), a.do_ld, a.L);
     const i32x4r docs = buffer_of(DOCS ? a.docs + z * a.docs_sz : nullptr, (int64_t)a.L * 4);
     const i32x4r stats = wave == 0 ? buffer_of(a.ref + ((int64_t)z * a.H + first_head) * 2 * a.rows, a.G * a.rows * 8) : buffer_of(a.delta + ((int64_t)z * a.H + first_head) * a.rows, a.G * a.rows * 4);
-    const uint32_t q_row = (uint32_t)a.q_ld * Q::ESZ, do_row = (uint32_t)a.do_ld * Q::ESZ;
+    const int per = apart((int)a.rows << (1 - wave)), lane_stat = (lane & 15) + (wave == 0 && half ? (int)a.rows : 0);
+    const float in = apart(a.in), out = apart(logit_factor<T, CAP>(a.out)), shift = CAP ? apart(logit_shift<T, CAP>(a.out)) : 0.f;
+    const float *slopes = BIAS ? apart(a.slopes + first_head) : nullptr;
     RowsLoad<T, D, LEAN> gq, gdo;
     gq.init(a.q_ld, lane);
     gdo.init(a.do_ld, lane);
+    int head_now = 0;                                   // the query head that q_rows and do_rows are of
     auto issue = [&](int stage_no, const Half &x) {
       const uint32_t st = lds_address(smem) + stage_no * Q::STAGE + wave * (16 * Q::RB), ex = lds_address(extra) + stage_no * Q::EXTRA;
       const int pos = wave ? x.hi : x.lo, hq = pos >> kHeadShift, lo = x.lo & kPosition, hi = x.hi & kPosition;
-      gq.issue(rows_buffer<T, D>(pq + hq * a.q_sh, a.q_ld, a.L), pos & kPosition, q_row, st);
-      gdo.issue(rows_buffer<T, D>(pdo + hq * a.do_sh, a.do_ld, a.L), pos & kPosition, do_row, st + Q::PIECE);
-      const int per = (int)a.rows << (1 - wave), at_lo = (x.lo >> kHeadShift) * per + lo, at_hi = (x.hi >> kHeadShift) * per + hi;
-      buffer_to_lds<4>(stats, (uint32_t)((lane & 16 ? at_hi : at_lo) + (lane & 15) + (wave == 0 && half ? (int)a.rows : 0)) * 4u, 0, ex + wave * 256);
+      if (hq != head_now) {
+        head_now = hq;
+        q_rows = move_buffer(q_rows, pq + hq * q_head);
+        do_rows = move_buffer(do_rows, pdo + hq * do_head);
+      }
+      gq.issue(q_rows, pos & kPosition, q_row, st);
+      gdo.issue(do_rows, pos & kPosition, do_row, st + Q::PIECE);
+      const int at_lo = (x.lo >> kHeadShift) * per + lo, at_hi = (x.hi >> kHeadShift) * per + hi;
+      buffer_to_lds<4>(stats, (uint32_t)((lane & 16 ? at_hi : at_lo) + lane_stat) * 4u, 0, ex + wave * 256);
       if (DOCS && wave == 1) load_documents(docs, lo, hi, lane, ex + 512);
     };
     issue(0, cur);
@@ -260,13 +273,13 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, CAP>())) k_rules_bwd_col
         f32x16 s = rows_times<T, D, Q0, LEAN>(smem, reads, xk, zeros16());
         float slope_lo = 0.f, slope_hi = 0.f;
         if constexpr (BIAS) {
-          slope_lo = as_floats(a.slopes)[first_head + (cur.lo >> kHeadShift)] * kLog2e;
-          slope_hi = as_floats(a.slopes)[first_head + (cur.hi >> kHeadShift)] * kLog2e;
+          slope_lo = as_floats(slopes)[cur.lo >> kHeadShift] * kLog2e;
+          slope_hi = as_floats(slopes)[cur.hi >> kHeadShift] * kLog2e;
         }
         const Logits<BIAS> logits(key - lo - 8 * half, key - hi - 8 * half, slope_lo, slope_hi);
         if constexpr (CAP)
 #pragma unroll
-          for (int i = 0; i < 16; i++) s[i] = cap_score<T>(s[i], a.in);
+          for (int i = 0; i < 16; i++) s[i] = cap_score<T>(s[i], in);
         // the rows' values, in the lane's order: 8 half .., 16 + 8 half ..
         const float *st = stat + 8 * half;
         float p[16], e[16];
@@ -274,7 +287,7 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, CAP>())) k_rules_bwd_col
           f32x4 ref[4];
 #pragma unroll
           for (int g = 0; g < 4; g++) ref[g] = *reinterpret_cast<const f32x4 *>(st + 16 * (g >> 1) + 4 * (g & 1));
-          logits.get(p, s, logit_factor<T, CAP>(a.out), [&](int i) { return ref[i >> 2][i & 3] - logit_shift<T, CAP>(a.out); });
+          logits.get(p, s, out, [&](int i) { return ref[i >> 2][i & 3] - shift; });
         }
 #pragma unroll
         for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f(p[i]);
@@ -286,8 +299,7 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, CAP>())) k_rules_bwd_col
             for (int j = 0; j < 4; j++) p[4 * g + j] *= f[j];
           }
         if (!whole)
-#pragma unroll
-          for (int i = 0; i < 16; i++) p[i] = keep_bit(p[i], seen, i);
+          for_16<0>([&](auto ic) { p[decltype(ic)::value] = keep(p[decltype(ic)::value], bit_mask<decltype(ic)::value>(seen)); });
         Shares<T> share;
         share.set(p);
         columns_times<T, D, O0, LEAN>(dv, smem, reads, share);
@@ -305,8 +317,7 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, CAP>())) k_rules_bwd_col
           if constexpr (CAP) e[i] *= cap_through<T, __is_same(T, bf16)>(s[i]);   // (fp16 keeps the factor: what is rounded next should be no smaller than it is)
         }
         if (!whole)
-#pragma unroll
-          for (int i = 0; i < 16; i++) e[i] = keep_bit(e[i], seen, i);
+          for_16<0>([&](auto ic) { e[decltype(ic)::value] = keep(e[decltype(ic)::value], bit_mask<decltype(ic)::value>(seen)); });
         share.set(e);
         columns_times<T, D, Q0, LEAN>(dk, smem, reads, share);
       }

@@ -36,17 +36,17 @@ __global__ void __launch_bounds__(128, (fwd_waves<T, D, BIAS, DOCS>())) k_rules_
   Walk<DOCS> walk;
   walk.init(a.lut + lut[2 * (h * a.R + line) + 1], line * 64 < a.L ? lut[2 * (h * a.R + line)] * 2 : 0);
   auto next = [&]() {
-    return walk.next(lane, [&](int lo, int hi, int bits, int hf, bool &full, bool &pad) { return rules.look(a, z, lo, hi, bits, hf, full, pad); });
+    return walk.next(lane, [&](int lo, int hi, int bits, int hf, bool &full, bool &pad) { return rules.look(lo, hi, bits, hf, full, pad); });
   };
   Half cur = next();
   if (cur.n >= 0) {
     held_t<T, D> xq;
     hold_operand<T, D>(xq, reinterpret_cast<const T *>(a.q) + z * a.q_sz + h * a.q_sh + row_in * a.q_ld, half, dead);
-    const float slope = BIAS ? as_floats(a.slopes)[h] * kLog2e : 0.f, factor = logit_factor<T, CAP>(a.out), shift = logit_shift<T, CAP>(a.out);
+    const float slope = BIAS ? as_floats(a.slopes)[h] * kLog2e : 0.f, factor = apart(logit_factor<T, CAP>(a.out)), shift = CAP ? apart(logit_shift<T, CAP>(a.out)) : 0.f, in = apart(a.in);
     const i32x4r pk = rows_buffer<T, D>(reinterpret_cast<const T *>(a.k) + z * a.k_sz + hk * a.k_sh, a.k_ld, a.L);
     const i32x4r pv = rows_buffer<T, D>(reinterpret_cast<const T *>(a.v) + z * a.v_sz + hk * a.v_sh, a.v_ld, a.L);
     const i32x4r docs = buffer_of(DOCS ? a.docs + z * a.docs_sz : nullptr, (int64_t)a.L * 4);
-    const uint32_t k_row = (uint32_t)a.k_ld * Q::ESZ, v_row = (uint32_t)a.v_ld * Q::ESZ;
+    const uint32_t k_row = apart((uint32_t)a.k_ld * Q::ESZ), v_row = apart((uint32_t)a.v_ld * Q::ESZ);
     RowsLoad<T, D, sizeof(T) == 4> gk, gv;
     gk.init(a.k_ld, lane);
     gv.init(a.v_ld, lane);
@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(128, (fwd_waves<T, D, BIAS, DOCS>())) k_rules_
         f32x16 s = rows_times<T, D, S * Q::STAGE, false>(smem, reads, xq, zeros16());
         if constexpr (CAP)
 #pragma unroll
-          for (int i = 0; i < 16; i++) s[i] = cap_score<T>(s[i], a.in);
+          for (int i = 0; i < 16; i++) s[i] = cap_score<T>(s[i], in);
         const Logits<BIAS> logits(row - cur.lo - 8 * half, row - cur.hi - 8 * half, slope);
         float e[16], sum;
         for (bool moved = false;; moved = true) {
@@ -96,8 +96,7 @@ __global__ void __launch_bounds__(128, (fwd_waves<T, D, BIAS, DOCS>())) k_rules_
 #pragma unroll
           for (int i = 0; i < 16; i++) e[i] = __builtin_amdgcn_exp2f(e[i]);
           if (!whole)
-#pragma unroll
-            for (int i = 0; i < 16; i++) e[i] = keep_bit(e[i], seen, i);
+            for_16<0>([&](auto ic) { e[decltype(ic)::value] = keep(e[decltype(ic)::value], bit_mask<decltype(ic)::value>(seen)); });
 #pragma unroll
           for (int i = 0; i < 16; i++) sum += e[i];
           if (moved || !__builtin_amdgcn_ballot_w64(sum > 8192.f || (m == -INFINITY && seen != 0))) break;
