@@ -516,6 +516,7 @@ typedef struct {
   int32_t *ranges;
   const int32_t *d_rows;
   float *stats;
+  void *o_rest;                    /* 16-bit types, with stats: [Z][H][length][D], what the rounding of o left out, written by fwd and read by bwd */
 } bsp_attention_rules_call;
 int bsp_attention_rules_fwd(const bsp_attention_rules_call *call, const void *q, const void *k, const void *v, void *o, void *stream);
 int bsp_attention_rules_bwd(const bsp_attention_rules_call *call, const void *d_o, const void *q, const void *k, const void *v, const void *o,

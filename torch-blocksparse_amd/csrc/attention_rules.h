@@ -27,6 +27,7 @@ struct RuleArgs {
   const void *q, *k, *v;
   const void *d_o, *o_in;          // backward: do, and the forward result (row kernel)
   void *o, *o2;                    // forward: o; row kernel: dq; column kernel: dk and dv
+  void *o_rest;                    // [Z][H][L][D]: what the rounding of o to a 16-bit type left out
   float *ref, *delta;              // ref: [Z][H][2][rows]: p = exp2(y - ref) * factor, y in the log2 domain; delta: [Z][H][rows], -sum_d do . o
   int64_t rows;                    // 64 * lines
   int64_t q_sz, q_sh, q_ld, k_sz, k_sh, k_ld, v_sz, v_sh, v_ld, do_sz, do_sh, do_ld, oin_sz, oin_sh, oin_ld;
@@ -109,53 +110,67 @@ template <typename T, int D, bool LEAN> struct RowsLoad {
   }
 };
 
-// Those of sixteen rows (from row0 on) of a stage's two pieces whose positions carry no document: zeros
+// Those of sixteen rows (from row0 on) of a piece whose positions carry no document: zeros
 template <typename T, int D> __device__ __forceinline__ void clear_rows(unsigned char *piece, int row0, const int32_t *docs_of_stage, int lane) {
   typedef Geo<T, D> Q;
   constexpr int RPL = 64 / Q::CPR;
 #pragma unroll 1
   for (int i = 0; i < 16 / RPL; i++) {
     const int r = row0 + i * RPL + lane / Q::CPR;
-    if (docs_of_stage[r] < 0) {
-      u32x4 *at = reinterpret_cast<u32x4 *>(piece + r * Q::RB + (lane % Q::CPR) * 16);
-      *at = u32x4{0, 0, 0, 0};
-      at[Q::PIECE / 16] = u32x4{0, 0, 0, 0};
-    }
+    if (docs_of_stage[r] < 0) *reinterpret_cast<u32x4 *>(piece + r * Q::RB + (lane % Q::CPR) * 16) = u32x4{0, 0, 0, 0};
   }
 }
 
-// The operand reads of a piece, along its rows and transposed
+// The operand reads of a piece, along its rows and transposed: LDS addresses in the piece at offset 0.  (Reads go through pointers to LDS made of them, so
+// that a stage's offset is a constant of the instruction; from a generic pointer each read costs an addition.)
 template <typename T, int D, bool LEAN> struct PieceReads {
   RowReads<D, LEAN> rows;
   TrReads<D, LEAN> tr;
   __device__ __forceinline__ void init(const unsigned char *smem, int lane) {
     rows.init(0, lane);
+#pragma unroll
+    for (int s = 0; s < (LEAN ? 1 : D / 16); s++) rows.a[s] += lds_address(smem);
     tr.init(lds_address(smem), 0, lane);
   }
 };
 template <int D, bool LEAN> struct PieceReads<float, D, LEAN> {
   uint32_t row, tr;                // the others are an exclusive-or of constants away
-  __device__ __forceinline__ void init(const unsigned char *, int lane) {
+  __device__ __forceinline__ void init(const unsigned char *smem, int lane) {
     const int half = lane >> 5, l32 = lane & 31, r = deal_row(l32);
-    row = (uint32_t)(r * Geo<float, D>::RB + ((half ^ rule_swz<float, D>(r)) << 4));
-    tr = (uint32_t)(8 * half * Geo<float, D>::RB + (((l32 >> 2) ^ (8 * half)) << 4) + ((l32 & 3) << 2));
+    row = lds_address(smem) + (uint32_t)(r * Geo<float, D>::RB + ((half ^ rule_swz<float, D>(r)) << 4));
+    tr = lds_address(smem) + (uint32_t)(8 * half * Geo<float, D>::RB + (((l32 >> 2) ^ (8 * half)) << 4) + ((l32 & 3) << 2));
   }
 };
+template <typename V> __device__ __forceinline__ V lds_read(uint32_t at) { return *(const V __attribute__((address_space(3))) *)(uintptr_t)at; }
 
-// acc + (32 rows of a piece, dealt by deal_row) . b: value i = row 16 (i / 8) + 8 (lane / 32) + i % 8 of the piece, column lane % 32
+// The operand fragment of chunk s of the lane's row, and the product with it
 template <typename T, int D, int OFF, bool LEAN>
-__device__ __forceinline__ f32x16 rows_times(const unsigned char *smem, const PieceReads<T, D, LEAN> &reads, const held_t<T, D> &b, f32x16 acc) {
+__device__ __forceinline__ typename RuleOperand<T>::type row_fragment(const PieceReads<T, D, LEAN> &reads, int s) {
+  uint32_t at;
+  if constexpr (sizeof(T) == 4) at = reads.row ^ (uint32_t)(s << 5);
+  else if constexpr (LEAN) at = reads.rows.a[0] ^ (uint32_t)(s << 5);
+  else at = reads.rows.a[s];
+  return lds_read<typename RuleOperand<T>::type>(at + OFF);
+}
+template <typename T> __device__ __forceinline__ f32x16 fragment_times(const typename RuleOperand<T>::type &f, const typename RuleOperand<T>::type &b, f32x16 acc) {
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int s = 0; s < Geo<T, D>::NF; s++) {
-      const f32x4 f = *reinterpret_cast<const f32x4 *>(smem + OFF + (reads.row ^ (uint32_t)(s << 5)));
-#pragma unroll
-      for (int j = 0; j < 4; j++) acc = Mma<float, 32>::run(f[j], b[s][j], acc);
-    }
+    for (int j = 0; j < 4; j++) acc = Mma<float, 32>::run(f[j], b[j], acc);
     return acc;
   } else {
-    return row_product<T, D, OFF, LEAN>(smem, reads.rows, b, acc);
+    return Mma<T, 32>::run(f, b, acc);
   }
+}
+// acc + (32 rows of a piece, dealt by deal_row) . b: value i = row 16 (i / 8) + 8 (lane / 32) + i % 8 of the piece, column lane % 32
+template <typename T, int D, int OFF, bool LEAN>
+__device__ __forceinline__ f32x16 rows_times(PieceReads<T, D, LEAN> reads, const held_t<T, D> &b, f32x16 acc) {
+  if constexpr (LEAN && sizeof(T) == 2) asm volatile("" : "+v"(reads.rows.a[0]));   // (the others are made when they are wanted, not held)
+  typename RuleOperand<T>::type f[Geo<T, D>::NF];
+#pragma unroll
+  for (int s = 0; s < Geo<T, D>::NF; s++) f[s] = row_fragment<T, D, OFF, LEAN>(reads, s);
+#pragma unroll
+  for (int s = 0; s < Geo<T, D>::NF; s++) acc = fragment_times<T>(f[s], b[s], acc);
+  return acc;
 }
 __device__ __forceinline__ f32x16 zeros16() {
   f32x16 z;
@@ -183,14 +198,14 @@ template <> struct Shares<float> {
 
 // acc[mt] += (32 rows of a piece, transposed)[column 32 mt ..][row] . b[row]
 template <typename T, int D, int OFF, bool LEAN>
-__device__ __forceinline__ void columns_times(f32x16 (&acc)[D / 32], const unsigned char *smem, const PieceReads<T, D, LEAN> &reads, const Shares<T> &b) {
+__device__ __forceinline__ void columns_times(f32x16 (&acc)[D / 32], const PieceReads<T, D, LEAN> &reads, const Shares<T> &b) {
   if constexpr (sizeof(T) == 4) {
     constexpr int RB = Geo<T, D>::RB;
 #pragma unroll
     for (int i = 0; i < 16; i++)
 #pragma unroll
       for (int mt = 0; mt < D / 32; mt++) {
-        const float x = *reinterpret_cast<const float *>(smem + OFF + (16 * (i / 8) + i % 8) * RB + (reads.tr ^ (uint32_t)((8 * mt ^ (i & 7)) << 4)));
+        const float x = lds_read<float>((reads.tr ^ (uint32_t)((8 * mt ^ (i & 7)) << 4)) + OFF + (16 * (i / 8) + i % 8) * RB);
         acc[mt] = Mma<float, 32>::run(x, b.e[i], acc[mt]);
       }
   } else {
@@ -375,6 +390,12 @@ template <bool BIAS> struct Logits {
         for (int g = 0; g < 2; g++) slope[g] *= sign, base[g] *= -slope[g];
       }
     }
+  }
+  // the logit of score i (STRAIGHT: of a wavefront whose scores lie on one side)
+  template <bool STRAIGHT> __device__ __forceinline__ float one(int i, float s, float out, float minus) const {
+    if constexpr (!BIAS) return fmaf(s, out, -minus);
+    else if constexpr (STRAIGHT) return fmaf(s, out, fmaf(slope[i >> 3], (float)(i & 7), base[i >> 3] - minus));
+    else return fmaf(s, out, fmaf(-slope[i >> 3], fabsf(base[i >> 3] - (float)(i & 7)), -minus));
   }
   // y(i) for i = 0 .. 15, minus(i) a value per score (a constant, usually)
   template <class S, class M> __device__ __forceinline__ void get(float (&y)[16], const S &s, float out, M &&minus) const {

@@ -1,6 +1,7 @@
 // Backward pass of attention with score rules (attention_rules.h), p = exp2(y - ref) * factor computed again:
 //     dv = p^T . do,   e = p * (dp - delta) * (1 - t^2)  (t the tanh of a capped score),   dq = scale * e . k,   dk = scale * e^T . q
-// with dp = do . v^T and delta = sum_d do_d o_d.
+// with dp = do . v^T and delta = sum_d do_d o_d, for which 16-bit types keep what the rounding of o left out as a second tensor: delta goes into every
+// gradient of its row, and with o alone the gradients are off by 1.8 times what the roundings of p, of e and of the result make them.
 //   row kernel    : a line of tiles per workgroup -> dq and -delta
 //   column kernel : a column of tiles (or a part of a long one) of a key head per workgroup -> dk and dv; the column's tiles are
 //                   those of all the query heads that share the key head, one after the other, so their sum needs no memory
@@ -44,6 +45,13 @@ __global__ void __launch_bounds__(128, (row_waves<T, D, CAP>())) k_rules_bwd_row
     for (int s = 0; s < Q::NF; s++)
 #pragma unroll
       for (int i = 0; i < Q::VEC; i++) delta = fmaf(to_float(xo[s][i]), to_float(of[s][i]), delta);
+    if constexpr (sizeof(T) == 2) {                      // ... and with what the rounding of o left out
+      hold_operand<T, D>(of, reinterpret_cast<const T *>(a.o_rest) + (((int64_t)z * a.H + h) * a.L + row_in) * D, half, dead);
+#pragma unroll
+      for (int s = 0; s < Q::NF; s++)
+#pragma unroll
+        for (int i = 0; i < Q::VEC; i++) delta = fmaf(to_float(xo[s][i]), to_float(of[s][i]), delta);
+    }
     delta += swap32(delta);
   }
   if (half == 0) a.delta[((int64_t)z * a.H + h) * a.rows + row] = -delta;   // (its negative: where the column kernel's dp starts from)
@@ -86,6 +94,7 @@ __global__ void __launch_bounds__(128, (row_waves<T, D, CAP>())) k_rules_bwd_row
       const int32_t *kd = reinterpret_cast<const int32_t *>(extra + S * Q::EXTRA);
       if (DOCS && cur.pad) {
         clear_rows<T, D>(smem + S * Q::STAGE, 16 * wave, kd, lane);
+        clear_rows<T, D>(smem + S * Q::STAGE + Q::PIECE, 16 * wave, kd, lane);
         lds_barrier();
       }
       if (nxt.n >= 0) issue(1 - S, nxt);
@@ -99,8 +108,8 @@ __global__ void __launch_bounds__(128, (row_waves<T, D, CAP>())) k_rules_bwd_row
         whole = __builtin_amdgcn_ballot_w64(seen != 0xffffu) == 0;
       }
       if (some) {
-        f32x16 s = rows_times<T, D, S * Q::STAGE, false>(smem, reads, xq, zeros16());
-        const f32x16 dp = rows_times<T, D, S * Q::STAGE + Q::PIECE, false>(smem, reads, xo, zeros16());
+        f32x16 s = rows_times<T, D, S * Q::STAGE, false>(reads, xq, zeros16());
+        const f32x16 dp = rows_times<T, D, S * Q::STAGE + Q::PIECE, false>(reads, xo, zeros16());
         const Logits<BIAS> logits(row - cur.lo - 8 * half, row - cur.hi - 8 * half, slope);
         if constexpr (CAP)
 #pragma unroll
@@ -116,7 +125,7 @@ __global__ void __launch_bounds__(128, (row_waves<T, D, CAP>())) k_rules_bwd_row
           for_16<0>([&](auto ic) { e[decltype(ic)::value] = keep(e[decltype(ic)::value], bit_mask<decltype(ic)::value>(seen)); });
         Shares<T> ds;
         ds.set(e);
-        columns_times<T, D, S * Q::STAGE, false>(dq, smem, reads, ds);
+        columns_times<T, D, S * Q::STAGE, false>(dq, reads, ds);
       }
       cur = nxt;
       return cur.n >= 0;
@@ -144,7 +153,9 @@ template <typename T, int D, bool CAP, bool BIAS, bool DOCS>
 __global__ void __launch_bounds__(128, (col_waves<T, D, CAP>())) k_rules_bwd_cols(RuleArgs a) {
   typedef Geo<T, D> Q;
   constexpr int MT = D / 32;
-  constexpr bool LEAN = D == 128 || sizeof(T) == 4;     // dk, dv, k and v alone take 192 registers there
+  // dk, dv, k and v alone take 192 registers at head dimension 128; at 64 what this saves is the third wavefront a SIMD, where no rule needs the registers
+  // (BigBird 12 x 16384: 76 -> 67 us; with a bias, which has two wavefronts either way: 312 -> 322)
+  constexpr bool LEAN = D == 128 || sizeof(T) == 4 || !(CAP || BIAS || DOCS);
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   unsigned char *extra = smem + Q::RING;                // per stage: ref of its 32 rows, their factors, their -delta (twice), their documents (twice)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -256,6 +267,7 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, CAP>())) k_rules_bwd_col
       const int32_t *rd = reinterpret_cast<const int32_t *>(extra + S * Q::EXTRA + 512);
       if (DOCS && cur.pad) {
         clear_rows<T, D>(smem + Q0, 16 * wave, rd, lane);
+        clear_rows<T, D>(smem + O0, 16 * wave, rd, lane);
         lds_barrier();
       }
       if (nxt.n >= 0) issue(1 - S, nxt);
@@ -270,7 +282,7 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, CAP>())) k_rules_bwd_col
       }
       if (some) {
         const bool factors = __builtin_amdgcn_ballot_w64(stat[32 + l32] != 1.f) != 0;
-        f32x16 s = rows_times<T, D, Q0, LEAN>(smem, reads, xk, zeros16());
+        f32x16 s = rows_times<T, D, Q0, LEAN>(reads, xk, zeros16());
         float slope_lo = 0.f, slope_hi = 0.f;
         if constexpr (BIAS) {
           slope_lo = as_floats(slopes)[cur.lo >> kHeadShift] * kLog2e;
@@ -302,7 +314,7 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, CAP>())) k_rules_bwd_col
           for_16<0>([&](auto ic) { p[decltype(ic)::value] = keep(p[decltype(ic)::value], bit_mask<decltype(ic)::value>(seen)); });
         Shares<T> share;
         share.set(p);
-        columns_times<T, D, O0, LEAN>(dv, smem, reads, share);
+        columns_times<T, D, O0, LEAN>(dv, reads, share);
         f32x16 dp;
 #pragma unroll
         for (int g = 0; g < 4; g++) {
@@ -310,7 +322,7 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, CAP>())) k_rules_bwd_col
 #pragma unroll
           for (int j = 0; j < 4; j++) dp[4 * g + j] = nd[j];
         }
-        dp = rows_times<T, D, O0, LEAN>(smem, reads, xv, dp);
+        dp = rows_times<T, D, O0, LEAN>(reads, xv, dp);
 #pragma unroll
         for (int i = 0; i < 16; i++) {
           e[i] = p[i] * dp[i];
@@ -319,7 +331,7 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, CAP>())) k_rules_bwd_col
         if (!whole)
           for_16<0>([&](auto ic) { e[decltype(ic)::value] = keep(e[decltype(ic)::value], bit_mask<decltype(ic)::value>(seen)); });
         share.set(e);
-        columns_times<T, D, Q0, LEAN>(dk, smem, reads, share);
+        columns_times<T, D, Q0, LEAN>(dk, reads, share);
       }
       cur = nxt;
       return cur.n >= 0;
@@ -416,7 +428,7 @@ extern "C" int bsp_attention_rules_bwd(const bsp_attention_rules_call *call, con
   const int rc = rules_args(call, a);
   if (rc != BSP_OK) return rc;
   const int64_t *s = call->strides;
-  if (!d_o || !q || !k || !v || !o || !dq || !neg_delta || !call->stats || (dk != nullptr) != (dv != nullptr)) return BSP_ERR_ARG;
+  if (!d_o || !q || !k || !v || !o || !dq || !neg_delta || !call->stats || (call->dtype != BSP_F32 && (!call->o_rest || off16(call->o_rest))) || (dk != nullptr) != (dv != nullptr)) return BSP_ERR_ARG;
   const void *ptrs[] = {d_o, q, k, v, o, dq, dk, dv, partial};
   for (const void *p : ptrs)
     if (off16(p)) return BSP_ERR_ARG;

@@ -1,7 +1,8 @@
 // Forward pass of attention with score rules (attention_rules.h): one sweep over a line's tiles with a running maximum and sum
 // per row.  As in attention_fwd.hip the maximum moves only when a lane's exponentials of a step add up to more than 8192.
 // Stores o and, for the backward pass, per row `ref` and `factor` with p = exp2(y - ref) * factor: ref = m + log2 l rounded to one
-// float, factor what the rounding left out (1 in 16-bit types while |ref| < 64, where it is below 2^-18).
+// float, factor what the rounding left out (1 in 16-bit types while |ref| < 64, where it is below 2^-18).  16-bit types keep what the rounding of o left out
+// as well.
 #include "attention_rules.h"
 
 namespace bsp {
@@ -70,6 +71,7 @@ __global__ void __launch_bounds__(128, (fwd_waves<T, D, BIAS, DOCS>())) k_rules_
       const int32_t *kd = reinterpret_cast<const int32_t *>(extra + S * Q::EXTRA);
       if (DOCS && cur.pad) {
         clear_rows<T, D>(smem + S * Q::STAGE, 16 * wave, kd, lane);
+        clear_rows<T, D>(smem + S * Q::STAGE + Q::PIECE, 16 * wave, kd, lane);
         lds_barrier();
       }
       if (nxt.n >= 0) issue(1 - S, nxt);
@@ -83,7 +85,7 @@ __global__ void __launch_bounds__(128, (fwd_waves<T, D, BIAS, DOCS>())) k_rules_
         whole = __builtin_amdgcn_ballot_w64(seen != 0xffffu) == 0;
       }
       if (some) {
-        f32x16 s = rows_times<T, D, S * Q::STAGE, false>(smem, reads, xq, zeros16());
+        f32x16 s = rows_times<T, D, S * Q::STAGE, false>(reads, xq, zeros16());
         if constexpr (CAP)
 #pragma unroll
           for (int i = 0; i < 16; i++) s[i] = cap_score<T>(s[i], in);
@@ -116,7 +118,7 @@ __global__ void __launch_bounds__(128, (fwd_waves<T, D, BIAS, DOCS>())) k_rules_
         l += sum;
         Shares<T> p;
         p.set(e);
-        columns_times<T, D, S * Q::STAGE + Q::PIECE, false>(o, smem, reads, p);
+        columns_times<T, D, S * Q::STAGE + Q::PIECE, false>(o, reads, p);
       }
       cur = nxt;
       return cur.n >= 0;
@@ -140,7 +142,17 @@ __global__ void __launch_bounds__(128, (fwd_waves<T, D, BIAS, DOCS>())) k_rules_
   quad_barrier();                                       // the ring is free
   T *po = reinterpret_cast<T *>(a.o) + z * a.o_sz + h * a.o_sh;
   const int first = line * 64 + 32 * wave;
-  store_some_rows<T, D>(smem + wave * (32 * (D + Q::VEC) * Q::ESZ), po + (int64_t)first * a.o_ld, a.L - first, po + (int64_t)(first + 16) * a.o_ld, a.L - first - 16, a.o_ld, o, lane);
+  unsigned char *stage = smem + wave * (32 * (D + Q::VEC) * Q::ESZ);
+  store_some_rows<T, D>(stage, po + (int64_t)first * a.o_ld, a.L - first, po + (int64_t)(first + 16) * a.o_ld, a.L - first - 16, a.o_ld, o, lane);
+  if constexpr (sizeof(T) == 2)
+    if (a.ref != nullptr) {                             // what the rounding left out, for the backward pass (attention_rules_bwd.hip)
+#pragma unroll
+      for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[mt][i] -= to_float(from_float<T>(o[mt][i]));
+      T *pr = reinterpret_cast<T *>(a.o_rest) + (((int64_t)z * a.H + h) * a.L + first) * D;
+      store_some_rows<T, D>(stage, pr, a.L - first, pr + 16 * D, a.L - first - 16, D, o, lane);
+    }
 }
 
 // The range of document numbers in each group of sixteen positions (see RuleArgs)
@@ -199,7 +211,7 @@ int rules_args(const bsp_attention_rules_call *c, RuleArgs &a) {
   logit_args(a, c->scale, c->softcap);
   a.slopes = c->slopes; a.causal = c->causal; a.prefix = c->prefix;
   a.docs = c->documents; a.docs_sz = c->documents_stride; a.ranges = c->ranges; a.groups = (int)((c->length + 15) / 16);
-  a.ref = c->stats; a.lut = c->d_rows;
+  a.ref = c->stats; a.o_rest = c->o_rest; a.lut = c->d_rows;
   return BSP_OK;
 }
 
@@ -215,6 +227,7 @@ extern "C" int bsp_attention_rules_fwd(const bsp_attention_rules_call *call, con
   if (rc != BSP_OK) return rc;
   const int64_t *s = call->strides;
   if (!q || !k || !v || !o || off16(q) || off16(k) || off16(v) || off16(o) || !s[2] || !s[5] || !s[8] || !s[11]) return BSP_ERR_ARG;
+  if (call->stats && call->dtype != BSP_F32 && (!call->o_rest || off16(call->o_rest))) return BSP_ERR_ARG;
   a.q = q; a.k = k; a.v = v; a.o = o;
   a.o_sz = s[9]; a.o_sh = s[10]; a.o_ld = s[11];
   const hipStream_t st = as_stream(stream);

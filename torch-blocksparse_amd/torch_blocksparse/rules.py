@@ -28,7 +28,7 @@ from . import _lib
 class _Call(ctypes.Structure):             # bsp_attention_rules_call
     _fields_ = ([(n, ctypes.c_int) for n in ('dtype', 'Z', 'H', 'kv_heads', 'lines', 'D')] + [('length', ctypes.c_int64), ('strides', ctypes.c_int64 * 24)]
                 + [(n, ctypes.c_float) for n in ('scale', 'softcap')] + [('causal', ctypes.c_int), ('slopes', ctypes.c_void_p), ('documents', ctypes.c_void_p),
-                   ('documents_stride', ctypes.c_int64), ('prefix', ctypes.c_void_p), ('ranges', ctypes.c_void_p), ('d_rows', ctypes.c_void_p), ('stats', ctypes.c_void_p)])
+                   ('documents_stride', ctypes.c_int64), ('prefix', ctypes.c_void_p), ('ranges', ctypes.c_void_p), ('d_rows', ctypes.c_void_p), ('stats', ctypes.c_void_p), ('o_rest', ctypes.c_void_p)])
 
 
 def _strides(t):
@@ -147,26 +147,27 @@ class _rules(torch.autograd.Function):
         keep = grad_enabled and any(ctx.needs_input_grad[:3])
         o = torch.empty((Z, H, L, D), dtype=q.dtype, device=q.device)
         stats = torch.empty((Z, H, 2, 64 * tables.lines), dtype=torch.float32, device=q.device) if keep else None
+        rest = torch.empty((Z, H, L, D), dtype=q.dtype, device=q.device) if keep and q.element_size() == 2 else None
         ranges = torch.empty((Z, (L + 15) // 16, 2), dtype=torch.int32, device=q.device) if documents is not None else None
-        call = _rules.call(q, k, v, o, tables, scale, softcap, slopes, causal, documents, prefix, ranges, stats)
+        call = _rules.call(q, k, v, o, tables, scale, softcap, slopes, causal, documents, prefix, ranges, stats, rest)
         _lib.check(lib.bsp_attention_rules_fwd(ctypes.byref(call), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _lib.stream_ptr(q.device)), 'bsp_attention_rules_fwd')
         if keep:
-            ctx.save_for_backward(q, k, v, o, stats, ranges, slopes, documents, prefix)
+            ctx.save_for_backward(q, k, v, o, rest, stats, ranges, slopes, documents, prefix)
             ctx.tables, ctx.numbers = tables, (scale, softcap, causal)
         return o
 
     @staticmethod
-    def call(q, k, v, o, tables, scale, softcap, slopes, causal, documents, prefix, ranges, stats, grads=()):
+    def call(q, k, v, o, tables, scale, softcap, slopes, causal, documents, prefix, ranges, stats, rest, grads=()):
         Z, H, L, D = q.shape
         strides = [s for t in (q, k, v, o) + tuple(grads) for s in (_strides(t) if t is not None else (0, 0, 0))]
         p = lambda t: None if t is None else t.data_ptr()   # noqa: E731
         return _Call(_lib.DTYPES[q.dtype], Z, H, k.size(1), tables.lines, D, L, (ctypes.c_int64 * 24)(*strides), scale, softcap, int(causal), p(slopes), p(documents),
-                     documents.stride(0) if documents is not None and Z > 1 else 0, p(prefix), p(ranges), tables.rows.data_ptr(), p(stats))
+                     documents.stride(0) if documents is not None and Z > 1 else 0, p(prefix), p(ranges), tables.rows.data_ptr(), p(stats), p(rest))
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        q, k, v, o, stats, ranges, slopes, documents, prefix = ctx.saved_tensors
+        q, k, v, o, rest, stats, ranges, slopes, documents, prefix = ctx.saved_tensors
         tables, (scale, softcap, causal) = ctx.tables, ctx.numbers
         need_q, need_k, need_v = ctx.needs_input_grad[:3]
         with _lib.on_device(q.device):
@@ -180,7 +181,7 @@ class _rules(torch.autograd.Function):
                 dk, dv = new(k), new(v)
                 items, n_items, splits, n_splits, slots = tables.columns(k.size(1), Z)
                 partial = torch.empty((Z, slots, 2, 64, D), dtype=torch.float32, device=q.device) if slots else None
-            call = _rules.call(q, k, v, o, tables, scale, softcap, slopes, causal, documents, prefix, ranges, stats, (do, dq, dk, dv))
+            call = _rules.call(q, k, v, o, tables, scale, softcap, slopes, causal, documents, prefix, ranges, stats, rest, (do, dq, dk, dv))
             p = _lib.ptr
             _lib.check(_lib.load().bsp_attention_rules_bwd(ctypes.byref(call), p(do), p(q), p(k), p(v), p(o), p(dq), p(dk), p(dv), p(delta), p(items), n_items,
                                                            p(partial), slots, p(splits), n_splits, _lib.stream_ptr(q.device)), 'bsp_attention_rules_bwd')
