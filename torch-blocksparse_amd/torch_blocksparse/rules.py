@@ -62,7 +62,7 @@ class _Tables:
         host, info = self._build(self.layout)
         self.lines = info.lines
         self.rows = host[:info.items_offset].to(device)
-        self._columns = dict()
+        self._columns, self._chosen = dict(), dict()
 
     def _build(self, lay):
         H, R, C = lay.shape
@@ -79,6 +79,12 @@ class _Tables:
 
     def columns(self, kv_heads, batches):
         """(items, their number per key head, splits, number of splits, slots), tensors on the device"""
+        made = self._chosen.get((kv_heads, batches))
+        if made is None:
+            made = self._chosen[kv_heads, batches] = self._choose(kv_heads, batches)
+        return made
+
+    def _choose(self, kv_heads, batches):
         H, R, C = self.layout.shape
         tiles = self._columns.get(kv_heads)
         if tiles is None:
