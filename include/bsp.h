@@ -545,14 +545,14 @@ int bsp_cache_read(int dtype, const void *pages, int n_pages, int block, int hea
  * h / (H / kv_heads).  rows: NULL, or what is seen beside that: the query heads of a key head form units of at most 16 (ceil(G / ceil(G / 16)) heads of G each,
  * the last may have fewer); per unit n_rows + 1 ints, from rows[0] on: the place in `rows` of the first entry of each block-row of the unit's
  * layout and the end of the last one's; an entry: block-column << 16 | a bit for each of the unit's heads that sees it.  The row is (n - 1) /
- * block.  splits: workgroups that a sequence's positions are split among (bsp_cache_attention_splits gives a good number for
- * rows of `blocks` blocks at most); workspace: bsp_cache_attention_workspace_bytes bytes, 16-byte aligned, or NULL where that is 0. */
+ * block.  most_blocks: no sequence sees more blocks (width, or the most entries of a row).  splits: workgroups that those are split among
+ * (bsp_cache_attention_splits gives a good number); workspace: bsp_cache_attention_workspace_bytes bytes, 16-byte aligned, or NULL where that is 0. */
 int bsp_cache_attention_splits(int B, int H, int kv_heads, int block, int64_t blocks);
 int64_t bsp_cache_attention_workspace_bytes(int B, int H, int kv_heads, int D, int splits);
 int bsp_cache_attention(int dtype, const void *q, int64_t q_stride_b, int64_t q_stride_h, void *o, int64_t o_stride_b, int64_t o_stride_h, int B, int H,
                         const void *pages, int n_pages, int block, int kv_heads, int D, int bits, const int32_t *table, int64_t table_stride, int width,
-                        const int32_t *lengths, const int32_t *rows, int n_rows, float scale, float softcap, const float *slopes, void *workspace,
-                        int64_t workspace_bytes, int splits, void *stream);
+                        const int32_t *lengths, const int32_t *rows, int n_rows, int64_t most_blocks, float scale, float softcap, const float *slopes,
+                        void *workspace, int64_t workspace_bytes, int splits, void *stream);
 
 /* ---------------------------------------------------------------------------------------------------
  * Dense utility ops of the reference package.

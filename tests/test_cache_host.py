@@ -57,10 +57,10 @@ def test_abi_refuses_before_it_launches():
         ('dtype', 0), ('pages', at), ('n', 1), ('block', 16), ('heads', 1), ('D', 64), ('bits', 4), ('k', at), ('v', at), ('slots', at), ('T', 1), ('stream', 0))])
     for bad in (dict(dtype=-1), dict(k=0), dict(v=at + 4), dict(bits=16), dict(T=-1)):
         assert read(**bad) < 0, bad
-    names = ('dtype q qb qh o ob oh B H pages n block kv D bits table ts width lengths rows n_rows scale cap slopes ws bytes splits stream').split()
-    good = dict(zip(names, (0, at, 64, 64, at, 64, 64, 1, 1, at, 1, 16, 1, 64, 4, at, 1, 1, at, 0, 0, 1., 0., 0, 0, 0, 1, 0)))
+    names = ('dtype q qb qh o ob oh B H pages n block kv D bits table ts width lengths rows n_rows most scale cap slopes ws bytes splits stream').split()
+    good = dict(zip(names, (0, at, 64, 64, at, 64, 64, 1, 1, at, 1, 16, 1, 64, 4, at, 1, 1, at, 0, 0, 1, 1., 0., 0, 0, 0, 1, 0)))
     for bad in (dict(dtype=2), dict(q=0), dict(q=at + 2), dict(qb=4), dict(o=at + 2), dict(oh=1), dict(B=0), dict(H=3, kv=2), dict(n=0), dict(block=20), dict(width=0),
-                dict(width=1 << 20), dict(lengths=0), dict(rows=at), dict(rows=at, n_rows=1 << 17), dict(scale=float('nan')), dict(cap=-1.), dict(splits=0), dict(splits=65),
+                dict(width=1 << 20), dict(lengths=0), dict(rows=at), dict(rows=at, n_rows=1 << 17), dict(most=0), dict(scale=float('nan')), dict(cap=-1.), dict(splits=0), dict(splits=65),
                 dict(splits=2), dict(splits=2, ws=at, bytes=16)):
         assert lib.bsp_cache_attention(*dict(good, **bad).values()) < 0, bad
 

@@ -7,10 +7,14 @@
 // codes and steps on their way while the one before is computed, and the wavefronts' results are joined in LDS.  Where sequences and
 // key heads do not fill the chip the positions are split among workgroups, and a second kernel joins what those leave.
 //
-// The codes are operands as they are: small integers are exact in fp16, so a score is the sum over the groups of step * (q . codes) +
+// The codes are operands as they are, bit patterns of fp16 numbers below the normal ones, so a score is the sum over the groups of step * (q . codes) +
 // least * (sum of the group's q), the products on the matrix units (16 x 16 x 32: a group each).  q is scaled by a power of two per head to the
 // range of fp16, which loses nothing that 2^-35 of its largest element would not.  Values are v = least + code * step rounded to fp16
 // (2^-12 of it, under the rounding of the shares) through LDS, where the product with the shares reads them transposed.
+//
+// Measured: sixteen sequences of up to 16384 positions, 32 query heads of 128 on 8 key heads, 4 bits (218 MB of pages): 51 us with the join, 4.3 TB/s;
+// loading the same bytes and nothing else takes 40.  The vector units are what is left: taking the codes out of their words for keys and
+// values was 240 of 390 operations a pair of tiles and is 140 of 270 with keys as they lie (63 us before).
 //
 // Scores lie with a position per lane and the query heads along the sixteen result rows of the matrix unit, dealt so that a head takes one
 // value in a quarter of the lanes: with at most four heads a key head (V = 1) a tile costs one exponential a lane, with up to eight two.
@@ -31,12 +35,13 @@ struct DecodeArgs {
   float scale, cap;
   float *partial;                  // [B][units][splits][heads a unit][D + 2]
   int B, H, kv_heads, block, tile_shift;                  // tile_shift: log2 of the tiles of sixteen positions a page
-  int G, per, units, splits;       // query heads a key head; heads of a unit (a workgroup's), units
+  int G, per, units, splits, chunk;   // query heads a key head; heads of a unit (a workgroup's), units; workgroups a unit, pairs of tiles a wavefront of them
 };
 
 namespace {
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 template <int BITS, int D> struct RawTile {
   static constexpr int QB = D * BITS / 32 / 4;            // 32-bit words of a quarter row
@@ -89,40 +94,89 @@ __global__ void __launch_bounds__(256, 3) k_cache_attention(DecodeArgs a, int dt
       tiles = (t[1] - t[0]) << a.tile_shift;
     }
   }
-  // this wavefront's pairs of tiles
-  const int pairs = (tiles + 1) >> 1, parts = a.splits * 4, part = split * 4 + wave;
-  const int p_end = (int)((int64_t)pairs * (part + 1) / parts);
-  int pair = (int)((int64_t)pairs * part / parts);
+  // this wavefront's pairs of tiles: the same number for all, whatever the sequences' lengths, so that no workgroup has much more to do than another
+  const int pairs = (tiles + 1) >> 1, part = split * 4 + wave;
+  const int p_end = pairs < (part + 1) * a.chunk ? pairs : (part + 1) * a.chunk;
+  int pair = part * a.chunk;
 
-  // the lane's heads: value j of the lane belongs to the unit's head c * V + j; row m of a product's first operand to head (m / 4) * V + m % 4
+  // row m of a product's first operand belongs to the unit's head (m / 4) * V + m % 4
+  const int row = (key >> 2) * V + (key & 3);
+  const bool row_here = (key & 3) < V && row < heads;
+  union { u32x4 raw; f16 h[8]; bf16 f[8]; } q[GR];
+#pragma unroll
+  for (int g = 0; g < GR; g++)
+    q[g].raw = *reinterpret_cast<const u32x4 *>(reinterpret_cast<const uint16_t *>(a.q) + b * a.q_sb + (first + (row_here ? row : 0)) * a.q_sh + 8 * c + 32 * g);
+
+  unsigned char *values = smem + wave * L::WAVE, *shares = values + 32 * L::VROW;
+  const int64_t page_bytes = P::bytes(a.block) * a.kv_heads;
+  const unsigned char *pages = a.pages + P::bytes(a.block) * hk;
+  const int value = P::codes(a.block, 1), k_meta = P::meta(a.block, 0);       // where a page's values lie behind its keys, and the steps behind the codes
+  const uint32_t own_codes = key * P::ROW + c * (P::ROW / 4), own_meta = key * P::META;
+
+  // 32 pairs at a time, a tile a lane: its page, its first position, how many of its positions count, the heads that see it
+  int base = pair, v_page = 0, v_pos = 0, v_info = 0;
+  auto look = [&]() {
+    const int t = 2 * base + lane;
+    int col = t >> a.tile_shift, mask = 0xffff;
+    const bool in = t < tiles && (t >> 1) < p_end;
+    if (a.rows) {
+      const uint32_t e = in ? (uint32_t)a.rows[entry + col] : 0u;
+      col = (int)(e >> 16);
+      mask = (int)(e & 0xffffu);
+    }
+    const int sub = t & ((1 << a.tile_shift) - 1);
+    v_pos = col * a.block + 16 * sub;
+    int n = in ? len - v_pos : 0, page = 0;
+    if (n > 0) page = a.table[b * a.table_sb + col];   // (col * block < len, so within the row of the table)
+    if (page < 0 || page >= a.n_pages) n = 0;
+    n = n < 0 ? 0 : n > 16 ? 16 : n;
+    v_page = n > 0 ? page : 0;
+    v_info = sub | n << 8 | mask << 16;
+  };
+  struct Tile { int pos, n, mask; };
+  auto fetch = [&](RawTile<BITS, D> &x, int at) {       // tile `at` of the lanes' 64
+    const int page = __builtin_amdgcn_readlane(v_page, at), info = __builtin_amdgcn_readlane(v_info, at);
+    const int sub = info & 0xff, n = (info >> 8) & 0xff;
+    // (addresses of the wavefront, and 32-bit ones of the lane from there)
+    const unsigned char *codes = pages + page * page_bytes + 16 * sub * P::ROW, *meta = pages + page * page_bytes + 16 * sub * P::META;
+    load_words(x.kc, codes + own_codes);
+    load_words(x.vc, codes + value + own_codes);
+    load_words(x.km, meta + k_meta + own_meta);
+    load_words(x.vm, meta + k_meta + value + own_meta);
+    return Tile{__builtin_amdgcn_readlane(v_pos, at), n, (info >> 16) & 0xffff};
+  };
+  RawTile<BITS, D> raw[2];
+  Tile tile[2];
+  if (pair < p_end) {                                     // (before q is looked at: loads of which each waits for the last)
+    look();
+#pragma unroll
+    for (int u = 0; u < 2; u++) tile[u] = fetch(raw[u], u);
+  }
+
+  // the lane's heads: value j of the lane belongs to the unit's head c * V + j
   float m[V], l[V], unscale[V], slope[V], qsum[V][GR];
   h8 qf[GR];
   {
-    const int r = (key >> 2) * V + (key & 3);
-    const bool here = (key & 3) < V && r < heads;
     float x[GR][8], top = 0.f;
-    const int64_t at = b * a.q_sb + (first + (here ? r : 0)) * a.q_sh + 8 * c;
 #pragma unroll
     for (int g = 0; g < GR; g++) {
-      union { u32x4 raw; f16 h[8]; bf16 f[8]; } u;
-      u.raw = *reinterpret_cast<const u32x4 *>(reinterpret_cast<const uint16_t *>(a.q) + at + 32 * g);
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        x[g][i] = here ? (dtype == BSP_F16 ? to_float(u.h[i]) : to_float(u.f[i])) : 0.f;
+        x[g][i] = row_here ? (dtype == BSP_F16 ? to_float(q[g].h[i]) : to_float(q[g].f[i])) : 0.f;
         top = fmaxf(top, fabsf(x[g][i]));
       }
     }
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
-    // 2^e so that the largest element is in [1024, 2048)
-    const int e = top > 0.f && top < INFINITY ? 10 - ilogbf(top) : 0;
+    // 2^e so that the largest element is in [2^14, 2^15)
+    const int e = top > 0.f && top < INFINITY ? 14 - ilogbf(top) : 0;
 #pragma unroll
     for (int g = 0; g < GR; g++) {
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        qf[g][i] = (_Float16)ldexpf(x[g][i], e);
-        sum += (float)qf[g][i];
+        qf[g][i] = (_Float16)ldexpf(x[g][i], e - code_up<BITS>(i));
+        sum += ldexpf((float)qf[g][i], code_up<BITS>(i) - 24);
       }
       sum += __shfl_xor(sum, 16);
       sum += __shfl_xor(sum, 32);
@@ -132,7 +186,7 @@ __global__ void __launch_bounds__(256, 3) k_cache_attention(DecodeArgs a, int dt
 #pragma unroll
     for (int j = 0; j < V; j++) {
       const int r2 = c * V + j, e2 = __shfl(e, 4 * c + j);
-      unscale[j] = ldexpf(1.f, -e2);
+      unscale[j] = ldexpf(1.f, 24 - e2);
       m[j] = r2 < heads ? -INFINITY : 0.f;
       l[j] = 0.f;
       slope[j] = a.slopes && r2 < heads ? a.slopes[first + r2] * kLog2e : 0.f;
@@ -143,68 +197,22 @@ __global__ void __launch_bounds__(256, 3) k_cache_attention(DecodeArgs a, int dt
 #pragma unroll
   for (int n = 0; n < NT; n++) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  unsigned char *values = smem + wave * L::WAVE, *shares = values + 32 * L::VROW;
-  const int64_t page_bytes = P::bytes(a.block) * a.kv_heads;
-  const unsigned char *pages = a.pages + P::bytes(a.block) * hk;
-  const int k_codes = P::codes(a.block, 0) + c * (P::ROW / 4), v_codes = P::codes(a.block, 1) + c * (P::ROW / 4), k_meta = P::meta(a.block, 0), v_meta = P::meta(a.block, 1);
-
   if (pair < p_end) {
-    // 32 pairs at a time, a tile a lane: its page, its first position, how many of its positions count, the heads that see it
-    int base = pair, v_page = 0, v_pos = 0, v_info = 0;
-    auto look = [&]() {
-      const int t = 2 * base + lane;
-      int col = t >> a.tile_shift, mask = 0xffff;
-      const bool in = t < tiles && (t >> 1) < p_end;
-      if (a.rows) {
-        const uint32_t e = in ? (uint32_t)a.rows[entry + col] : 0u;
-        col = (int)(e >> 16);
-        mask = (int)(e & 0xffffu);
-      }
-      const int sub = t & ((1 << a.tile_shift) - 1);
-      v_pos = col * a.block + 16 * sub;
-      int n = in ? len - v_pos : 0, page = 0;
-      if (n > 0) page = a.table[b * a.table_sb + col];   // (col * block < len, so within the row of the table)
-      if (page < 0 || page >= a.n_pages) n = 0;
-      n = n < 0 ? 0 : n > 16 ? 16 : n;
-      v_page = n > 0 ? page : 0;
-      v_info = sub | n << 8 | mask << 16;
-    };
-    look();
-    struct Tile { int pos, n, mask; };
-    auto fetch = [&](RawTile<BITS, D> &x, int at) {       // tile `at` of the lanes' 64
-      const int page = __builtin_amdgcn_readlane(v_page, at), info = __builtin_amdgcn_readlane(v_info, at);
-      const int row = 16 * (info & 0xff) + key, n = (info >> 8) & 0xff;
-      const unsigned char *from = pages + page * page_bytes;
-      load_words(x.kc, from + k_codes + row * P::ROW);
-      load_words(x.vc, from + v_codes + row * P::ROW);
-      load_words(x.km, from + k_meta + row * P::META);
-      load_words(x.vm, from + v_meta + row * P::META);
-      const bool here = key < n;                          // what lies behind the sequence's end stands for zeros
-#pragma unroll
-      for (int g = 0; g < GR; g++) x.km[g] = here ? x.km[g] : 0u, x.vm[g] = here ? x.vm[g] : 0u;
-      return Tile{__builtin_amdgcn_readlane(v_pos, at), n, (info >> 16) & 0xffff};
-    };
-    RawTile<BITS, D> raw[2];
-    Tile tile[2];
-#pragma unroll
-    for (int u = 0; u < 2; u++) tile[u] = fetch(raw[u], u);
     while (true) {
       // scores and values of the pair
       float y[2][V];
       uint32_t seen = 0;                                  // bit 4 u + j
 #pragma unroll
       for (int u = 0; u < 2; u++) {
+        const bool here = key < tile[u].n;                // what lies behind the sequence's end stands for zeros (looked at here and not where it is loaded, which would be waiting for it)
         float s[V];
 #pragma unroll
         for (int j = 0; j < V; j++) s[j] = 0.f;
 #pragma unroll
         for (int g = 0; g < GR; g++) {
-          f16x2 p[4];
-          chunk_codes<BITS>(raw[u].kc + g * (BITS / 4), p);
-          h8 kf;
-#pragma unroll
-          for (int i = 0; i < 8; i++) kf[i] = p[i >> 1][i & 1];
-          const f32x4 dot = __builtin_amdgcn_mfma_f32_16x16x32_f16(qf[g], kf, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+          uint32_t p[4];
+          chunk_bits<BITS>(raw[u].kc + g * (BITS / 4), p);
+          const f32x4 dot = __builtin_amdgcn_mfma_f32_16x16x32_f16(qf[g], __builtin_bit_cast(h8, u32x4{p[0], p[1], p[2], p[3]}), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
           const float step = step_of(raw[u].km[g]), least = least_of(raw[u].km[g]);
 #pragma unroll
           for (int j = 0; j < V; j++) s[j] = fmaf(step, dot[j], fmaf(least, qsum[j][g], s[j]));
@@ -213,23 +221,32 @@ __global__ void __launch_bounds__(256, 3) k_cache_attention(DecodeArgs a, int dt
 #pragma unroll
         for (int j = 0; j < V; j++) {
           float x = s[j] * unscale[j];
-          if (capped) x = a.cap * kLog2e * fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * (2.f * kLog2e * a.scale / a.cap)) + 1.f), 1.f);
-          else x *= a.scale * kLog2e;
+          if (capped) {
+            asm volatile("");                             // (a branch: not computed where there is no cap)
+            x = a.cap * kLog2e * fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * (2.f * kLog2e * a.scale / a.cap)) + 1.f), 1.f);
+          } else {
+            x *= a.scale * kLog2e;
+          }
           y[u][j] = fmaf(-slope[j], behind, x);
-          seen |= (key < tile[u].n && (tile[u].mask >> (c * V + j) & 1)) ? 1u << (4 * u + j) : 0u;
+          seen |= (here && (tile[u].mask >> (c * V + j) & 1)) ? 1u << (4 * u + j) : 0u;
         }
 #pragma unroll
         for (int g = 0; g < GR; g++) {
           f16x2 p[4];
           chunk_codes<BITS>(raw[u].vc + g * (BITS / 4), p);
-          const f16 step = __builtin_bit_cast(f16, (uint16_t)raw[u].vm[g]), least = __builtin_bit_cast(f16, (uint16_t)(raw[u].vm[g] >> 16));
+          const uint32_t meta = here ? raw[u].vm[g] : 0u;
+          const f16 step = __builtin_bit_cast(f16, (uint16_t)meta), least = __builtin_bit_cast(f16, (uint16_t)(meta >> 16));
           union { u32x4 w; f16x2 h[4]; } v;
 #pragma unroll
           for (int i = 0; i < 4; i++) v.h[i] = __builtin_elementwise_fma(p[i], f16x2{step, step}, f16x2{least, least});
           *reinterpret_cast<u32x4 *>(values + (16 * u + key) * L::VROW + 64 * g + 16 * c) = v.w;
         }
       }
-      // the next pair on its way
+      // the next pair on its way (into the registers that the scores have come from)
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int j = 0; j < V; j++) asm volatile("" : "+v"(y[u][j]));
       pair++;
       const bool more = pair < p_end;
       if (more) {
@@ -241,7 +258,8 @@ __global__ void __launch_bounds__(256, 3) k_cache_attention(DecodeArgs a, int dt
         for (int u = 0; u < 2; u++) tile[u] = fetch(raw[u], 2 * (pair - base) + u);
       }
       // shares relative to the running maximum, which moves when they grow past 8192
-      float e[2][V], sum[V];
+      f16 e[2][V];
+      float sum[V];
       auto exponentials = [&]() {
 #pragma unroll
         for (int j = 0; j < V; j++) {
@@ -249,8 +267,8 @@ __global__ void __launch_bounds__(256, 3) k_cache_attention(DecodeArgs a, int dt
           sum[j] = 0.f;
 #pragma unroll
           for (int u = 0; u < 2; u++) {
-            e[u][j] = seen >> (4 * u + j) & 1 ? __builtin_amdgcn_exp2f(y[u][j] - ms) : 0.f;
-            sum[j] += e[u][j];
+            e[u][j] = (f16)(seen >> (4 * u + j) & 1 ? __builtin_amdgcn_exp2f(y[u][j] - ms) : 0.f);
+            sum[j] += (float)e[u][j];                     // as the product below has them
           }
         }
       };
@@ -276,7 +294,7 @@ __global__ void __launch_bounds__(256, 3) k_cache_attention(DecodeArgs a, int dt
       for (int j = 0; j < V; j++) {
         l[j] += sum[j];
 #pragma unroll
-        for (int u = 0; u < 2; u++) *reinterpret_cast<f16 *>(shares + (4 * c + j) * L::PROW + 2 * (16 * u + key)) = (f16)e[u][j];
+        for (int u = 0; u < 2; u++) *reinterpret_cast<f16 *>(shares + (4 * c + j) * L::PROW + 2 * (16 * u + key)) = e[u][j];
       }
       asm volatile("" ::: "memory");
       __builtin_amdgcn_wave_barrier();                    // LDS operations of one wavefront complete in order; this only pins the code order
@@ -327,9 +345,8 @@ __global__ void __launch_bounds__(256, 3) k_cache_attention(DecodeArgs a, int dt
     }
     if (a.splits > 1) {
       float *to = a.partial + ((((int64_t)b * a.units + unit) * a.splits + split) * a.per + r) * ONE;
-      if (d == 0) to[0] = top, to[1] = sum;
-      to[2 + d] = x0;
-      to[3 + d] = x1;
+      if (d == 0) *reinterpret_cast<f32x2 *>(to) = f32x2{top, sum};
+      *reinterpret_cast<f32x2 *>(to + 2 + d) = f32x2{x0, x1};
     } else {
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       uint16_t *to = reinterpret_cast<uint16_t *>(a.o) + b * a.o_sb + (first + r) * a.o_sh + d;
@@ -342,31 +359,56 @@ __global__ void __launch_bounds__(256, 3) k_cache_attention(DecodeArgs a, int dt
   }
 }
 
-// The splits of a head joined: two elements a thread
+// The splits of a head joined, a head a wavefront: a split's maximum and sum a lane (so at most 64 splits), then D / 64 elements a lane, the
+// loads of eight splits under way at a time.  Splits that saw nothing left zeros and a factor of 0.
 template <int D> __global__ void __launch_bounds__(256) k_cache_attention_join(DecodeArgs a, int dtype) {
-  constexpr int ONE = D + 2;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (int64_t)a.B * a.H * (D / 2)) return;
-  const int d = (int)(i % (D / 2)) * 2, h = (int)(i / (D / 2) % a.H), b = (int)(i / (D / 2) / a.H);
+  constexpr int ONE = D + 2, N = D / 64;
+  const int lane = threadIdx.x & 63;
+  const int64_t i = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (i >= (int64_t)a.B * a.H) return;
+  const int h = (int)(i % a.H), b = (int)(i / a.H);
   const int per_key = (a.G + a.per - 1) / a.per, in_key = h % a.G, unit = h / a.G * per_key + in_key / a.per, r = in_key % a.per;
   const float *from = a.partial + (((int64_t)b * a.units + unit) * a.splits * a.per + r) * ONE;
-  float top = -INFINITY;
-  for (int s = 0; s < a.splits; s++) top = fmaxf(top, from[(int64_t)s * a.per * ONE]);
-  float sum = 0.f, x0 = 0.f, x1 = 0.f;
-  for (int s = 0; s < a.splits; s++) {
-    const float *p = from + (int64_t)s * a.per * ONE;
-    const float f = p[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(p[0] - top);
-    sum = fmaf(f, p[1], sum);
-    x0 = fmaf(f, p[2 + d], x0);
-    x1 = fmaf(f, p[3 + d], x1);
+  const int64_t next = (int64_t)a.per * ONE;
+  f32x2 own = {-INFINITY, 0.f};
+  if (lane < a.splits) own = *reinterpret_cast<const f32x2 *>(from + lane * next);
+  float top = own[0];
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+  const float f = own[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(own[0] - top);
+  float sum = f * own[1];
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+  float x[N] = {};
+  for (int s = 0; s < a.splits; s += 8) {
+    float v[8][N];
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      const float *p = from + (s + u < a.splits ? s + u : a.splits - 1) * next + 2 + N * lane;
+      if constexpr (N == 2) {
+        const f32x2 w = *reinterpret_cast<const f32x2 *>(p);
+        v[u][0] = w[0], v[u][1] = w[1];
+      } else {
+        v[u][0] = *p;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      const float g = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s + u));    // (0 past the last split)
+#pragma unroll
+      for (int e = 0; e < N; e++) x[e] = fmaf(g, v[u][e], x[e]);
+    }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  x0 = sum == 0.f ? 0.f : x0 * inv;
-  x1 = sum == 0.f ? 0.f : x1 * inv;
-  uint16_t *to = reinterpret_cast<uint16_t *>(a.o) + b * a.o_sb + h * a.o_sh + d;
-  *reinterpret_cast<uint32_t *>(to) = dtype == BSP_F16
-      ? (uint32_t)__builtin_bit_cast(uint16_t, (f16)x0) | (uint32_t)__builtin_bit_cast(uint16_t, (f16)x1) << 16
-      : (uint32_t)__builtin_bit_cast(uint16_t, (bf16)x0) | (uint32_t)__builtin_bit_cast(uint16_t, (bf16)x1) << 16;
+  uint16_t *to = reinterpret_cast<uint16_t *>(a.o) + b * a.o_sb + h * a.o_sh + N * lane;
+  uint32_t bits = 0;
+#pragma unroll
+  for (int e = 0; e < N; e++) {
+    const float y = sum == 0.f ? 0.f : x[e] * inv;
+    bits |= (uint32_t)(dtype == BSP_F16 ? __builtin_bit_cast(uint16_t, (f16)y) : __builtin_bit_cast(uint16_t, (bf16)y)) << (16 * e);
+  }
+  if constexpr (N == 2) *reinterpret_cast<uint32_t *>(to) = bits;
+  else *to = (uint16_t)bits;
 }
 
 template <int BITS, int D> int launch_decode(const DecodeArgs &a, int dtype, hipStream_t st) {
@@ -374,7 +416,7 @@ template <int BITS, int D> int launch_decode(const DecodeArgs &a, int dtype, hip
   if (a.per <= 4) hipLaunchKernelGGL((k_cache_attention<BITS, D, 1>), grid, dim3(256), 0, st, a, dtype);
   else if (a.per <= 8) hipLaunchKernelGGL((k_cache_attention<BITS, D, 2>), grid, dim3(256), 0, st, a, dtype);
   else hipLaunchKernelGGL((k_cache_attention<BITS, D, 4>), grid, dim3(256), 0, st, a, dtype);
-  if (a.splits > 1) hipLaunchKernelGGL(k_cache_attention_join<D>, dim3((unsigned)cdiv((int64_t)a.B * a.H * (D / 2), 256)), dim3(256), 0, st, a, dtype);
+  if (a.splits > 1) hipLaunchKernelGGL(k_cache_attention_join<D>, dim3((unsigned)cdiv((int64_t)a.B * a.H, 4)), dim3(256), 0, st, a, dtype);
   BSP_LAUNCH_CHECK();
   return BSP_OK;
 }
@@ -387,13 +429,13 @@ inline int heads_a_unit(int G) { return (G + (G + 15) / 16 - 1) / ((G + 15) / 16
 
 using namespace bsp;
 
-// Workgroups to split a sequence's positions over: enough for four a compute unit, each with eight pairs of tiles a wavefront
-// at least if the longest sequence fills its row of the table (lengths are on the device).
+// Workgroups to split a sequence's positions over, `blocks` blocks at most (lengths are on the device): enough for three a compute unit, each with at
+// least eight pairs of tiles a wavefront.
 extern "C" int bsp_cache_attention_splits(int B, int H, int kv_heads, int block, int64_t blocks) {
   if (B <= 0 || H <= 0 || kv_heads <= 0 || H % kv_heads || block <= 0 || blocks <= 0) return BSP_ERR_ARG;
   const int G = H / kv_heads, per = heads_a_unit(G);
   const int64_t groups = (int64_t)B * kv_heads * ((G + per - 1) / per), pairs = (blocks * block + 31) / 32;
-  int64_t n = (1024 + groups - 1) / groups;
+  int64_t n = (768 + groups - 1) / groups;
   if (n > pairs / 32) n = pairs / 32;
   return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }
@@ -406,12 +448,12 @@ extern "C" int64_t bsp_cache_attention_workspace_bytes(int B, int H, int kv_head
 
 extern "C" int bsp_cache_attention(int dtype, const void *q, int64_t q_stride_b, int64_t q_stride_h, void *o, int64_t o_stride_b, int64_t o_stride_h, int B, int H,
                                    const void *pages, int n_pages, int block, int kv_heads, int D, int bits, const int32_t *table, int64_t table_stride, int width,
-                                   const int32_t *lengths, const int32_t *rows, int n_rows, float scale, float softcap, const float *slopes, void *workspace,
-                                   int64_t workspace_bytes, int splits, void *stream) {
+                                   const int32_t *lengths, const int32_t *rows, int n_rows, int64_t most_blocks, float scale, float softcap, const float *slopes,
+                                   void *workspace, int64_t workspace_bytes, int splits, void *stream) {
   if (!q || !o || !pages || !table || !lengths || B <= 0 || H <= 0 || kv_heads <= 0 || H % kv_heads || n_pages <= 0 || width <= 0 || splits < 1 || splits > 64) return BSP_ERR_ARG;
   if ((dtype != BSP_F16 && dtype != BSP_BF16) || bsp_cache_page_bytes(block, kv_heads, D, bits) <= 0) return BSP_ERR_UNSUPPORTED;
   if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(pages)) & 15) || (reinterpret_cast<uintptr_t>(o) & 3) || q_stride_b % 8 || q_stride_h % 8 || o_stride_b % 2 || o_stride_h % 2) return BSP_ERR_ARG;
-  if (!(scale - scale == 0.f) || !(softcap >= 0.f) || !(softcap - softcap == 0.f) || (rows && n_rows <= 0)) return BSP_ERR_ARG;
+  if (!(scale - scale == 0.f) || !(softcap >= 0.f) || !(softcap - softcap == 0.f) || (rows && n_rows <= 0) || most_blocks <= 0) return BSP_ERR_ARG;
   if ((int64_t)width * block >= ((int64_t)1 << 24) || (int64_t)n_pages * block >= ((int64_t)1 << 31) || (rows && n_rows > 65536)) return BSP_ERR_UNSUPPORTED;
   const int64_t need = bsp_cache_attention_workspace_bytes(B, H, kv_heads, D, splits);
   if (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < need)) return BSP_ERR_CAPACITY;
@@ -426,6 +468,8 @@ extern "C" int bsp_cache_attention(int dtype, const void *q, int64_t q_stride_b,
   a.rows = rows; a.n_rows = n_rows; a.slopes = slopes; a.scale = scale; a.cap = softcap;
   a.partial = reinterpret_cast<float *>(workspace);
   a.B = B; a.H = H; a.kv_heads = kv_heads; a.block = block; a.splits = splits;
+  const int64_t pairs = (most_blocks * block + 31) / 32;
+  a.chunk = (int)((pairs + 4 * splits - 1) / (4 * splits));
   a.tile_shift = block == 16 ? 0 : block == 32 ? 1 : block == 64 ? 2 : 3;
   const hipStream_t st = as_stream(stream);
   if (bits == 4) return D == 64 ? launch_decode<4, 64>(a, dtype, st) : launch_decode<4, 128>(a, dtype, st);

@@ -101,7 +101,7 @@ SIGNATURES = {
     'bsp_cache_read': (_i, [_i, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _i, _vp]),
     'bsp_cache_attention_splits': (_i, [_i, _i, _i, _i, _i64]),
     'bsp_cache_attention_workspace_bytes': (_i64, [_i] * 5),
-    'bsp_cache_attention': (_i, [_i, _vp, _i64, _i64, _vp, _i64, _i64, _i, _i, _vp, _i, _i, _i, _i, _i, _vp, _i64, _i, _vp, _vp, _i, _f, _f, _vp, _vp, _i64, _i, _vp]),
+    'bsp_cache_attention': (_i, [_i, _vp, _i64, _i64, _vp, _i64, _i64, _i, _i, _vp, _i, _i, _i, _i, _i, _vp, _i64, _i, _vp, _vp, _i, _i64, _f, _f, _vp, _vp, _i64, _i, _vp]),
     'bsp_layout_fixed': (_i, [_vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp]),
     'bsp_layout_sparse_transformer': (_i, [_vp, _i, _i, _i, _i, _i, _vp]),
     'bsp_layout_bigbird': (_i, [_vp, _i, _i, _i, _i, _i, _vp, _i, _vp]),

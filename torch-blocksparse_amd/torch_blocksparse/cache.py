@@ -191,7 +191,7 @@ class CacheAttention:
             workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
             rc = lib.bsp_cache_attention(_lib.DTYPES[q.dtype], q.data_ptr(), q.stride(0) if B > 1 else 0, q.stride(1) if H > 1 else 0, o.data_ptr(), H * D, D, B, H,
                                          cache.data.data_ptr(), cache.pages, self.block, cache.heads, D, cache.bits, table.data_ptr(), table.stride(0) if B > 1 else 0,
-                                         table.size(1), lengths.data_ptr(), _lib.ptr(rows), n_rows, scale, softcap, _lib.ptr(slopes), _lib.ptr(workspace), need, splits,
+                                         table.size(1), lengths.data_ptr(), _lib.ptr(rows), n_rows, blocks, scale, softcap, _lib.ptr(slopes), _lib.ptr(workspace), need, splits,
                                          _lib.stream_ptr(q.device))
             _lib.check(rc, 'bsp_cache_attention')
         return o
