@@ -5,8 +5,11 @@
 // reads back as NaN.  The codes are those of exact arithmetic: a quotient is computed in fp32 and, where that lies close to the middle of two
 // integers, decided in 64 bits.
 //
-// Both kernels move each byte once (16384 positions of 16 heads of 64, fp16, 8 bits: 67 MB in, 38 MB out).  A thread has a
-// chunk of eight elements: 16 bytes in 16-bit types, and the four threads of a group agree on its range by two exchanges within the quad.
+// Both kernels move each byte once and are bound by that.  A thread has a chunk of eight elements: 16 bytes in 16-bit types, and the four
+// threads of a group agree on its range by two exchanges within the quad.  Measured, 16384 positions of 16 heads of 64, fp16, 8 bits (67 MB and 38 MB): written
+// in 26 us, 2.4 of them before to see which position of a slot counts, read in 17; 32750 of 8 heads of 128, bf16, 4 bits (176 MB) read in 38.
+// Writing was bound by its operations before the rounded quotient was taken from the low bits of one sum (33 us); reading by the
+// divisions that found a thread's place (20 and 42 us).
 #include "cache.h"
 
 namespace bsp {
@@ -19,7 +22,7 @@ struct CacheArgs {
   int32_t *owner;
   unsigned char *pages;
   int64_t capacity;                // positions of the cache
-  int T, heads, block;
+  int T, heads, block, block_shift;
 };
 
 namespace {
@@ -71,25 +74,30 @@ template <typename T, int BITS, int D, bool SCAN> __global__ void __launch_bound
     if (last != t + 1) return;
     if (tid == 0) a.owner[slot] = 0;                    // (another position of the slot that looks from now on finds 0: not the last either)
   }
-  const int page = slot / a.block, at = slot % a.block, n = 2 * a.heads * CHUNKS;
-  for (int i = tid; i < n; i += 256) {
-    const int j = i % CHUNKS, head = i / CHUNKS % a.heads, value = i / (CHUNKS * a.heads), g = j >> 2, c = j & 3;
+  const int page = slot >> a.block_shift, at = slot & (a.block - 1);
+  const int j = tid % CHUNKS, g = j >> 2, c = j & 3;
+  for (int m = tid / CHUNKS; m < 2 * a.heads; m += 256 / CHUNKS) {
+    const int value = m >= a.heads, head = value ? m - a.heads : m;
     float x[8];
     load8<T>(x, (value ? reinterpret_cast<const T *>(a.v) + t * a.v_st + head * a.v_sh : reinterpret_cast<const T *>(a.k) + t * a.k_st + head * a.k_sh) + 8 * j);
-    float lo = INFINITY, hi = -INFINITY, bad = 0.f;
+    // the group's range, into that of fp16 here: elements outside get the codes of its ends below
+    bool nan = false;
+    float lo = x[0], hi = x[0];
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      bad = x[e] != x[e] ? 1.f : bad;
-      x[e] = fminf(fmaxf(x[e], -65504.f), 65504.f);
-      lo = fminf(lo, x[e]);
-      hi = fmaxf(hi, x[e]);
+    for (int e = 0; e < 8; e += 2) {
+      nan |= __builtin_isunordered(x[e], x[e + 1]);
+      lo = fminf(fminf(lo, x[e]), x[e + 1]);
+      hi = fmaxf(fmaxf(hi, x[e]), x[e + 1]);
     }
+    float bad = nan ? 1.f : 0.f;
     lo = fminf(lo, quad1(lo));
     hi = fmaxf(hi, quad1(hi));
     bad = fmaxf(bad, quad1(bad));
     lo = fminf(lo, quad2(lo));
     hi = fmaxf(hi, quad2(hi));
     bad = fmaxf(bad, quad2(bad));
+    lo = fminf(fmaxf(lo, -65504.f), 65504.f);
+    hi = fminf(fmaxf(hi, -65504.f), 65504.f);
     constexpr int MOST = (1 << BITS) - 1;
     f16 least = (f16)lo, step;
     {
@@ -98,79 +106,83 @@ template <typename T, int BITS, int D, bool SCAN> __global__ void __launch_bound
       step = (f16)((double)r == range ? r / (float)MOST : (float)(range / (double)MOST));   // (the same number: both quotients are rounded to the nearest)
     }
     if (bad != 0.f) least = __builtin_bit_cast(f16, (uint16_t)0x7e00), step = (f16)0.f;
-    const float l32 = (float)least, s32 = (float)step, inv = s32 > 0.f ? 1.f / s32 : 0.f;
-    uint32_t code[8];
-    bool close = false;
-    float q[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      q[e] = bad != 0.f ? 0.f : (x[e] - l32) * inv;
-      const float n0 = __builtin_rintf(q[e]);
-      close |= fabsf(q[e] - n0) > 0.5f - 2e-4f;          // (the quotient is off by 3 * 2^-24 of itself at most, 5e-5 at 255)
-      code[e] = (uint32_t)(int)fminf(fmaxf(n0, 0.f), (float)MOST);
-    }
-    if (close && s32 > 0.f) {
-      const double h = 0.5 * (double)s32;
+    const float l32 = (float)least, s32 = (float)step;
+    uint32_t w[2] = {0u, 0u};
+    if (s32 > 0.f) {
+      // the quotient rounded in the low bits of 1.5 * 2^23 + it
+      const float inv = __builtin_amdgcn_rcpf(s32), magic = 12582912.f;
+      uint32_t code[8];
+      float off = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        const float n0 = __builtin_rintf(q[e]);
-        const double rem = ((double)x[e] - (double)l32) - (double)n0 * (double)s32;
-        const bool odd = (int)n0 & 1;
-        const int m = (int)n0 + (rem > h || (rem == h && odd) ? 1 : 0) - (rem < -h || (rem == -h && odd) ? 1 : 0);
-        code[e] = (uint32_t)(m < 0 ? 0 : m > MOST ? MOST : m);
+        const float d = x[e] - l32, r = fmaf(d, inv, magic);
+        off = fmaxf(off, fabsf(fmaf(d, inv, magic - r)));
+        code[e] = __builtin_bit_cast(uint32_t, fminf(fmaxf(r, magic), magic + (float)MOST));
+      }
+      // x - least is off by 2^-24 of itself, the reciprocal by 2^-23, so the quotient by 3 * 2^-24 * MOST: decided in 64 bits where the middle is as near
+      if (off > 0.5f - MOST * 0x1p-22f) {
+        const double h = 0.5 * (double)s32;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const int n0 = (int)(code[e] & 0x1ffu);
+          const double rem = ((double)x[e] - (double)l32) - (double)n0 * (double)s32;
+          const bool odd = n0 & 1;
+          const int m = n0 + (rem > h || (rem == h && odd) ? 1 : 0) - (rem < -h || (rem == -h && odd) ? 1 : 0);
+          code[e] = (uint32_t)(m < 0 ? 0 : m > MOST ? MOST : m);
+        }
+      }
+      if constexpr (BITS == 4) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) w[0] |= (code[e] & 15u) << (4 * (e >> 1) + 16 * (e & 1));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+          w[e] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(code[4 * e + 3], code[4 * e + 2], 0x0c0c0400u), __builtin_amdgcn_perm(code[4 * e + 1], code[4 * e], 0x0c0c0400u), 0x05040100u);
       }
     }
     unsigned char *base = a.pages + ((int64_t)page * a.heads + head) * P::bytes(a.block);
     unsigned char *to = base + P::codes(a.block, value) + at * P::ROW + P::chunk(c, g);
-    if constexpr (BITS == 4) {
-      uint32_t w = 0;
-#pragma unroll
-      for (int e = 0; e < 8; e++) w |= code[e] << (4 * (e >> 1) + 16 * (e & 1));
-      *reinterpret_cast<uint32_t *>(to) = w;
-    } else {
-      *reinterpret_cast<u32x2 *>(to) = u32x2{code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24, code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24};
-    }
+    if constexpr (BITS == 4) *reinterpret_cast<uint32_t *>(to) = w[0];
+    else *reinterpret_cast<u32x2 *>(to) = u32x2{w[0], w[1]};
     if (c == 0)
       *reinterpret_cast<uint32_t *>(base + P::meta(a.block, value) + at * P::META + 4 * g) =
           (uint32_t)__builtin_bit_cast(uint16_t, step) | (uint32_t)__builtin_bit_cast(uint16_t, least) << 16;
   }
 }
 
-// A thread has a chunk of one position.  Slots outside the cache read as zeros.
+// A workgroup per position, a chunk a thread.  Slots outside the cache read as zeros.
 template <typename T, int BITS, int D> __global__ void __launch_bounds__(256) k_cache_read(CacheArgs a) {
   typedef Page<BITS, D> P;
   constexpr int CHUNKS = D / 8;
-  const int64_t n = (int64_t)a.T * 2 * a.heads * CHUNKS, i = xcd_remap(blockIdx.x, gridDim.x) * 256 + threadIdx.x;
-  if (i >= n) return;
-  const int j = (int)(i % CHUNKS);
-  const int64_t rest = i / CHUNKS;
-  const int head = (int)(rest % a.heads), value = (int)(rest / a.heads % 2), t = (int)(rest / a.heads / 2), g = j >> 2, c = j & 3;
-  const int slot = a.slots[t];
-  float x[8];
-  if (slot < 0 || slot >= a.capacity) {
+  const int t = (int)xcd_remap(blockIdx.x, a.T), tid = threadIdx.x;
+  const int slot = as_table(a.slots)[t];
+  const bool here = slot >= 0 && slot < a.capacity;
+  const int page = here ? slot >> a.block_shift : 0, at = here ? slot & (a.block - 1) : 0;
+  const int j = tid % CHUNKS, g = j >> 2, c = j & 3;
+  for (int m = tid / CHUNKS; m < 2 * a.heads; m += 256 / CHUNKS) {
+    const int value = m >= a.heads, head = value ? m - a.heads : m;
+    float x[8] = {};
+    if (here) {
+      const unsigned char *base = a.pages + ((int64_t)page * a.heads + head) * P::bytes(a.block);
+      const uint32_t *from = reinterpret_cast<const uint32_t *>(base + P::codes(a.block, value) + at * P::ROW + P::chunk(c, g));
+      const uint32_t meta = *reinterpret_cast<const uint32_t *>(base + P::meta(a.block, value) + at * P::META + 4 * g);
+      const float step = (float)__builtin_bit_cast(f16, (uint16_t)meta), least = (float)__builtin_bit_cast(f16, (uint16_t)(meta >> 16));
+      uint32_t w[2] = {from[0], BITS == 8 ? from[BITS == 8 ? 1 : 0] : 0u};
+      f16x2 p[4];
+      chunk_codes<BITS>(w, p);
 #pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = 0.f;
-  } else {
-    const int page = slot / a.block, at = slot % a.block;
-    const unsigned char *base = a.pages + ((int64_t)page * a.heads + head) * P::bytes(a.block);
-    const uint32_t *from = reinterpret_cast<const uint32_t *>(base + P::codes(a.block, value) + at * P::ROW + P::chunk(c, g));
-    const uint32_t meta = *reinterpret_cast<const uint32_t *>(base + P::meta(a.block, value) + at * P::META + 4 * g);
-    const float step = (float)__builtin_bit_cast(f16, (uint16_t)meta), least = (float)__builtin_bit_cast(f16, (uint16_t)(meta >> 16));
-    uint32_t w[2] = {from[0], BITS == 8 ? from[BITS == 8 ? 1 : 0] : 0u};
-    f16x2 p[4];
-    chunk_codes<BITS>(w, p);
+      for (int e = 0; e < 8; e++) x[e] = fmaf((float)p[e >> 1][e & 1], step, least);
+    }
+    T *to = reinterpret_cast<T *>(value ? a.vo : a.ko) + ((int64_t)t * a.heads + head) * D + 8 * j;
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<f32x4 *>(to) = f32x4{x[0], x[1], x[2], x[3]};
+      *reinterpret_cast<f32x4 *>(to + 4) = f32x4{x[4], x[5], x[6], x[7]};
+    } else {
+      union { u32x4 raw; T e[8]; } u;
 #pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = fmaf((float)p[e >> 1][e & 1], step, least);
-  }
-  T *to = reinterpret_cast<T *>(value ? a.vo : a.ko) + ((int64_t)t * a.heads + head) * D + 8 * j;
-  if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<f32x4 *>(to) = f32x4{x[0], x[1], x[2], x[3]};
-    *reinterpret_cast<f32x4 *>(to + 4) = f32x4{x[4], x[5], x[6], x[7]};
-  } else {
-    union { u32x4 raw; T e[8]; } u;
-#pragma unroll
-    for (int e = 0; e < 8; e++) u.e[e] = from_float<T>(x[e]);
-    *reinterpret_cast<u32x4 *>(to) = u.raw;
+      for (int e = 0; e < 8; e++) u.e[e] = from_float<T>(x[e]);
+      *reinterpret_cast<u32x4 *>(to) = u.raw;
+    }
   }
 }
 
@@ -179,7 +191,7 @@ constexpr int kScan = 512;
 
 template <typename T, int BITS, int D> int launch_cache(const CacheArgs &a, bool write, hipStream_t st) {
   if (!write) {
-    hipLaunchKernelGGL((k_cache_read<T, BITS, D>), dim3((unsigned)cdiv((int64_t)a.T * 2 * a.heads * (D / 8), 256)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((k_cache_read<T, BITS, D>), dim3((unsigned)a.T), dim3(256), 0, st, a);
   } else if (a.T <= kScan) {
     hipLaunchKernelGGL((k_cache_write<T, BITS, D, true>), dim3((unsigned)a.T), dim3(256), 0, st, a);
   } else {
@@ -204,7 +216,7 @@ int cache_args(int dtype, const void *pages, int n_pages, int block, int heads, 
   a = CacheArgs{};
   a.pages = reinterpret_cast<unsigned char *>(const_cast<void *>(pages));
   a.capacity = (int64_t)n_pages * block;
-  a.block = block; a.heads = heads; a.slots = slots; a.T = T;
+  a.block = block; a.block_shift = __builtin_ctz(block); a.heads = heads; a.slots = slots; a.T = T;
   return BSP_OK;
 }
 
