@@ -6,6 +6,9 @@ Differences from the reference, all deliberate: the per-sequence-length operator
 configuration instead of the sequence length alone (deepspeedsparseselfattention.py:67-106 shares operators
 between modules with different layouts), and a key given as [..., head_dim, seq] is made contiguous after it is
 transposed back (:119-123 hands a strided view to kernels that assume a unit inner stride).
+
+Beyond the reference, `forward` takes score rules (`Attention`): a cap, a bias by distance, documents, a causal order with a prefix, keys and values
+of fewer heads; and `decode` answers for one new position a sequence from a `KeyValueCache` over the same layout.
 """
 import collections
 
@@ -13,8 +16,10 @@ import torch
 import torch.nn as nn
 
 from .attention_core import attention_chain
+from .cache import CacheAttention
 from .layouts import fixed_layout
 from .matmul import MatMul
+from .rules import Attention
 from .softmax import Softmax
 
 
@@ -68,6 +73,31 @@ class DeepSpeedSparseSelfAttention(nn.Module):
             cache.popitem(last=False)
         return cache[key]
 
+    # Operators with rules and of decoding that a captured graph has in it: its replays use their tables, so these stay.
+    captured = dict()
+
+    def _kept(self, kind, H, num_blocks, make):
+        """the operator `make` makes of the configuration's layout for so many blocks of any number, kept among `ops`"""
+        cfg = self.sparsity_config
+        key = (kind, H, num_blocks) + cfg.key()
+        cache = DeepSpeedSparseSelfAttention.ops
+        if key not in cache:
+            if key in DeepSpeedSparseSelfAttention.captured:
+                cache[key] = DeepSpeedSparseSelfAttention.captured[key]
+            else:
+                block_stride = cfg.stride // cfg.block
+                if block_stride != cfg.stride / cfg.block:
+                    raise ValueError('Stride %d must be dividable by block size %d' % (cfg.stride, cfg.block))
+                whole = -(-num_blocks // block_stride) * block_stride        # the layout is made of whole windows
+                layout = DeepSpeedSparseSelfAttention._make_layout(H, whole, cfg.mode, block_stride, cfg.attention, cfg.numverts, cfg.vertsize)
+                cache[key] = make(layout[:, :num_blocks, :num_blocks].to(torch.uint8))
+        cache.move_to_end(key)
+        while len(cache) > DeepSpeedSparseSelfAttention.OPS_CACHE_SIZE:
+            cache.popitem(last=False)
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            DeepSpeedSparseSelfAttention.captured[key] = cache[key]
+        return cache[key]
+
     def __init__(self, sparsity_config=SparsityConfig(), key_padding_mask_mode='add', attn_mask_mode='mul'):
         super().__init__()
         self.sparsity_config = sparsity_config
@@ -88,7 +118,20 @@ class DeepSpeedSparseSelfAttention(nn.Module):
             return x
         return x.squeeze()
 
-    def forward(self, query, key, value, rpe=None, key_padding_mask=None, attn_mask=None):
+    def forward(self, query, key, value, rpe=None, key_padding_mask=None, attn_mask=None, *, softcap=0., slopes=None, causal=False,
+                documents=None, prefix=None):
+        """Attention over the configuration's layout, scores scaled by head_dim ** -0.5.  With one of softcap, slopes, causal, documents and prefix, or with
+        keys and values of fewer heads than the query, it is that of `Attention` with these rules: any length, and no rpe or masks beside them."""
+        fewer_heads = query.dim() == key.dim() == 4 and key.size(1) < query.size(1)
+        if softcap or slopes is not None or causal or documents is not None or prefix is not None or fewer_heads:
+            if rpe is not None or key_padding_mask is not None or attn_mask is not None:
+                raise ValueError('softcap, slopes, causal, documents, prefix and shared key heads do not go with rpe, key_padding_mask and attn_mask')
+            if query.dim() != 4 or key.dim() != 4:
+                raise ValueError('query and key must have shape [batch, heads, length, head_dim]')
+            key = self.transpose_key_for_scores(key, query.size(2))
+            block = self.sparsity_config.block
+            op = self._kept('rules', query.size(1), -(-query.size(2) // block), lambda layout: Attention(layout, block))
+            return op(query, key, value, scale=float(query.size(3)) ** -0.5, softcap=softcap, slopes=slopes, causal=causal, documents=documents, prefix=prefix)
         bsz, num_heads, tgt_len, head_dim = query.size()
         key = self.transpose_key_for_scores(key, tgt_len)
         if query.shape != key.shape or key.shape != value.shape:
@@ -103,6 +146,16 @@ class DeepSpeedSparseSelfAttention(nn.Module):
         return attention_chain(sdd_nt, softmax, dsd_nn, query, key, value, scale=scaling, rpe=rpe,
                                key_padding_mask=key_padding_mask, attn_mask=attn_mask,
                                key_padding_mask_mode=self.key_padding_mask_mode, attn_mask_mode=self.attn_mask_mode)
+
+    def decode(self, query, cache, table, lengths, *, softcap=0., slopes=None):
+        """One new position a sequence: query [batch, heads, head_dim] over the pages `table` [batch, width] of `cache`, which hold `lengths` [batch]
+        positions of each sequence, the new one among them (`CacheAttention`).  It is what `forward` with causal=True and the same softcap and slopes gives
+        for each sequence's last position, over keys and values as the cache holds them."""
+        if query.dim() != 3 or table.dim() != 2:
+            raise ValueError('query must have shape [batch, heads, head_dim], table [batch, width]')
+        cfg = self.sparsity_config
+        op = self._kept('decode', query.size(1), table.size(1), lambda layout: CacheAttention(cfg.block, None if cfg.mode == 'dense' else layout))
+        return op(query, cache, table, lengths, scale=float(query.size(2)) ** -0.5, softcap=softcap, slopes=slopes)
 
 
 SparseSelfAttention = DeepSpeedSparseSelfAttention
