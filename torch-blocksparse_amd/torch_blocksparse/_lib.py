@@ -168,6 +168,11 @@ def stream_ptr(device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def raw_stream(device):
+    """the handle of the current stream of a tensor's device, as a number"""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 class _Nothing:
     def __enter__(self):
         return None

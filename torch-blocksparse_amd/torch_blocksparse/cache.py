@@ -72,7 +72,7 @@ class KeyValueCache:
             return
         with _lib.on_device(self.device):
             rc = _lib.load().bsp_cache_write(_lib.DTYPES[k.dtype], self.data.data_ptr(), self.pages, self.block, self.heads, self.head_dim, self.bits, k.data_ptr(), k_st, k_sh,
-                                             v.data_ptr(), v_st, v_sh, slots.data_ptr(), T, self._owner.data_ptr(), _lib.stream_ptr(self.device))
+                                             v.data_ptr(), v_st, v_sh, slots.data_ptr(), T, self._owner.data_ptr(), _lib.raw_stream(self.device))
         _lib.check(rc, 'bsp_cache_write')
 
     def read(self, slots, dtype=torch.float16):
@@ -84,7 +84,7 @@ class KeyValueCache:
         if slots.numel():
             with _lib.on_device(self.device):
                 rc = _lib.load().bsp_cache_read(_lib.DTYPES[dtype], self.data.data_ptr(), self.pages, self.block, self.heads, self.head_dim, self.bits, k.data_ptr(),
-                                                v.data_ptr(), slots.data_ptr(), slots.numel(), _lib.stream_ptr(self.device))
+                                                v.data_ptr(), slots.data_ptr(), slots.numel(), _lib.raw_stream(self.device))
             _lib.check(rc, 'bsp_cache_read')
         return k, v
 
@@ -191,7 +191,8 @@ class CacheAttention:
             workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
             rc = lib.bsp_cache_attention(_lib.DTYPES[q.dtype], q.data_ptr(), q.stride(0) if B > 1 else 0, q.stride(1) if H > 1 else 0, o.data_ptr(), H * D, D, B, H,
                                          cache.data.data_ptr(), cache.pages, self.block, cache.heads, D, cache.bits, table.data_ptr(), table.stride(0) if B > 1 else 0,
-                                         table.size(1), lengths.data_ptr(), _lib.ptr(rows), n_rows, blocks, scale, softcap, _lib.ptr(slopes), _lib.ptr(workspace), need, splits,
-                                         _lib.stream_ptr(q.device))
+                                         table.size(1), lengths.data_ptr(), rows.data_ptr() if rows is not None else None, n_rows, blocks, scale, softcap,
+                                         slopes.data_ptr() if slopes is not None else None, workspace.data_ptr() if need else None, need, splits,
+                                         _lib.raw_stream(q.device))
             _lib.check(rc, 'bsp_cache_attention')
         return o

@@ -18,6 +18,7 @@ bsp_attention_rules_bwd).  The results of a call are the same bits every time.
 """
 import ctypes
 import math
+import struct
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -25,27 +26,28 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 
 
-class _Call(ctypes.Structure):             # bsp_attention_rules_call
-    _fields_ = ([(n, ctypes.c_int) for n in ('dtype', 'Z', 'H', 'kv_heads', 'lines', 'D')] + [('length', ctypes.c_int64), ('strides', ctypes.c_int64 * 24)]
-                + [(n, ctypes.c_float) for n in ('scale', 'softcap')] + [('causal', ctypes.c_int), ('slopes', ctypes.c_void_p), ('documents', ctypes.c_void_p),
-                   ('documents_stride', ctypes.c_int64), ('prefix', ctypes.c_void_p), ('ranges', ctypes.c_void_p), ('d_rows', ctypes.c_void_p), ('stats', ctypes.c_void_p), ('o_rest', ctypes.c_void_p)])
+# bsp_attention_rules_call: dtype, Z, H, kv_heads, lines, D; length, strides[24]; scale, softcap, causal; slopes, documents, documents_stride, prefix, ranges, d_rows, stats, o_rest
+_CALL = struct.Struct('@6i25q2fiPPqPPPPP')
 
 
-def _strides(t):
-    """batch, head and row stride; those that no address depends on as the kernels want them"""
-    z, h, row, _ = t.stride()
-    return (z if t.size(0) > 1 else 0, h if t.size(1) > 1 else 0, row if t.size(2) > 1 else t.size(3))
+def _operand(t, Z, heads, L, D):
+    """(t, or a copy of it where the kernels could not address t: unit inner stride, 16-byte vectors, rows that do not overlap and lie within 4 GiB of a
+    head's first; its batch, head and row stride, those that no address depends on as the kernels want them)"""
+    z, h, row, one = t.stride()
+    z, h, row = z if Z > 1 else 0, h if heads > 1 else 0, row if L > 1 else D
+    size = t.element_size()
+    if one == 1 and not (z | h | row) * size % 16 and row >= D and not t.data_ptr() % 16 and row * (L + 64) * size < 1 << 32:
+        return t, (z, h, row)
+    return t.clone(memory_format=torch.contiguous_format), _own(Z, heads, L, D)
 
 
-def _addressable(t):
-    """t, or a copy of it where the kernels could not address t: unit inner stride, 16-byte vectors, rows that do not overlap and lie
-    within 4 GiB of a head's first"""
-    z, h, row = _strides(t)
-    unit = 16 // t.element_size()
-    if (t.stride(3) == 1 and not (z | h | row) % unit and row >= t.size(3) and not t.data_ptr() % 16
-            and row * (t.size(2) + 64) * t.element_size() < 2 ** 32):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+def _own(Z, heads, L, D):
+    """the strides of a contiguous tensor"""
+    return (heads * L * D if Z > 1 else 0, L * D if heads > 1 else 0, D)
+
+
+def _at(t):
+    return 0 if t is None else t.data_ptr()
 
 
 class _Tables:
@@ -147,28 +149,28 @@ class _rules(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, tables, scale, softcap, slopes, causal, documents, prefix, grad_enabled):
-        lib = _lib.load()
-        q, k, v = _addressable(q), _addressable(k), _addressable(v)
         Z, H, L, D = q.shape
+        kv, device = k.size(1), q.device
+        (q, q_at), (k, k_at), (v, v_at) = _operand(q, Z, H, L, D), _operand(k, Z, kv, L, D), _operand(v, Z, kv, L, D)
         keep = grad_enabled and any(ctx.needs_input_grad[:3])
-        o = torch.empty((Z, H, L, D), dtype=q.dtype, device=q.device)
-        stats = torch.empty((Z, H, 2, 64 * tables.lines), dtype=torch.float32, device=q.device) if keep else None
-        rest = torch.empty((Z, H, L, D), dtype=q.dtype, device=q.device) if keep and q.element_size() == 2 else None
-        ranges = torch.empty((Z, (L + 15) // 16, 2), dtype=torch.int32, device=q.device) if documents is not None else None
-        call = _rules.call(q, k, v, o, tables, scale, softcap, slopes, causal, documents, prefix, ranges, stats, rest)
-        _lib.check(lib.bsp_attention_rules_fwd(ctypes.byref(call), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _lib.stream_ptr(q.device)), 'bsp_attention_rules_fwd')
+        o = torch.empty((Z, H, L, D), dtype=q.dtype, device=device)
+        stats = torch.empty((Z, H, 2, 64 * tables.lines), dtype=torch.float32, device=device) if keep else None
+        rest = torch.empty((Z, H, L, D), dtype=q.dtype, device=device) if keep and q.element_size() == 2 else None
+        ranges = torch.empty((Z, (L + 15) // 16, 2), dtype=torch.int32, device=device) if documents is not None else None
+        call = _rules.call(q, kv, q_at + k_at + v_at + _own(Z, H, L, D) + (0,) * 12, tables, scale, softcap, slopes, causal, documents, prefix, ranges, stats, rest)
+        rc = _lib.load().bsp_attention_rules_fwd(call, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _lib.raw_stream(device))
+        if rc:
+            _lib.check(rc, 'bsp_attention_rules_fwd')
         if keep:
             ctx.save_for_backward(q, k, v, o, rest, stats, ranges, slopes, documents, prefix)
             ctx.tables, ctx.numbers = tables, (scale, softcap, causal)
         return o
 
     @staticmethod
-    def call(q, k, v, o, tables, scale, softcap, slopes, causal, documents, prefix, ranges, stats, rest, grads=()):
+    def call(q, kv, strides, tables, scale, softcap, slopes, causal, documents, prefix, ranges, stats, rest):
         Z, H, L, D = q.shape
-        strides = [s for t in (q, k, v, o) + tuple(grads) for s in (_strides(t) if t is not None else (0, 0, 0))]
-        p = lambda t: None if t is None else t.data_ptr()   # noqa: E731
-        return _Call(_lib.DTYPES[q.dtype], Z, H, k.size(1), tables.lines, D, L, (ctypes.c_int64 * 24)(*strides), scale, softcap, int(causal), p(slopes), p(documents),
-                     documents.stride(0) if documents is not None and Z > 1 else 0, p(prefix), p(ranges), tables.rows.data_ptr(), p(stats), p(rest))
+        return _CALL.pack(_lib.DTYPES[q.dtype], Z, H, kv, tables.lines, D, L, *strides, scale, softcap, causal, _at(slopes), _at(documents),
+                          documents.stride(0) if documents is not None and Z > 1 else 0, _at(prefix), _at(ranges), tables.rows.data_ptr(), _at(stats), _at(rest))
 
     @staticmethod
     @once_differentiable
@@ -176,22 +178,27 @@ class _rules(torch.autograd.Function):
         q, k, v, o, rest, stats, ranges, slopes, documents, prefix = ctx.saved_tensors
         tables, (scale, softcap, causal) = ctx.tables, ctx.numbers
         need_q, need_k, need_v = ctx.needs_input_grad[:3]
-        with _lib.on_device(q.device):
-            do = _addressable(do)
+        device, dtype = q.device, q.dtype
+        with _lib.on_device(device):
             Z, H, L, D = q.shape
-            new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)   # noqa: E731
-            dq, dk, dv = new(q), None, None
-            delta = torch.empty((Z, H, 64 * tables.lines), dtype=torch.float32, device=q.device)
+            kv = k.size(1)
+            # (what was saved may have been elsewhere in between and have come back in other strides)
+            (q, q_at), (k, k_at), (v, v_at) = _operand(q, Z, H, L, D), _operand(k, Z, kv, L, D), _operand(v, Z, kv, L, D)
+            (o, o_at), (do, do_at) = _operand(o, Z, H, L, D), _operand(do, Z, H, L, D)
+            dq, dk, dv = torch.empty((Z, H, L, D), dtype=dtype, device=device), None, None
+            delta = torch.empty((Z, H, 64 * tables.lines), dtype=torch.float32, device=device)
             items, n_items, splits, n_splits, slots, partial = None, 0, None, 0, 0, None
             if need_k or need_v:
-                dk, dv = new(k), new(v)
-                items, n_items, splits, n_splits, slots = tables.columns(k.size(1), Z)
-                partial = torch.empty((Z, slots, 2, 64, D), dtype=torch.float32, device=q.device) if slots else None
-            call = _rules.call(q, k, v, o, tables, scale, softcap, slopes, causal, documents, prefix, ranges, stats, rest, (do, dq, dk, dv))
-            p = _lib.ptr
-            _lib.check(_lib.load().bsp_attention_rules_bwd(ctypes.byref(call), p(do), p(q), p(k), p(v), p(o), p(dq), p(dk), p(dv), p(delta), p(items), n_items,
-                                                           p(partial), slots, p(splits), n_splits, _lib.stream_ptr(q.device)), 'bsp_attention_rules_bwd')
-        return (dq if need_q else None, dk if need_k else None, dv if need_v else None) + (None,) * 8
+                dk, dv = torch.empty((Z, kv, L, D), dtype=dtype, device=device), torch.empty((Z, kv, L, D), dtype=dtype, device=device)
+                items, n_items, splits, n_splits, slots = tables.columns(kv, Z)
+                partial = torch.empty((Z, slots, 2, 64, D), dtype=torch.float32, device=device) if slots else None
+            own = _own(Z, kv, L, D)
+            call = _rules.call(q, kv, q_at + k_at + v_at + o_at + do_at + _own(Z, H, L, D) + own + own, tables, scale, softcap, slopes, causal, documents, prefix, ranges, stats, rest)
+            rc = _lib.load().bsp_attention_rules_bwd(call, do.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), dq.data_ptr(), _at(dk), _at(dv), delta.data_ptr(),
+                                                     _at(items), n_items, _at(partial), slots, _at(splits), n_splits, _lib.raw_stream(device))
+            if rc:
+                _lib.check(rc, 'bsp_attention_rules_bwd')
+        return dq if need_q else None, dk if need_k else None, dv if need_v else None, None, None, None, None, None, None, None, None
 
 
 class Attention:
