@@ -291,3 +291,25 @@ def test_far_positions():
     dv = p.t() @ do[0, 0, rows].double().cpu()
     assert bool(((got[3][0, 0, keys].double().cpu() - dv).abs() <= 8e-5 * (p.t() @ do[0, 0, rows].double().cpu().abs())).all())
     assert not bool(got[0][0, 0, :first].any())
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('name', ['causal', 'all'])
+def test_a_launch_of_few_lines_and_one_of_many(dtype, D, name):
+    """Few lines have two pairs of wavefronts each, many one: the same sequence alone and 120 times over."""
+    H, kv, L, block, times = 4, 2, 300, 32, 120
+    lay = random_layout((H, 10, 10), 0.6, 9)
+    lay[:, 3] = 0                                        # rows that see nothing, and a line of an odd number of halves
+    op = tb.Attention(lay, block)
+    q, k, v, do = inputs(1, H, kv, L, D, dtype, 21)
+    rules = dict(rules_of(name, 1, H, L), scale=D ** -0.5)
+    compare(op, lay, block, q, k, v, do, 'few %s %d %s' % (name, D, dtype), **rules)
+    want = rules_oracle.attention(q, k, v, lay, block, do, **rules)
+    many = {n: t.expand(times, *t.shape[1:]).contiguous() if n in ('documents', 'prefix') else t for n, t in rules.items()}
+    got = run(op, *[t.expand(times, -1, -1, -1).contiguous() for t in (q, k, v, do)], **many)
+    for z in (0, 57, times - 1):
+        for g, n in zip(got, ('o', 'dq', 'dk', 'dv')):
+            rules_oracle.check(g[z:z + 1], want[n], 'many %s' % n)
+    for g in got:
+        assert torch.equal(g[:1].expand_as(g), g)

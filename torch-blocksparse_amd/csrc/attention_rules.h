@@ -477,6 +477,21 @@ template <typename T, int D> constexpr int rules_lds() {
   return ring > out ? ring : out;
 }
 
+// A launch of few lines has two pairs of wavefronts to a line, each of which takes every other half of a tile, with a ring of its own; at the end the second
+// pair's sums are added to the first's through its ring.
+template <typename T, int D, int PAIRS> constexpr int pair_lds() {
+  constexpr int sums = 2 * 64 * 4 * (D / 2 + 2);        // two wavefronts' accumulators, maxima and sums
+  return PAIRS == 1 || rules_lds<T, D>() > sums ? rules_lds<T, D>() : sums;
+}
+// The halves of the pair of wavefronts `group`; more: some pair has one; pads: one of them has padding
+struct Halves { Half own; bool more, pads; };
+template <int PAIRS, class F> __device__ __forceinline__ Halves next_halves(int group, F &&next) {
+  const Half a = next();
+  if constexpr (PAIRS == 1) return Halves{a, a.n >= 0, a.pad};
+  const Half b = a.n >= 0 ? next() : a;
+  return Halves{group ? b : a, a.n >= 0, a.pad || b.pad};
+}
+
 // Which of n work items of which of `units` heads (all of equal cost, item 0 the longest) a workgroup does.  Workgroups go round the eight
 // XCDs, each with an L2 of its own: the heads are dealt to the XCDs whole, so that a head's k and v are fetched into one L2, four heads at a
 // time, their longest items first.  Heads past a multiple of eight go first, an item here, an item there: every XCD gets the same
@@ -517,9 +532,15 @@ __device__ __forceinline__ void lds_barrier() {
   asm volatile("" ::: "memory");
 }
 
-template <typename K> int rules_launch(K kernel, int64_t n_wg, int lds, std::atomic<uint64_t> &done, const RuleArgs &a, hipStream_t st) {
+// Two pairs of wavefronts a line in launches of few lines, whose wavefronts would leave SIMDs idle or with nobody to change places with.  Causal layouts without
+// holes, forward pass, one pair -> two: 512 lines of 1024 positions fp32 104 -> 61 us (128 elements: 148 -> 102), bf16 24 -> 18 (34 -> 25); 1024 lines of 4096 positions
+// 456 -> 318 (578 -> 642), 82 -> 63 (126 -> 104); 2048 of them 693 -> 577 (1130 -> 1261), 124 -> 116 (198 -> 217); 3072 lines of BigBird fp16 51 -> 59.
+template <typename T, int D> inline bool few_lines(const RuleArgs &a) {
+  return a.R >= 4 && (int64_t)a.Z * a.H * a.R <= (D == 64 ? 2048 : sizeof(T) == 4 ? 512 : 1024);
+}
+template <typename K> int rules_launch(K kernel, int64_t n_wg, int threads, int lds, std::atomic<uint64_t> &done, const RuleArgs &a, hipStream_t st) {
   if (lds > 65536 && !raise_lds_limit(reinterpret_cast<const void *>(kernel), lds, done)) return BSP_ERR_HIP;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)n_wg), dim3(128), lds, st, a);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)n_wg), dim3((unsigned)threads), lds, st, a);
   return BSP_OK;
 }
 

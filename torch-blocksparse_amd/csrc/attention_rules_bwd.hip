@@ -11,15 +11,16 @@ namespace bsp {
 namespace {
 
 template <typename T, int D, bool CAP> constexpr int row_waves() { return sizeof(T) == 4 ? (D == 64 ? 2 : 1) : D == 64 ? (CAP ? 2 : 3) : 2; }
-template <typename T, int D, bool CAP> constexpr int col_waves() { return sizeof(T) == 4 ? 1 : D == 64 ? 2 : 1; }
+template <typename T, int D, bool CAP> constexpr int col_waves() { return D == 64 ? 2 : 1; }
 
-template <typename T, int D, bool CAP, bool BIAS, bool DOCS>
-__global__ void __launch_bounds__(128, (row_waves<T, D, CAP>())) k_rules_bwd_rows(RuleArgs a) {
+template <typename T, int D, bool CAP, bool BIAS, bool DOCS, int PAIRS>
+__global__ void __launch_bounds__(128 * PAIRS, (row_waves<T, D, CAP>())) k_rules_bwd_rows(RuleArgs a) {
   typedef Geo<T, D> Q;
   constexpr int MT = D / 32;
-  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  unsigned char *extra = smem + Q::RING;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  extern __shared__ __attribute__((aligned(1024))) unsigned char all_smem[];
+  const int group = PAIRS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 7);
+  unsigned char *smem = all_smem + group * pair_lds<T, D, PAIRS>(), *extra = smem + Q::RING;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 1);
   const int l32 = lane & 31, half = lane >> 5;
   const Place place = rules_place(blockIdx.x, a.Z * a.H, a.R);
   if (place.unit < 0) return;
@@ -54,7 +55,7 @@ __global__ void __launch_bounds__(128, (row_waves<T, D, CAP>())) k_rules_bwd_row
     }
     delta += swap32(delta);
   }
-  if (half == 0) a.delta[((int64_t)z * a.H + h) * a.rows + row] = -delta;   // (its negative: where the column kernel's dp starts from)
+  if (half == 0 && (PAIRS == 1 || group == 0)) a.delta[((int64_t)z * a.H + h) * a.rows + row] = -delta;   // (its negative: where the column kernel's dp starts from)
 
   Walk<DOCS> walk;
   walk.init(a.lut + lut[2 * (h * a.R + line) + 1], line * 64 < a.L ? lut[2 * (h * a.R + line)] * 2 : 0);
@@ -63,8 +64,8 @@ __global__ void __launch_bounds__(128, (row_waves<T, D, CAP>())) k_rules_bwd_row
   };
   const float *stats = a.ref + ((int64_t)z * a.H + h) * 2 * a.rows + row;
   const float ref = stats[0], factor = stats[a.rows];
-  Half cur = next();
-  if (cur.n >= 0) {
+  Halves halves = next_halves<PAIRS>(group, next);
+  if (halves.more) {
     held_t<T, D> xq;
     hold_operand<T, D>(xq, reinterpret_cast<const T *>(a.q) + z * a.q_sz + h * a.q_sh + row_in * a.q_ld, half, dead);
     const float slope = BIAS ? as_floats(a.slopes)[h] * kLog2e : 0.f, out = apart(logit_factor<T, CAP>(a.out)), in = apart(a.in), minus = ref - logit_shift<T, CAP>(a.out) - (CAP && sizeof(T) != 4 ? 2.f : 0.f);   // (e^y times four: see cap_through)
@@ -83,21 +84,24 @@ __global__ void __launch_bounds__(128, (row_waves<T, D, CAP>())) k_rules_bwd_row
       gv.issue(pv, pos, v_row, st + Q::PIECE);
       if (DOCS && wave == 0) load_documents(docs, x.lo, x.hi, lane, lds_address(extra) + stage_no * Q::EXTRA);
     };
-    issue(0, cur);
+    if (PAIRS == 1 || halves.own.n >= 0) issue(0, halves.own);
     PieceReads<T, D, false> reads;                      // the same for the k and the v piece
     reads.init(smem, lane);
 
     auto step = [&](auto stage_no) {
       constexpr int S = decltype(stage_no)::value;
-      const Half nxt = next();
+      const Halves all = halves, nxt = next_halves<PAIRS>(group, next);
+      const Half &cur = all.own;
       quad_barrier();
       const int32_t *kd = reinterpret_cast<const int32_t *>(extra + S * Q::EXTRA);
-      if (DOCS && cur.pad) {
-        clear_rows<T, D>(smem + S * Q::STAGE, 16 * wave, kd, lane);
-        clear_rows<T, D>(smem + S * Q::STAGE + Q::PIECE, 16 * wave, kd, lane);
+      if (DOCS && all.pads) {
+        if (PAIRS == 1 || cur.pad) {
+          clear_rows<T, D>(smem + S * Q::STAGE, 16 * wave, kd, lane);
+          clear_rows<T, D>(smem + S * Q::STAGE + Q::PIECE, 16 * wave, kd, lane);
+        }
         lds_barrier();
       }
-      if (nxt.n >= 0) issue(1 - S, nxt);
+      if (nxt.own.n >= 0) issue(1 - S, nxt.own);
       uint32_t seen = 0xffffu;                          // as in the forward kernel
       bool some = true, whole = true;
       if (!cur.full) {
@@ -127,10 +131,22 @@ __global__ void __launch_bounds__(128, (row_waves<T, D, CAP>())) k_rules_bwd_row
         ds.set(e);
         columns_times<T, D, S * Q::STAGE, false>(dq, reads, ds);
       }
-      cur = nxt;
-      return cur.n >= 0;
+      halves = nxt;
+      return halves.more;
     };
     while (step(Const<0>{}) && step(Const<1>{})) {}
+  }
+  if constexpr (PAIRS == 2) {                           // the second pair's sums to the first
+    quad_barrier();
+    float *sums = reinterpret_cast<float *>(all_smem + pair_lds<T, D, PAIRS>()) + wave * (64 * 16 * MT) + lane;
+    if (group) {
+#pragma unroll
+      for (int i = 0; i < 16 * MT; i++) sums[64 * i] = dq[i >> 4][i & 15];
+    }
+    lds_barrier();
+    if (group) return;
+#pragma unroll
+    for (int i = 0; i < 16 * MT; i++) dq[i >> 4][i & 15] += sums[64 * i];
   }
   const float last = a.scale * factor;
 #pragma unroll
@@ -391,11 +407,13 @@ template <typename T, int D> __global__ void __launch_bounds__(256) k_rules_bwd_
 
 template <typename T, int D, bool CAP, bool BIAS, bool DOCS> int launch_rules_bwd(const RuleArgs &a, bool cols, hipStream_t st) {
   if (!cols) {
-    static std::atomic<uint64_t> done{0};
-    return rules_launch(k_rules_bwd_rows<T, D, CAP, BIAS, DOCS>, rules_grid((int64_t)a.Z * a.H, a.R), rules_lds<T, D>(), done, a, st);
+    static std::atomic<uint64_t> done{0}, done2{0};
+    const int64_t grid = rules_grid((int64_t)a.Z * a.H, a.R);
+    if (few_lines<T, D>(a)) return rules_launch(k_rules_bwd_rows<T, D, CAP, BIAS, DOCS, 2>, grid, 256, 2 * pair_lds<T, D, 2>(), done2, a, st);
+    return rules_launch(k_rules_bwd_rows<T, D, CAP, BIAS, DOCS, 1>, grid, 128, rules_lds<T, D>(), done, a, st);
   }
   static std::atomic<uint64_t> done{0};
-  const int rc = rules_launch(k_rules_bwd_cols<T, D, CAP, BIAS, DOCS>, rules_grid((int64_t)a.Z * (a.H / a.G), a.R), rules_lds<T, D>(), done, a, st);
+  const int rc = rules_launch(k_rules_bwd_cols<T, D, CAP, BIAS, DOCS>, rules_grid((int64_t)a.Z * (a.H / a.G), a.R), 128, rules_lds<T, D>(), done, a, st);
   if (rc != BSP_OK) return rc;
   if (a.n_split > 0)
     hipLaunchKernelGGL((k_rules_bwd_cols_sum<T, D>), dim3((unsigned)((int64_t)a.Z * a.n_split * (2 * 64 * D / 4 / 256))), dim3(256), 0, st, a);

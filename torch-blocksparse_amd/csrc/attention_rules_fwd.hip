@@ -11,13 +11,14 @@ namespace {
 // (four wavefronts a SIMD leave 128 registers, which a bias or documents overrun)
 template <typename T, int D, bool BIAS, bool DOCS> constexpr int fwd_waves() { return sizeof(T) == 4 ? (D == 64 ? 2 : 1) : D == 64 ? (BIAS || DOCS ? 3 : 4) : 2; }
 
-template <typename T, int D, bool CAP, bool BIAS, bool DOCS>
-__global__ void __launch_bounds__(128, (fwd_waves<T, D, BIAS, DOCS>())) k_rules_fwd(RuleArgs a) {
+template <typename T, int D, bool CAP, bool BIAS, bool DOCS, int PAIRS>
+__global__ void __launch_bounds__(128 * PAIRS, (fwd_waves<T, D, BIAS, DOCS>())) k_rules_fwd(RuleArgs a) {
   typedef Geo<T, D> Q;
   constexpr int MT = D / 32;
-  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  unsigned char *extra = smem + Q::RING;                // per stage: the documents of its 32 keys, twice
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  extern __shared__ __attribute__((aligned(1024))) unsigned char all_smem[];
+  const int group = PAIRS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 7);
+  unsigned char *smem = all_smem + group * pair_lds<T, D, PAIRS>(), *extra = smem + Q::RING;                // per stage: the documents of its 32 keys, twice
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 1);
   const int l32 = lane & 31, half = lane >> 5;
   const Place place = rules_place(blockIdx.x, a.Z * a.H, a.R);
   if (place.unit < 0) return;
@@ -39,8 +40,8 @@ __global__ void __launch_bounds__(128, (fwd_waves<T, D, BIAS, DOCS>())) k_rules_
   auto next = [&]() {
     return walk.next(lane, [&](int lo, int hi, int bits, int hf, bool &full, bool &pad) { return rules.look(lo, hi, bits, hf, full, pad); });
   };
-  Half cur = next();
-  if (cur.n >= 0) {
+  Halves halves = next_halves<PAIRS>(group, next);
+  if (halves.more) {
     held_t<T, D> xq;
     hold_operand<T, D>(xq, reinterpret_cast<const T *>(a.q) + z * a.q_sz + h * a.q_sh + row_in * a.q_ld, half, dead);
     const float slope = BIAS ? as_floats(a.slopes)[h] * kLog2e : 0.f, factor = apart(logit_factor<T, CAP>(a.out)), shift = CAP ? apart(logit_shift<T, CAP>(a.out)) : 0.f, in = apart(a.in);
@@ -59,22 +60,25 @@ __global__ void __launch_bounds__(128, (fwd_waves<T, D, BIAS, DOCS>())) k_rules_
       gv.issue(pv, pos, v_row, st + Q::PIECE);
       if (DOCS && wave == 0) load_documents(docs, x.lo, x.hi, lane, lds_address(extra) + stage_no * Q::EXTRA);
     };
-    issue(0, cur);
+    if (PAIRS == 1 || halves.own.n >= 0) issue(0, halves.own);
     PieceReads<T, D, false> reads;
     reads.init(smem, lane);
 
     // one half of a tile; false: it was the last
     auto step = [&](auto stage_no) {
       constexpr int S = decltype(stage_no)::value;
-      const Half nxt = next();
+      const Halves all = halves, nxt = next_halves<PAIRS>(group, next);
+      const Half &cur = all.own;
       quad_barrier();
       const int32_t *kd = reinterpret_cast<const int32_t *>(extra + S * Q::EXTRA);
-      if (DOCS && cur.pad) {
-        clear_rows<T, D>(smem + S * Q::STAGE, 16 * wave, kd, lane);
-        clear_rows<T, D>(smem + S * Q::STAGE + Q::PIECE, 16 * wave, kd, lane);
+      if (DOCS && all.pads) {
+        if (PAIRS == 1 || cur.pad) {
+          clear_rows<T, D>(smem + S * Q::STAGE, 16 * wave, kd, lane);
+          clear_rows<T, D>(smem + S * Q::STAGE + Q::PIECE, 16 * wave, kd, lane);
+        }
         lds_barrier();
       }
-      if (nxt.n >= 0) issue(1 - S, nxt);
+      if (nxt.own.n >= 0) issue(1 - S, nxt.own);
       uint32_t seen = 0xffffu;                          // bit i: the lane's row sees its key i
       bool some = true, whole = true;
       if (!cur.full) {
@@ -120,12 +124,29 @@ __global__ void __launch_bounds__(128, (fwd_waves<T, D, BIAS, DOCS>())) k_rules_
         p.set(e);
         columns_times<T, D, S * Q::STAGE + Q::PIECE, false>(o, reads, p);
       }
-      cur = nxt;
-      return cur.n >= 0;
+      halves = nxt;
+      return halves.more;
     };
     while (step(Const<0>{}) && step(Const<1>{})) {}
   }
 
+  if constexpr (PAIRS == 2) {                           // the second pair's maxima, sums and accumulators to the first
+    quad_barrier();
+    float *sums = reinterpret_cast<float *>(all_smem + pair_lds<T, D, PAIRS>()) + wave * (64 * (16 * MT + 2)) + lane;
+    if (group) {
+      sums[0] = m;
+      sums[64] = l;
+#pragma unroll
+      for (int i = 0; i < 16 * MT; i++) sums[64 * (2 + i)] = o[i >> 4][i & 15];
+    }
+    lds_barrier();
+    if (group) return;
+    const float m2 = sums[0], top = fmaxf(m, m2), to = top == -INFINITY ? 0.f : top, f1 = __builtin_amdgcn_exp2f(m - to), f2 = __builtin_amdgcn_exp2f(m2 - to);
+    m = top;
+    l = l * f1 + sums[64] * f2;
+#pragma unroll
+    for (int i = 0; i < 16 * MT; i++) o[i >> 4][i & 15] = o[i >> 4][i & 15] * f1 + sums[64 * (2 + i)] * f2;
+  }
   l += swap32(l);
   const bool none = dead || l == 0.f;                   // a row that sees no key: zeros, and no share of anything in the backward pass
   const float inv = none ? 0.f : 1.f / l;
@@ -174,8 +195,10 @@ __global__ void __launch_bounds__(256) k_rules_ranges(const int32_t *docs, int64
 }
 
 template <typename T, int D, bool CAP, bool BIAS, bool DOCS> int launch_rules_fwd(const RuleArgs &a, hipStream_t st) {
-  static std::atomic<uint64_t> done{0};
-  return rules_launch(k_rules_fwd<T, D, CAP, BIAS, DOCS>, rules_grid((int64_t)a.Z * a.H, a.R), rules_lds<T, D>(), done, a, st);
+  static std::atomic<uint64_t> done{0}, done2{0};
+  const int64_t grid = rules_grid((int64_t)a.Z * a.H, a.R);
+  if (few_lines<T, D>(a)) return rules_launch(k_rules_fwd<T, D, CAP, BIAS, DOCS, 2>, grid, 256, 2 * pair_lds<T, D, 2>(), done2, a, st);
+  return rules_launch(k_rules_fwd<T, D, CAP, BIAS, DOCS, 1>, grid, 128, rules_lds<T, D>(), done, a, st);
 }
 template <typename T, int D, bool CAP, bool BIAS> int launch_rules_fwd(const RuleArgs &a, hipStream_t st) {
   return a.docs ? launch_rules_fwd<T, D, CAP, BIAS, true>(a, st) : launch_rules_fwd<T, D, CAP, BIAS, false>(a, st);
