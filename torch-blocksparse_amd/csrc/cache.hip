@@ -6,10 +6,10 @@
 // integers, decided in 64 bits.
 //
 // Both kernels move each byte once and are bound by that.  A thread has a chunk of eight elements: 16 bytes in 16-bit types, and the four
-// threads of a group agree on its range by two exchanges within the quad.  Measured, 16384 positions of 16 heads of 64, fp16, 8 bits (67 MB and 38 MB): written
-// in 26 us, 2.4 of them before to see which position of a slot counts, read in 17; 32750 of 8 heads of 128, bf16, 4 bits (176 MB) read in 38.
-// Writing was bound by its operations before the rounded quotient was taken from the low bits of one sum (33 us); reading by the
-// divisions that found a thread's place (20 and 42 us).
+// threads of a group agree on its range by two exchanges within the quad.  Tensors outside the cache are streamed past the L2 (non-temporal): nothing reads them
+// soon.  Measured: 16384 positions of 16 heads of 64, fp16, 8 bits (67 MB and 38 MB) written and read back in 45 us, 51 without the streaming, 58 before a
+// thread's place was found without divisions and the rounded quotient taken from the low bits of one sum; 32749 positions of 8 heads of 128, bf16, 4 bits
+// (176 MB) read in 41 us, 52 without the streaming.
 #include "cache.h"
 
 namespace bsp {
@@ -35,13 +35,13 @@ template <typename T> __device__ __forceinline__ void load8(float (&x)[8], const
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-      const f32x4 v = *reinterpret_cast<const f32x4 *>(p + 4 * i);
+      const f32x4 v = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(p + 4 * i));
 #pragma unroll
       for (int j = 0; j < 4; j++) x[4 * i + j] = v[j];
     }
   } else {
     union { u32x4 raw; T e[8]; } u;
-    u.raw = *reinterpret_cast<const u32x4 *>(p);
+    u.raw = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p));
 #pragma unroll
     for (int i = 0; i < 8; i++) x[i] = to_float(u.e[i]);
   }
@@ -175,13 +175,13 @@ template <typename T, int BITS, int D> __global__ void __launch_bounds__(256) k_
     }
     T *to = reinterpret_cast<T *>(value ? a.vo : a.ko) + ((int64_t)t * a.heads + head) * D + 8 * j;
     if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<f32x4 *>(to) = f32x4{x[0], x[1], x[2], x[3]};
-      *reinterpret_cast<f32x4 *>(to + 4) = f32x4{x[4], x[5], x[6], x[7]};
+      __builtin_nontemporal_store(f32x4{x[0], x[1], x[2], x[3]}, reinterpret_cast<f32x4 *>(to));
+      __builtin_nontemporal_store(f32x4{x[4], x[5], x[6], x[7]}, reinterpret_cast<f32x4 *>(to + 4));
     } else {
       union { u32x4 raw; T e[8]; } u;
 #pragma unroll
       for (int e = 0; e < 8; e++) u.e[e] = from_float<T>(x[e]);
-      *reinterpret_cast<u32x4 *>(to) = u.raw;
+      __builtin_nontemporal_store(u.raw, reinterpret_cast<u32x4 *>(to));
     }
   }
 }

@@ -12,7 +12,7 @@
 // range of fp16, which loses nothing that 2^-35 of its largest element would not.  Values are v = least + code * step rounded to fp16
 // (2^-12 of it, under the rounding of the shares) through LDS, where the product with the shares reads them transposed.
 //
-// Measured: sixteen sequences of up to 16384 positions, 32 query heads of 128 on 8 key heads, 4 bits (218 MB of pages): 51 us with the join, 4.3 TB/s;
+// Measured: sixteen sequences of up to 16384 positions, 32 query heads of 128 on 8 key heads, 4 bits (218 MB of pages): 52 us with the join, 4.2 TB/s;
 // loading the same bytes and nothing else takes 40.  The vector units are what is left: taking the codes out of their words for keys and
 // values was 240 of 390 operations a pair of tiles and is 140 of 270 with keys as they lie (63 us before).
 //
@@ -48,14 +48,15 @@ template <int BITS, int D> struct RawTile {
   static constexpr int GROUPS = D / 32;
   uint32_t kc[QB], vc[QB], km[GROUPS], vm[GROUPS];
 };
+// (each byte is read once: streamed past the L2, 54.5 -> 52 us)
 template <int N> __device__ __forceinline__ void load_words(uint32_t (&w)[N], const unsigned char *p) {
   if constexpr (N == 2) {
-    const u32x2 x = *reinterpret_cast<const u32x2 *>(p);
+    const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(p));
     w[0] = x[0], w[1] = x[1];
   } else {
 #pragma unroll
     for (int i = 0; i < N / 4; i++) {
-      const u32x4 x = *reinterpret_cast<const u32x4 *>(p + 16 * i);
+      const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p + 16 * i));
 #pragma unroll
       for (int j = 0; j < 4; j++) w[4 * i + j] = x[j];
     }
