@@ -77,7 +77,7 @@ class _Tables:
     # Work items of the columns for a launch over `batches` sequences: a column of many tiles is cut into parts, so that the longest do not
     # outlast the launch (twice the average, as in the tables of the other kernels, or half of what each of some WANTED workgroups at a time
     # has to do: the longest go first) and a small launch still has some WANTED items for its 256 compute units; every part costs a slot of 512 D bytes
-    # written and read (fp16 8 x 16 x 4096, blocks of 16, stride 64: parts of 21, 40 and 64 tiles 334, 328 and 329 us).
+    # written and read (fp16 8 x 16 x 4096, blocks of 16, stride 64: parts of 21, 32 and 64 tiles 334, 322 and 329 us).
     WANTED = 1024
 
     def columns(self, kv_heads, batches):
@@ -111,7 +111,7 @@ class _Tables:
             tiles = self._columns[kv_heads] = (heads[whole], first[whole], count, entries, dict())
         heads, first, count, entries, made = tiles
         total, n = int(count.sum()), count.numel()
-        part = max(16, -(-2 * total // n), batches * total // (2 * self.WANTED))
+        part = max(16, min(max(-(-2 * total // n), batches * total // (2 * self.WANTED) // 16 * 16), int(count.max())))    # (few different ones: each is a table that is kept)
         while part > 4 and batches * int(((count + part - 1) // part).clamp(min=1).sum()) < self.WANTED:
             part //= 2
         if part not in made:
