@@ -487,7 +487,7 @@ int bsp_attention_f32_bwd(const bsp_attention_f32_call *call, const float *d_o, 
                           int n_split, void *stream);
 
 /* Block-sparse attention with score rules: o = softmax(y) . v and its gradients without any sparse tensor, with
- *     y_ij = cap * tanh(scale * q_i . k_j / cap) - slope_h * |i - j|      (softcap 0: scale * q_i . k_j - ...)
+ *     y_ij = cap * tanh(scale * q_i . k_j / cap) - slope_h * |i - j|      (softcap 0: scale * q_i . k_j - ...; else 2^-10 .. 1024)
  * over the keys j that row i sees: block (h, i / block, j / block) is in the layout; documents[z][i] = documents[z][j] >= 0
  * (where documents is not NULL); and, with causal, j <= i or j < prefix[z] (prefix NULL: none).  A row that sees no key gets zeros
  * in o and dq.  Positions with a negative document number reach nothing, whatever q, k, v and d_o hold there.  Query head h
@@ -539,7 +539,7 @@ int bsp_cache_read(int dtype, const void *pages, int n_pages, int block, int hea
                    void *stream);
 
 /* Attention of one position a sequence over such a cache: o = softmax(y) . v, y_j = softcap * tanh(scale * q . k_j / softcap) - slope_h *
- * (n - 1 - j) (softcap 0: no cap), over the positions j < n = lengths[b] of the sequence: position j is in page table[b * table_stride
+ * (n - 1 - j) (softcap 0: no cap, else 2^-10 .. 1024), over the positions j < n = lengths[b] of the sequence: position j is in page table[b * table_stride
  * + j / block] (numbers outside 0 .. n_pages - 1: not held, not seen).  A length of at most 0 gives zeros, one past width * block (n_rows *
  * block) counts as that.  q, o: [B, H, D] in fp16 or bf16, q 16-byte aligned with strides that are multiples of 8; query head h uses key head
  * h / (H / kv_heads).  rows: NULL, or what is seen beside that: the query heads of a key head form units of at most 16 (ceil(G / ceil(G / 16)) heads of G each,

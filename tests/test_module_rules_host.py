@@ -65,3 +65,25 @@ def test_refusals(empty):
         mod.decode(q, None, torch.zeros(1, 3, dtype=torch.int32), torch.ones(1, dtype=torch.int32))
     with pytest.raises(ValueError):
         mod.decode(q[:, :, 0], None, torch.zeros(3, dtype=torch.int32), torch.ones(1, dtype=torch.int32))
+
+
+@pytest.mark.parametrize('bad', [dict(softcap=1e-4), dict(softcap=2000.), dict(softcap=1e30), dict(softcap=-1.), dict(softcap=float('nan')), dict(scale=1e30), dict(scale=float('-inf'))])
+def test_caps_and_scales_that_fp32_cannot_keep(bad, monkeypatch):
+    from torch_blocksparse import _lib, rules
+    numbers = dict(dict(scale=1., softcap=0.), **bad)
+    with pytest.raises(ValueError):
+        rules.check_scores(**numbers)
+    lib = _lib.load()
+    import ctypes
+    at = 1 << 20
+    call = rules._CALL.pack(0, 1, 1, 1, 1, 64, 16, *([64] * 12 + [0] * 12), numbers['scale'] if abs(numbers['scale']) < 1e38 else float('inf'), numbers['softcap'], 0, 0, 0, 0, 0, 0, at, 0, 0)
+    assert lib.bsp_attention_rules_fwd(call, at, at, at, at, 0) < 0
+    names = ('dtype q qb qh o ob oh B H pages n block kv D bits table ts width lengths rows n_rows most scale softcap slopes ws bytes splits stream').split()
+    good = dict(zip(names, (0, at, 64, 64, at, 64, 64, 1, 1, at, 1, 16, 1, 64, 4, at, 1, 1, at, 0, 0, 1, 1., 0., 0, 0, 0, 1, 0)))
+    assert lib.bsp_cache_attention(*[ctypes.c_float(v) if n in ('scale', 'softcap') else v for n, v in dict(good, **numbers).items()]) < 0
+
+
+def test_good_caps_and_scales():
+    from torch_blocksparse import rules
+    for scale, softcap in ((1., 0.), (0., 1024.), (-3., 2. ** -10), (2. ** 64, 30.)):
+        rules.check_scores(scale, softcap)

@@ -214,7 +214,7 @@ template <typename T> int launch_rules_fwd(const RuleArgs &a, int D, hipStream_t
 int rules_args(const bsp_attention_rules_call *c, RuleArgs &a) {
   if (!c || c->Z <= 0 || c->H <= 0 || c->kv_heads <= 0 || c->H % c->kv_heads || c->length <= 0 || c->length >= (1 << 24) || !c->d_rows) return BSP_ERR_ARG;
   if ((c->dtype != BSP_F16 && c->dtype != BSP_BF16 && c->dtype != BSP_F32) || (c->D != 64 && c->D != 128)) return BSP_ERR_UNSUPPORTED;
-  if (c->H / c->kv_heads > 127 || !(c->softcap >= 0.f) || !(c->scale - c->scale == 0.f) || !(c->softcap - c->softcap == 0.f)) return BSP_ERR_ARG;
+  if (c->H / c->kv_heads > 127 || !scores_ok(c->scale, c->softcap)) return BSP_ERR_ARG;
   if ((c->documents != nullptr) != (c->ranges != nullptr) || (c->prefix && !c->causal)) return BSP_ERR_ARG;
   const int64_t lines = c->lines, unit = c->dtype == BSP_F32 ? 4 : 8, size = c->dtype == BSP_F32 ? 4 : 2;
   if (lines < (c->length + 63) / 64 || lines > (1 << 18)) return BSP_ERR_ARG;

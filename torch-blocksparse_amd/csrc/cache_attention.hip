@@ -454,7 +454,7 @@ extern "C" int bsp_cache_attention(int dtype, const void *q, int64_t q_stride_b,
   if (!q || !o || !pages || !table || !lengths || B <= 0 || H <= 0 || kv_heads <= 0 || H % kv_heads || n_pages <= 0 || width <= 0 || splits < 1 || splits > 64) return BSP_ERR_ARG;
   if ((dtype != BSP_F16 && dtype != BSP_BF16) || bsp_cache_page_bytes(block, kv_heads, D, bits) <= 0) return BSP_ERR_UNSUPPORTED;
   if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(pages)) & 15) || (reinterpret_cast<uintptr_t>(o) & 3) || q_stride_b % 8 || q_stride_h % 8 || o_stride_b % 2 || o_stride_h % 2) return BSP_ERR_ARG;
-  if (!(scale - scale == 0.f) || !(softcap >= 0.f) || !(softcap - softcap == 0.f) || (rows && n_rows <= 0) || most_blocks <= 0) return BSP_ERR_ARG;
+  if (!scores_ok(scale, softcap) || (rows && n_rows <= 0) || most_blocks <= 0) return BSP_ERR_ARG;
   if ((int64_t)width * block >= ((int64_t)1 << 24) || (int64_t)n_pages * block >= ((int64_t)1 << 31) || (rows && n_rows > 65536)) return BSP_ERR_UNSUPPORTED;
   const int64_t need = bsp_cache_attention_workspace_bytes(B, H, kv_heads, D, splits);
   if (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < need)) return BSP_ERR_CAPACITY;

@@ -12,11 +12,10 @@ In the cache 32 neighbouring elements of a head share a least value and a step, 
 (2^bits - 1), and an element is least + code * step with the nearest code (ties to the even one), in exact arithmetic.  Elements are taken into
 float16's range first; a group with a NaN reads back as NaN.  A position of a head takes 5 / 8 (4 bits) or 9 / 8 (8 bits) bytes an element.
 """
-import math
-
 import torch
 
 from . import _lib
+from .rules import check_scores
 
 
 class KeyValueCache:
@@ -61,7 +60,8 @@ class KeyValueCache:
 
     def write(self, k, v, slots):
         """Quantises k and v [tokens, heads, head_dim] (of one type) into positions slots[t] = page * block + offset of the cache.  Tokens with a
-        negative slot, or one past the cache, are left out; of tokens with the same slot the last is written.  No gradient."""
+        negative slot, or one past the cache, are left out; of tokens with the same slot the last is written.  No gradient.  Two writes that run at
+        the same time (on two streams) and have a slot in common leave it as one of them, or half of each."""
         slots = self._check_slots(slots)
         T = slots.numel()
         k, k_st, k_sh = self._operand(k, 'k', T)
@@ -116,7 +116,7 @@ class CacheAttention:
     their `lengths` [batch] int32, the new position among them (its key and value are in the cache already).  Position j of sequence b is in page
     table[b, j // block] at offset j % block.  Returns o [batch, query heads, head_dim]:
 
-        y_j = softcap * tanh(scale * q . k_j / softcap) - slopes[h] * (n - 1 - j),   o = sum_j softmax_j(y_j) v_j      (softcap 0: no cap)
+        y_j = softcap * tanh(scale * q . k_j / softcap) - slopes[h] * (n - 1 - j),   o = sum_j softmax_j(y_j) v_j      (softcap 0: no cap; else 2^-10 to 1024)
 
     over j < n = lengths[b], with a layout those in blocks that row (n - 1) // block of head h has: what `Attention` with causal=True gives for its last
     row.  A page number outside the cache (-1, say) stands for a page that is not held: its positions are not seen, so pages that no later
@@ -163,8 +163,7 @@ class CacheAttention:
         for name, t, shape, dtype in (('lengths', lengths, (B,), torch.int32), ('slopes', slopes, (H,), torch.float32)):
             if (t is not None or name == 'lengths') and (tuple(t.shape) != shape or t.dtype != dtype or t.device != q.device):
                 raise ValueError('%s must be %s %s on %s (got %s %s on %s)' % (name, dtype, list(shape), q.device, t.dtype, list(t.shape), t.device))
-        if not (softcap >= 0 and math.isfinite(softcap) and math.isfinite(scale)):
-            raise ValueError('softcap must be finite and not negative, scale finite (got %s and %s)' % (softcap, scale))
+        check_scores(scale, softcap)
 
     def __call__(self, q, cache, table, lengths, scale=1., softcap=0., slopes=None):
         scale, softcap = float(scale), float(softcap or 0.)

@@ -17,7 +17,6 @@ One kernel forward, two backward (rows: dq; columns: dk and dv), none of which s
 bsp_attention_rules_bwd).  The results of a call are the same bits every time.
 """
 import ctypes
-import math
 import struct
 
 import torch
@@ -44,6 +43,14 @@ def _operand(t, Z, heads, L, D):
 def _own(Z, heads, L, D):
     """the strides of a contiguous tensor"""
     return (heads * L * D if Z > 1 else 0, L * D if heads > 1 else 0, D)
+
+
+def check_scores(scale, softcap):
+    """a capped score is off by softcap * 2^-23 (the tanh comes of an exponential in fp32), so a cap has an upper end"""
+    if not (softcap == 0. or 2. ** -10 <= softcap <= 1024.):
+        raise ValueError('softcap must be 0 or between 2^-10 and 1024 (got %s)' % softcap)
+    if not abs(scale) <= 2. ** 64:
+        raise ValueError('scale must be finite, 2^64 at most (got %s)' % scale)
 
 
 def _at(t):
@@ -210,7 +217,7 @@ class Attention:
     layout's last block.
 
     scale     factor of the scores
-    softcap   0 for none, else the scores are softcap * tanh(scale * q . k / softcap)
+    softcap   0 for none, else the scores are softcap * tanh(scale * q . k / softcap); 2^-10 to 1024
     slopes    None, or [heads] float32: slopes[h] * |i - j| is taken off the scores (constants: no gradient)
     causal    row i sees the keys up to i only
     documents None, or [batch, length] int32: a row sees keys of its own document only; negative: padding
@@ -253,13 +260,14 @@ class Attention:
             raise ValueError('head dimensions are 64 and 128 (got %d)' % D)
         if k.shape != v.shape or tuple(k.shape) != (Z, kv, L, D) or kv == 0 or H % kv:
             raise ValueError('q %s, k %s and v %s do not fit together' % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+        if (L + 64) * D * q.element_size() >= 1 << 32:
+            raise ValueError('the rows of a head lie within 4 GiB (got length %d)' % L)
         if H // kv > 127:
             raise ValueError('at most 127 query heads share a key head (got %d)' % (H // kv))
         heads, blocks = self.layout.shape[:2]
         if H != heads or -(-L // self.block) != blocks:
             raise ValueError('q %s does not fit a layout of %d heads and %d blocks of %d' % (tuple(q.shape), heads, blocks, self.block))
-        if not (softcap >= 0 and math.isfinite(softcap) and math.isfinite(scale)):
-            raise ValueError('softcap must be finite and not negative, scale finite (got %s and %s)' % (softcap, scale))
+        check_scores(scale, softcap)
         if prefix is not None and not causal:
             raise ValueError('a prefix needs causal=True')
         for name, t, shape, dtype in (('slopes', slopes, (H,), torch.float32), ('documents', documents, (Z, L), torch.int32), ('prefix', prefix, (Z,), torch.int32)):
