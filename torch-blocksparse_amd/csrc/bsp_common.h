@@ -54,7 +54,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 // a cap of scores (0: none) whose error, softcap * 2^-23 of fp32's exponential, stays below that of a score itself, and a scale that cannot make it overflow
-inline bool scores_ok(float scale, float softcap) { return (softcap == 0.f || (softcap >= 0x1p-10f && softcap <= 1024.f)) && scale >= -0x1p64f && scale <= 0x1p64f; }
+inline bool scores_ok(float scale, float softcap) { return (softcap == 0.f || (softcap >= 0x1p-10f && softcap <= 1024.f)) && scale >= -0x1p100f && scale <= 0x1p100f; }
 static inline int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 static inline hipStream_t as_stream(void *s) { return reinterpret_cast<hipStream_t>(s); }
 

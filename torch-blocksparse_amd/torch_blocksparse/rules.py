@@ -49,8 +49,8 @@ def check_scores(scale, softcap):
     """a capped score is off by softcap * 2^-23 (the tanh comes of an exponential in fp32), so a cap has an upper end"""
     if not (softcap == 0. or 2. ** -10 <= softcap <= 1024.):
         raise ValueError('softcap must be 0 or between 2^-10 and 1024 (got %s)' % softcap)
-    if not abs(scale) <= 2. ** 64:
-        raise ValueError('scale must be finite, 2^64 at most (got %s)' % scale)
+    if not abs(scale) <= 2. ** 100:
+        raise ValueError('scale must be finite, 2^100 at most (got %s)' % scale)
 
 
 def _at(t):
