@@ -12,8 +12,9 @@
 // range of fp16, which loses nothing that 2^-35 of its largest element would not.  Values are v = least + code * step rounded to fp16
 // (2^-12 of it, under the rounding of the shares) through LDS, where the product with the shares reads them transposed.
 //
-// Measured: sixteen sequences of up to 16384 positions, 32 query heads of 128 on 8 key heads, 4 bits (218 MB of pages): 52 us with the join, 4.2 TB/s;
-// loading the same bytes and nothing else takes 40.  The vector units are what is left: taking the codes out of their words for keys and
+// Measured: sixteen sequences of up to 16384 positions, 32 query heads of 128 on 8 key heads, 4 bits (218 MB of pages): 51 us with the join, 4.3 TB/s
+// (all of 16384 positions: 64 us, 5.2 TB/s, the rate of a copy);
+// loading the same bytes and nothing else takes 40.  What is left is that compute units get unequal shares of ragged sequences, and the vector units: taking the codes out of their words for keys and
 // values was 240 of 390 operations a pair of tiles and is 140 of 270 with keys as they lie (63 us before).
 //
 // Scores lie with a position per lane and the query heads along the sixteen result rows of the matrix unit, dealt so that a head takes one
@@ -78,8 +79,10 @@ __global__ void __launch_bounds__(256, 3) k_cache_attention(DecodeArgs a, int dt
   constexpr int GR = D / 32, NT = D / 16;
   __shared__ __attribute__((aligned(16))) unsigned char smem[L::bytes(V)];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), key = lane & 15, c = lane >> 4;
-  const int64_t wg = xcd_remap(blockIdx.x, (int64_t)a.B * a.units * a.splits);
-  const int split = (int)(wg % a.splits), unit = (int)(wg / a.splits % a.units), b = (int)(wg / a.splits / a.units);
+  // the first pieces of all sequences and heads, then the second ones: the workgroups that find nothing to do come last, and every XCD (they take workgroups
+  // in turn) gets the same share of the long sequences
+  const uint32_t groups = (uint32_t)(a.B * a.units), split = blockIdx.x / groups, group = blockIdx.x % groups;
+  const int unit = (int)(group % (uint32_t)a.units), b = (int)(group / (uint32_t)a.units);
   const int per_key = (a.G + a.per - 1) / a.per, hk = unit / per_key, first = hk * a.G + unit % per_key * a.per;
   const int heads = hk * a.G + a.G - first < a.per ? hk * a.G + a.G - first : a.per;     // the unit's query heads: first ..
   const int held = a.width * a.block, most = a.rows && a.n_rows * a.block < held ? a.n_rows * a.block : held;
