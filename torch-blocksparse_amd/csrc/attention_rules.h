@@ -534,7 +534,7 @@ __device__ __forceinline__ void lds_barrier() {
 
 // Two pairs of wavefronts a line in launches of few lines, whose wavefronts would leave SIMDs idle or with nobody to change places with.  Causal layouts without
 // holes, forward pass, one pair -> two: 512 lines of 1024 positions fp32 104 -> 61 us (128 elements: 148 -> 102), bf16 24 -> 18 (34 -> 25); 1024 lines of 4096 positions
-// 456 -> 318 (578 -> 642), 82 -> 63 (126 -> 104); 2048 of them 693 -> 577 (1130 -> 1261), 124 -> 116 (198 -> 217); 3072 lines of BigBird fp16 51 -> 59.
+// 456 -> 318 (578 -> 642), 82 -> 63 (126 -> 104); 2048 of them 693 -> 577 (1130 -> 1261), 124 -> 116 (198 -> 217); twelve heads of 256 lines of BigBird fp16 51 -> 59.
 template <typename T, int D> inline bool few_lines(const RuleArgs &a) {
   return a.R >= 4 && (int64_t)a.Z * a.H * a.R <= (D == 64 ? 2048 : sizeof(T) == 4 ? 512 : 1024);
 }
