@@ -1,0 +1,33 @@
+"""CPU: which operators SparseSelfAttention keeps, and for how long."""
+import collections
+
+import pytest
+import torch
+
+import torch_blocksparse as tb
+
+CLS = tb.DeepSpeedSparseSelfAttention
+
+
+@pytest.fixture
+def empty(monkeypatch):
+    monkeypatch.setattr(CLS, 'ops', collections.OrderedDict())
+    monkeypatch.setattr(CLS, 'captured', dict())
+
+
+def module():
+    return tb.SparseSelfAttention(tb.SparsityConfig(block=16, stride=64))
+
+
+def test_a_kind_of_operators_takes_no_place_of_another(empty):
+    mod = module()
+    chain = mod.get_ops(2, 64)
+    rules = mod._kept('rules', 2, 4, lambda layout: tb.Attention(layout, 16))
+    for blocks in range(1, 2 * CLS.OPS_CACHE_SIZE):
+        mod._kept('decode', 2, blocks, lambda layout: tb.CacheAttention(16, layout))
+    assert mod.get_ops(2, 64) is chain and mod._kept('rules', 2, 4, None) is rules
+    for blocks in range(1, 2 * CLS.OPS_CACHE_SIZE):
+        mod.get_ops(2, 64 * blocks + 64)
+    assert mod._kept('rules', 2, 4, None) is rules
+    assert mod.get_ops(2, 64) is not chain               # (its own kind has as many places as ever)
+    assert len(CLS.ops) == 2 * CLS.OPS_CACHE_SIZE + 1

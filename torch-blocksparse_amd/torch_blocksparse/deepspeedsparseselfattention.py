@@ -45,9 +45,18 @@ class DeepSpeedSparseSelfAttention(nn.Module):
     _make_layout = staticmethod(fixed_layout)
 
     # Operators by (heads, sequence length, configuration, device), shared by all modules like the reference's class-level
-    # cache, but bounded: the least recently used entry goes when more than OPS_CACHE_SIZE are held.
+    # cache, but bounded: the least recently used entry of a kind (the chain's, those with rules, those of decoding) goes when
+    # more than OPS_CACHE_SIZE of the kind are held.
     ops = collections.OrderedDict()
     OPS_CACHE_SIZE = 16
+
+    @staticmethod
+    def _drop_the_oldest(key):
+        """of the kind of `key`, where there are too many of it"""
+        cache, kind = DeepSpeedSparseSelfAttention.ops, lambda k: k[0] if isinstance(k[0], str) else 'chain'
+        alike = [k for k in cache if kind(k) == kind(key)]
+        for old in alike[:-DeepSpeedSparseSelfAttention.OPS_CACHE_SIZE]:
+            del cache[old]
 
     def get_ops(self, H, L, device=None):
         cfg = self.sparsity_config
@@ -69,8 +78,7 @@ class DeepSpeedSparseSelfAttention(nn.Module):
         dsd_nn = MatMul(layout, cfg.block, 'dsd', trans_a=False, trans_b=False)
         softmax = Softmax(layout, cfg.block)
         cache[key] = (sdd_nt, dsd_nn, softmax)
-        while len(cache) > DeepSpeedSparseSelfAttention.OPS_CACHE_SIZE:
-            cache.popitem(last=False)
+        DeepSpeedSparseSelfAttention._drop_the_oldest(key)
         return cache[key]
 
     # Operators with rules and of decoding that a captured graph has in it: its replays use their tables, so these stay.
@@ -91,9 +99,8 @@ class DeepSpeedSparseSelfAttention(nn.Module):
                 whole = -(-num_blocks // block_stride) * block_stride        # the layout is made of whole windows
                 layout = DeepSpeedSparseSelfAttention._make_layout(H, whole, cfg.mode, block_stride, cfg.attention, cfg.numverts, cfg.vertsize)
                 cache[key] = make(layout[:, :num_blocks, :num_blocks].to(torch.uint8))
+            DeepSpeedSparseSelfAttention._drop_the_oldest(key)
         cache.move_to_end(key)
-        while len(cache) > DeepSpeedSparseSelfAttention.OPS_CACHE_SIZE:
-            cache.popitem(last=False)
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             DeepSpeedSparseSelfAttention.captured[key] = cache[key]
         return cache[key]
