@@ -1,4 +1,4 @@
-"""CPU: which operators SparseSelfAttention keeps, and for how long."""
+"""CPU: which operators SparseSelfAttention keeps: each kind has places of its own, and what a captured graph has in it stays."""
 import collections
 
 import pytest
@@ -13,6 +13,11 @@ CLS = tb.DeepSpeedSparseSelfAttention
 def empty(monkeypatch):
     monkeypatch.setattr(CLS, 'ops', collections.OrderedDict())
     monkeypatch.setattr(CLS, 'captured', dict())
+
+
+def capturing(monkeypatch, yes):
+    monkeypatch.setattr(torch.cuda, 'is_available', lambda: True)
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: yes)
 
 
 def module():
@@ -31,3 +36,16 @@ def test_a_kind_of_operators_takes_no_place_of_another(empty):
     assert mod._kept('rules', 2, 4, None) is rules
     assert mod.get_ops(2, 64) is not chain               # (its own kind has as many places as ever)
     assert len(CLS.ops) == 2 * CLS.OPS_CACHE_SIZE + 1
+
+
+def test_the_chain_of_a_graph_stays(empty, monkeypatch):
+    mod = module()
+    capturing(monkeypatch, False)
+    mod.get_ops(2, 128)
+    capturing(monkeypatch, True)
+    chain = mod.get_ops(2, 64)
+    capturing(monkeypatch, False)
+    for blocks in range(2, 2 * CLS.OPS_CACHE_SIZE):
+        mod.get_ops(2, 64 * blocks)
+    assert [c for c in CLS.captured.values()] == [chain]
+    assert mod.get_ops(2, 64) is chain

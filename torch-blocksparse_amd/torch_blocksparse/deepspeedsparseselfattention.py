@@ -61,10 +61,10 @@ class DeepSpeedSparseSelfAttention(nn.Module):
     def get_ops(self, H, L, device=None):
         cfg = self.sparsity_config
         key = (H, L, str(device)) + cfg.key()
-        cache = DeepSpeedSparseSelfAttention.ops
-        if key in cache:
-            cache.move_to_end(key)
-            return cache[key]
+        return self._held(key, lambda: self._chain(H, L, device))
+
+    def _chain(self, H, L, device):
+        cfg = self.sparsity_config
         num_blocks = L // cfg.block
         if num_blocks != L / cfg.block:
             raise ValueError('Sequence length %d must be dividable by block size %d' % (L, cfg.block))
@@ -77,33 +77,36 @@ class DeepSpeedSparseSelfAttention(nn.Module):
         sdd_nt = MatMul(layout, cfg.block, 'sdd', trans_a=False, trans_b=True)
         dsd_nn = MatMul(layout, cfg.block, 'dsd', trans_a=False, trans_b=False)
         softmax = Softmax(layout, cfg.block)
-        cache[key] = (sdd_nt, dsd_nn, softmax)
-        DeepSpeedSparseSelfAttention._drop_the_oldest(key)
-        return cache[key]
+        return sdd_nt, dsd_nn, softmax
 
-    # Operators with rules and of decoding that a captured graph has in it: its replays use their tables, so these stay.
+    # Operators that a captured graph has in it: its replays use their tables, so these stay.
     captured = dict()
+
+    @staticmethod
+    def _held(key, make):
+        """what `ops` holds under `key`, made where it holds nothing"""
+        cls = DeepSpeedSparseSelfAttention
+        if key not in cls.ops:
+            cls.ops[key] = cls.captured[key] if key in cls.captured else make()
+            cls._drop_the_oldest(key)
+        cls.ops.move_to_end(key)
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            cls.captured[key] = cls.ops[key]
+        return cls.ops[key]
 
     def _kept(self, kind, H, num_blocks, make):
         """the operator `make` makes of the configuration's layout for so many blocks of any number, kept among `ops`"""
         cfg = self.sparsity_config
-        key = (kind, H, num_blocks) + cfg.key()
-        cache = DeepSpeedSparseSelfAttention.ops
-        if key not in cache:
-            if key in DeepSpeedSparseSelfAttention.captured:
-                cache[key] = DeepSpeedSparseSelfAttention.captured[key]
-            else:
-                block_stride = cfg.stride // cfg.block
-                if block_stride != cfg.stride / cfg.block:
-                    raise ValueError('Stride %d must be dividable by block size %d' % (cfg.stride, cfg.block))
-                whole = -(-num_blocks // block_stride) * block_stride        # the layout is made of whole windows
-                layout = DeepSpeedSparseSelfAttention._make_layout(H, whole, cfg.mode, block_stride, cfg.attention, cfg.numverts, cfg.vertsize)
-                cache[key] = make(layout[:, :num_blocks, :num_blocks].to(torch.uint8))
-            DeepSpeedSparseSelfAttention._drop_the_oldest(key)
-        cache.move_to_end(key)
-        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
-            DeepSpeedSparseSelfAttention.captured[key] = cache[key]
-        return cache[key]
+
+        def operator():
+            block_stride = cfg.stride // cfg.block
+            if block_stride != cfg.stride / cfg.block:
+                raise ValueError('Stride %d must be dividable by block size %d' % (cfg.stride, cfg.block))
+            whole = -(-num_blocks // block_stride) * block_stride        # the layout is made of whole windows
+            layout = DeepSpeedSparseSelfAttention._make_layout(H, whole, cfg.mode, block_stride, cfg.attention, cfg.numverts, cfg.vertsize)
+            return make(layout[:, :num_blocks, :num_blocks].to(torch.uint8))
+
+        return self._held((kind, H, num_blocks) + cfg.key(), operator)
 
     def __init__(self, sparsity_config=SparsityConfig(), key_padding_mask_mode='add', attn_mask_mode='mul'):
         super().__init__()
