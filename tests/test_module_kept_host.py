@@ -1,5 +1,6 @@
 """CPU: which operators SparseSelfAttention keeps: each kind has places of its own, and what a captured graph has in it stays."""
 import collections
+import threading
 
 import pytest
 import torch
@@ -49,3 +50,29 @@ def test_the_chain_of_a_graph_stays(empty, monkeypatch):
         mod.get_ops(2, 64 * blocks)
     assert [c for c in CLS.captured.values()] == [chain]
     assert mod.get_ops(2, 64) is chain
+
+
+@pytest.mark.parametrize('kind', ['chain', 'rules'])
+def test_another_thread_may_drop_operators(empty, monkeypatch, kind):
+    """While a call has found its operators and not yet returned them, a second thread makes as many others as there are places."""
+    mod, made, workers = module(), [], []
+
+    def call(n):
+        return mod.get_ops(2, 64 * n) if kind == 'chain' else mod._kept('rules', 2, n, lambda layout: tb.Attention(layout, 16))
+
+    def others():
+        for n in range(2, 3 + CLS.OPS_CACHE_SIZE):
+            made.append(call(n))
+
+    class Racing(collections.OrderedDict):
+        def move_to_end(self, key):
+            if not workers:
+                workers.append(threading.Thread(target=others))
+                workers[0].start()
+                workers[0].join(0.5)                     # (as long as it takes, or waiting for this call)
+            super().move_to_end(key)
+
+    monkeypatch.setattr(CLS, 'ops', Racing())
+    assert call(1) is not None
+    workers[0].join(30)
+    assert len(made) == 1 + CLS.OPS_CACHE_SIZE and len(CLS.ops) == CLS.OPS_CACHE_SIZE

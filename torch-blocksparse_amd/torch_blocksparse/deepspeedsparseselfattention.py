@@ -11,6 +11,7 @@ Beyond the reference, `forward` takes score rules (`Attention`): a cap, a bias b
 of fewer heads; and `decode` answers for one new position a sequence from a `KeyValueCache` over the same layout.
 """
 import collections
+import threading
 
 import torch
 import torch.nn as nn
@@ -49,6 +50,7 @@ class DeepSpeedSparseSelfAttention(nn.Module):
     # more than OPS_CACHE_SIZE of the kind are held.
     ops = collections.OrderedDict()
     OPS_CACHE_SIZE = 16
+    _lock = threading.RLock()                            # of `ops` and `captured`
 
     @staticmethod
     def _drop_the_oldest(key):
@@ -86,13 +88,14 @@ class DeepSpeedSparseSelfAttention(nn.Module):
     def _held(key, make):
         """what `ops` holds under `key`, made where it holds nothing"""
         cls = DeepSpeedSparseSelfAttention
-        if key not in cls.ops:
-            cls.ops[key] = cls.captured[key] if key in cls.captured else make()
-            cls._drop_the_oldest(key)
-        cls.ops.move_to_end(key)
-        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
-            cls.captured[key] = cls.ops[key]
-        return cls.ops[key]
+        with cls._lock:
+            if key not in cls.ops:
+                cls.ops[key] = cls.captured[key] if key in cls.captured else make()
+                cls._drop_the_oldest(key)
+            cls.ops.move_to_end(key)
+            if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+                cls.captured[key] = cls.ops[key]
+            return cls.ops[key]
 
     def _kept(self, kind, H, num_blocks, make):
         """the operator `make` makes of the configuration's layout for so many blocks of any number, kept among `ops`"""
