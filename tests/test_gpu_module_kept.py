@@ -1,8 +1,13 @@
-"""GPU: the operators that SparseSelfAttention keeps: a captured chain outlives what other calls make."""
+"""GPU: the operators that SparseSelfAttention keeps: a captured chain outlives what other calls make, and tables of dropped operators are not given away
+while a stream reads them."""
+import collections
+import gc
+
 import pytest
 import torch
 
 import torch_blocksparse as tb
+from torch_blocksparse import _lib
 
 pytestmark = pytest.mark.gpu
 DEV = 'cuda'
@@ -51,3 +56,88 @@ def test_a_captured_chain_outlives_the_operators_of_decoding_and_of_other_length
         for a, b in zip(out, eager):
             assert torch.equal(a, b)
     del filler
+
+
+def round_up(n):
+    return -(-n // 512) * 512                            # (the allocator's unit)
+
+
+@pytest.mark.parametrize('block', [16, 32, 64])
+def test_all_that_a_chain_holds_on_the_gpu_is_found(block, monkeypatch):
+    """What stays allocated when a chain was used in all ways is what a drop tells of the streams."""
+    monkeypatch.setattr(tb.DeepSpeedSparseSelfAttention, 'ops', collections.OrderedDict())    # (no operator of another test is dropped meanwhile)
+    mod = tb.SparseSelfAttention(tb.SparsityConfig(block=block, stride=2 * block, numverts=2))
+    B, H, L, D = 2, 4, 8 * block, 64
+    x = {t: torch.randn(B, H, L, D, device=DEV).to(t) for t in (torch.float16, torch.bfloat16, torch.float32)}
+    mask = {t: torch.ones(L, L, dtype=t, device=DEV) for t in x}
+
+    def use(length):
+        for t in x:
+            for attn_mask in (None, mask[t][:length, :length].contiguous()):
+                leaves = [x[t][:, :, :length].contiguous().requires_grad_(True) for _ in range(3)]
+                mod(*leaves, attn_mask=attn_mask).sum().backward()
+
+    use(4 * block)                                       # (what the libraries keep for themselves)
+    torch.cuda.synchronize()
+    gc.collect()
+    before = torch.cuda.memory_allocated()
+    use(8 * block)
+    torch.cuda.synchronize()
+    gc.collect()
+    held = torch.cuda.memory_allocated() - before
+    found = {t.untyped_storage().data_ptr(): t.untyped_storage().nbytes() for t in _lib.tensors_of(mod.get_ops(H, L, x[torch.float16].device)) if t.is_cuda}
+    assert held == sum(round_up(n) for n in found.values()) > 0
+
+
+def busy_stream(seconds=0.3):
+    """a stream with work of that length under way"""
+    start, stop = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+    start.record()
+    torch.cuda._sleep(1 << 22)                           # (of a clock that differs between cards)
+    stop.record()
+    stop.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(int((1 << 22) * 1e3 * seconds / start.elapsed_time(stop)))
+    return stream
+
+
+def addresses(tensors):
+    return [(t.untyped_storage().data_ptr(), t.untyped_storage().data_ptr() + t.untyped_storage().nbytes()) for t in tensors if t.is_cuda]
+
+
+def test_tables_are_not_given_away_while_another_stream_reads_them():
+    """Operators made on one stream, in use on another one when they are dropped: their memory stays theirs until that is done."""
+    cls = tb.DeepSpeedSparseSelfAttention
+    B, H, D, block, L = 2, 2, 64, 16, 256
+    mod = tb.SparseSelfAttention(tb.SparsityConfig(block=block, stride=32))
+    q, k, v = [torch.randn(B, H, L, D, device=DEV).half() for _ in range(3)]
+    lay = tb.fixed_layout(H, L // block, 'fixed', 2, 'unidirectional', 1, 1)
+    cache = tb.KeyValueCache(2 * L // block, block, H, D)
+    cache.write(k.transpose(1, 2).flatten(0, 1), v.transpose(1, 2).flatten(0, 1), torch.arange(B * L, dtype=torch.int32, device=DEV))
+    table, lengths = torch.arange(2 * L // block, dtype=torch.int32, device=DEV).view(B, -1), torch.full((B,), L, dtype=torch.int32, device=DEV)
+    ops = dict(rules=tb.Attention(lay, block), decode=tb.CacheAttention(block, lay))
+    work = dict(chain=lambda: mod(q, k, v), rules=lambda: ops['rules'](q, k, v, causal=True), decode=lambda: ops['decode'](q[:, :, -1].contiguous(), cache, table, lengths))
+    want = {n: w() for n, w in work.items()}
+    torch.cuda.synchronize()
+    for name in work:
+        held = _lib.tensors_of(mod.get_ops(H, L, q.device) if name == 'chain' else ops[name])
+        places = addresses(held)
+        sizes = sorted({b - a for a, b in places})
+        assert places
+        del held
+        stream = busy_stream()
+        with torch.cuda.stream(stream):
+            got = work[name]()                           # behind the sleep
+        if name == 'chain':
+            for n in range(1, cls.OPS_CACHE_SIZE + 1):
+                mod.get_ops(H, L + 32 * n, q.device)
+        else:
+            del ops[name]
+        gc.collect()
+        fresh = [torch.empty(n, dtype=torch.uint8, device=DEV) for _ in range(20) for n in sizes]
+        new = addresses(fresh)
+        assert not stream.query()                        # (still under way)
+        assert not any(a < d and c < b for a, b in places for c, d in new), name
+        stream.synchronize()
+        assert torch.equal(got, want[name])

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import torch_blocksparse as tb
+from torch_blocksparse import _lib
 
 CLS = tb.DeepSpeedSparseSelfAttention
 
@@ -76,3 +77,53 @@ def test_another_thread_may_drop_operators(empty, monkeypatch, kind):
     assert call(1) is not None
     workers[0].join(30)
     assert len(made) == 1 + CLS.OPS_CACHE_SIZE and len(CLS.ops) == CLS.OPS_CACHE_SIZE
+
+
+class Table:
+    """a device tensor that says which streams it was told of"""
+    is_cuda = True
+
+    def __init__(self):
+        self.told = []
+
+    def record_stream(self, stream):
+        self.told.append(stream)
+
+
+def test_tables_are_told_of_every_stream_that_reads_them(monkeypatch):
+    now = [1]
+    monkeypatch.setattr(_lib, 'raw_stream', lambda device: now[0])
+    monkeypatch.setattr(torch.cuda, 'current_stream', lambda device=None: 'stream %d' % now[0])
+    early, late, readers = Table(), Table(), _lib.Readers()
+    readers.table(early, None, torch.zeros(1))           # (one that is on the host needs nothing)
+    for now[0] in (1, 2, 1):
+        readers.read('device')
+    readers.table(late)
+    now[0] = 3
+    readers.read('device')
+    assert early.told == ['stream 1', 'stream 2', 'stream 3'] and sorted(late.told) == ['stream 1', 'stream 2', 'stream 3']
+
+
+def test_the_tensors_of_an_operator_are_found_wherever_they_are():
+    op, plan, t = tb.MatMul(torch.ones(1, 1, 1), 16, 'dsd'), tb.Softmax(torch.ones(1, 1, 1), 16), [torch.zeros(i + 1) for i in range(6)]
+    plan.table, t[1].gplan, inside = t[0], plan, t[5]
+    op.lut_cache['key'] = ([t[1], (t[2], None)], dict(a=t[3], b=op))
+    op.build = lambda: inside
+    op._products[0] = [t[4]]
+    found = {id(x) for x in _lib.tensors_of((op, 3, 'text'))}
+    assert found == {id(x) for x in t + [op.layout, plan.layout]}
+
+
+def test_a_dropped_chain_tells_its_tables(empty, monkeypatch):
+    told, now = [], [7]
+    monkeypatch.setattr(CLS, '_readers', dict())
+    monkeypatch.setattr(_lib, 'raw_stream', lambda device: now[0])
+    monkeypatch.setattr(torch.cuda, 'current_stream', lambda device=None: now[0])
+    monkeypatch.setattr(_lib.Readers, 'table', lambda self, *tensors: told.append((sorted(self.streams), len(tensors))))
+    monkeypatch.setattr(CLS, '_chain', lambda self, H, L, device: (torch.zeros(H), torch.zeros(L)))
+    mod, device = module(), torch.device('cuda', 0)
+    for now[0] in (7, 8, 7):
+        mod.get_ops(2, 64, device)
+    for n in range(2, 2 + CLS.OPS_CACHE_SIZE):
+        mod.get_ops(2, 64 * n, device)
+    assert told == [([7, 8], 2)] and len(CLS._readers) == CLS.OPS_CACHE_SIZE

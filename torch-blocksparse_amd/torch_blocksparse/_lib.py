@@ -8,6 +8,7 @@ import ctypes
 import importlib.machinery
 import importlib.util
 import os
+import types
 
 import torch
 
@@ -187,6 +188,51 @@ _nothing = _Nothing()
 def on_device(device):
     """a context in which `device` is the current one (launches go to it); costs nothing where it is already"""
     return _nothing if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def tensors_of(operator):
+    """the tensors that an operator of this package holds, in whatever it is made of"""
+    found, seen, open_ = [], dict(), [operator]
+    while open_:
+        x = open_.pop()
+        if id(x) in seen:
+            continue
+        seen[id(x)] = x                                  # (kept, so that the number stays its own)
+        if isinstance(x, torch.Tensor):
+            found.append(x)
+        if isinstance(x, dict):
+            open_.extend(x.values())
+        elif isinstance(x, (list, tuple)):
+            open_.extend(x)
+        elif isinstance(x, types.FunctionType):          # (tables that are made on demand: what the maker has at hand)
+            open_.extend(c.cell_contents for c in x.__closure__ or ())
+        if isinstance(x, torch.Tensor) or type(x).__module__.startswith(__package__):
+            open_.extend(getattr(x, '__dict__', dict()).values())
+    return found
+
+
+class Readers:
+    """The streams that read an operator's tables.  Memory that is given back goes to the stream it was allocated on as soon as nobody holds
+    it; the allocator has to be told of other streams that may still be at work on it."""
+
+    def __init__(self):
+        self.streams, self.tables = dict(), []
+
+    def table(self, *tensors):
+        """tables that the operator keeps from now on"""
+        for t in tensors:
+            if t is not None and t.is_cuda:
+                self.tables.append(t)
+                for stream in list(self.streams.values()):
+                    t.record_stream(stream)
+
+    def read(self, device):
+        """the current stream of `device` reads them, those made later too"""
+        raw = raw_stream(device)
+        if raw not in self.streams:
+            self.streams[raw] = stream = torch.cuda.current_stream(device)
+            for t in list(self.tables):
+                t.record_stream(stream)
 
 
 def ptr(t):

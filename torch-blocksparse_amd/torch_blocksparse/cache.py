@@ -141,7 +141,8 @@ class CacheAttention:
         made = self._rows.get((kv_heads, device))
         if made is None:
             rows, longest = _rows_table(self.layout.cpu(), kv_heads)
-            made = self._rows[kv_heads, device] = (rows.to(device), longest)
+            made = self._rows[kv_heads, device] = (rows.to(device), longest, _lib.Readers())
+            made[2].table(made[0])
         return made
 
     def _check(self, q, cache, table, lengths, scale, softcap, slopes):
@@ -183,7 +184,8 @@ class CacheAttention:
         with _lib.on_device(q.device):
             rows, blocks, n_rows = None, table.size(1), 0
             if self.layout is not None:
-                rows, longest = self._table(cache.heads, q.device)
+                rows, longest, readers = self._table(cache.heads, q.device)
+                readers.read(q.device)
                 blocks, n_rows = max(1, min(blocks, longest)), self.layout.size(1)
             splits = lib.bsp_cache_attention_splits(B, H, cache.heads, self.block, blocks)
             need = lib.bsp_cache_attention_workspace_bytes(B, H, cache.heads, D, splits)

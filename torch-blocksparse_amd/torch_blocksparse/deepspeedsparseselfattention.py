@@ -16,6 +16,7 @@ import threading
 import torch
 import torch.nn as nn
 
+from . import _lib
 from .attention_core import attention_chain
 from .cache import CacheAttention
 from .layouts import fixed_layout
@@ -50,7 +51,8 @@ class DeepSpeedSparseSelfAttention(nn.Module):
     # more than OPS_CACHE_SIZE of the kind are held.
     ops = collections.OrderedDict()
     OPS_CACHE_SIZE = 16
-    _lock = threading.RLock()                            # of `ops` and `captured`
+    _lock = threading.RLock()                            # of `ops`, `captured` and `_readers`
+    _readers = dict()                                    # of the chain's operators (those with rules and of decoding know their own)
 
     @staticmethod
     def _drop_the_oldest(key):
@@ -58,12 +60,15 @@ class DeepSpeedSparseSelfAttention(nn.Module):
         cache, kind = DeepSpeedSparseSelfAttention.ops, lambda k: k[0] if isinstance(k[0], str) else 'chain'
         alike = [k for k in cache if kind(k) == kind(key)]
         for old in alike[:-DeepSpeedSparseSelfAttention.OPS_CACHE_SIZE]:
+            readers = DeepSpeedSparseSelfAttention._readers.pop(old, None)
+            if readers is not None:
+                readers.table(*_lib.tensors_of(cache[old]))
             del cache[old]
 
     def get_ops(self, H, L, device=None):
         cfg = self.sparsity_config
         key = (H, L, str(device)) + cfg.key()
-        return self._held(key, lambda: self._chain(H, L, device))
+        return self._held(key, lambda: self._chain(H, L, device), device)
 
     def _chain(self, H, L, device):
         cfg = self.sparsity_config
@@ -85,8 +90,8 @@ class DeepSpeedSparseSelfAttention(nn.Module):
     captured = dict()
 
     @staticmethod
-    def _held(key, make):
-        """what `ops` holds under `key`, made where it holds nothing"""
+    def _held(key, make, device=None):
+        """what `ops` holds under `key`, made where it holds nothing, for the current stream of `device`"""
         cls = DeepSpeedSparseSelfAttention
         with cls._lock:
             if key not in cls.ops:
@@ -95,6 +100,11 @@ class DeepSpeedSparseSelfAttention(nn.Module):
             cls.ops.move_to_end(key)
             if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
                 cls.captured[key] = cls.ops[key]
+            if isinstance(device, torch.device) and device.type == 'cuda' and device.index is not None:
+                readers = cls._readers.get(key)
+                if readers is None:
+                    readers = cls._readers[key] = _lib.Readers()
+                readers.read(device)
             return cls.ops[key]
 
     def _kept(self, kind, H, num_blocks, make):

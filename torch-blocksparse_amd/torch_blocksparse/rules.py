@@ -72,6 +72,8 @@ class _Tables:
         self.lines = info.lines
         self.rows = host[:info.items_offset].to(device)
         self._columns, self._chosen = dict(), dict()
+        self.readers = _lib.Readers()
+        self.readers.table(self.rows)
 
     def _build(self, lay):
         H, R, C = lay.shape
@@ -123,6 +125,7 @@ class _Tables:
             part //= 2
         if part not in made:
             made[part] = self._cut(heads, first, count, entries, part)
+            self.readers.table(made[part][0], made[part][2])
         return made[part]
 
     def _cut(self, heads, first, count, entries, part):
@@ -242,6 +245,11 @@ class Attention:
             made = self._tables[device] = _Tables(self.layout, self.block, device)
         return made
 
+    def _tables_for_a_launch(self, device):
+        made = self.tables(device)
+        made.readers.read(device)
+        return made
+
     def __getstate__(self):
         return dict(self.__dict__, _tables=dict())
 
@@ -288,4 +296,4 @@ class Attention:
         if documents is not None and documents.size(1) > 1 and documents.stride(1) != 1:
             documents = documents.contiguous()
         with _lib.on_device(q.device):
-            return _rules.apply(q, k, v, self.tables(q.device), scale, softcap, slopes, bool(causal), documents, prefix, torch.is_grad_enabled())
+            return _rules.apply(q, k, v, self._tables_for_a_launch(q.device), scale, softcap, slopes, bool(causal), documents, prefix, torch.is_grad_enabled())
