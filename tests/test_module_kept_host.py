@@ -127,3 +127,15 @@ def test_a_dropped_chain_tells_its_tables(empty, monkeypatch):
     for n in range(2, 2 + CLS.OPS_CACHE_SIZE):
         mod.get_ops(2, 64 * n, device)
     assert told == [([7, 8], 2)] and len(CLS._readers) == CLS.OPS_CACHE_SIZE
+
+
+def test_decoding_without_a_layout_makes_none(empty, monkeypatch):
+    mod = tb.SparseSelfAttention(tb.SparsityConfig('dense', block=16, stride=64))
+    sizes, used = [], []
+    make = CLS._make_layout
+    monkeypatch.setattr(CLS, '_make_layout', staticmethod(lambda H, blocks, *args, **k: sizes.append(blocks) or make(H, blocks, *args, **k)))
+    monkeypatch.setattr(tb.CacheAttention, '__call__', lambda self, q, cache, table, lengths, **rules: used.append(self) or q)
+    q, lengths = torch.zeros(1, 16, 64, dtype=torch.float16), torch.ones(1, dtype=torch.int32)
+    for width in (1, 7, 300, 1 << 19):
+        mod.decode(q, None, torch.zeros(1, 1, dtype=torch.int32).expand(1, width), lengths)
+    assert used == [used[0]] * 4 and used[0].layout is None and not any(sizes)

@@ -177,7 +177,11 @@ class DeepSpeedSparseSelfAttention(nn.Module):
         if query.dim() != 3 or table.dim() != 2:
             raise ValueError('query must have shape [batch, heads, head_dim], table [batch, width]')
         cfg = self.sparsity_config
-        op = self._kept('decode', query.size(1), table.size(1), lambda layout: CacheAttention(cfg.block, None if cfg.mode == 'dense' else layout))
+        if cfg.mode == 'dense':                          # (no layout is needed where everything is seen)
+            blocks, make = 0, lambda layout: CacheAttention(cfg.block)
+        else:
+            blocks, make = table.size(1), lambda layout: CacheAttention(cfg.block, layout)
+        op = self._kept('decode', query.size(1), blocks, make)
         return op(query, cache, table, lengths, scale=float(query.size(2)) ** -0.5, softcap=softcap, slopes=slopes)
 
 
