@@ -141,3 +141,26 @@ def test_tables_are_not_given_away_while_another_stream_reads_them():
         assert not any(a < d and c < b for a, b in places for c, d in new), name
         stream.synchronize()
         assert torch.equal(got, want[name])
+
+
+@pytest.mark.parametrize('mode,attention', [('fixed', 'unidirectional'), ('fixed', 'bidirectional'), ('dense', 'unidirectional')])
+@pytest.mark.parametrize('width', [1, 3, 16, 17, 39, 130])
+def test_decoding_over_tables_of_all_widths(mode, attention, width):
+    """The same as CacheAttention over the layout of exactly so many blocks: for one direction bit by bit, and where later blocks count as
+    work (that nobody sees) up to the order of sums: 2^-10 of a value for each of the two."""
+    B, H, kv, D, block = 3, 4, 2, 64, 16
+    mod = tb.SparseSelfAttention(tb.SparsityConfig(mode, block, 64, attention, numverts=2))
+    g = torch.Generator().manual_seed(width)
+    cache = tb.KeyValueCache(B * width, block, kv, D, bits=8)
+    k, v = [torch.randn(B * width * block, kv, D, generator=g).half().to(DEV) for _ in range(2)]
+    cache.write(k, v, torch.arange(B * width * block, dtype=torch.int32, device=DEV))
+    table = torch.randperm(B * width, generator=g).int().view(B, width).to(DEV)
+    q = torch.randn(B, H, D, generator=g).half().to(DEV)
+    lengths = torch.tensor([width * block, 1 + width * block // 2, width * block + 99], dtype=torch.int32, device=DEV)
+    lay = None if mode == 'dense' else tb.fixed_layout(H, -(-width // 4) * 4, mode, 4, attention, 2, 1)[:, :width, :width]
+    want = tb.CacheAttention(block, lay)(q, cache, table, lengths, scale=D ** -0.5, softcap=9.)
+    got = mod.decode(q, cache, table, lengths, softcap=9.)
+    if attention == 'unidirectional':
+        assert torch.equal(got, want)
+    else:
+        assert float((got.float() - want.float()).abs().max()) <= 2 * 2. ** -10 * float(v.abs().max())

@@ -129,6 +129,25 @@ def test_a_dropped_chain_tells_its_tables(empty, monkeypatch):
     assert told == [([7, 8], 2)] and len(CLS._readers) == CLS.OPS_CACHE_SIZE
 
 
+@pytest.mark.parametrize('attention', ['unidirectional', 'bidirectional'])
+@pytest.mark.parametrize('stride,numverts,vertsize', [(64, 1, 1), (64, 2, 2), (112, 7, 1)])
+def test_a_table_of_pages_that_grows_finds_its_operator(empty, monkeypatch, attention, stride, numverts, vertsize):
+    mod = tb.SparseSelfAttention(tb.SparsityConfig(block=16, stride=stride, attention=attention, numverts=numverts, vertsize=vertsize))
+    used = []
+    monkeypatch.setattr(tb.CacheAttention, '__call__', lambda self, q, cache, table, lengths, **rules: used.append(self) or q)
+    H, window = 9, stride // 16
+    q, lengths = torch.zeros(1, H, 64, dtype=torch.float16), torch.ones(1, dtype=torch.int32)
+    for width in range(1, 257):
+        mod.decode(q, None, torch.zeros(1, width, dtype=torch.int32), lengths)
+        lay = used[-1].layout
+        # ... at most a quarter longer (short ones: sixteen blocks), with what each position of the table sees
+        assert tuple(lay.shape) == (H,) + (lay.size(1),) * 2 and width <= lay.size(1) <= max(width + 15, 1.25 * width)
+        if width % 37 == 0:
+            exact = tb.fixed_layout(H, -(-width // window) * window, 'fixed', window, attention, numverts, vertsize)[:, :width, :width]
+            assert torch.equal(lay[:, :width, :width].long(), exact)
+    assert len({id(op) for op in used}) <= 16
+
+
 def test_decoding_without_a_layout_makes_none(empty, monkeypatch):
     mod = tb.SparseSelfAttention(tb.SparsityConfig('dense', block=16, stride=64))
     sizes, used = [], []
@@ -139,3 +158,13 @@ def test_decoding_without_a_layout_makes_none(empty, monkeypatch):
     for width in (1, 7, 300, 1 << 19):
         mod.decode(q, None, torch.zeros(1, 1, dtype=torch.int32).expand(1, width), lengths)
     assert used == [used[0]] * 4 and used[0].layout is None and not any(sizes)
+
+
+def test_the_widest_layout_of_pages_is_made(empty, monkeypatch):
+    mod = tb.SparseSelfAttention(tb.SparsityConfig(block=16, stride=16))
+    widths = []
+    monkeypatch.setattr(CLS, '_kept', lambda self, kind, H, blocks, make: widths.append(blocks) or (lambda *a, **k: None))
+    q, lengths = torch.zeros(1, 1, 64, dtype=torch.float16), torch.ones(1, dtype=torch.int32)
+    for width in (40000, 57344, 57345, 65535, 65536):
+        mod.decode(q, None, torch.zeros(1, 1, dtype=torch.int32).expand(1, width), lengths)
+    assert widths == [40960, 57344, 65535, 65535, 65536]

@@ -140,8 +140,9 @@ class CacheAttention:
     def _table(self, kv_heads, device):
         made = self._rows.get((kv_heads, device))
         if made is None:
-            rows, longest = _rows_table(self.layout.cpu(), kv_heads)
-            made = self._rows[kv_heads, device] = (rows.to(device), longest, _lib.Readers())
+            layout = self.layout.cpu()
+            longest = (layout != 0).any(0).sum(1).cummax(0).values.tolist()       # the most entries of the rows up to each
+            made = self._rows[kv_heads, device] = (_rows_table(layout, kv_heads)[0].to(device), longest, _lib.Readers())
             made[2].table(made[0])
         return made
 
@@ -186,7 +187,8 @@ class CacheAttention:
             if self.layout is not None:
                 rows, longest, readers = self._table(cache.heads, q.device)
                 readers.read(q.device)
-                blocks, n_rows = max(1, min(blocks, longest)), self.layout.size(1)
+                n_rows = self.layout.size(1)
+                blocks = max(1, min(blocks, longest[min(blocks, n_rows) - 1]))
             splits = lib.bsp_cache_attention_splits(B, H, cache.heads, self.block, blocks)
             need = lib.bsp_cache_attention_workspace_bytes(B, H, cache.heads, D, splits)
             workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None

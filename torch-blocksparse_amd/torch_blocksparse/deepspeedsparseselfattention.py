@@ -116,8 +116,9 @@ class DeepSpeedSparseSelfAttention(nn.Module):
             if block_stride != cfg.stride / cfg.block:
                 raise ValueError('Stride %d must be dividable by block size %d' % (cfg.stride, cfg.block))
             whole = -(-num_blocks // block_stride) * block_stride        # the layout is made of whole windows
-            layout = DeepSpeedSparseSelfAttention._make_layout(H, whole, cfg.mode, block_stride, cfg.attention, cfg.numverts, cfg.vertsize)
-            return make(layout[:, :num_blocks, :num_blocks].to(torch.uint8))
+            alike = min(H, cfg.numverts)                                  # (every numverts-th head has the same one)
+            layout = DeepSpeedSparseSelfAttention._make_layout(alike, whole, cfg.mode, block_stride, cfg.attention, cfg.numverts, cfg.vertsize)
+            return make(layout[:, :num_blocks, :num_blocks].to(torch.uint8)[torch.arange(H) % alike])
 
         return self._held((kind, H, num_blocks) + cfg.key(), operator)
 
@@ -177,10 +178,15 @@ class DeepSpeedSparseSelfAttention(nn.Module):
         if query.dim() != 3 or table.dim() != 2:
             raise ValueError('query must have shape [batch, heads, head_dim], table [batch, width]')
         cfg = self.sparsity_config
-        if cfg.mode == 'dense':                          # (no layout is needed where everything is seen)
+        # Rows of the layout are the same in a longer one, as far as a position sees: one operator serves a quarter of an octave of widths, and a
+        # table that grows by a page finds it made.  Where everything is seen no layout is needed.
+        if cfg.mode == 'dense':
             blocks, make = 0, lambda layout: CacheAttention(cfg.block)
         else:
-            blocks, make = table.size(1), lambda layout: CacheAttention(cfg.block, layout)
+            unit = max(16, 1 << max(0, table.size(1).bit_length() - 3))
+            blocks, make = -(-max(1, table.size(1)) // unit) * unit, lambda layout: CacheAttention(cfg.block, layout)
+            if blocks > 65535 >= table.size(1):
+                blocks = 65535                           # (the longest that CacheAttention takes)
         op = self._kept('decode', query.size(1), blocks, make)
         return op(query, cache, table, lengths, scale=float(query.size(2)) ** -0.5, softcap=softcap, slopes=slopes)
 
