@@ -531,7 +531,7 @@ int bsp_attention_rules_bwd(const bsp_attention_rules_call *call, const void *d_
  * write: k, v: element (t, head, d) at t * stride_t + head * stride_h + d, 16-byte aligned, strides multiples of 8 elements (fp32: 4);
  *   slots: [T]; those outside the cache (negative ones) are left out; of positions with one slot the last is written.  owner: [n_pages *
  *   block] ints, zero before the first call (each call leaves them so).
- * read: k, v: [T, heads, D], contiguous; slots outside the cache give zeros. */
+ * read: k, v: [T, heads, D], contiguous; slots outside the cache give zeros.  A step that was rounded up may take an element past 65504: fp16 has it as 65504. */
 int64_t bsp_cache_page_bytes(int block, int heads, int D, int bits);
 int bsp_cache_write(int dtype, void *pages, int n_pages, int block, int heads, int D, int bits, const void *k, int64_t k_stride_t, int64_t k_stride_h,
                     const void *v, int64_t v_stride_t, int64_t v_stride_h, const int32_t *slots, int T, int32_t *owner, void *stream);

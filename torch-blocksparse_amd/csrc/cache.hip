@@ -172,6 +172,10 @@ template <typename T, int BITS, int D> __global__ void __launch_bounds__(256) k_
       chunk_codes<BITS>(w, p);
 #pragma unroll
       for (int e = 0; e < 8; e++) x[e] = fmaf((float)p[e >> 1][e & 1], step, least);
+      if constexpr (__is_same(T, f16)) {                // (where the rounding of the step takes an element past fp16's range: NaN stays NaN)
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = x[e] > 65504.f ? 65504.f : x[e];
+      }
     }
     T *to = reinterpret_cast<T *>(value ? a.vo : a.ko) + ((int64_t)t * a.heads + head) * D + 8 * j;
     if constexpr (sizeof(T) == 4) {
