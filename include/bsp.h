@@ -540,7 +540,7 @@ int bsp_cache_read(int dtype, const void *pages, int n_pages, int block, int hea
 
 /* Attention of one position a sequence over such a cache: o = softmax(y) . v, y_j = softcap * tanh(scale * q . k_j / softcap) - slope_h *
  * (n - 1 - j) (softcap 0: no cap, else 2^-10 .. 1024), over the positions j < n = lengths[b] of the sequence: position j is in page table[b * table_stride
- * + j / block] (numbers outside 0 .. n_pages - 1: not held, not seen).  A length of at most 0 gives zeros, one past width * block (n_rows *
+ * + j / block] (numbers outside 0 .. n_pages - 1: not held, not seen).  Values are rounded to fp16, at most 65504.  A length of at most 0 gives zeros, one past width * block (n_rows *
  * block) counts as that.  q, o: [B, H, D] in fp16 or bf16, q 16-byte aligned with strides that are multiples of 8; query head h uses key head
  * h / (H / kv_heads).  rows: NULL, or what is seen beside that: the query heads of a key head form units of at most 16 (ceil(G / ceil(G / 16)) heads of G each,
  * the last may have fewer); per unit n_rows + 1 ints, from rows[0] on: the place in `rows` of the first entry of each block-row of the unit's

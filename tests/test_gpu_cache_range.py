@@ -1,11 +1,11 @@
-"""GPU: the quantised cache at the ends of float16's range."""
+"""GPU: the quantised cache and attention over it at the ends of float16's range."""
 import math
 
 import pytest
 import torch
 
 import torch_blocksparse as tb
-from test_gpu_cache import quantised
+from test_gpu_cache import check, oracle, quantised
 
 pytestmark = pytest.mark.gpu
 DEV = 'cuda'
@@ -39,3 +39,39 @@ def test_what_is_finite_reads_back_finite(bits, dtype):
         once = (want.clamp(max=65504.) if other == torch.float16 else want).float().to(other)
         assert bool(torch.isnan(got[5, 0, 32:]).all()) and int(torch.isnan(got).sum()) == 32
         assert bool(((got == once) | (torch.isnan(got) & torch.isnan(once))).all()) and not bool(torch.isinf(got).any())
+
+
+@pytest.mark.parametrize('bits', [4, 8])
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('H,kv', [(2, 2), (7, 1), (16, 1)])
+def test_decoding_over_values_at_the_ends(bits, D, dtype, H, kv):
+    """... and attention takes them as 65504 too: where a head's share is nothing, or its layout hides the block that another head of the
+    workgroup sees, nothing comes of them."""
+    B, block, width = 2, 16, 4
+    T = B * width * block
+    k, v = saturated(T, kv, D, dtype, 3)
+    cache = tb.KeyValueCache(B * width, block, kv, D, bits=bits)
+    cache.write(k, v, torch.arange(T, dtype=torch.int32, device=DEV))
+    table = torch.arange(B * width, dtype=torch.int32, device=DEV).view(B, width)
+    g = torch.Generator().manual_seed(7)
+    q = (40 * torch.randn(B, H, D, generator=g)).to(dtype).to(DEV)            # (most shares are below 2^-24)
+    lengths = torch.tensor([64, 51], dtype=torch.int32, device=DEV)
+    lay = torch.ones(H, width, width, dtype=torch.int64)
+    lay[::2, :, 1] = 0
+    lay[1::2, :, 2] = 0
+    (kq, step, least), vq = quantised(k, bits), quantised(v, bits)[0].clamp(max=65504.)
+    held = [t.view(B, -1, kv, D) for t in (kq, vq, least, step)]
+    everything = torch.ones(B, width * block, dtype=torch.bool)
+    for layout in (None, lay):
+        for scale in (1., 1e-4):
+            o = tb.CacheAttention(block, layout)(q, cache, table, lengths, scale=scale)
+            out, bound = oracle(q, *held[:2], held[2], held[3], bits, lengths, layout, block, scale, 0., None, everything)
+            # a result in fp16 whose bound reaches past the type's range may be infinite: from above it is held to nothing, from below, as any
+            # result, to |got| >= |out| - bound (sums of values of both signs may have a bound that is wide)
+            fits = (out.abs() + bound <= 65504.) if dtype == torch.float16 else torch.ones_like(out, dtype=torch.bool)
+            assert bool(fits.float().mean() > 0.5)
+            got = o.double().cpu()
+            assert not bool(torch.isnan(got).any())
+            check(torch.where(fits, got, out), (out, bound), 'scale %g' % scale)
+            assert bool((got.abs() >= out.abs() - bound)[~fits].all())

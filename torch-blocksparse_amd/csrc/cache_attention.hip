@@ -10,7 +10,7 @@
 // The codes are operands as they are, bit patterns of fp16 numbers below the normal ones, so a score is the sum over the groups of step * (q . codes) +
 // least * (sum of the group's q), the products on the matrix units (16 x 16 x 32: a group each).  q is scaled by a power of two per head to the
 // range of fp16, which loses nothing that 2^-35 of its largest element would not.  Values are v = least + code * step rounded to fp16
-// (2^-12 of it, under the rounding of the shares) through LDS, where the product with the shares reads them transposed.
+// (2^-12 of it, under the rounding of the shares; 65504 at most) through LDS, where the product with the shares reads them transposed.
 //
 // Measured: sixteen sequences of up to 16384 positions, 32 query heads of 128 on 8 key heads, 4 bits (218 MB of pages): 51 us with the join, 4.3 TB/s
 // (all of 16384 positions: 64 us, 5.2 TB/s, the rate of a copy);
@@ -206,6 +206,7 @@ __global__ void __launch_bounds__(256, 3) k_cache_attention(DecodeArgs a, int dt
       // scores and values of the pair
       float y[2][V];
       uint32_t seen = 0;                                  // bit 4 u + j
+      uint32_t most = 0;                                  // the greatest step and the greatest least value of the lane's groups, if above zero (or NaN)
 #pragma unroll
       for (int u = 0; u < 2; u++) {
         const bool here = key < tile[u].n;                // what lies behind the sequence's end stands for zeros (looked at here and not where it is loaded, which would be waiting for it)
@@ -245,7 +246,12 @@ __global__ void __launch_bounds__(256, 3) k_cache_attention(DecodeArgs a, int dt
           for (int i = 0; i < 4; i++) v.h[i] = __builtin_elementwise_fma(p[i], f16x2{step, step}, f16x2{least, least});
           *reinterpret_cast<u32x4 *>(values + (16 * u + key) * L::VROW + 64 * g + 16 * c) = v.w;
         }
+#pragma unroll
+        for (int g = 0; g < GR; g += 2) asm("v_pk_maximum3_f16 %0, %0, %1, %2" : "+v"(most) : "v"(raw[u].vm[g]), "v"(raw[u].vm[g + 1]));
       }
+      // A step that was rounded up takes the last codes of a group that reaches the end of fp16's range past it: 65504 then, not infinity, which would make
+      // NaN of every share that is zero.  least + (2^BITS - 1) * step > 65504 takes a step or a least value of half of that.
+      const bool large = __builtin_amdgcn_ballot_w64((most & 0xffffu) >= (BITS == 4 ? 0x6800u : 0x5800u) || most >= 0x78000000u) != 0;    // (2048, 128; 32768)
       // the next pair on its way (into the registers that the scores have come from)
 #pragma unroll
       for (int u = 0; u < 2; u++)
@@ -280,19 +286,33 @@ __global__ void __launch_bounds__(256, 3) k_cache_attention(DecodeArgs a, int dt
       bool move = false;
 #pragma unroll
       for (int j = 0; j < V; j++) move |= sum[j] > 8192.f || (m[j] == -INFINITY && (seen & (0x11u << j)));
-      if (__builtin_amdgcn_ballot_w64(move)) {
+      const uint64_t moves = __builtin_amdgcn_ballot_w64(move);
+      if (large || moves) {                               // (one branch in the usual case)
+        if (moves) {
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-          float top = fmaxf(seen >> j & 1 ? y[0][j] : -INFINITY, seen >> (4 + j) & 1 ? y[1][j] : -INFINITY);
+          for (int j = 0; j < V; j++) {
+            float top = fmaxf(seen >> j & 1 ? y[0][j] : -INFINITY, seen >> (4 + j) & 1 ? y[1][j] : -INFINITY);
 #pragma unroll
-          for (int d = 1; d < 16; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-          const float mn = fmaxf(m[j], top), f = __builtin_amdgcn_exp2f(m[j] - (mn == -INFINITY ? 0.f : mn));
-          l[j] *= f;
+            for (int d = 1; d < 16; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+            const float mn = fmaxf(m[j], top), f = __builtin_amdgcn_exp2f(m[j] - (mn == -INFINITY ? 0.f : mn));
+            l[j] *= f;
 #pragma unroll
-          for (int n = 0; n < NT; n++) o[n][j] *= f;
-          m[j] = mn;
+            for (int n = 0; n < NT; n++) o[n][j] *= f;
+            m[j] = mn;
+          }
+          exponentials();
         }
-        exponentials();
+        if (large) {
+#pragma unroll 1
+          for (int n = 0; n < 2 * GR; n++) {
+            union { u32x4 w; f16 h[8]; } v;
+            u32x4 *at = reinterpret_cast<u32x4 *>(values + (16 * (n / GR) + key) * L::VROW + 64 * (n % GR) + 16 * c);
+            v.w = *at;
+#pragma unroll
+            for (int i = 0; i < 8; i++) v.h[i] = v.h[i] > (f16)65504.f ? (f16)65504.f : v.h[i];
+            *at = v.w;
+          }
+        }
       }
 #pragma unroll
       for (int j = 0; j < V; j++) {
