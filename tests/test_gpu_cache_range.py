@@ -75,3 +75,28 @@ def test_decoding_over_values_at_the_ends(bits, D, dtype, H, kv):
             assert not bool(torch.isnan(got).any())
             check(torch.where(fits, got, out), (out, bound), 'scale %g' % scale)
             assert bool((got.abs() >= out.abs() - bound)[~fits].all())
+
+
+@pytest.mark.parametrize('bits', [4, 8])
+@pytest.mark.parametrize('softcap', [0., 9.])
+@pytest.mark.parametrize('exponent', [-120, 100, 117, 118, 122, 126])
+def test_queries_at_the_ends_of_bfloat16(bits, softcap, exponent):
+    """Queries so large (or small) that only the scale makes scores of them, keys that are zero among the others."""
+    B, H, kv, D, block, width = 2, 4, 2, 64, 16, 4
+    T = B * width * block
+    g = torch.Generator().manual_seed(exponent)
+    k, v = [torch.randn(T, kv, D, generator=g).bfloat16().to(DEV) for _ in range(2)]
+    k[::3] = 0.
+    cache = tb.KeyValueCache(B * width, block, kv, D, bits=bits)
+    cache.write(k, v, torch.arange(T, dtype=torch.int32, device=DEV))
+    table = torch.arange(B * width, dtype=torch.int32, device=DEV).view(B, width)
+    q = (torch.rand(B, H, D, generator=g) * 1.9 - 0.95).double().mul(2. ** exponent).bfloat16().to(DEV)
+    q[1, :, 3] = 2. ** exponent
+    lengths = torch.tensor([64, 51], dtype=torch.int32, device=DEV)
+    (kq, step, least), vq = quantised(k, bits), quantised(v, bits)[0]
+    held = [t.view(B, -1, kv, D) for t in (kq, vq, least, step)]
+    everything = torch.ones(B, width * block, dtype=torch.bool)
+    scale = max(2. ** -exponent, 2. ** -100) if exponent > 0 else 2. ** 100
+    for scale in (scale, 2. ** -exponent if exponent > 0 else scale, -scale):
+        o = tb.CacheAttention(block)(q, cache, table, lengths, scale=scale, softcap=softcap)
+        check(o, oracle(q, *held[:2], held[2], held[3], bits, lengths, None, block, scale, softcap, None, everything), 'scale %g' % scale)

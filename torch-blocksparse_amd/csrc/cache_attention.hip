@@ -158,7 +158,8 @@ __global__ void __launch_bounds__(256, 3) k_cache_attention(DecodeArgs a, int dt
   }
 
   // the lane's heads: value j of the lane belongs to the unit's head c * V + j
-  float m[V], l[V], unscale[V], slope[V], qsum[V][GR];
+  const bool capped = a.cap > 0.f;
+  float m[V], l[V], factor[V], slope[V], qsum[V][GR];
   h8 qf[GR];
   {
     float x[GR][8], top = 0.f;
@@ -190,13 +191,13 @@ __global__ void __launch_bounds__(256, 3) k_cache_attention(DecodeArgs a, int dt
 #pragma unroll
     for (int j = 0; j < V; j++) {
       const int r2 = c * V + j, e2 = __shfl(e, 4 * c + j);
-      unscale[j] = ldexpf(1.f, 24 - e2);
+      // what a score is multiplied by: the power of two alone may be past fp32's range, and a product that is turns a score of zero into NaN
+      factor[j] = fminf(fmaxf(ldexpf(capped ? 2.f * kLog2e * a.scale / a.cap : a.scale * kLog2e, 24 - e2), -__FLT_MAX__), __FLT_MAX__);
       m[j] = r2 < heads ? -INFINITY : 0.f;
       l[j] = 0.f;
       slope[j] = a.slopes && r2 < heads ? a.slopes[first + r2] * kLog2e : 0.f;
     }
   }
-  const bool capped = a.cap > 0.f;
   f32x4 o[NT];
 #pragma unroll
   for (int n = 0; n < NT; n++) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -225,12 +226,10 @@ __global__ void __launch_bounds__(256, 3) k_cache_attention(DecodeArgs a, int dt
         const float behind = (float)(len - 1 - tile[u].pos - key);
 #pragma unroll
         for (int j = 0; j < V; j++) {
-          float x = s[j] * unscale[j];
+          float x = s[j] * factor[j];
           if (capped) {
             asm volatile("");                             // (a branch: not computed where there is no cap)
-            x = a.cap * kLog2e * fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * (2.f * kLog2e * a.scale / a.cap)) + 1.f), 1.f);
-          } else {
-            x *= a.scale * kLog2e;
+            x = a.cap * kLog2e * fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x) + 1.f), 1.f);
           }
           y[u][j] = fmaf(-slope[j], behind, x);
           seen |= (here && (tile[u].mask >> (c * V + j) & 1)) ? 1u << (4 * u + j) : 0u;
