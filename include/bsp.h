@@ -527,7 +527,7 @@ int bsp_attention_rules_bwd(const bsp_attention_rules_call *call, const void *d_
  * heads of D = 64 or 128 elements in `bits` = 4 or 8: bsp_cache_page_bytes bytes, pages back to back at a 16-byte aligned address.
  * Position `at` of page p is slot p * block + at.  Of 32 neighbouring elements, taken into [-65504, 65504], least = fp16(min), step =
  * fp16((max - least) / (2^bits - 1)), code = (x - least) / step to the nearest integer, ties to even, in 0 .. 2^bits - 1 (0 where step is 0),
- * all in exact arithmetic; the element then is least + code * step.  A group with a NaN becomes NaN.  How they lie in a page: csrc/cache.h.
+ * all in exact arithmetic but for step's quotient, which is rounded to fp32 and then to fp16 (it is below zero where least is rounded up past the max); the element then is least + code * step.  A group with a NaN becomes NaN.  How they lie in a page: csrc/cache.h.
  * write: k, v: element (t, head, d) at t * stride_t + head * stride_h + d, 16-byte aligned, strides multiples of 8 elements (fp32: 4);
  *   slots: [T]; those outside the cache (negative ones) are left out; of positions with one slot the last is written.  owner: [n_pages *
  *   block] ints, zero before the first call (each call leaves them so).

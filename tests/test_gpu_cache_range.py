@@ -100,3 +100,25 @@ def test_queries_at_the_ends_of_bfloat16(bits, softcap, exponent):
     for scale in (scale, 2. ** -exponent if exponent > 0 else scale, -scale):
         o = tb.CacheAttention(block)(q, cache, table, lengths, scale=scale, softcap=softcap)
         check(o, oracle(q, *held[:2], held[2], held[3], bits, lengths, None, block, scale, softcap, None, everything), 'scale %g' % scale)
+
+
+@pytest.mark.parametrize('bits', [4, 8])
+@pytest.mark.parametrize('D', [64, 128])
+def test_groups_whose_least_value_is_rounded_up_past_them(bits, D):
+    """Elements closer together than float16's numbers: the least value rounded to float16 may lie above all of them, and the step below zero."""
+    g = torch.Generator().manual_seed(5)
+    base = torch.tensor([1000.3, 1000.1, -1000.1, 0.1, 65500., -65490., 3e-8, 12.003, -7.7e-5, 1 / 3])
+    spread = torch.tensor([0., 2. ** -15, 2. ** -13, 2. ** -12, 2. ** -11])
+    x = (base[:, None, None] * (1 + spread[:, None] * torch.rand(len(base), len(spread), D, generator=g))).view(-1, 1, D)
+    cache = tb.KeyValueCache(4, 16, 1, D, bits=bits)
+    slots = torch.arange(x.size(0), dtype=torch.int32, device=DEV)
+    cache.write(x.to(DEV), x.flip(0).to(DEV), slots)
+    # from the definition (a code is 0 where the step is 0), in 64 bits
+    groups, most = x.double().clamp(-65504., 65504.).unflatten(-1, (-1, 32)), 2 ** bits - 1
+    least = groups.amin(-1, keepdim=True).float().half().double()
+    step = ((groups.amax(-1, keepdim=True) - least) / most).float().half().double()
+    assert 10 < int((step < 0).sum()) < step.numel() - 10
+    code = torch.where(step != 0, ((groups - least) / torch.where(step != 0, step, 1.)).round().clamp(0, most), 0.)
+    want = (least + code * step).flatten(-2)
+    for got, value in zip(cache.read(slots, torch.float32), (want, want.flip(0))):
+        assert torch.equal(got.double().cpu(), value.float().double())

@@ -1,7 +1,7 @@
 // Keys and values into the pages of a quantised cache, and back (layout: cache.h).
 //
 // Of 32 neighbouring elements x (taken into [-65504, 65504], the range of fp16) least = fp16(min x), step = fp16((max x - least) /
-// (2^bits - 1)), code = the integer nearest to (x - least) / step, ties to the even one, within 0 .. 2^bits - 1.  A group with a NaN
+// (2^bits - 1)), code = the integer nearest to (x - least) / step, ties to the even one, within 0 .. 2^bits - 1; step's quotient is rounded to fp32 first, and below zero where least is rounded up past the max.  A group with a NaN
 // reads back as NaN.  The codes are those of exact arithmetic: a quotient is computed in fp32 and, where that lies close to the middle of two
 // integers, decided in 64 bits.
 //
@@ -108,7 +108,7 @@ template <typename T, int BITS, int D, bool SCAN> __global__ void __launch_bound
     if (bad != 0.f) least = __builtin_bit_cast(f16, (uint16_t)0x7e00), step = (f16)0.f;
     const float l32 = (float)least, s32 = (float)step;
     uint32_t w[2] = {0u, 0u};
-    if (s32 > 0.f) {
+    if (s32 != 0.f) {                                   // (below zero where the least value was rounded up past the greatest one)
       // the quotient rounded in the low bits of 1.5 * 2^23 + it
       const float inv = __builtin_amdgcn_rcpf(s32), magic = 12582912.f;
       uint32_t code[8];
@@ -121,11 +121,11 @@ template <typename T, int BITS, int D, bool SCAN> __global__ void __launch_bound
       }
       // x - least is off by 2^-24 of itself, the reciprocal by 2^-23, so the quotient by 3 * 2^-24 * MOST: decided in 64 bits where the middle is as near
       if (off > 0.5f - MOST * 0x1p-22f) {
-        const double h = 0.5 * (double)s32;
+        const double h = 0.5 * fabs((double)s32);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           const int n0 = (int)(code[e] & 0x1ffu);
-          const double rem = ((double)x[e] - (double)l32) - (double)n0 * (double)s32;
+          const double rest = ((double)x[e] - (double)l32) - (double)n0 * (double)s32, rem = s32 < 0.f ? -rest : rest;
           const bool odd = n0 & 1;
           const int m = n0 + (rem > h || (rem == h && odd) ? 1 : 0) - (rem < -h || (rem == -h && odd) ? 1 : 0);
           code[e] = (uint32_t)(m < 0 ? 0 : m > MOST ? MOST : m);

@@ -9,7 +9,7 @@ its row of the layout names, and reads no other.
     o = CacheAttention(block, layout)(q, cache, table, lengths, scale=head_dim ** -0.5)     # q, o [batch, query heads, head_dim]
 
 In the cache 32 neighbouring elements of a head share a least value and a step, both float16: least = min x, step = (max x - least) /
-(2^bits - 1), and an element is least + code * step with the nearest code (ties to the even one), in exact arithmetic.  Elements are taken into
+(2^bits - 1), and an element is least + code * step with the nearest code (ties to the even one), in exact arithmetic (the step is below zero where the least value is rounded up past all of them).  Elements are taken into
 float16's range first; where the rounding of a step takes one past it again, float16 reads 65504 and attention takes a value as 65504.  A group with a NaN reads back as NaN.  A position of a head takes 5 / 8 (4 bits) or 9 / 8 (8 bits) bytes an element.
 """
 import torch
