@@ -84,8 +84,8 @@ __device__ __forceinline__ i32x4r move_buffer(const i32x4r &b, const char *p) { 
 // load_to_lds from a buffer
 template <int BYTES> __device__ __forceinline__ void buffer_to_lds(const i32x4r &rsrc, uint32_t off, uint32_t add, uint32_t dst) {
   uint32_t at;                                            // (the addition also is the instruction that must lie between m0 and its use)
-  if constexpr (BYTES == 16) asm volatile("s_mov_b32 m0, %4\n\tv_add_u32 %0, %2, %1\n\tbuffer_load_dwordx4 %0, %3, 0 offen lds" : "=&v"(at) : "v"(off), "s"(add), "s"(rsrc), "s"(dst) : "memory");
-  else asm volatile("s_mov_b32 m0, %4\n\tv_add_u32 %0, %2, %1\n\tbuffer_load_dword %0, %3, 0 offen lds" : "=&v"(at) : "v"(off), "s"(add), "s"(rsrc), "s"(dst) : "memory");
+  if constexpr (BYTES == 16) asm volatile("s_mov_b32 m0, %4\n\tv_add_u32 %0, %2, %1\n\tbuffer_load_dwordx4 %0, %3, 0 offen lds" : "=&v"(at) : "v"(off), "s"(add), "s"(rsrc), "s"(dst) : "m0", "memory");
+  else asm volatile("s_mov_b32 m0, %4\n\tv_add_u32 %0, %2, %1\n\tbuffer_load_dword %0, %3, 0 offen lds" : "=&v"(at) : "v"(off), "s"(add), "s"(rsrc), "s"(dst) : "m0", "memory");
 }
 
 // Sixteen consecutive rows, global -> LDS.  Rows behind the last one come as zeros.
