@@ -221,7 +221,7 @@ class Attention:
 
     scale     factor of the scores
     softcap   0 for none, else the scores are softcap * tanh(scale * q . k / softcap); 2^-10 to 1024
-    slopes    None, or [heads] float32: slopes[h] * |i - j| is taken off the scores (constants: no gradient)
+    slopes    None, or [heads] float32: slopes[h] * |i - j| is taken off the scores (constants: refused where they require a gradient, but under no_grad)
     causal    row i sees the keys up to i only
     documents None, or [batch, length] int32: a row sees keys of its own document only; negative: padding
     prefix    None, or [batch] int32, with causal: keys before prefix[z] are seen by every row
@@ -281,7 +281,7 @@ class Attention:
         for name, t, shape, dtype in (('slopes', slopes, (H,), torch.float32), ('documents', documents, (Z, L), torch.int32), ('prefix', prefix, (Z,), torch.int32)):
             if t is not None and (tuple(t.shape) != shape or t.dtype != dtype or t.device != q.device):
                 raise ValueError('%s must be %s %s on %s (got %s %s on %s)' % (name, dtype, list(shape), q.device, t.dtype, list(t.shape), t.device))
-        if slopes is not None and slopes.requires_grad:
+        if slopes is not None and slopes.requires_grad and torch.is_grad_enabled():
             raise ValueError('slopes are constants: they get no gradient')
 
     def __call__(self, q, k, v, scale=1., softcap=0., slopes=None, causal=False, documents=None, prefix=None):
