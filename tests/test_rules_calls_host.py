@@ -1,4 +1,4 @@
-"""CPU: slopes that are a parameter of the model: refused where a gradient would be expected of them, taken where none is."""
+"""CPU: calls of Attention that launch nothing, and slopes that are a parameter of the model."""
 import pytest
 import torch
 
@@ -21,3 +21,14 @@ def test_slopes_that_are_a_parameter(monkeypatch):
         with torch.inference_mode():
             check(slopes, q_grad)
         check(slopes.detach(), q_grad)
+
+
+@pytest.mark.parametrize('Z,L', [(0, 40), (2, 0), (0, 0)])
+def test_no_positions_or_no_sequences(monkeypatch, Z, L):
+    monkeypatch.setattr(tb.rules._lib, 'require_gpu_tensor', lambda t, what: None)
+    q, k, v = [torch.zeros(Z, h, L, 64, dtype=torch.float16, requires_grad=True) for h in (4, 2, 2)]
+    blocks = -(-L // 16)
+    o = tb.Attention(torch.ones(4, blocks, blocks), 16)(q, k, v, causal=True, documents=torch.zeros(Z, L, dtype=torch.int32))
+    assert o.shape == q.shape and o.dtype == q.dtype
+    grads = torch.autograd.grad(o, (q, k, v), torch.zeros_like(o))
+    assert [g.shape for g in grads] == [q.shape, k.shape, v.shape]

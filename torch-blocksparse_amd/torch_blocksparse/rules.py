@@ -287,7 +287,7 @@ class Attention:
     def __call__(self, q, k, v, scale=1., softcap=0., slopes=None, causal=False, documents=None, prefix=None):
         scale, softcap = float(scale), float(softcap or 0.)
         self._check(q, k, v, softcap, scale, slopes, causal, documents, prefix)
-        if q.size(0) == 0:
+        if q.numel() == 0:
             return torch.empty_like(q) + 0 * (q.sum() + k.sum() + v.sum())
         if slopes is not None:
             slopes = slopes.contiguous()
