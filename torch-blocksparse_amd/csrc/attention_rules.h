@@ -391,12 +391,6 @@ template <bool BIAS> struct Logits {
       }
     }
   }
-  // the logit of score i (STRAIGHT: of a wavefront whose scores lie on one side)
-  template <bool STRAIGHT> __device__ __forceinline__ float one(int i, float s, float out, float minus) const {
-    if constexpr (!BIAS) return fmaf(s, out, -minus);
-    else if constexpr (STRAIGHT) return fmaf(s, out, fmaf(slope[i >> 3], (float)(i & 7), base[i >> 3] - minus));
-    else return fmaf(s, out, fmaf(-slope[i >> 3], fabsf(base[i >> 3] - (float)(i & 7)), -minus));
-  }
   // y(i) for i = 0 .. 15, minus(i) a value per score (a constant, usually)
   template <class S, class M> __device__ __forceinline__ void get(float (&y)[16], const S &s, float out, M &&minus) const {
     if constexpr (!BIAS) {
