@@ -492,7 +492,7 @@ int bsp_attention_f32_bwd(const bsp_attention_f32_call *call, const float *d_o, 
  * (where documents is not NULL); and, with causal, j <= i or j < prefix[z] (prefix NULL: none).  A row that sees no key gets zeros
  * in o and dq.  Positions with a negative document number reach nothing, whatever q, k, v and d_o hold there.  Query head h
  * uses head h / (H / kv_heads) of k and v; their gradients are the sums over the query heads that share them.
- * dtype: any; D = 64 or 128.  length: positions of q, k, v and o, 1 .. 2^24 - 1, any number up to 64 lines.
+ * dtype: any; D = 64 or 128.  length: positions of q, k, v and o, 1 .. 2^24 - 1, any number up to 64 lines; Z * H * lines < 2^25 - 64.
  * strides: of batch, head and row, in elements, three per tensor: q, k, v, o, d_o, dq, dk, dv (those that a call does not use: 0);
  * multiples of 8 elements (fp32: 4), unit inner stride, 16-byte aligned pointers, rows of a head within 4 GiB.
  * d_rows, lines: the table of the lines of bsp_attention_tables_build (blocks of 16, 32, 64; larger ones are given as blocks of 64).
@@ -529,7 +529,7 @@ int bsp_attention_rules_bwd(const bsp_attention_rules_call *call, const void *d_
  * fp16((max - least) / (2^bits - 1)), code = (x - least) / step to the nearest integer, ties to even, in 0 .. 2^bits - 1 (0 where step is 0),
  * all in exact arithmetic but for step's quotient, which is rounded to fp32 and then to fp16 (it is below zero where least is rounded up past the max); the element then is least + code * step.  A group with a NaN becomes NaN.  How they lie in a page: csrc/cache.h.
  * write: k, v: element (t, head, d) at t * stride_t + head * stride_h + d, 16-byte aligned, strides multiples of 8 elements (fp32: 4);
- *   slots: [T]; those outside the cache (negative ones) are left out; of positions with one slot the last is written.  owner: [n_pages *
+ *   slots: [T], T < 2^24; those outside the cache (negative ones) are left out; of positions with one slot the last is written.  owner: [n_pages *
  *   block] ints, zero before the first call (each call leaves them so).
  * read: k, v: [T, heads, D], contiguous; slots outside the cache give zeros.  A step that was rounded up may take an element past 65504: fp16 has it as 65504. */
 int64_t bsp_cache_page_bytes(int block, int heads, int D, int bits);

@@ -1,0 +1,43 @@
+"""CPU: launches of more threads than a grid holds (2^32) are refused before anything is launched."""
+import pytest
+import torch
+
+import torch_blocksparse as tb
+from torch_blocksparse import _lib, rules
+
+UNSUPPORTED = -2
+
+
+def aligned():
+    x = torch.zeros(1 << 14, dtype=torch.uint8)
+    return x, x.data_ptr() + -x.data_ptr() % 16
+
+
+def test_a_cache_call_of_many_positions():
+    """... of which the first of two launches would have left marks that later calls take for their own."""
+    lib, (held, at) = _lib.load(), aligned()
+    for T in (1 << 24, (1 << 31) - 1):
+        assert lib.bsp_cache_write(0, at, 1 << 20, 16, 1, 64, 4, at, 64, 64, at, 64, 64, at, T, at, 0) == UNSUPPORTED
+        assert lib.bsp_cache_read(0, at, 1 << 20, 16, 1, 64, 4, at, at, at, T, 0) == UNSUPPORTED
+
+
+def test_attention_over_a_cache_of_many_sequences():
+    lib, (held, at) = _lib.load(), aligned()
+    for B, kv in ((1 << 24, 1), (1 << 20, 16)):
+        assert lib.bsp_cache_attention(0, at, 64, 64, at, 64, 64, B, kv, at, 1, 16, kv, 64, 4, at, 1, 1, at, 0, 0, 1, 1., 0., 0, 0, 0, 1, 0) == UNSUPPORTED
+
+
+def test_attention_of_many_lines():
+    lib, (held, at) = _lib.load(), aligned()
+    for Z, H, length in ((1 << 25, 1, 64), (1 << 20, 32, 1), (1 << 12, 8, 1 << 16)):
+        lines = (length + 63) // 64
+        call = rules._CALL.pack(0, Z, H, H, lines, 64, length, *([64] * 24), 1., 0., 0, 0, 0, 0, 0, 0, at, 0, 0)
+        assert lib.bsp_attention_rules_fwd(call, at, at, at, at, 0) == UNSUPPORTED
+
+
+def test_too_many_tokens_are_refused_by_name():
+    cache = tb.KeyValueCache.__new__(tb.KeyValueCache)
+    cache.device = torch.device('cpu')
+    with pytest.raises(ValueError, match='tokens'):
+        cache._check_slots(torch.zeros(1, dtype=torch.int32).expand(1 << 24))
+    cache._check_slots(torch.zeros(5, dtype=torch.int32))

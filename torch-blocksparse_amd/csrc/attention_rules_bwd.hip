@@ -456,7 +456,7 @@ extern "C" int bsp_attention_rules_bwd(const bsp_attention_rules_call *call, con
   for (int i = 2; i < 24; i += 3)
     if (!s[i] && (dk || i < 18)) return BSP_ERR_ARG;
   if (dk && (!d_items || n_items <= 0 || n_slots < 0 || n_split < 0 || (n_slots > 0) != (n_split > 0) || (n_slots > 0 && (!partial || !d_split)))) return BSP_ERR_ARG;
-  if (dk && ((int64_t)a.Z * call->kv_heads * n_items >= ((int64_t)1 << 31) - 64 || (int64_t)a.Z * n_split * 16 >= ((int64_t)1 << 31) || a.rows * 2 * a.G >= ((int64_t)1 << 30))) return BSP_ERR_UNSUPPORTED;
+  if (dk && ((int64_t)a.Z * call->kv_heads * n_items >= ((int64_t)1 << 25) - 64 || (int64_t)a.Z * n_split * (32 * call->D) >= ((int64_t)1 << 32) || a.rows * 2 * a.G >= ((int64_t)1 << 30))) return BSP_ERR_UNSUPPORTED;
   a.q = q; a.k = k; a.v = v; a.d_o = d_o; a.o_in = o; a.delta = neg_delta;
   a.oin_sz = s[9]; a.oin_sh = s[10]; a.oin_ld = s[11];
   a.do_sz = s[12]; a.do_sh = s[13]; a.do_ld = s[14];

@@ -221,7 +221,7 @@ int rules_args(const bsp_attention_rules_call *c, RuleArgs &a) {
   if ((c->documents != nullptr) != (c->ranges != nullptr) || (c->prefix && !c->causal)) return BSP_ERR_ARG;
   const int64_t lines = c->lines, unit = c->dtype == BSP_F32 ? 4 : 8, size = c->dtype == BSP_F32 ? 4 : 2;
   if (lines < (c->length + 63) / 64 || lines > (1 << 18)) return BSP_ERR_ARG;
-  if ((int64_t)c->Z * c->H * lines >= ((int64_t)1 << 31) - 64) return BSP_ERR_UNSUPPORTED;
+  if ((int64_t)c->Z * c->H * lines >= ((int64_t)1 << 25) - 64) return BSP_ERR_UNSUPPORTED;   // (a grid has fewer than 2^32 threads, 128 a line)
   for (int i = 0; i < 24; i++)
     if (c->strides[i] % unit) return BSP_ERR_ARG;
   // the rows of q, k, v and do are fetched by byte offsets of 32 bits from a head's first

@@ -216,7 +216,7 @@ int launch_cache(int dtype, const CacheArgs &a, int bits, int D, bool write, hip
 int cache_args(int dtype, const void *pages, int n_pages, int block, int heads, int D, int bits, const int32_t *slots, int T, CacheArgs &a) {
   if (!pages || (reinterpret_cast<uintptr_t>(pages) & 15) || n_pages <= 0 || heads <= 0 || !slots || T <= 0) return BSP_ERR_ARG;
   if (bsp_cache_page_bytes(block, heads, D, bits) <= 0 || (dtype != BSP_F16 && dtype != BSP_BF16 && dtype != BSP_F32)) return BSP_ERR_UNSUPPORTED;
-  if ((int64_t)n_pages * block >= ((int64_t)1 << 31) || (int64_t)T * 2 * heads * (D / 8) >= ((int64_t)1 << 38)) return BSP_ERR_UNSUPPORTED;
+  if ((int64_t)n_pages * block >= ((int64_t)1 << 31) || (int64_t)T * 256 >= ((int64_t)1 << 32)) return BSP_ERR_UNSUPPORTED;   // (a grid has fewer than 2^32 threads)
   a = CacheArgs{};
   a.pages = reinterpret_cast<unsigned char *>(const_cast<void *>(pages));
   a.capacity = (int64_t)n_pages * block;

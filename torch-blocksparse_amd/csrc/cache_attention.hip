@@ -484,7 +484,7 @@ extern "C" int bsp_cache_attention(int dtype, const void *q, int64_t q_stride_b,
   a.G = H / kv_heads;
   a.per = heads_a_unit(a.G);
   a.units = kv_heads * ((a.G + a.per - 1) / a.per);
-  if ((int64_t)B * a.units * splits >= ((int64_t)1 << 31)) return BSP_ERR_UNSUPPORTED;
+  if ((int64_t)B * a.units * splits * 256 >= ((int64_t)1 << 32) || (int64_t)B * H * 64 + 256 >= ((int64_t)1 << 32)) return BSP_ERR_UNSUPPORTED;   // (a grid has fewer than 2^32 threads)
   a.q = q; a.q_sb = q_stride_b; a.q_sh = q_stride_h; a.o = o; a.o_sb = o_stride_b; a.o_sh = o_stride_h;
   a.pages = reinterpret_cast<const unsigned char *>(pages); a.n_pages = n_pages;
   a.table = table; a.table_sb = table_stride; a.width = width; a.lengths = lengths;

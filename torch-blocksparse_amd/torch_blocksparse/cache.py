@@ -43,6 +43,8 @@ class KeyValueCache:
     def _check_slots(self, slots):
         if slots.dim() != 1 or slots.dtype != torch.int32 or slots.device != self.device:
             raise ValueError('slots must be a vector of int32 on %s (got %s %s on %s)' % (self.device, slots.dtype, list(slots.shape), slots.device))
+        if slots.numel() >= 1 << 24:
+            raise ValueError('a call takes fewer than 2^24 tokens (got %d)' % slots.numel())
         return slots.contiguous()
 
     def _operand(self, t, name, tokens):
