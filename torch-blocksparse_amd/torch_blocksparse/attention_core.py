@@ -35,7 +35,7 @@ def _stored_tables(layout, block, ids=None, part=0):
     S = 64 // block
     info = _lib.AttentionTables()
     cap = 2 * H * R + 20 * H * C + (20 if S == 1 else 28 + 2 * S * S) * int(torch.count_nonzero(lay))
-    host = torch.empty(max(cap, 1), dtype=torch.int32)
+    host = torch.empty(max(cap, 1), dtype=torch.int32, device='cpu')
     ids = None if ids is None else ids.to(torch.int32).contiguous()
     _lib.check(_lib.load().bsp_attention_stored_tables_build(_lib.ptr(lay), _lib.ptr(ids), H, R, C, block, part, _lib.ptr(host), cap,
                                                              ctypes.byref(info)), 'bsp_attention_stored_tables_build')
@@ -106,7 +106,7 @@ class _QuadTables:
         info = _lib.AttentionTables()
         blocks = int(torch.count_nonzero(lay))
         cap = 32 * H * (R + C) + 16 * blocks + 64
-        host = torch.empty(cap, dtype=torch.int32)
+        host = torch.empty(cap, dtype=torch.int32, device='cpu')
         _lib.check(lib.bsp_attention_tables_build(_lib.ptr(lay), H, R, C, block, _lib.ptr(host), cap, ctypes.byref(info)),
                    'bsp_attention_tables_build')
         self.rows = host[:info.total].to(device)

@@ -99,12 +99,12 @@ def _rows_table(layout, kv_heads):
     units = [(g * G + u, min(per, G - u)) for g in range(kv_heads) for u in range(0, G, per)]
     starts, entries, at = [], [], len(units) * (R + 1)
     for first, n in units:
-        seen = torch.zeros((R, C), dtype=torch.int64)
+        seen = torch.zeros((R, C), dtype=torch.int64, device='cpu')
         for i in range(n):
             seen |= (layout[first + i] != 0).long() << i
         where = torch.nonzero(seen)
         counts = torch.bincount(where[:, 0], minlength=R)
-        starts.append(torch.cat([torch.zeros(1, dtype=torch.int64), counts.cumsum(0)]) + at)
+        starts.append(torch.cat([torch.zeros(1, dtype=torch.int64, device='cpu'), counts.cumsum(0)]) + at)
         entries.append((where[:, 1] << 16) | seen[where[:, 0], where[:, 1]])
         at += len(where)
     table = torch.cat(starts + entries)

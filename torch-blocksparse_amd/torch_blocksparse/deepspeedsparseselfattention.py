@@ -118,7 +118,7 @@ class DeepSpeedSparseSelfAttention(nn.Module):
             whole = -(-num_blocks // block_stride) * block_stride        # the layout is made of whole windows
             alike = min(H, cfg.numverts)                                  # (every numverts-th head has the same one)
             layout = DeepSpeedSparseSelfAttention._make_layout(alike, whole, cfg.mode, block_stride, cfg.attention, cfg.numverts, cfg.vertsize)
-            return make(layout[:, :num_blocks, :num_blocks].to(torch.uint8)[torch.arange(H) % alike])
+            return make(layout[:, :num_blocks, :num_blocks].to(torch.uint8)[torch.arange(H, device=layout.device) % alike])
 
         return self._held((kind, H, num_blocks) + cfg.key(), operator)
 

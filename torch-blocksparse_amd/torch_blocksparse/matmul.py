@@ -216,7 +216,7 @@ class GroupPlan:
         H, R, C = lay.shape
         n, lib = ctypes.c_int64(0), _lib.load()
         cap = 148 * (int(lay.sum()) // 16 + H * (-(-R // 16)) * (C // 16 + 1))
-        host = torch.empty(cap, dtype=torch.int32)
+        host = torch.empty(cap, dtype=torch.int32, device='cpu')
         _lib.check(lib.bsp_sdd_tiles_build(_lib.ptr(lay), H, R, C, _lib.ptr(host), cap, ctypes.byref(n)), 'bsp_sdd_tiles_build')
         return GroupPlan(host[:148 * n.value].to(device), n.value, R)
 
@@ -236,7 +236,7 @@ class GroupPlan:
         if not always and (L * 8 < -(-L // 16) * 16 * 7 or nnz > .45 * H * R * C):
             return None
         cap = H * -(-L // 16) * (36 + 32 * -(-K // 4)) + 32 * (nnz // 9)      # a chunk has four reduction blocks, or nine blocks of the layout
-        host = torch.empty(cap, dtype=torch.int32)
+        host = torch.empty(cap, dtype=torch.int32, device='cpu')
         _lib.check(lib.bsp_xsd_chunks_build(_lib.ptr(lay), H, R, C, int(rows), _lib.ptr(host), cap, ctypes.byref(groups), ctypes.byref(n)), 'bsp_xsd_chunks_build')
         if not always and nnz < 11 * ((n.value - 4 * groups.value) // 32):
             return None

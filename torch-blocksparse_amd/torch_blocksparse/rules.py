@@ -79,7 +79,7 @@ class _Tables:
         H, R, C = lay.shape
         info = _lib.AttentionTables()
         cap = 32 * H * (R + C) + 16 * int(torch.count_nonzero(lay)) + 64
-        host = torch.empty(cap, dtype=torch.int32)
+        host = torch.empty(cap, dtype=torch.int32, device='cpu')
         _lib.check(_lib.load().bsp_attention_tables_build(_lib.ptr(lay), H, R, C, self.block, _lib.ptr(host), cap, ctypes.byref(info)), 'bsp_attention_tables_build')
         return host, info
 
@@ -113,10 +113,10 @@ class _Tables:
             order = torch.argsort(column * (len(entries) + 1) + (heads[:, 1] - begin) // 8)
             heads, column = heads[order], column[order]
             first = (heads[:, 1].long() - begin) // 8
-            whole = torch.ones(info.n_items, dtype=torch.bool)
+            whole = torch.ones(info.n_items, dtype=torch.bool, device='cpu')
             whole[1:] = column[1:] != column[:-1]
             group = whole.cumsum(0) - 1
-            count = torch.zeros(int(group[-1]) + 1, dtype=torch.long).index_add_(0, group, heads[:, 0].long())
+            count = torch.zeros(int(group[-1]) + 1, dtype=torch.long, device='cpu').index_add_(0, group, heads[:, 0].long())
             tiles = self._columns[kv_heads] = (heads[whole], first[whole], count, entries, dict())
         heads, first, count, entries, made = tiles
         total, n = int(count.sum()), count.numel()
@@ -130,8 +130,8 @@ class _Tables:
 
     def _cut(self, heads, first, count, entries, part):
         parts = ((count + part - 1) // part).clamp(min=1)
-        of = torch.repeat_interleave(torch.arange(count.numel()), parts)
-        k = torch.arange(of.numel()) - (parts.cumsum(0) - parts)[of]
+        of = torch.repeat_interleave(torch.arange(count.numel(), device='cpu'), parts)
+        k = torch.arange(of.numel(), device='cpu') - (parts.cumsum(0) - parts)[of]
         base, rest = (count // parts)[of], (count % parts)[of]
         items = heads[of].clone()
         items[:, 0] = (base + (k < rest)).int()
@@ -146,9 +146,9 @@ class _Tables:
         order = torch.argsort(items[:, 2].long() * (1 << 32) - items[:, 0], stable=True)
         items, number = items[order], torch.bincount(items[:, 2].long(), minlength=kv_heads)
         n_items = int(number.max())
-        rank = torch.arange(of.numel()) - (number.cumsum(0) - number)[items[:, 2].long()]
+        rank = torch.arange(of.numel(), device='cpu') - (number.cumsum(0) - number)[items[:, 2].long()]
         begin = 12 * kv_heads * n_items
-        lists = torch.zeros((kv_heads, n_items, 12), dtype=torch.int32)
+        lists = torch.zeros((kv_heads, n_items, 12), dtype=torch.int32, device='cpu')
         lists[:, :, 1], lists[:, :, 3], lists[:, :, 4] = begin, -1, -1
         lists[items[:, 2].long(), rank] = items
         lists[:, :, 1] += begin * (lists[:, :, 3] >= 0)
