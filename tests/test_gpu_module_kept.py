@@ -164,3 +164,27 @@ def test_decoding_over_tables_of_all_widths(mode, attention, width):
         assert torch.equal(got, want)
     else:
         assert float((got.float() - want.float()).abs().max()) <= 2 * 2. ** -10 * float(v.abs().max())
+
+
+def test_a_cache_is_not_given_away_while_another_stream_writes_it():
+    H, D, block, pages = 2, 64, 16, 64
+    T = pages * block
+    k, v = [torch.randn(T, H, D, device=DEV).half() for _ in range(2)]
+    slots = torch.arange(T, dtype=torch.int32, device=DEV)
+    cache = tb.KeyValueCache(pages, block, H, D, bits=8)
+    cache.write(k, v, slots)
+    want = cache.read(slots)
+    places = addresses([cache.data, cache._owner])
+    torch.cuda.synchronize()
+    stream = busy_stream()
+    with torch.cuda.stream(stream):
+        cache.write(v, k, slots)
+        got = cache.read(slots)
+    del cache
+    gc.collect()
+    fresh = [torch.empty(b - a, dtype=torch.uint8, device=DEV) for _ in range(20) for a, b in places]
+    new = addresses(fresh)
+    assert not stream.query()
+    assert not any(a < d and c < b for a, b in places for c, d in new)
+    stream.synchronize()
+    assert torch.equal(got[0], want[1]) and torch.equal(got[1], want[0])

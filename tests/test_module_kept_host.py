@@ -1,5 +1,6 @@
 """CPU: which operators SparseSelfAttention keeps: each kind has places of its own, and what a captured graph has in it stays."""
 import collections
+import copy
 import threading
 
 import pytest
@@ -89,6 +90,9 @@ class Table:
     def record_stream(self, stream):
         self.told.append(stream)
 
+    def data_ptr(self):
+        return 0
+
 
 def test_tables_are_told_of_every_stream_that_reads_them(monkeypatch):
     now = [1]
@@ -168,3 +172,38 @@ def test_the_widest_layout_of_pages_is_made(empty, monkeypatch):
     for width in (40000, 57344, 57345, 65535, 65536):
         mod.decode(q, None, torch.zeros(1, 1, dtype=torch.int32).expand(1, width), lengths)
     assert widths == [40960, 57344, 65535, 65535, 65536]
+
+
+def bare_cache(monkeypatch):
+    cache = tb.KeyValueCache.__new__(tb.KeyValueCache)
+    cache.__setstate__(dict(pages=4, block=16, heads=2, head_dim=64, bits=4, device=torch.device('cpu'), data=Table(), _owner=Table()))
+    return cache
+
+
+def test_a_cache_tells_its_memory_of_the_streams_that_use_it(monkeypatch):
+    now = [1]
+    monkeypatch.setattr(_lib, 'raw_stream', lambda device: now[0])
+    monkeypatch.setattr(_lib, 'on_device', lambda device: _lib._nothing)
+    monkeypatch.setattr(torch.cuda, 'current_stream', lambda device=None: now[0])
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *args: 0
+    monkeypatch.setattr(_lib, 'load', lambda: Library())
+    cache, slots, k = bare_cache(monkeypatch), torch.zeros(3, dtype=torch.int32), torch.zeros(3, 2, 64)
+    cache.write(k, k, slots)
+    now[0] = 2
+    cache.read(slots)
+    now[0] = 3
+    q, table, lengths = torch.zeros(1, 2, 64, dtype=torch.float16), torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    tb.CacheAttention(16)(q, cache, table, lengths)
+    assert cache.data.told == cache._owner.told == [1, 2, 3]
+
+
+def test_a_cache_can_be_copied(monkeypatch):
+    monkeypatch.setattr(_lib, 'raw_stream', lambda device: 1)
+    monkeypatch.setattr(torch.cuda, 'current_stream', lambda device=None: object())
+    cache = bare_cache(monkeypatch)
+    cache._users.read(cache.device)
+    for other in (copy.deepcopy(cache), copy.copy(cache)):
+        assert other.pages == 4 and other._users is not cache._users and not other._users.streams and other._users.tables == [other.data, other._owner]

@@ -39,6 +39,18 @@ class KeyValueCache:
         self.pages, self.block, self.heads, self.head_dim, self.bits, self.device = int(pages), block, int(heads), head_dim, bits, device
         self.data = torch.zeros((self.pages, _lib.load().bsp_cache_page_bytes(block, self.heads, head_dim, bits)), dtype=torch.uint8, device=device)
         self._owner = torch.zeros(self.pages * block, dtype=torch.int32, device=device)     # (zero between calls: bsp_cache_write)
+        self._note_users()
+
+    def _note_users(self):
+        self._users = _lib.Readers()                       # (the streams of all calls: memory that is given back while one writes it would change under its next owner)
+        self._users.table(self.data, self._owner)
+
+    def __getstate__(self):
+        return {n: x for n, x in self.__dict__.items() if n != '_users'}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._note_users()
 
     def _check_slots(self, slots):
         if slots.dim() != 1 or slots.dtype != torch.int32 or slots.device != self.device:
@@ -73,8 +85,11 @@ class KeyValueCache:
         if T == 0:
             return
         with _lib.on_device(self.device):
+            stream = _lib.raw_stream(self.device)
+            if stream not in self._users.streams:
+                self._users.read(self.device)
             rc = _lib.load().bsp_cache_write(_lib.DTYPES[k.dtype], self.data.data_ptr(), self.pages, self.block, self.heads, self.head_dim, self.bits, k.data_ptr(), k_st, k_sh,
-                                             v.data_ptr(), v_st, v_sh, slots.data_ptr(), T, self._owner.data_ptr(), _lib.raw_stream(self.device))
+                                             v.data_ptr(), v_st, v_sh, slots.data_ptr(), T, self._owner.data_ptr(), stream)
         _lib.check(rc, 'bsp_cache_write')
 
     def read(self, slots, dtype=torch.float16):
@@ -85,8 +100,11 @@ class KeyValueCache:
         k, v = [torch.empty((slots.numel(), self.heads, self.head_dim), dtype=dtype, device=self.device) for _ in range(2)]
         if slots.numel():
             with _lib.on_device(self.device):
+                stream = _lib.raw_stream(self.device)
+                if stream not in self._users.streams:
+                    self._users.read(self.device)
                 rc = _lib.load().bsp_cache_read(_lib.DTYPES[dtype], self.data.data_ptr(), self.pages, self.block, self.heads, self.head_dim, self.bits, k.data_ptr(),
-                                                v.data_ptr(), slots.data_ptr(), slots.numel(), _lib.raw_stream(self.device))
+                                                v.data_ptr(), slots.data_ptr(), slots.numel(), stream)
             _lib.check(rc, 'bsp_cache_read')
         return k, v
 
@@ -185,10 +203,14 @@ class CacheAttention:
         slopes = slopes.detach().contiguous() if slopes is not None else None
         lib = _lib.load()
         with _lib.on_device(q.device):
+            stream = _lib.raw_stream(q.device)
+            if stream not in cache._users.streams:
+                cache._users.read(q.device)
             rows, blocks, n_rows = None, table.size(1), 0
             if self.layout is not None:
                 rows, longest, readers = self._table(cache.heads, q.device)
-                readers.read(q.device)
+                if stream not in readers.streams:
+                    readers.read(q.device)
                 n_rows = self.layout.size(1)
                 blocks = max(1, min(blocks, longest[min(blocks, n_rows) - 1]))
             splits = lib.bsp_cache_attention_splits(B, H, cache.heads, self.block, blocks)
@@ -198,6 +220,6 @@ class CacheAttention:
                                          cache.data.data_ptr(), cache.pages, self.block, cache.heads, D, cache.bits, table.data_ptr(), table.stride(0) if B > 1 else 0,
                                          table.size(1), lengths.data_ptr(), rows.data_ptr() if rows is not None else None, n_rows, blocks, scale, softcap,
                                          slopes.data_ptr() if slopes is not None else None, workspace.data_ptr() if need else None, need, splits,
-                                         _lib.raw_stream(q.device))
+                                         stream)
             _lib.check(rc, 'bsp_cache_attention')
         return o
