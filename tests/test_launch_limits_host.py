@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import torch_blocksparse as tb
-from torch_blocksparse import _lib, rules
+from torch_blocksparse import _lib, cache, rules
 
 UNSUPPORTED = -2
 
@@ -36,8 +36,19 @@ def test_attention_of_many_lines():
 
 
 def test_too_many_tokens_are_refused_by_name():
-    cache = tb.KeyValueCache.__new__(tb.KeyValueCache)
-    cache.device = torch.device('cpu')
+    held = tb.KeyValueCache.__new__(tb.KeyValueCache)
+    held.device = torch.device('cpu')
     with pytest.raises(ValueError, match='tokens'):
-        cache._check_slots(torch.zeros(1, dtype=torch.int32).expand(1 << 24))
-    cache._check_slots(torch.zeros(5, dtype=torch.int32))
+        held._check_slots(torch.zeros(1, dtype=torch.int32).expand(1 << 24))
+    held._check_slots(torch.zeros(5, dtype=torch.int32))
+
+
+def test_a_layout_whose_rows_do_not_fit_32_bits(monkeypatch):
+    """Places in the table of a layout's rows are 32 bits wide: a longer table is refused."""
+    lay = torch.ones(2, 5, 5)
+    whole = cache._rows_table(lay, 2)[0].numel()
+    monkeypatch.setattr(cache, 'MOST_ROWS', whole)
+    assert cache._rows_table(lay, 2)[0].numel() == whole
+    monkeypatch.setattr(cache, 'MOST_ROWS', whole - 1)
+    with pytest.raises(ValueError, match='layout'):
+        cache._rows_table(lay, 2)

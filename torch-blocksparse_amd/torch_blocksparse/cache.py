@@ -109,6 +109,9 @@ class KeyValueCache:
         return k, v
 
 
+MOST_ROWS = 2 ** 31 - 1       # places in the table of a layout's rows are 32-bit numbers
+
+
 def _rows_table(layout, kv_heads):
     """what bsp_cache_attention takes of a layout [H, R, C] (host): per unit of query heads the block-rows' first entries, then the entries"""
     H, R, C = layout.shape
@@ -125,6 +128,8 @@ def _rows_table(layout, kv_heads):
         starts.append(torch.cat([torch.zeros(1, dtype=torch.int64, device='cpu'), counts.cumsum(0)]) + at)
         entries.append((where[:, 1] << 16) | seen[where[:, 0], where[:, 1]])
         at += len(where)
+    if at > MOST_ROWS:
+        raise ValueError('the rows of the layout take %d entries, more than %d' % (at, MOST_ROWS))
     table = torch.cat(starts + entries)
     return torch.where(table >= 1 << 31, table - (1 << 32), table).to(torch.int32), int((layout != 0).any(0).sum(1).max()) if R else 0
 
