@@ -52,3 +52,19 @@ def test_a_layout_whose_rows_do_not_fit_32_bits(monkeypatch):
     monkeypatch.setattr(cache, 'MOST_ROWS', whole - 1)
     with pytest.raises(ValueError, match='layout'):
         cache._rows_table(lay, 2)
+
+
+def test_a_layout_whose_tables_do_not_fit_32_bits(monkeypatch):
+    lay = torch.ones(2, 8, 8)
+    made = rules._Tables(lay, 64, torch.device('cpu'))
+    rows, columns = made.rows.numel(), made.columns(2, 1)[0].numel()
+    assert columns > rows
+    monkeypatch.setattr(rules, 'MOST_PLACES', columns)
+    assert rules._Tables(lay, 64, torch.device('cpu')).columns(2, 1)[0].numel() == columns
+    monkeypatch.setattr(rules, 'MOST_PLACES', columns - 1)
+    made = rules._Tables(lay, 64, torch.device('cpu'))
+    with pytest.raises(ValueError, match='layout'):
+        made.columns(2, 1)
+    monkeypatch.setattr(rules, 'MOST_PLACES', rows - 1)
+    with pytest.raises(ValueError, match='layout'):
+        rules._Tables(lay, 64, torch.device('cpu'))

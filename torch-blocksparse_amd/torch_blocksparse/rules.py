@@ -57,6 +57,14 @@ def _at(t):
     return 0 if t is None else t.data_ptr()
 
 
+MOST_PLACES = 2 ** 31 - 1     # places in a table are 32-bit numbers
+
+
+def _places(n):
+    if n > MOST_PLACES:
+        raise ValueError('the tables of the layout take %d numbers, more than %d' % (n, MOST_PLACES))
+
+
 class _Tables:
     """The tables of a layout on one device: the lines of 64 rows, and per number of query heads that share a key head the columns of
     64 keys (bsp_attention_tables_build)."""
@@ -69,6 +77,7 @@ class _Tables:
         S = 64 // self.block
         self.layout = torch.nn.functional.pad(lay.to(torch.uint8), (0, -lay.size(2) % S, 0, -lay.size(1) % S)).contiguous()
         host, info = self._build(self.layout)
+        _places(info.items_offset)
         self.lines = info.lines
         self.rows = host[:info.items_offset].to(device)
         self._columns, self._chosen = dict(), dict()
@@ -148,6 +157,7 @@ class _Tables:
         n_items = int(number.max())
         rank = torch.arange(of.numel(), device='cpu') - (number.cumsum(0) - number)[items[:, 2].long()]
         begin = 12 * kv_heads * n_items
+        _places(begin + entries.numel())
         lists = torch.zeros((kv_heads, n_items, 12), dtype=torch.int32, device='cpu')
         lists[:, :, 1], lists[:, :, 3], lists[:, :, 4] = begin, -1, -1
         lists[items[:, 2].long(), rank] = items
