@@ -32,3 +32,24 @@ def test_no_positions_or_no_sequences(monkeypatch, Z, L):
     assert o.shape == q.shape and o.dtype == q.dtype
     grads = torch.autograd.grad(o, (q, k, v), torch.zeros_like(o))
     assert [g.shape for g in grads] == [q.shape, k.shape, v.shape]
+
+
+def test_gradients_that_the_backward_pass_cannot_address_are_refused_in_the_forward_pass(monkeypatch):
+    monkeypatch.setattr(tb.rules._lib, 'require_gpu_tensor', lambda t, what: None)
+    G, block = 127, 128
+    length = -(-(1 << 29) // G)                          # G * length is just past 2^29
+    for L, refused in ((length, True), (length - block, False)):
+        blocks = -(-L // block)
+        op = tb.Attention(torch.ones(1, 1, 1, dtype=torch.uint8).expand(G, blocks, blocks), block)
+        q = torch.zeros(1, 1, 1, 64, dtype=torch.float16).expand(1, G, L, 64)
+        k, leaf = q[:, :1], torch.zeros(1, 1, 1, 64, dtype=torch.float16, requires_grad=True).expand(1, 1, L, 64)
+        args = (0., 1., None, True, None, None)
+        op._check(q, k, k, *args)
+        with torch.no_grad():
+            op._check(q, leaf, leaf, *args)
+        for keys, values in ((leaf, k), (k, leaf)):
+            if refused:
+                with pytest.raises(ValueError, match='gradient'):
+                    op._check(q, keys, values, *args)
+            else:
+                op._check(q, keys, values, *args)

@@ -282,6 +282,8 @@ class Attention:
             raise ValueError('the rows of a head lie within 4 GiB (got length %d)' % L)
         if H // kv > 127:
             raise ValueError('at most 127 query heads share a key head (got %d)' % (H // kv))
+        if 128 * -(-L // 64) * (H // kv) >= 1 << 30 and torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+            raise ValueError('the gradient of a key head reads the rows of fewer than 2^29 positions (got %d query heads of %d)' % (H // kv, L))
         heads, blocks = self.layout.shape[:2]
         if H != heads or -(-L // self.block) != blocks:
             raise ValueError('q %s does not fit a layout of %d heads and %d blocks of %d' % (tuple(q.shape), heads, blocks, self.block))
