@@ -89,7 +89,7 @@ def test_all_that_a_chain_holds_on_the_gpu_is_found(block, monkeypatch):
     assert held == sum(round_up(n) for n in found.values()) > 0
 
 
-def busy_stream(seconds=0.3):
+def busy_stream(seconds=2.):
     """a stream with work of that length under way"""
     start, stop = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
     start.record()
