@@ -120,6 +120,7 @@ def test_the_tensors_of_an_operator_are_found_wherever_they_are():
 
 def test_a_dropped_chain_tells_its_tables(empty, monkeypatch):
     told, now = [], [7]
+    capturing(monkeypatch, False)
     monkeypatch.setattr(CLS, '_readers', dict())
     monkeypatch.setattr(_lib, 'raw_stream', lambda device: now[0])
     monkeypatch.setattr(torch.cuda, 'current_stream', lambda device=None: now[0])

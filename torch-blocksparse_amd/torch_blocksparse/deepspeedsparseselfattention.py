@@ -93,14 +93,15 @@ class DeepSpeedSparseSelfAttention(nn.Module):
     def _held(key, make, device=None):
         """what `ops` holds under `key`, made where it holds nothing, for the current stream of `device`"""
         cls = DeepSpeedSparseSelfAttention
+        on_gpu = isinstance(device, torch.device) and device.type == 'cuda' and device.index is not None
         with cls._lock:
             if key not in cls.ops:
                 cls.ops[key] = cls.captured[key] if key in cls.captured else make()
                 cls._drop_the_oldest(key)
             cls.ops.move_to_end(key)
-            if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            if (on_gpu or torch.cuda.is_available()) and torch.cuda.is_current_stream_capturing():
                 cls.captured[key] = cls.ops[key]
-            if isinstance(device, torch.device) and device.type == 'cuda' and device.index is not None:
+            if on_gpu:
                 readers = cls._readers.get(key)
                 if readers is None:
                     readers = cls._readers[key] = _lib.Readers()
