@@ -180,7 +180,8 @@ __device__ __forceinline__ f32x16 zeros16() {
 }
 
 // Sixteen values a lane, one per row of a piece as rows_times deals them, as the operand of columns_times: rounded to the
-// operands' type (the products take no other), in fp32 as they are
+// operands' type (the products take no other; the two-term form that loses nothing is twice the products), in fp32 as they are.  The forward pass has its shares
+// relative to the running maximum, the backward pass normalised ones: in fp16 those below 2^-14 are off by up to 2^-25, as every fp16 number.
 template <typename T> struct Shares {
   typename Mma<T, 32>::frag_t f[2];
   __device__ __forceinline__ void set(const float (&e)[16]) {
@@ -526,9 +527,11 @@ __device__ __forceinline__ void lds_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// Two pairs of wavefronts a line in launches of few lines, whose wavefronts would leave SIMDs idle or with nobody to change places with.  Causal layouts without
-// holes, forward pass, one pair -> two: 512 lines of 1024 positions fp32 104 -> 61 us (128 elements: 148 -> 102), bf16 24 -> 18 (34 -> 25); 1024 lines of 4096 positions
+// Two pairs of wavefronts a line in launches of few lines, whose wavefronts would leave SIMDs idle or with nobody to change places with.  The rule knows the number
+// of lines, not of their tiles (which documents and a prefix change from call to call).  Causal layouts without holes, forward pass, one pair -> two: 512 lines of 1024 positions fp32 104 -> 61 us (128 elements: 148 -> 102), bf16 24 -> 18 (34 -> 25); 1024 lines of 4096 positions
 // 456 -> 318 (578 -> 642), 82 -> 63 (126 -> 104); 2048 of them 693 -> 577 (1130 -> 1261), 124 -> 116 (198 -> 217); twelve heads of 256 lines of BigBird fp16 51 -> 59.
+// Short lines, of 7 tiles (BigBird): fp16 768 lines 18.0 -> 17.3, 1536 29.7 -> 31.9; bf16 of 128 elements 512 lines 22.9 -> 19.2, 1024 30.6 -> 35.6; fp32 512 lines 68.6 -> 43.3, 1024 76.8 ->
+// 78.7, of 128 elements 256 74.3 -> 45.3, 512 80.2 -> 91.6; of one tile: fp16 768 lines 7.1 -> 8.1, bf16 of 128 elements 1024 14.5 -> 19.4, fp32 512 12.6 -> 11.8, of 128 elements 21.8 -> 29.0.
 template <typename T, int D> inline bool few_lines(const RuleArgs &a) {
   return a.R >= 4 && (int64_t)a.Z * a.H * a.R <= (D == 64 ? 2048 : sizeof(T) == 4 ? 512 : 1024);
 }

@@ -5,9 +5,9 @@
 //   row kernel    : a line of tiles per workgroup -> dq and -delta
 //   column kernel : a column of tiles (or a part of a long one) of a key head per workgroup -> dk and dv; the column's tiles are
 //                   those of all the query heads that share the key head, one after the other, so their sum needs no memory
-// Measured: fp16 8 x 16 x 4096 over blocks of 16 with stride 64 and a bias by distance: rows 186 us (vector operations 54 % of the cycles, matrix units 29 %), columns 285 (41 %,
-// 26 %), sums of their parts 16; bf16 2 x 16 (4 key heads) x 4001 x 128, six documents, capped scores: 142, 224 and 14, where the longest document's lines and columns are what takes so
-// long; fp32 2 x 8 x 2023, two documents: 76, 104 and 6.
+// Measured: fp16 8 x 16 x 4096 over blocks of 16 with stride 64 and a bias by distance: rows 176 us (vector operations 54 % of the cycles, matrix units 29 %), columns 258 (42 %,
+// 26 %), sums of their parts 15; bf16 2 x 16 (4 key heads) x 4001 x 128, six documents, capped scores: 132, 205 and 14, where the longest document's lines and columns are what takes so
+// long; fp32 2 x 8 x 2023, two documents: 71, 97 and 7.
 #include "attention_rules.h"
 
 namespace bsp {

@@ -3,9 +3,9 @@
 // Stores o and, for the backward pass, per row `ref` and `factor` with p = exp2(y - ref) * factor: ref = m + log2 l rounded to one
 // float, factor what the rounding left out (1 in 16-bit types while |ref| < 64, where it is below 2^-18).  16-bit types keep what the rounding of o left out
 // as well.
-// Measured: a causal prompt of 8192 positions in 16 heads of 128 (8 key heads), bf16, capped scores: 391 us, 705 TFLOP/s, vector operations 53 % of the cycles, matrix
-// units 30 %, which two wavefronts a SIMD overlap little (more do not fit the registers); fp16 8 x 16 x 4096 over blocks of 16 with stride 64 and a bias by distance: 174 us,
-// 68 % and 20 %.
+// Measured: a causal prompt of 8192 positions in 16 heads of 128 (8 key heads), bf16, capped scores: 396 us, 695 TFLOP/s, vector operations 53 % of the cycles, matrix
+// units 29 %, which two wavefronts a SIMD overlap little (more do not fit the registers); fp16 8 x 16 x 4096 over blocks of 16 with stride 64 and a bias by distance: 153 us,
+// 70 % and 21 %.
 #include "attention_rules.h"
 
 namespace bsp {

@@ -7,9 +7,10 @@
 //
 // Both kernels move each byte once and are bound by that.  A thread has a chunk of eight elements: 16 bytes in 16-bit types, and the four
 // threads of a group agree on its range by two exchanges within the quad.  Tensors outside the cache are streamed past the L2 (non-temporal): nothing reads them
-// soon.  Measured: 16384 positions of 16 heads of 64, fp16, 8 bits (67 MB and 38 MB) written and read back in 45 us, 51 without the streaming, 58 before a
-// thread's place was found without divisions and the rounded quotient taken from the low bits of one sum; 32749 positions of 8 heads of 128, bf16, 4 bits
-// (176 MB) read in 41 us, 52 without the streaming.
+// soon.  Measured: 16384 positions of 16 heads of 64, fp16, 8 bits (67 MB and 38 MB): written in 33 us (4 of them the launch that says whose a slot is), read back in 27, or
+// in 16 where a cache level still holds them.  One after the other 45 us: 51 without the streaming, 58 before a thread's place was found without divisions and the rounded
+// quotient taken from the low bits of one sum.  The write's vector units are busy for 68 % of its cycles, 85 to 100 % over more positions.
+// 32749 positions of 8 heads of 128, bf16, 4 bits (176 MB) read in 41 us, 52 without the streaming.
 #include "cache.h"
 
 namespace bsp {

@@ -146,7 +146,7 @@ class CacheAttention:
     over j < n = lengths[b], with a layout those in blocks that row (n - 1) // block of head h has: what `Attention` with causal=True gives for its last
     row.  A page number outside the cache (-1, say) stands for a page that is not held: its positions are not seen, so pages that no later
     row of the layout names can be given to others.  A sequence of length 0, or one that sees nothing, gets zeros.  Lengths count as
-    at most width * block and as at most the layout's positions.  Query head h uses key head h // (query heads / key heads).  No gradient.
+    at most width * block and as at most the layout's positions.  A NaN in a value that one query head of a key head sees can reach its other query heads.  Query head h uses key head h // (query heads / key heads).  No gradient.
 
     With a layout a table is made at the first call for a number of key heads on a device, so a call that is captured into a graph needs one like it
     before."""
