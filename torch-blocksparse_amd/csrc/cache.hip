@@ -5,7 +5,7 @@
 // reads back as NaN.  The codes are those of exact arithmetic: a quotient is computed in fp32 and, where that lies close to the middle of two
 // integers, decided in 64 bits.
 //
-// Both kernels move each byte once and are bound by that.  A thread has a chunk of eight elements: 16 bytes in 16-bit types, and the four
+// Both kernels move each byte once; the read is bound by that, the write by its vector operations.  A thread has a chunk of eight elements: 16 bytes in 16-bit types, and the four
 // threads of a group agree on its range by two exchanges within the quad.  Tensors outside the cache are streamed past the L2 (non-temporal): nothing reads them
 // soon.  Measured: 16384 positions of 16 heads of 64, fp16, 8 bits (67 MB and 38 MB): written in 33 us (4 of them the launch that says whose a slot is), read back in 27, or
 // in 16 where a cache level still holds them.  One after the other 45 us: 51 without the streaming, 58 before a thread's place was found without divisions and the rounded
