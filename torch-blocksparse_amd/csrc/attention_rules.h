@@ -214,6 +214,31 @@ __device__ __forceinline__ void columns_times(f32x16 (&acc)[D / 32], const Piece
   }
 }
 
+// ... + (32 rows of a piece, transposed) . e for sixteen values a lane in two operands, what they are rounded to and what that leaves out: as exact as
+// products of fp32 numbers, for half as many products again
+template <typename T, int D, int OFF, bool LEAN>
+__device__ __forceinline__ void columns_times_exact(f32x16 (&acc)[D / 32], const PieceReads<T, D, LEAN> &reads, float (&e)[16]) {
+  typedef Mma<T, 32> M;
+  Shares<T> most, rest;
+  most.set(e);
+#pragma unroll
+  for (int i = 0; i < 16; i++) e[i] -= to_float(most.f[i >> 3][i & 7]);
+  rest.set(e);
+  uint32_t lo[D / 32], hi[D / 32];
+  reads.tr.get(lo, hi);
+#pragma unroll
+  for (int mt = 0; mt < D / 32; mt += 2) {
+    constexpr int HI = LEAN ? 4 * 2 * D : 0;
+    typename M::frag_t f[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) f[i] = tr_fragment<T>(lo[mt + (i & 1)] + OFF + (i >> 1) * (16 * 2 * D), hi[mt + (i & 1)] + OFF + HI + (i >> 1) * (16 * 2 * D));
+#pragma unroll
+    for (int i = 0; i < 4; i++) acc[mt + (i & 1)] = M::run(f[i], most.f[i >> 1], acc[mt + (i & 1)]);
+#pragma unroll
+    for (int i = 0; i < 4; i++) acc[mt + (i & 1)] = M::run(f[i], rest.f[i >> 1], acc[mt + (i & 1)]);
+  }
+}
+
 // Capped scores.  With x = scale * s / cap, tanh(x) = 1 - 2 r and 1 - tanh(x)^2 = 4 (r - r^2), r = 1 / (exp(2 x) + 1): the kernels for 16-bit
 // types keep r, whose error of 2^-24 cap * log2 e takes to the logit: little beside what the operands' rounding leaves of it.  In fp32 they keep
 // the tanh, from its series where x is small (in trained models nearly everywhere) with its relative precision: up to x = 0.45 the

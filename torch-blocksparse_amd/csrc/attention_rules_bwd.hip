@@ -58,7 +58,10 @@ __global__ void __launch_bounds__(128 * PAIRS, (row_waves<T, D, CAP>())) k_rules
     }
     delta += swap32(delta);
   }
-  if (half == 0 && (PAIRS == 1 || group == 0)) a.delta[((int64_t)z * a.H + h) * a.rows + row] = -delta;   // (its negative: where the column kernel's dp starts from)
+  // delta is also sum_j p_j dp_j.  The two differ by what the rounding of the forward pass's shares made of o, in bfloat16 enough to see in the gradients: what the
+  // row's sum of p (dp - delta) is off zero by is added for the column kernel.
+  constexpr bool FINE = __is_same(T, bf16);
+  float off = 0.f;
 
   Walk<DOCS> walk;
   walk.init(a.lut + lut[2 * (h * a.R + line) + 1], line * 64 < a.L ? lut[2 * (h * a.R + line)] * 2 : 0);
@@ -124,15 +127,29 @@ __global__ void __launch_bounds__(128 * PAIRS, (row_waves<T, D, CAP>())) k_rules
         float e[16];
         logits.get(e, s, out, [&](int) { return minus; });
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          e[i] = __builtin_amdgcn_exp2f(e[i]) * (dp[i] - delta);
-          if constexpr (CAP) e[i] *= cap_through<T, true>(s[i]);
+        for (int i = 0; i < 16; i++) e[i] = __builtin_amdgcn_exp2f(e[i]) * (dp[i] - delta);
+        auto keep_seen = [&]() {
+          if (!whole)
+            for_16<0>([&](auto ic) { e[decltype(ic)::value] = keep(e[decltype(ic)::value], bit_mask<decltype(ic)::value>(seen)); });
+        };
+        if constexpr (FINE) {
+          keep_seen();
+          float sums[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) sums[i] = (e[i] + e[4 + i]) + (e[8 + i] + e[12 + i]);
+          off += (sums[0] + sums[1]) + (sums[2] + sums[3]);
         }
-        if (!whole)
-          for_16<0>([&](auto ic) { e[decltype(ic)::value] = keep(e[decltype(ic)::value], bit_mask<decltype(ic)::value>(seen)); });
-        Shares<T> ds;
-        ds.set(e);
-        columns_times<T, D, S * Q::STAGE, false>(dq, reads, ds);
+        if constexpr (CAP)
+#pragma unroll
+          for (int i = 0; i < 16; i++) e[i] *= cap_through<T, true>(s[i]);
+        if constexpr (CAP || !FINE) keep_seen();
+        if constexpr (FINE) {
+          columns_times_exact<T, D, S * Q::STAGE, false>(dq, reads, e);
+        } else {
+          Shares<T> ds;
+          ds.set(e);
+          columns_times<T, D, S * Q::STAGE, false>(dq, reads, ds);
+        }
       }
       halves = nxt;
       return halves.more;
@@ -141,16 +158,20 @@ __global__ void __launch_bounds__(128 * PAIRS, (row_waves<T, D, CAP>())) k_rules
   }
   if constexpr (PAIRS == 2) {                           // the second pair's sums to the first
     quad_barrier();
-    float *sums = reinterpret_cast<float *>(all_smem + pair_lds<T, D, PAIRS>()) + wave * (64 * 16 * MT) + lane;
+    float *sums = reinterpret_cast<float *>(all_smem + pair_lds<T, D, PAIRS>()) + wave * (64 * (16 * MT + 2)) + lane;
     if (group) {
+      sums[0] = off;
 #pragma unroll
-      for (int i = 0; i < 16 * MT; i++) sums[64 * i] = dq[i >> 4][i & 15];
+      for (int i = 0; i < 16 * MT; i++) sums[64 * (1 + i)] = dq[i >> 4][i & 15];
     }
     lds_barrier();
     if (group) return;
+    off += sums[0];
 #pragma unroll
-    for (int i = 0; i < 16 * MT; i++) dq[i >> 4][i & 15] += sums[64 * i];
+    for (int i = 0; i < 16 * MT; i++) dq[i >> 4][i & 15] += sums[64 * (1 + i)];
   }
+  if constexpr (FINE) delta += (off + swap32(off)) * factor * (CAP ? 0.25f : 1.f);
+  if (half == 0) a.delta[((int64_t)z * a.H + h) * a.rows + row] = -delta;   // (its negative: where the column kernel's dp starts from)
   const float last = a.scale * factor;
 #pragma unroll
   for (int mt = 0; mt < MT; mt++)
