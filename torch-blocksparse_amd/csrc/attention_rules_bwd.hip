@@ -60,9 +60,9 @@ __global__ void __launch_bounds__(128 * PAIRS, (row_waves<T, D, CAP>())) k_rules
     }
     delta += swap32(delta);
   }
-  // delta is also sum_j p_j dp_j.  The two differ by what the rounding of the forward pass's shares made of o, in bfloat16 enough to see in the gradients: what the
+  // delta is also sum_j p_j dp_j.  The two differ by what the rounding of the forward pass's shares made of o, in 16-bit types enough to see in the gradients: what the
   // row's sum of p (dp - delta) is off zero by is added for the column kernel.
-  constexpr bool FINE = __is_same(T, bf16);
+  constexpr bool FINE = sizeof(T) == 2;
   float off = 0.f;
 
   Walk<DOCS> walk;
