@@ -122,3 +122,28 @@ def test_groups_whose_least_value_is_rounded_up_past_them(bits, D):
     want = (least + code * step).flatten(-2)
     for got, value in zip(cache.read(slots, torch.float32), (want, want.flip(0))):
         assert torch.equal(got.double().cpu(), value.float().double())
+
+
+@pytest.mark.parametrize('bits', [4, 8])
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('H', [1, 6, 16])
+@pytest.mark.parametrize('length', [64, 4096])
+def test_shares_of_a_float16_result_are_not_those_of_its_type(bits, D, H, length):
+    """Half of the positions have scores of zero, the others scores whose exponential is off by 4e-4 of itself when it is rounded to float16, to
+    what makes their values cancel.  (Groups of one value each: the cache holds them as they are.)"""
+    block, score = 16, -497 / 1024
+    k, v = [torch.zeros(length, 1, D) for _ in range(2)]
+    e = math.exp(score)
+    low = -float(torch.tensor(e).half())
+    k[1::2], v[0::2], v[1::2] = score, low, 1.
+    cache = tb.KeyValueCache(length // block, block, 1, D, bits=bits)
+    cache.write(k.half().to(DEV), v.half().to(DEV), torch.arange(length, dtype=torch.int32, device=DEV))
+    q = torch.zeros(1, H, D, dtype=torch.float16, device=DEV)
+    q[..., 5] = 1.
+    o = tb.CacheAttention(block)(q, cache, torch.arange(length // block, dtype=torch.int32, device=DEV)[None], torch.tensor([length], dtype=torch.int32, device=DEV))
+    want, size = (low + e) / (1 + e), (abs(low) + e) / (1 + e)
+    # sums in fp32 of terms of that size, shares in two terms of eleven bits each, the result
+    c = 2. ** -24 * (2 * D + length / 8 + 8 + 32)         # (a lane's sum is of a sixteenth of the positions)
+    bound = (c + 2. ** -22) * size + 2. ** -11 * abs(want) + 2. ** -25
+    assert abs(want) > 4 * bound                         # (with shares rounded to float16 it is zero)
+    assert float((o.double() - want).abs().max()) <= bound

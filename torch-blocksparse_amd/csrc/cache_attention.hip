@@ -10,7 +10,7 @@
 // The codes are operands as they are, bit patterns of fp16 numbers below the normal ones, so a score is the sum over the groups of step * (q . codes) +
 // least * (sum of the group's q), the products on the matrix units (16 x 16 x 32: a group each).  q is scaled by a power of two per head to the
 // range of fp16, which loses nothing that 2^-35 of its largest element would not.  Values are v = least + code * step rounded to fp16
-// (2^-12 of it, under the rounding of the shares; 65504 at most) through LDS, where the product with the shares reads them transposed.
+// (2^-12 of it; 65504 at most) through LDS, where the product with the shares reads them transposed.
 //
 // Measured: sixteen sequences of up to 16384 positions, 32 query heads of 128 on 8 key heads, 4 bits (218 MB of pages): 53 us with the join, 4.1 TB/s
 // (all of 16384 positions: 61 us, 5.5 TB/s); loading the same bytes and nothing else takes 40.  What is left is that compute units get unequal shares of ragged
@@ -67,17 +67,19 @@ __device__ __forceinline__ float step_of(uint32_t meta) { return (float)__builti
 __device__ __forceinline__ float least_of(uint32_t meta) { return (float)__builtin_bit_cast(f16, (uint16_t)(meta >> 16)); }
 template <int BITS, int D> struct DecodeLds {
   static constexpr int VROW = 2 * D + 16, PROW = 80;      // bytes of a position's values, of a head's 32 shares
-  static constexpr int WAVE = 32 * VROW + 16 * PROW;
   static constexpr int join(int V) { return 4 * 4 * V * (D + 2) * 4; }
-  static constexpr int bytes(int V) { return 4 * WAVE > join(V) ? 4 * WAVE : join(V); }
+  static constexpr int wave(bool fine) { return 32 * VROW + (fine ? 2 : 1) * 16 * PROW; }
+  static constexpr int bytes(int V, bool fine) { return 4 * wave(fine) > join(V) ? 4 * wave(fine) : join(V); }
 };
 
-template <int BITS, int D, int V>
-__global__ void __launch_bounds__(256, 3) k_cache_attention(DecodeArgs a, int dtype) {
+// FINE: float16, whose results have eleven bits: the shares in two terms, what they are rounded to and what that leaves out.  (In bfloat16 their rounding is nothing beside
+// the result's.)
+template <int BITS, int D, int V, bool FINE>
+__global__ void __launch_bounds__(256, 3) k_cache_attention(DecodeArgs a) {
   typedef Page<BITS, D> P;
   typedef DecodeLds<BITS, D> L;
   constexpr int GR = D / 32, NT = D / 16;
-  __shared__ __attribute__((aligned(16))) unsigned char smem[L::bytes(V)];
+  __shared__ __attribute__((aligned(16))) unsigned char smem[L::bytes(V, FINE)];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), key = lane & 15, c = lane >> 4;
   // the first pieces of all sequences and heads, then the second ones: the workgroups that find nothing to do come last, and every XCD (they take workgroups
   // in turn) gets the same share of the long sequences
@@ -111,7 +113,7 @@ __global__ void __launch_bounds__(256, 3) k_cache_attention(DecodeArgs a, int dt
   for (int g = 0; g < GR; g++)
     q[g].raw = *reinterpret_cast<const u32x4 *>(reinterpret_cast<const uint16_t *>(a.q) + b * a.q_sb + (first + (row_here ? row : 0)) * a.q_sh + 8 * c + 32 * g);
 
-  unsigned char *values = smem + wave * L::WAVE, *shares = values + 32 * L::VROW;
+  unsigned char *values = smem + wave * L::wave(FINE), *shares = values + 32 * L::VROW;
   const int64_t page_bytes = P::bytes(a.block) * a.kv_heads;
   const unsigned char *pages = a.pages + P::bytes(a.block) * hk;
   const int value = P::codes(a.block, 1), k_meta = P::meta(a.block, 0);       // where a page's values lie behind its keys, and the steps behind the codes
@@ -167,7 +169,7 @@ __global__ void __launch_bounds__(256, 3) k_cache_attention(DecodeArgs a, int dt
     for (int g = 0; g < GR; g++) {
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        x[g][i] = row_here ? (dtype == BSP_F16 ? to_float(q[g].h[i]) : to_float(q[g].f[i])) : 0.f;
+        x[g][i] = row_here ? (FINE ? to_float(q[g].h[i]) : to_float(q[g].f[i])) : 0.f;
         top = fmaxf(top, fabsf(x[g][i]));
       }
     }
@@ -267,8 +269,7 @@ __global__ void __launch_bounds__(256, 3) k_cache_attention(DecodeArgs a, int dt
         for (int u = 0; u < 2; u++) tile[u] = fetch(raw[u], 2 * (pair - base) + u);
       }
       // shares relative to the running maximum, which moves when they grow past 8192
-      f16 e[2][V];
-      float sum[V];
+      float e[2][V], sum[V];
       auto exponentials = [&]() {
 #pragma unroll
         for (int j = 0; j < V; j++) {
@@ -276,8 +277,8 @@ __global__ void __launch_bounds__(256, 3) k_cache_attention(DecodeArgs a, int dt
           sum[j] = 0.f;
 #pragma unroll
           for (int u = 0; u < 2; u++) {
-            e[u][j] = (f16)(seen >> (4 * u + j) & 1 ? __builtin_amdgcn_exp2f(y[u][j] - ms) : 0.f);
-            sum[j] += (float)e[u][j];                     // as the product below has them
+            e[u][j] = seen >> (4 * u + j) & 1 ? __builtin_amdgcn_exp2f(y[u][j] - ms) : 0.f;
+            sum[j] += FINE ? e[u][j] : (float)(f16)e[u][j];   // as the product below has them
           }
         }
       };
@@ -317,20 +318,35 @@ __global__ void __launch_bounds__(256, 3) k_cache_attention(DecodeArgs a, int dt
       for (int j = 0; j < V; j++) {
         l[j] += sum[j];
 #pragma unroll
-        for (int u = 0; u < 2; u++) *reinterpret_cast<f16 *>(shares + (4 * c + j) * L::PROW + 2 * (16 * u + key)) = e[u][j];
+        for (int u = 0; u < 2; u++) *reinterpret_cast<f16 *>(shares + (4 * c + j) * L::PROW + 2 * (16 * u + key)) = (f16)e[u][j];
       }
+      if constexpr (FINE)
+#pragma unroll
+        for (int j = 0; j < V; j++)
+#pragma unroll
+          for (int u = 0; u < 2; u++) *reinterpret_cast<f16 *>(shares + (16 + 4 * c + j) * L::PROW + 2 * (16 * u + key)) = (f16)(e[u][j] - (float)(f16)e[u][j]);
       asm volatile("" ::: "memory");
       __builtin_amdgcn_wave_barrier();                    // LDS operations of one wavefront complete in order; this only pins the code order
       // (rows of no head hold whatever was there: they come out as rows of no head)
       const h8 pf = *reinterpret_cast<const h8 *>(shares + key * L::PROW + 16 * c);
       const uint32_t vat = (uint32_t)(uintptr_t)BSP_LDS_PTR(values) + (8 * c + (key >> 2)) * L::VROW + 8 * (key & 3);
-#pragma unroll
-      for (int n = 0; n < NT; n++) {
+      auto value_operand = [&](int n) {
         typedef s16x4 __attribute__((address_space(3))) * lds_ptr;
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(uintptr_t)(vat + 32 * n)), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(uintptr_t)(vat + 32 * n + 4 * L::VROW));
         typedef short s16x8 __attribute__((ext_vector_type(8)));
-        const h8 vf = __builtin_bit_cast(h8, (s16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-        o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pf, vf, o[n], 0, 0, 0);
+        return __builtin_bit_cast(h8, (s16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      };
+      if constexpr (FINE) {
+        const h8 pr = *reinterpret_cast<const h8 *>(shares + (16 + key) * L::PROW + 16 * c);
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          const h8 vf = value_operand(n);
+          o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pf, vf, o[n], 0, 0, 0);
+          o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pr, vf, o[n], 0, 0, 0);
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < NT; n++) o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pf, value_operand(n), o[n], 0, 0, 0);
       }
       asm volatile("" ::: "memory");
       __builtin_amdgcn_wave_barrier();
@@ -375,7 +391,7 @@ __global__ void __launch_bounds__(256, 3) k_cache_attention(DecodeArgs a, int dt
       uint16_t *to = reinterpret_cast<uint16_t *>(a.o) + b * a.o_sb + (first + r) * a.o_sh + d;
       x0 = sum == 0.f ? 0.f : x0 * inv;
       x1 = sum == 0.f ? 0.f : x1 * inv;
-      *reinterpret_cast<uint32_t *>(to) = dtype == BSP_F16
+      *reinterpret_cast<uint32_t *>(to) = FINE
           ? (uint32_t)__builtin_bit_cast(uint16_t, (f16)x0) | (uint32_t)__builtin_bit_cast(uint16_t, (f16)x1) << 16
           : (uint32_t)__builtin_bit_cast(uint16_t, (bf16)x0) | (uint32_t)__builtin_bit_cast(uint16_t, (bf16)x1) << 16;
     }
@@ -434,11 +450,15 @@ template <int D> __global__ void __launch_bounds__(256) k_cache_attention_join(D
   else *to = (uint16_t)bits;
 }
 
-template <int BITS, int D> int launch_decode(const DecodeArgs &a, int dtype, hipStream_t st) {
+template <int BITS, int D, bool FINE> void launch_decode(const DecodeArgs &a, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)a.B * a.units * a.splits));
-  if (a.per <= 4) hipLaunchKernelGGL((k_cache_attention<BITS, D, 1>), grid, dim3(256), 0, st, a, dtype);
-  else if (a.per <= 8) hipLaunchKernelGGL((k_cache_attention<BITS, D, 2>), grid, dim3(256), 0, st, a, dtype);
-  else hipLaunchKernelGGL((k_cache_attention<BITS, D, 4>), grid, dim3(256), 0, st, a, dtype);
+  if (a.per <= 4) hipLaunchKernelGGL((k_cache_attention<BITS, D, 1, FINE>), grid, dim3(256), 0, st, a);
+  else if (a.per <= 8) hipLaunchKernelGGL((k_cache_attention<BITS, D, 2, FINE>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((k_cache_attention<BITS, D, 4, FINE>), grid, dim3(256), 0, st, a);
+}
+template <int BITS, int D> int launch_decode(const DecodeArgs &a, int dtype, hipStream_t st) {
+  if (dtype == BSP_F16) launch_decode<BITS, D, true>(a, st);
+  else launch_decode<BITS, D, false>(a, st);
   if (a.splits > 1) hipLaunchKernelGGL(k_cache_attention_join<D>, dim3((unsigned)cdiv((int64_t)a.B * a.H, 4)), dim3(256), 0, st, a, dtype);
   BSP_LAUNCH_CHECK();
   return BSP_OK;
