@@ -1,14 +1,14 @@
 // Backward pass of attention with score rules (attention_rules.h), p = exp2(y - ref) * factor computed again:
 //     dv = p^T . do,   e = p * (dp - delta) * (1 - t^2)  (t the tanh of a capped score),   dq = scale * e . k,   dk = scale * e^T . q
 // with dp = do . v^T and delta = sum_d do_d o_d, for which 16-bit types keep what the rounding of o left out as a second tensor: delta goes into every
-// gradient of its row, and with o alone the gradients are off by 1.8 times what the roundings of p, of e and of the result make them.  Where those roundings are of
-// eight bits (bfloat16), dq takes e in two terms and dk a delta that the row kernel has corrected: errors against 64 bits (relative 2-norm) of dq 2.5e-3 -> 1.9e-3, of dk
-// 2.5e-3 -> 2.35e-3, where rounding the results alone is 1.66e-3.  In fp16 they are 3.0e-4 of 2.1e-4.
+// gradient of its row, and with o alone the gradients are off by 1.8 times what the roundings of p, of e and of the result make them.  16-bit types
+// also take e in two terms for dq, and for dk a delta that the row kernel has corrected: errors against 64 bits (relative 2-norm) of dq 2.5e-3 -> 1.9e-3 in bf16, 3.0e-4 -> 2.2e-4 in
+// fp16, of dk 2.5e-3 -> 2.35e-3, 3.0e-4 -> 2.95e-4, where rounding the results alone is 1.66e-3 and 2.07e-4.
 //   row kernel    : a line of tiles per workgroup -> dq and -delta
 //   column kernel : a column of tiles (or a part of a long one) of a key head per workgroup -> dk and dv; the column's tiles are
 //                   those of all the query heads that share the key head, one after the other, so their sum needs no memory
-// Measured: fp16 8 x 16 x 4096 over blocks of 16 with stride 64 and a bias by distance: rows 176 us (vector operations 54 % of the cycles, matrix units 29 %), columns 258 (42 %,
-// 26 %), sums of their parts 15; bf16 2 x 16 (4 key heads) x 4001 x 128, six documents, capped scores: 155 (132 with score gradients in one term), 205 and 14, where the longest document's lines and columns are what takes so
+// Measured: fp16 8 x 16 x 4096 over blocks of 16 with stride 64 and a bias by distance: rows 196 us (vector operations 64 % of the cycles, matrix units 34 %; 176 with e in one term), columns 255 (42 %,
+// 26 %), sums of their parts 16; bf16 2 x 16 (4 key heads) x 4001 x 128, six documents, capped scores: 153 (132 with e in one term), 204 and 14, where the longest document's lines and columns are what takes so
 // long; fp32 2 x 8 x 2023, two documents: 71, 97 and 7.
 #include "attention_rules.h"
 

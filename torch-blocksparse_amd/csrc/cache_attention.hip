@@ -12,10 +12,10 @@
 // range of fp16, which loses nothing that 2^-35 of its largest element would not.  Values are v = least + code * step rounded to fp16
 // (2^-12 of it; 65504 at most) through LDS, where the product with the shares reads them transposed.
 //
-// Measured: sixteen sequences of up to 16384 positions, 32 query heads of 128 on 8 key heads, 4 bits (218 MB of pages): 53 us with the join, 4.1 TB/s
+// Measured: sixteen sequences of up to 16384 positions, 32 query heads of 128 on 8 key heads, 4 bits (218 MB of pages): 52 us with the join, 4.2 TB/s
 // (all of 16384 positions: 61 us, 5.5 TB/s); loading the same bytes and nothing else takes 40.  What is left is that compute units get unequal shares of ragged
 // sequences, and the vector units: taking the codes out of their words for keys and values was 240 of 390 operations a pair of tiles and is 140 of 270 with keys as
-// they lie (63 us before).  Looking for values past fp16's range (see `large`) is 1.3 of the 53.
+// they lie (63 us before).  Looking for values past fp16's range (see `large`) is 1.3 of the 52.
 //
 // Scores lie with a position per lane and the query heads along the sixteen result rows of the matrix unit, dealt so that a head takes one
 // value in a quarter of the lanes: with at most four heads a key head (V = 1) a tile costs one exponential a lane, with up to eight two.
