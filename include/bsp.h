@@ -523,6 +523,16 @@ int bsp_attention_rules_bwd(const bsp_attention_rules_call *call, const void *d_
                             void *dq, void *dk, void *dv, float *neg_delta, const int32_t *d_items, int n_items, float *partial, int n_slots,
                             const int32_t *d_split, int n_split, void *stream);
 
+/* Rotated positions: y = x with the pairs of the first 2 * pairs of each row's D elements turned by position * frequency (back: minus that),
+ *     (a, b) -> (a cos - b sin, a sin + b cos),
+ * pair p being elements p and pairs + p, or 2 p and 2 p + 1 (neighbours); the others are copied.  fractions: [pairs], frequency / (2 pi) less whole turns, in units of
+ * 2^-64.  pairs and D: multiples of 8.  One or two operands (H1 = 0: one) of any type: element (z, head, l, d) at z * strides[0] + head * strides[1] + l * strides[2] + d,
+ * of y with strides[3 .. 5]; multiples of 8 elements (fp32: 4), 16-byte aligned.  positions: element (z, l) at z * pos_stride_z + l * pos_stride_l, or
+ * NULL: l.  Z * length * D < 2^32.  x and y do not overlap. */
+int bsp_rotate(int dtype, int Z, int64_t length, int D, int pairs, int neighbours, int back, const uint64_t *fractions, const int32_t *positions,
+               int64_t pos_stride_z, int64_t pos_stride_l, const void *x0, void *y0, int H0, const int64_t *strides0, const void *x1, void *y1, int H1,
+               const int64_t *strides1, void *stream);
+
 /* A quantised cache of keys and values.  A page holds `block` (16, 32, 64, 128) consecutive positions of a sequence for `heads` key
  * heads of D = 64 or 128 elements in `bits` = 4 or 8: bsp_cache_page_bytes bytes, pages back to back at a 16-byte aligned address.
  * Position `at` of page p is slot p * block + at.  Of 32 neighbouring elements, taken into [-65504, 65504], least = fp16(min), step =
@@ -531,10 +541,14 @@ int bsp_attention_rules_bwd(const bsp_attention_rules_call *call, const void *d_
  * write: k, v: element (t, head, d) at t * stride_t + head * stride_h + d, 16-byte aligned, strides multiples of 8 elements (fp32: 4);
  *   slots: [T], T < 2^24; those outside the cache (negative ones) are left out; of positions with one slot the last is written.  owner: [n_pages *
  *   block] ints, zero before the first call (each call leaves them so).
+ * write_rotated: the keys are turned first (bsp_rotate; positions: [T]), in 64 bits, and the least of 32 turned elements is rounded to fp32 on its way to fp16.
  * read: k, v: [T, heads, D], contiguous; slots outside the cache give zeros.  A step that was rounded up may take an element past 65504: fp16 has it as 65504. */
 int64_t bsp_cache_page_bytes(int block, int heads, int D, int bits);
 int bsp_cache_write(int dtype, void *pages, int n_pages, int block, int heads, int D, int bits, const void *k, int64_t k_stride_t, int64_t k_stride_h,
                     const void *v, int64_t v_stride_t, int64_t v_stride_h, const int32_t *slots, int T, int32_t *owner, void *stream);
+int bsp_cache_write_rotated(int dtype, void *pages, int n_pages, int block, int heads, int D, int bits, const void *k, int64_t k_stride_t, int64_t k_stride_h,
+                            const void *v, int64_t v_stride_t, int64_t v_stride_h, const int32_t *slots, int T, int32_t *owner, const uint64_t *fractions,
+                            int pairs, int neighbours, const int32_t *positions, void *stream);
 int bsp_cache_read(int dtype, const void *pages, int n_pages, int block, int heads, int D, int bits, void *k, void *v, const int32_t *slots, int T,
                    void *stream);
 
@@ -553,6 +567,28 @@ int bsp_cache_attention(int dtype, const void *q, int64_t q_stride_b, int64_t q_
                         const void *pages, int n_pages, int block, int kv_heads, int D, int bits, const int32_t *table, int64_t table_stride, int width,
                         const int32_t *lengths, const int32_t *rows, int n_rows, int64_t most_blocks, float scale, float softcap, const float *slopes,
                         void *workspace, int64_t workspace_bytes, int splits, void *stream);
+
+/* A cache of latent vectors: row `slot` = page * block + offset has a position's `latent` (128, 256, 512) elements and behind them the 64 of the key part that all heads
+ * share, in dtype (fp16 or bf16), rows and pages back to back at a 16-byte aligned address; block 16, 32, 64 or 128.
+ * write: c: element (t, d) at t * c_stride_t + d, 16-byte aligned, strides multiples of 8; r: [T, 64] at any stride.  slots, owner, T: as in bsp_cache_write.  fractions (NULL: no rotation), pairs,
+ *   neighbours: as in bsp_rotate, with D = 64; positions: [T].
+ * read: c: [T, latent], r: [T, 64], contiguous; slots outside the cache give zeros. */
+int bsp_latent_write(int dtype, void *pages, int n_pages, int block, int latent, const void *c, int64_t c_stride_t, const void *r, int64_t r_stride_t, const int32_t *slots,
+                     int T, int32_t *owner, const uint64_t *fractions, int pairs, int neighbours, const int32_t *positions, void *stream);
+int bsp_latent_read(int dtype, const void *pages, int n_pages, int block, int latent, void *c, void *r, const int32_t *slots, int T, void *stream);
+
+/* Attention of one position a sequence over such a cache, of which every head reads the same: o = sum_j softmax_j(y) c_j, y_j = softcap * tanh(scale * (q . c_j + q_r . r_j) / softcap) - slope_h *
+ * (n - 1 - j) (softcap 0: no cap, else 2^-10 .. 1024), over the positions j < n = lengths[b]; table, lengths, width, n_pages: as in bsp_cache_attention.  q, o: [B, H, latent], q_r: [B, H, 64], all
+ * 16-byte aligned with strides that are multiples of 8; B * H < 2^24.  rows: NULL, or what is seen beside that, for units of bsp_latent_attention_heads(H) heads (the last may have fewer): per unit n_rows + 1
+ * ints, the number of the first entry of each block-row and the end of the last one's; behind all of them the entries, three ints each: block-column, and 64 bits (low
+ * ones first), one for each of the unit's heads that sees it; one more entry behind the last.  The row is (n - 1) / block.  most_blocks: no sequence sees more blocks (width, or the most entries of a row).  workspace:
+ * bsp_latent_attention_workspace_bytes bytes, 16-byte aligned, no initialisation; calls that overlap need one each.  No atomics: the same call gives the same bits. */
+int bsp_latent_attention_heads(int H);
+int64_t bsp_latent_attention_workspace_bytes(int B, int H, int latent, int block, int64_t most_blocks);
+int bsp_latent_attention(int dtype, const void *q, int64_t q_stride_b, int64_t q_stride_h, const void *q_r, int64_t qr_stride_b, int64_t qr_stride_h, void *o,
+                         int64_t o_stride_b, int64_t o_stride_h, int B, int H, const void *pages, int n_pages, int block, int latent, const int32_t *table,
+                         int64_t table_stride, int width, const int32_t *lengths, const int32_t *rows, int n_rows, int64_t most_blocks, float scale, float softcap,
+                         const float *slopes, void *workspace, int64_t workspace_bytes, void *stream);
 
 /* ---------------------------------------------------------------------------------------------------
  * Dense utility ops of the reference package.

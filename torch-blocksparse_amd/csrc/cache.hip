@@ -11,7 +11,11 @@
 // in 16 where a cache level still holds them.  One after the other 45 us: 51 without the streaming, 58 before a thread's place was found without divisions and the rounded
 // quotient taken from the low bits of one sum.  The write's vector units are busy for 68 % of its cycles, 85 to 100 % over more positions.
 // 32749 positions of 8 heads of 128, bf16, 4 bits (176 MB) read in 41 us, 52 without the streaming.
+//
+// With a rotation (rotation.h) the keys are turned first, all of it in 64 bits, as what rounding in between would leave out decides codes: the vector units do fp64 at the
+// rate of fp32.  A workgroup computes its position's sines and cosines once, into LDS, and a thread takes the other chunk of its pairs from the lane that has it.
 #include "cache.h"
+#include "rotation.h"
 
 namespace bsp {
 
@@ -24,6 +28,9 @@ struct CacheArgs {
   unsigned char *pages;
   int64_t capacity;                // positions of the cache
   int T, heads, block, block_shift;
+  const int32_t *positions;        // write, with a rotation
+  const uint64_t *fractions;
+  int pairs, neighbours;
 };
 
 namespace {
@@ -31,6 +38,20 @@ namespace {
 // value of the neighbour xor 1, xor 2 in the quad
 __device__ __forceinline__ float quad1(float v) { return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xf, 0xf, true)); }
 __device__ __forceinline__ float quad2(float v) { return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xf, 0xf, true)); }
+
+__device__ __forceinline__ double quad_f64(double v, int control) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const int lo = (int)(uint32_t)b, hi = (int)(uint32_t)(b >> 32);
+  const uint32_t l = control == 1 ? __builtin_amdgcn_update_dpp(0, lo, 0xB1, 0xf, 0xf, true) : __builtin_amdgcn_update_dpp(0, lo, 0x4E, 0xf, 0xf, true);
+  const uint32_t h = control == 1 ? __builtin_amdgcn_update_dpp(0, hi, 0xB1, 0xf, 0xf, true) : __builtin_amdgcn_update_dpp(0, hi, 0x4E, 0xf, 0xf, true);
+  return __builtin_bit_cast(double, (uint64_t)h << 32 | l);
+}
+__device__ __forceinline__ double quad1(double v) { return quad_f64(v, 1); }
+__device__ __forceinline__ double quad2(double v) { return quad_f64(v, 2); }
+__device__ __forceinline__ float lesser(float a, float b) { return fminf(a, b); }
+__device__ __forceinline__ double lesser(double a, double b) { return fmin(a, b); }
+__device__ __forceinline__ float greater(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ double greater(double a, double b) { return fmax(a, b); }
 
 template <typename T> __device__ __forceinline__ void load8(float (&x)[8], const T *p) {
   if constexpr (sizeof(T) == 4) {
@@ -57,8 +78,105 @@ __global__ void __launch_bounds__(256) k_cache_owner(CacheArgs a) {
   if (slot >= 0 && slot < a.capacity) atomicMax(a.owner + slot, t + 1);
 }
 
+// The codes of the thread's eight elements (words), least value and step of their group, which the four threads of a quad have.  X: float, or double for what a rotation
+// left (whose least element is rounded to fp32 on its way to fp16)
+template <int BITS, typename X> __device__ __forceinline__ void quantise(const X (&x)[8], uint32_t (&w)[2], f16 &least, f16 &step) {
+    // the group's range, into that of fp16 here: elements outside get the codes of its ends below
+    bool nan = false;
+    X lo = x[0], hi = x[0];
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    nan |= __builtin_isunordered(x[e], x[e + 1]);
+    lo = lesser(lesser(lo, x[e]), x[e + 1]);
+    hi = greater(greater(hi, x[e]), x[e + 1]);
+  }
+  float bad = nan ? 1.f : 0.f;
+  lo = lesser(lo, quad1(lo));
+  hi = greater(hi, quad1(hi));
+  bad = fmaxf(bad, quad1(bad));
+  lo = lesser(lo, quad2(lo));
+  hi = greater(hi, quad2(hi));
+  bad = fmaxf(bad, quad2(bad));
+  lo = lesser(greater(lo, (X)-65504), (X)65504);
+  hi = lesser(greater(hi, (X)-65504), (X)65504);
+  constexpr int MOST = (1 << BITS) - 1;
+  float lo32 = (float)lo;
+  if constexpr (sizeof(X) == 8) asm("" : "+v"(lo32));   // (or the compiler makes one rounding of the two)
+  least = (f16)lo32;
+  {
+    const double range = (double)hi - (double)(float)least;
+    const float r = (float)range;
+    step = (f16)((double)r == range ? r / (float)MOST : (float)(range / (double)MOST));   // (the same number: both quotients are rounded to the nearest)
+  }
+  if (bad != 0.f) least = __builtin_bit_cast(f16, (uint16_t)0x7e00), step = (f16)0.f;
+    const float l32 = (float)least, s32 = (float)step;
+    if (s32 != 0.f) {                                   // (below zero where the least value was rounded up past the greatest one)
+      // the quotient rounded in the low bits of 1.5 * 2^23 + it
+      const float inv = __builtin_amdgcn_rcpf(s32), magic = 12582912.f;
+      uint32_t code[8];
+      float off = 0.f;
+  #pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float d = (float)(x[e] - (X)l32), r = fmaf(d, inv, magic);
+        off = fmaxf(off, fabsf(fmaf(d, inv, magic - r)));
+        code[e] = __builtin_bit_cast(uint32_t, fminf(fmaxf(r, magic), magic + (float)MOST));
+      }
+      // x - least is off by 2^-24 of itself, the reciprocal by 2^-23, so the quotient by 3 * 2^-24 * MOST: decided in 64 bits where the middle is as near
+      if (off > 0.5f - MOST * 0x1p-22f) {
+        const double h = 0.5 * fabs((double)s32);
+  #pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const int n0 = (int)(code[e] & 0x1ffu);
+          const double rest = ((double)x[e] - (double)l32) - (double)n0 * (double)s32, rem = s32 < 0.f ? -rest : rest;
+          const bool odd = n0 & 1;
+          const int m = n0 + (rem > h || (rem == h && odd) ? 1 : 0) - (rem < -h || (rem == -h && odd) ? 1 : 0);
+          code[e] = (uint32_t)(m < 0 ? 0 : m > MOST ? MOST : m);
+        }
+      }
+      if constexpr (BITS == 4) {
+  #pragma unroll
+        for (int e = 0; e < 8; e++) w[0] |= (code[e] & 15u) << (4 * (e >> 1) + 16 * (e & 1));
+      } else {
+  #pragma unroll
+        for (int e = 0; e < 2; e++)
+          w[e] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(code[4 * e + 3], code[4 * e + 2], 0x0c0c0400u), __builtin_amdgcn_perm(code[4 * e + 1], code[4 * e], 0x0c0c0400u), 0x05040100u);
+      }
+    }
+}
+
+// The turned elements of the thread's chunk j
+template <int CHUNKS> __device__ __forceinline__ void turn_chunk(double (&y)[8], const float (&x)[8], int j, int pairs, bool neighbours, const TurnF64 *turns) {
+  if (neighbours) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const double p = x[2 * i], q = x[2 * i + 1];
+      if (4 * j < pairs) {                                // (a multiple of four)
+        const TurnF64 t = turns[4 * j + i];
+        y[2 * i] = fma(p, t.cos, -q * t.sin);
+        y[2 * i + 1] = fma(p, t.sin, q * t.cos);
+      } else {
+        y[2 * i] = p;
+        y[2 * i + 1] = q;
+      }
+    }
+    return;
+  }
+  const int half = pairs >> 3;                            // chunks
+  const bool low = j < half, turned = j < 2 * half;
+  const int lane = threadIdx.x & 63, other = turned ? (low ? lane + half : lane - half) : lane;   // (of the same head, so of the same wavefront)
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    const float b = __shfl(x[e], other);
+    y[e] = x[e];
+    if (turned) {
+      const TurnF64 t = turns[8 * (low ? j : j - half) + e];
+      y[e] = fma((double)x[e], t.cos, (low ? -(double)b : (double)b) * t.sin);
+    }
+  }
+}
+
 // A workgroup per position.  SCAN: few positions, a later one with the same slot is looked for here; else owner says which is last.
-template <typename T, int BITS, int D, bool SCAN> __global__ void __launch_bounds__(256) k_cache_write(CacheArgs a) {
+template <typename T, int BITS, int D, bool SCAN, bool ROTATED> __global__ void __launch_bounds__(256) k_cache_write(CacheArgs a) {
   typedef Page<BITS, D> P;
   constexpr int CHUNKS = D / 8;
   const int t = (int)xcd_remap(blockIdx.x, a.T), tid = threadIdx.x;
@@ -75,71 +193,25 @@ template <typename T, int BITS, int D, bool SCAN> __global__ void __launch_bound
     if (last != t + 1) return;
     if (tid == 0) a.owner[slot] = 0;                    // (another position of the slot that looks from now on finds 0: not the last either)
   }
+  __shared__ TurnF64 turns[ROTATED ? D / 2 : 1];
+  if constexpr (ROTATED) {
+    if (tid < a.pairs) turns[tid] = turn_of_f64(as_table(a.positions)[t], a.fractions[tid]);
+    __syncthreads();
+  }
   const int page = slot >> a.block_shift, at = slot & (a.block - 1);
   const int j = tid % CHUNKS, g = j >> 2, c = j & 3;
   for (int m = tid / CHUNKS; m < 2 * a.heads; m += 256 / CHUNKS) {
     const int value = m >= a.heads, head = value ? m - a.heads : m;
     float x[8];
     load8<T>(x, (value ? reinterpret_cast<const T *>(a.v) + t * a.v_st + head * a.v_sh : reinterpret_cast<const T *>(a.k) + t * a.k_st + head * a.k_sh) + 8 * j);
-    // the group's range, into that of fp16 here: elements outside get the codes of its ends below
-    bool nan = false;
-    float lo = x[0], hi = x[0];
-#pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      nan |= __builtin_isunordered(x[e], x[e + 1]);
-      lo = fminf(fminf(lo, x[e]), x[e + 1]);
-      hi = fmaxf(fmaxf(hi, x[e]), x[e + 1]);
-    }
-    float bad = nan ? 1.f : 0.f;
-    lo = fminf(lo, quad1(lo));
-    hi = fmaxf(hi, quad1(hi));
-    bad = fmaxf(bad, quad1(bad));
-    lo = fminf(lo, quad2(lo));
-    hi = fmaxf(hi, quad2(hi));
-    bad = fmaxf(bad, quad2(bad));
-    lo = fminf(fmaxf(lo, -65504.f), 65504.f);
-    hi = fminf(fmaxf(hi, -65504.f), 65504.f);
-    constexpr int MOST = (1 << BITS) - 1;
-    f16 least = (f16)lo, step;
-    {
-      const double range = (double)hi - (double)(float)least;
-      const float r = (float)range;
-      step = (f16)((double)r == range ? r / (float)MOST : (float)(range / (double)MOST));   // (the same number: both quotients are rounded to the nearest)
-    }
-    if (bad != 0.f) least = __builtin_bit_cast(f16, (uint16_t)0x7e00), step = (f16)0.f;
-    const float l32 = (float)least, s32 = (float)step;
     uint32_t w[2] = {0u, 0u};
-    if (s32 != 0.f) {                                   // (below zero where the least value was rounded up past the greatest one)
-      // the quotient rounded in the low bits of 1.5 * 2^23 + it
-      const float inv = __builtin_amdgcn_rcpf(s32), magic = 12582912.f;
-      uint32_t code[8];
-      float off = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const float d = x[e] - l32, r = fmaf(d, inv, magic);
-        off = fmaxf(off, fabsf(fmaf(d, inv, magic - r)));
-        code[e] = __builtin_bit_cast(uint32_t, fminf(fmaxf(r, magic), magic + (float)MOST));
-      }
-      // x - least is off by 2^-24 of itself, the reciprocal by 2^-23, so the quotient by 3 * 2^-24 * MOST: decided in 64 bits where the middle is as near
-      if (off > 0.5f - MOST * 0x1p-22f) {
-        const double h = 0.5 * fabs((double)s32);
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const int n0 = (int)(code[e] & 0x1ffu);
-          const double rest = ((double)x[e] - (double)l32) - (double)n0 * (double)s32, rem = s32 < 0.f ? -rest : rest;
-          const bool odd = n0 & 1;
-          const int m = n0 + (rem > h || (rem == h && odd) ? 1 : 0) - (rem < -h || (rem == -h && odd) ? 1 : 0);
-          code[e] = (uint32_t)(m < 0 ? 0 : m > MOST ? MOST : m);
-        }
-      }
-      if constexpr (BITS == 4) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) w[0] |= (code[e] & 15u) << (4 * (e >> 1) + 16 * (e & 1));
-      } else {
-#pragma unroll
-        for (int e = 0; e < 2; e++)
-          w[e] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(code[4 * e + 3], code[4 * e + 2], 0x0c0c0400u), __builtin_amdgcn_perm(code[4 * e + 1], code[4 * e], 0x0c0c0400u), 0x05040100u);
-      }
+    f16 least, step;
+    if (ROTATED && !value) {
+      double y[8];
+      turn_chunk<CHUNKS>(y, x, j, a.pairs, a.neighbours, turns);
+      quantise<BITS>(y, w, least, step);
+    } else {
+      quantise<BITS>(x, w, least, step);
     }
     unsigned char *base = a.pages + ((int64_t)page * a.heads + head) * P::bytes(a.block);
     unsigned char *to = base + P::codes(a.block, value) + at * P::ROW + P::chunk(c, g);
@@ -194,15 +266,18 @@ template <typename T, int BITS, int D> __global__ void __launch_bounds__(256) k_
 // few positions: each workgroup reads the slots behind its own, which costs less than the launch that says whose a slot is
 constexpr int kScan = 512;
 
-template <typename T, int BITS, int D> int launch_cache(const CacheArgs &a, bool write, hipStream_t st) {
-  if (!write) {
-    hipLaunchKernelGGL((k_cache_read<T, BITS, D>), dim3((unsigned)a.T), dim3(256), 0, st, a);
-  } else if (a.T <= kScan) {
-    hipLaunchKernelGGL((k_cache_write<T, BITS, D, true>), dim3((unsigned)a.T), dim3(256), 0, st, a);
+template <typename T, int BITS, int D, bool ROTATED> void launch_cache_write(const CacheArgs &a, hipStream_t st) {
+  if (a.T <= kScan) {
+    hipLaunchKernelGGL((k_cache_write<T, BITS, D, true, ROTATED>), dim3((unsigned)a.T), dim3(256), 0, st, a);
   } else {
     hipLaunchKernelGGL(k_cache_owner, dim3((unsigned)cdiv(a.T, 256)), dim3(256), 0, st, a);
-    hipLaunchKernelGGL((k_cache_write<T, BITS, D, false>), dim3((unsigned)a.T), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((k_cache_write<T, BITS, D, false, ROTATED>), dim3((unsigned)a.T), dim3(256), 0, st, a);
   }
+}
+template <typename T, int BITS, int D> int launch_cache(const CacheArgs &a, bool write, hipStream_t st) {
+  if (!write) hipLaunchKernelGGL((k_cache_read<T, BITS, D>), dim3((unsigned)a.T), dim3(256), 0, st, a);
+  else if (a.fractions) launch_cache_write<T, BITS, D, true>(a, st);
+  else launch_cache_write<T, BITS, D, false>(a, st);
   BSP_LAUNCH_CHECK();
   return BSP_OK;
 }
@@ -235,9 +310,8 @@ extern "C" int64_t bsp_cache_page_bytes(int block, int heads, int D, int bits) {
   return 2 * (int64_t)block * heads * (D * bits / 8 + D / 8);
 }
 
-extern "C" int bsp_cache_write(int dtype, void *pages, int n_pages, int block, int heads, int D, int bits, const void *k, int64_t k_stride_t, int64_t k_stride_h,
-                               const void *v, int64_t v_stride_t, int64_t v_stride_h, const int32_t *slots, int T, int32_t *owner, void *stream) {
-  CacheArgs a;
+static int cache_write(int dtype, void *pages, int n_pages, int block, int heads, int D, int bits, const void *k, int64_t k_stride_t, int64_t k_stride_h,
+                       const void *v, int64_t v_stride_t, int64_t v_stride_h, const int32_t *slots, int T, int32_t *owner, CacheArgs &a) {
   const int rc = cache_args(dtype, pages, n_pages, block, heads, D, bits, slots, T, a);
   if (rc != BSP_OK) return rc;
   const int unit = dtype == BSP_F32 ? 4 : 8;
@@ -245,6 +319,24 @@ extern "C" int bsp_cache_write(int dtype, void *pages, int n_pages, int block, i
   if (k_stride_t % unit || k_stride_h % unit || v_stride_t % unit || v_stride_h % unit) return BSP_ERR_ARG;
   a.k = k; a.v = v; a.k_st = k_stride_t; a.k_sh = k_stride_h; a.v_st = v_stride_t; a.v_sh = v_stride_h;
   a.owner = owner;
+  return BSP_OK;
+}
+
+extern "C" int bsp_cache_write(int dtype, void *pages, int n_pages, int block, int heads, int D, int bits, const void *k, int64_t k_stride_t, int64_t k_stride_h,
+                               const void *v, int64_t v_stride_t, int64_t v_stride_h, const int32_t *slots, int T, int32_t *owner, void *stream) {
+  CacheArgs a;
+  const int rc = cache_write(dtype, pages, n_pages, block, heads, D, bits, k, k_stride_t, k_stride_h, v, v_stride_t, v_stride_h, slots, T, owner, a);
+  return rc != BSP_OK ? rc : launch_cache(dtype, a, bits, D, true, as_stream(stream));
+}
+
+extern "C" int bsp_cache_write_rotated(int dtype, void *pages, int n_pages, int block, int heads, int D, int bits, const void *k, int64_t k_stride_t, int64_t k_stride_h,
+                                       const void *v, int64_t v_stride_t, int64_t v_stride_h, const int32_t *slots, int T, int32_t *owner, const uint64_t *fractions, int pairs,
+                                       int neighbours, const int32_t *positions, void *stream) {
+  CacheArgs a;
+  const int rc = cache_write(dtype, pages, n_pages, block, heads, D, bits, k, k_stride_t, k_stride_h, v, v_stride_t, v_stride_h, slots, T, owner, a);
+  if (rc != BSP_OK) return rc;
+  if (!rotation_ok(fractions, pairs, D) || !positions) return BSP_ERR_ARG;
+  a.fractions = fractions; a.pairs = pairs; a.neighbours = neighbours != 0; a.positions = positions;
   return launch_cache(dtype, a, bits, D, true, as_stream(stream));
 }
 

@@ -97,9 +97,16 @@ SIGNATURES = {
     'bsp_attention_f32_bwd': (_i, [_vp] * 9 + [_i, _vp, _i, _vp, _i, _vp]),
     'bsp_attention_rules_fwd': (_i, [_vp] * 6),
     'bsp_attention_rules_bwd': (_i, [_vp] * 11 + [_i, _vp, _i, _vp, _i, _vp]),
+    'bsp_rotate': (_i, [_i, _i, _i64, _i, _i, _i, _i, _vp, _vp, _i64, _i64, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp]),
     'bsp_cache_page_bytes': (_i64, [_i] * 4),
     'bsp_cache_write': (_i, [_i, _vp, _i, _i, _i, _i, _i, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i, _vp, _vp]),
+    'bsp_cache_write_rotated': (_i, [_i, _vp, _i, _i, _i, _i, _i, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i, _vp, _vp, _i, _i, _vp, _vp]),
     'bsp_cache_read': (_i, [_i, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _i, _vp]),
+    'bsp_latent_write': (_i, [_i, _vp, _i, _i, _i, _vp, _i64, _vp, _i64, _vp, _i, _vp, _vp, _i, _i, _vp, _vp]),
+    'bsp_latent_read': (_i, [_i, _vp, _i, _i, _i, _vp, _vp, _vp, _i, _vp]),
+    'bsp_latent_attention_heads': (_i, [_i]),
+    'bsp_latent_attention_workspace_bytes': (_i64, [_i, _i, _i, _i, _i64]),
+    'bsp_latent_attention': (_i, [_i, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i, _i, _vp, _i, _i, _i, _vp, _i64, _i, _vp, _vp, _i, _i64, _f, _f, _vp, _vp, _i64, _vp]),
     'bsp_cache_attention_splits': (_i, [_i, _i, _i, _i, _i64]),
     'bsp_cache_attention_workspace_bytes': (_i64, [_i] * 5),
     'bsp_cache_attention': (_i, [_i, _vp, _i64, _i64, _vp, _i64, _i64, _i, _i, _vp, _i, _i, _i, _i, _i, _vp, _i64, _i, _vp, _vp, _i, _i64, _f, _f, _vp, _vp, _i64, _i, _vp]),

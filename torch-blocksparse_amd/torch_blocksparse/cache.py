@@ -15,10 +15,49 @@ float16's range first; where the rounding of a step takes one past it again, flo
 import torch
 
 from . import _lib
+from .rotation import Rotation
 from .rules import check_scores
 
 
-class KeyValueCache:
+def check_rotation(rotation, positions, tokens, dim, device):
+    """the positions [tokens] that a cache is given with a rotation of `dim` elements, as its kernels read them"""
+    if rotation is None:
+        if positions is not None:
+            raise ValueError('positions go with a rotation')
+        return None
+    if not isinstance(rotation, Rotation):
+        raise ValueError('rotation must be a Rotation (got %s)' % type(rotation).__name__)
+    if 2 * rotation.pairs > dim:
+        raise ValueError('a rotation of %d pairs does not fit %d elements' % (rotation.pairs, dim))
+    if positions is None:
+        raise ValueError('a rotation needs positions')
+    rotation.check_positions(positions, ((tokens,),), device)
+    return positions.contiguous()
+
+
+class Pages:
+    """what the caches of this package have in common: positions in pages, named by slots, written by whatever stream is current"""
+
+    def _note_users(self):
+        self._users = _lib.Readers()                       # (the streams of all calls: memory that is given back while one writes it would change under its next owner)
+        self._users.table(self.data, self._owner)
+
+    def __getstate__(self):
+        return {n: x for n, x in self.__dict__.items() if n != '_users'}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._note_users()
+
+    def _check_slots(self, slots):
+        if slots.dim() != 1 or slots.dtype != torch.int32 or slots.device != self.device:
+            raise ValueError('slots must be a vector of int32 on %s (got %s %s on %s)' % (self.device, slots.dtype, list(slots.shape), slots.device))
+        if slots.numel() >= 1 << 24:
+            raise ValueError('a call takes fewer than 2^24 tokens (got %d)' % slots.numel())
+        return slots.contiguous()
+
+
+class KeyValueCache(Pages):
     """pages of `block` (16, 32, 64 or 128) positions of `heads` key heads of 64 or 128 elements, in 4 or 8 bits.  `data` holds the pages
     ([pages, bytes of a page]; zeros at first, which stand for zeros); what a page means to a program, a table of its own says."""
 
@@ -41,24 +80,6 @@ class KeyValueCache:
         self._owner = torch.zeros(self.pages * block, dtype=torch.int32, device=device)     # (zero between calls: bsp_cache_write)
         self._note_users()
 
-    def _note_users(self):
-        self._users = _lib.Readers()                       # (the streams of all calls: memory that is given back while one writes it would change under its next owner)
-        self._users.table(self.data, self._owner)
-
-    def __getstate__(self):
-        return {n: x for n, x in self.__dict__.items() if n != '_users'}
-
-    def __setstate__(self, state):
-        self.__dict__.update(state)
-        self._note_users()
-
-    def _check_slots(self, slots):
-        if slots.dim() != 1 or slots.dtype != torch.int32 or slots.device != self.device:
-            raise ValueError('slots must be a vector of int32 on %s (got %s %s on %s)' % (self.device, slots.dtype, list(slots.shape), slots.device))
-        if slots.numel() >= 1 << 24:
-            raise ValueError('a call takes fewer than 2^24 tokens (got %d)' % slots.numel())
-        return slots.contiguous()
-
     def _operand(self, t, name, tokens):
         if t.device != self.device:
             raise _lib.BlocksparseLibraryError('torch_blocksparse: %s must live on %s (got device %s)' % (name, self.device, t.device))
@@ -72,12 +93,16 @@ class KeyValueCache:
             t = t.clone(memory_format=torch.contiguous_format)
         return t, (t.stride(0) if t.size(0) > 1 else 0), (t.stride(1) if t.size(1) > 1 else 0)
 
-    def write(self, k, v, slots):
+    def write(self, k, v, slots, rotation=None, positions=None):
         """Quantises k and v [tokens, heads, head_dim] (of one type) into positions slots[t] = page * block + offset of the cache.  Tokens with a
         negative slot, or one past the cache, are left out; of tokens with the same slot the last is written.  No gradient.  Two writes that run at
-        the same time (on two streams) and have a slot in common leave it as one of them, or half of each."""
+        the same time (on two streams) and have a slot in common leave it as one of them, or half of each.
+
+        With a `Rotation` and the tokens' positions [tokens] int32 the keys are turned on the way, in 64 bits and with no rounding before their codes (so a NaN or an infinity makes
+        its pair's other element one too); what `rotation(k, positions=positions)` gives is rounded to the type of k."""
         slots = self._check_slots(slots)
         T = slots.numel()
+        positions = check_rotation(rotation, positions, T, self.head_dim, self.device)
         k, k_st, k_sh = self._operand(k, 'k', T)
         v, v_st, v_sh = self._operand(v, 'v', T)
         if k.dtype != v.dtype:
@@ -88,8 +113,12 @@ class KeyValueCache:
             stream = _lib.raw_stream(self.device)
             if stream not in self._users.streams:
                 self._users.read(self.device)
-            rc = _lib.load().bsp_cache_write(_lib.DTYPES[k.dtype], self.data.data_ptr(), self.pages, self.block, self.heads, self.head_dim, self.bits, k.data_ptr(), k_st, k_sh,
-                                             v.data_ptr(), v_st, v_sh, slots.data_ptr(), T, self._owner.data_ptr(), stream)
+            args = (_lib.DTYPES[k.dtype], self.data.data_ptr(), self.pages, self.block, self.heads, self.head_dim, self.bits, k.data_ptr(), k_st, k_sh,
+                    v.data_ptr(), v_st, v_sh, slots.data_ptr(), T, self._owner.data_ptr())
+            if rotation is None:
+                rc = _lib.load().bsp_cache_write(*args, stream)
+            else:
+                rc = _lib.load().bsp_cache_write_rotated(*args, rotation.fractions(self.device).data_ptr(), rotation.pairs, rotation.neighbours, positions.data_ptr(), stream)
         _lib.check(rc, 'bsp_cache_write')
 
     def read(self, slots, dtype=torch.float16):
@@ -176,6 +205,8 @@ class CacheAttention:
             raise _lib.BlocksparseLibraryError('torch_blocksparse: q must live on %s, where the cache is (got device %s)' % (cache.device, q.device))
         if q.dtype not in (torch.float16, torch.bfloat16):
             raise ValueError('CacheAttention supports float16 and bfloat16 (got %s)' % q.dtype)
+        if not isinstance(cache, KeyValueCache):
+            raise ValueError('CacheAttention reads a KeyValueCache (got %s)' % type(cache).__name__)
         if cache.block != self.block:
             raise ValueError('the cache has pages of %d, the attention blocks of %d' % (cache.block, self.block))
         if q.dim() != 3 or q.size(2) != cache.head_dim or q.size(1) == 0 or q.size(1) % cache.heads:
