@@ -523,6 +523,20 @@ int bsp_attention_rules_bwd(const bsp_attention_rules_call *call, const void *d_
                             void *dq, void *dk, void *dv, float *neg_delta, const int32_t *d_items, int n_items, float *partial, int n_slots,
                             const int32_t *d_split, int n_split, void *stream);
 
+/* The same with keys of which all heads share a part (the expanded form of latent attention): scale * (q_i . k_j + q'_i . k'_j) in the place of scale * q_i . k_j, q' [Z, H, length, 64] and k'
+ * [Z, length, 64] (part->q, part->k) in the call's type.  bwd also writes dq' = part->dq and, where dk and dv are written, dk' = part->dk, the sum over all heads, of which part->dk_heads keeps each key head's: [Z][kv_heads]
+ * [length][64] floats of scratch; partial is [Z][n_slots][64 * (2 * D + 64)] floats then.  strides: q' batch, head, row; k' batch, row; dq' batch, head, row; dk' batch, row; with the rules of the others.  Z < 65536. */
+typedef struct {
+  const void *q, *k;
+  int64_t strides[10];
+  void *dq, *dk;
+  float *dk_heads;
+} bsp_attention_shared_part;
+int bsp_attention_shared_fwd(const bsp_attention_rules_call *call, const bsp_attention_shared_part *part, const void *q, const void *k, const void *v, void *o, void *stream);
+int bsp_attention_shared_bwd(const bsp_attention_rules_call *call, const bsp_attention_shared_part *part, const void *d_o, const void *q, const void *k, const void *v, const void *o,
+                             void *dq, void *dk, void *dv, float *neg_delta, const int32_t *d_items, int n_items, float *partial, int n_slots, const int32_t *d_split,
+                             int n_split, void *stream);
+
 /* Rotated positions: y = x with the pairs of the first 2 * pairs of each row's D elements turned by position * frequency (back: minus that),
  *     (a, b) -> (a cos - b sin, a sin + b cos),
  * pair p being elements p and pairs + p, or 2 p and 2 p + 1 (neighbours); the others are copied.  fractions: [pairs], frequency / (2 pi) less whole turns, in units of

@@ -40,9 +40,14 @@ struct RuleArgs {
   const int32_t *ranges; int groups;   // per batch and group of sixteen positions the least and the greatest document number (least: -1 if any is negative)
   int causal, capped;
   const int32_t *lut;
-  float *partial;                  // column kernel: slots of the parts of long columns, [Z][n_slots][dk, dv][64][D]
+  float *partial;                  // column kernel: slots of the parts of long columns, [Z][n_slots][dk, dv][64][D] (and [64][X])
   const int32_t *split_lut;
   int n_slots, n_split;
+  // the kernels with X > 0: what every query head adds to its rows and all key heads share, X elements a row (logits of q . k + qx . kx)
+  const void *qx, *kx;
+  void *ox;                        // row kernel: the gradient of qx
+  float *kx_heads;                 // column kernel: the gradient of kx for each key head, [Z][key heads][L][X]
+  int64_t qx_sz, qx_sh, qx_ld, kx_sz, kx_ld, ox_sz, ox_sh, ox_ld;
   int Z, H, G, R, L;               // G: query heads a key head; R: lines of the table per head, 64 R >= L (column kernel: work items of a key head)
 };
 
@@ -50,9 +55,12 @@ namespace {
 
 template <typename T, int D> struct Geo {
   static constexpr int ESZ = sizeof(T), RB = D * ESZ, CPR = RB / 16, NF = RB / 32, VEC = 16 / ESZ;   // bytes and 16-byte chunks of a row; operand fragments; elements a chunk
-  static constexpr int PIECE = 32 * RB, STAGE = 2 * PIECE, RING = 2 * STAGE;
+  static constexpr int PIECE = 32 * RB;
   static constexpr int EXTRA = 768;                      // bytes behind each stage's pieces: documents, statistics
 };
+template <typename T> struct Geo<T, 0> { static constexpr int RB = 0, PIECE = 0, NF = 0; };
+// Two stages of the pieces of 32 rows: two of D elements, and one of the X elements that are shared
+template <typename T, int D, int X> struct RuleRing { static constexpr int THIRD = 2 * Geo<T, D>::PIECE, STAGE = THIRD + Geo<T, X>::PIECE, RING = 2 * STAGE; };
 template <typename T> struct RuleOperand { typedef typename Mma<T, 32>::frag_t type; };
 template <> struct RuleOperand<float> { typedef f32x4 type; };
 template <typename T, int D> using held_t = typename RuleOperand<T>::type[Geo<T, D>::NF];
@@ -216,14 +224,15 @@ __device__ __forceinline__ void columns_times(f32x16 (&acc)[D / 32], const Piece
 
 // ... + (32 rows of a piece, transposed) . e for sixteen values a lane in two operands, what they are rounded to and what that leaves out: as exact as
 // products of fp32 numbers, for half as many products again
-template <typename T, int D, int OFF, bool LEAN>
-__device__ __forceinline__ void columns_times_exact(f32x16 (&acc)[D / 32], const PieceReads<T, D, LEAN> &reads, float (&e)[16]) {
-  typedef Mma<T, 32> M;
-  Shares<T> most, rest;
+template <typename T> __device__ __forceinline__ void two_terms(float (&e)[16], Shares<T> &most, Shares<T> &rest) {
   most.set(e);
 #pragma unroll
   for (int i = 0; i < 16; i++) e[i] -= to_float(most.f[i >> 3][i & 7]);
   rest.set(e);
+}
+template <typename T, int D, int OFF, bool LEAN>
+__device__ __forceinline__ void columns_times_exact(f32x16 (&acc)[D / 32], const PieceReads<T, D, LEAN> &reads, const Shares<T> &most, const Shares<T> &rest) {
+  typedef Mma<T, 32> M;
   uint32_t lo[D / 32], hi[D / 32];
   reads.tr.get(lo, hi);
 #pragma unroll
@@ -492,16 +501,16 @@ template <typename T, int D> __device__ __forceinline__ void store_some_rows(uns
   }
   __builtin_amdgcn_wave_barrier();
 }
-template <typename T, int D> constexpr int rules_lds() {
-  constexpr int ring = Geo<T, D>::RING + 2 * Geo<T, D>::EXTRA, out = 64 * (D + Geo<T, D>::VEC) * Geo<T, D>::ESZ;
+template <typename T, int D, int X> constexpr int rules_lds() {
+  constexpr int ring = RuleRing<T, D, X>::RING + 2 * Geo<T, D>::EXTRA, out = 64 * (D + Geo<T, D>::VEC) * Geo<T, D>::ESZ;
   return ring > out ? ring : out;
 }
 
 // A launch of few lines has two pairs of wavefronts to a line, each of which takes every other half of a tile, with a ring of its own; at the end the second
 // pair's sums are added to the first's through its ring.
-template <typename T, int D, int PAIRS> constexpr int pair_lds() {
-  constexpr int sums = 2 * 64 * 4 * (D / 2 + 2);        // two wavefronts' accumulators, maxima and sums
-  return PAIRS == 1 || rules_lds<T, D>() > sums ? rules_lds<T, D>() : sums;
+template <typename T, int D, int X, int PAIRS> constexpr int pair_lds() {
+  constexpr int sums = 2 * 64 * 4 * (D / 2 + X / 2 + 2);        // two wavefronts' accumulators, maxima and sums
+  return PAIRS == 1 || rules_lds<T, D, X>() > sums ? rules_lds<T, D, X>() : sums;
 }
 // The halves of the pair of wavefronts `group`; more: some pair has one; pads: one of them has padding
 struct Halves { Half own; bool more, pads; };
@@ -557,6 +566,7 @@ __device__ __forceinline__ void lds_barrier() {
 // 456 -> 318 (578 -> 642), 82 -> 63 (126 -> 104); 2048 of them 693 -> 577 (1130 -> 1261), 124 -> 116 (198 -> 217); twelve heads of 256 lines of BigBird fp16 51 -> 59.
 // Short lines, of 7 tiles (BigBird): fp16 768 lines 18.0 -> 17.3, 1536 29.7 -> 31.9; bf16 of 128 elements 512 lines 22.9 -> 19.2, 1024 30.6 -> 35.6; fp32 512 lines 68.6 -> 43.3, 1024 76.8 ->
 // 78.7, of 128 elements 256 74.3 -> 45.3, 512 80.2 -> 91.6; of one tile: fp16 768 lines 7.1 -> 8.1, bf16 of 128 elements 1024 14.5 -> 19.4, fp32 512 12.6 -> 11.8, of 128 elements 21.8 -> 29.0.
+constexpr int kLdsBytes = 160 * 1024;                     // of a compute unit
 template <typename T, int D> inline bool few_lines(const RuleArgs &a) {
   return a.R >= 4 && (int64_t)a.Z * a.H * a.R <= (D == 64 ? 2048 : sizeof(T) == 4 ? 512 : 1024);
 }
@@ -568,7 +578,15 @@ template <typename K> int rules_launch(K kernel, int64_t n_wg, int threads, int 
 
 }  // namespace
 
-// call -> kernel arguments, checked (attention_rules_fwd.hip)
+constexpr int kShared = 64;                               // elements of a key part that all heads share (attention_shared_fwd.hip, attention_shared_bwd.hip)
+int shared_args(const bsp_attention_rules_call *call, const bsp_attention_shared_part *part, bool backward, RuleArgs &a);
+
+// call -> kernel arguments, checked (attention_rules_fwd.hip, attention_rules_bwd.hip)
 int rules_args(const bsp_attention_rules_call *c, RuleArgs &a);
+int rules_fwd_args(const bsp_attention_rules_call *call, const void *q, const void *k, const void *v, void *o, RuleArgs &a);
+void rules_ranges(const RuleArgs &a, int32_t *ranges, hipStream_t st);
+int rules_bwd_args(const bsp_attention_rules_call *call, const void *d_o, const void *q, const void *k, const void *v, const void *o, void *dq, void *dk, void *dv, float *neg_delta,
+                   const int32_t *d_items, int n_items, float *partial, int n_slots, const int32_t *d_split, int n_split, RuleArgs &a);
+void rules_bwd_columns(const bsp_attention_rules_call *call, void *dk, void *dv, const int32_t *d_items, int n_items, float *partial, int n_slots, const int32_t *d_split, int n_split, RuleArgs &a);
 }  // namespace bsp
 #endif

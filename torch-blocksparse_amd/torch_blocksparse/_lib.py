@@ -97,6 +97,8 @@ SIGNATURES = {
     'bsp_attention_f32_bwd': (_i, [_vp] * 9 + [_i, _vp, _i, _vp, _i, _vp]),
     'bsp_attention_rules_fwd': (_i, [_vp] * 6),
     'bsp_attention_rules_bwd': (_i, [_vp] * 11 + [_i, _vp, _i, _vp, _i, _vp]),
+    'bsp_attention_shared_fwd': (_i, [_vp] * 7),
+    'bsp_attention_shared_bwd': (_i, [_vp] * 12 + [_i, _vp, _i, _vp, _i, _vp]),
     'bsp_rotate': (_i, [_i, _i, _i64, _i, _i, _i, _i, _vp, _vp, _i64, _i64, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp]),
     'bsp_cache_page_bytes': (_i64, [_i] * 4),
     'bsp_cache_write': (_i, [_i, _vp, _i, _i, _i, _i, _i, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i, _vp, _vp]),

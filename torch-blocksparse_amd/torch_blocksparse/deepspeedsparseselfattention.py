@@ -19,9 +19,10 @@ import torch.nn as nn
 from . import _lib
 from .attention_core import attention_chain
 from .cache import CacheAttention
+from .latent import LatentAttention, LatentCache
 from .layouts import fixed_layout
 from .matmul import MatMul
-from .rules import Attention
+from .rules import SHARED, Attention
 from .softmax import Softmax
 
 
@@ -144,11 +145,12 @@ class DeepSpeedSparseSelfAttention(nn.Module):
         return x.squeeze()
 
     def forward(self, query, key, value, rpe=None, key_padding_mask=None, attn_mask=None, *, softcap=0., slopes=None, causal=False,
-                documents=None, prefix=None):
+                documents=None, prefix=None, shared=None):
         """Attention over the configuration's layout, scores scaled by head_dim ** -0.5.  With one of softcap, slopes, causal, documents and prefix, or with
-        keys and values of fewer heads than the query, it is that of `Attention` with these rules: any length, and no rpe or masks beside them."""
+        keys and values of fewer heads than the query, it is that of `Attention` with these rules: any length, and no rpe or masks beside them.  With shared too, whose 64 elements
+        then count as the head's: the scale is (head_dim + 64) ** -0.5."""
         fewer_heads = query.dim() == key.dim() == 4 and key.size(1) < query.size(1)
-        if softcap or slopes is not None or causal or documents is not None or prefix is not None or fewer_heads:
+        if softcap or slopes is not None or causal or documents is not None or prefix is not None or shared is not None or fewer_heads:
             if rpe is not None or key_padding_mask is not None or attn_mask is not None:
                 raise ValueError('softcap, slopes, causal, documents, prefix and shared key heads do not go with rpe, key_padding_mask and attn_mask')
             if query.dim() != 4 or key.dim() != 4:
@@ -156,7 +158,8 @@ class DeepSpeedSparseSelfAttention(nn.Module):
             key = self.transpose_key_for_scores(key, query.size(2))
             block = self.sparsity_config.block
             op = self._kept('rules', query.size(1), -(-query.size(2) // block), lambda layout: Attention(layout, block))
-            return op(query, key, value, scale=float(query.size(3)) ** -0.5, softcap=softcap, slopes=slopes, causal=causal, documents=documents, prefix=prefix)
+            width = query.size(3) + (SHARED if shared is not None else 0)
+            return op(query, key, value, scale=float(width) ** -0.5, softcap=softcap, slopes=slopes, causal=causal, documents=documents, prefix=prefix, shared=shared)
         bsz, num_heads, tgt_len, head_dim = query.size()
         key = self.transpose_key_for_scores(key, tgt_len)
         if query.shape != key.shape or key.shape != value.shape:
@@ -172,23 +175,32 @@ class DeepSpeedSparseSelfAttention(nn.Module):
                                key_padding_mask=key_padding_mask, attn_mask=attn_mask,
                                key_padding_mask_mode=self.key_padding_mask_mode, attn_mask_mode=self.attn_mask_mode)
 
-    def decode(self, query, cache, table, lengths, *, softcap=0., slopes=None):
+    def decode(self, query, cache, table, lengths, *, softcap=0., slopes=None, shared=None, scale=None):
         """One new position a sequence: query [batch, heads, head_dim] over the pages `table` [batch, width] of `cache`, which hold `lengths` [batch]
         positions of each sequence, the new one among them (`CacheAttention`).  It is what `forward` with causal=True and the same softcap and slopes gives
-        for each sequence's last position, over keys and values as the cache holds them."""
+        for each sequence's last position, over keys and values as the cache holds them.
+
+        Over a `LatentCache` (`LatentAttention`) query [batch, heads, latent] has the key matrices in it already, shared [batch, heads, 64] is its other part, scale is that of the
+        expanded heads, (head_dim + 64) ** -0.5, and the value matrices are for what is returned."""
         if query.dim() != 3 or table.dim() != 2:
             raise ValueError('query must have shape [batch, heads, head_dim], table [batch, width]')
         cfg = self.sparsity_config
+        latent = isinstance(cache, LatentCache)
+        if latent != (shared is not None) or latent != (scale is not None):
+            raise ValueError('a LatentCache, and no other, takes shared and scale')
+        Decode = LatentAttention if latent else CacheAttention
         # Rows of the layout are the same in a longer one, as far as a position sees: one operator serves a quarter of an octave of widths, and a
         # table that grows by a page finds it made.  Where everything is seen no layout is needed.
         if cfg.mode == 'dense':
-            blocks, make = 0, lambda layout: CacheAttention(cfg.block)
+            blocks, make = 0, lambda layout: Decode(cfg.block)
         else:
             unit = max(16, 1 << max(0, table.size(1).bit_length() - 3))
-            blocks, make = -(-max(1, table.size(1)) // unit) * unit, lambda layout: CacheAttention(cfg.block, layout)
+            blocks, make = -(-max(1, table.size(1)) // unit) * unit, lambda layout: Decode(cfg.block, layout)
             if blocks > 65535 >= table.size(1):
                 blocks = 65535                           # (the longest that CacheAttention takes)
-        op = self._kept('decode', query.size(1), blocks, make)
+        op = self._kept('latent' if latent else 'decode', query.size(1), blocks, make)
+        if latent:
+            return op(query, shared, cache, table, lengths, scale=scale, softcap=softcap, slopes=slopes)
         return op(query, cache, table, lengths, scale=float(query.size(2)) ** -0.5, softcap=softcap, slopes=slopes)
 
 

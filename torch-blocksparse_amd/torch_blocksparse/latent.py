@@ -14,9 +14,7 @@ import torch
 
 from . import _lib
 from .cache import Pages, check_rotation
-from .rules import check_scores
-
-SHARED = 64                   # elements of the key part that all heads share
+from .rules import SHARED, check_scores
 
 
 class LatentCache(Pages):

@@ -226,6 +226,74 @@ class _rules(torch.autograd.Function):
         return dq if need_q else None, dk if need_k else None, dv if need_v else None, None, None, None, None, None, None, None, None
 
 
+# bsp_attention_shared_part: q, k; strides[10]; dq, dk, dk_heads
+_PART = struct.Struct('@2P10q3P')
+SHARED = 64                   # elements of a key part that all heads share
+
+
+class _shared_rules(torch.autograd.Function):
+    """_rules with a part q_s [Z, H, L, 64] . k_s [Z, L, 64] of the scores, k_s for all heads"""
+
+    @staticmethod
+    def _parts(q_s, k_s):
+        Z, H, L, _ = q_s.shape
+        (q_s, q_at), (k_s, k_at) = _operand(q_s, Z, H, L, SHARED), _operand(k_s.unsqueeze(1), Z, 1, L, SHARED)
+        return q_s, q_at, k_s, (k_at[0], k_at[2])
+
+    @staticmethod
+    def forward(ctx, q, k, v, q_s, k_s, tables, scale, softcap, slopes, causal, documents, prefix, grad_enabled):
+        Z, H, L, D = q.shape
+        kv, device = k.size(1), q.device
+        (q, q_at), (k, k_at), (v, v_at) = _operand(q, Z, H, L, D), _operand(k, Z, kv, L, D), _operand(v, Z, kv, L, D)
+        own_k_s = k_s
+        q_s, qs_at, k_s, ks_at = _shared_rules._parts(q_s, k_s)
+        keep = grad_enabled and any(ctx.needs_input_grad[:5])
+        o = torch.empty((Z, H, L, D), dtype=q.dtype, device=device)
+        stats = torch.empty((Z, H, 2, 64 * tables.lines), dtype=torch.float32, device=device) if keep else None
+        rest = torch.empty((Z, H, L, D), dtype=q.dtype, device=device) if keep and q.element_size() == 2 else None
+        ranges = torch.empty((Z, (L + 15) // 16, 2), dtype=torch.int32, device=device) if documents is not None else None
+        call = _rules.call(q, kv, q_at + k_at + v_at + _own(Z, H, L, D) + (0,) * 12, tables, scale, softcap, slopes, causal, documents, prefix, ranges, stats, rest)
+        part = _PART.pack(q_s.data_ptr(), k_s.data_ptr(), *qs_at, *ks_at, 0, 0, 0, 0, 0, 0, 0, 0)
+        rc = _lib.load().bsp_attention_shared_fwd(call, part, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _lib.raw_stream(device))
+        if rc:
+            _lib.check(rc, 'bsp_attention_shared_fwd')
+        if keep:
+            ctx.save_for_backward(q, k, v, q_s, own_k_s, o, rest, stats, ranges, slopes, documents, prefix)
+            ctx.tables, ctx.numbers = tables, (scale, softcap, causal)
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        q, k, v, q_s, k_s, o, rest, stats, ranges, slopes, documents, prefix = ctx.saved_tensors
+        tables, (scale, softcap, causal) = ctx.tables, ctx.numbers
+        need = ctx.needs_input_grad[:5]
+        device, dtype = q.device, q.dtype
+        with _lib.on_device(device):
+            Z, H, L, D = q.shape
+            kv = k.size(1)
+            (q, q_at), (k, k_at), (v, v_at) = _operand(q, Z, H, L, D), _operand(k, Z, kv, L, D), _operand(v, Z, kv, L, D)
+            (o, o_at), (do, do_at) = _operand(o, Z, H, L, D), _operand(do, Z, H, L, D)
+            q_s, qs_at, k_s, ks_at = _shared_rules._parts(q_s, k_s)
+            dq, dq_s = [torch.empty((Z, H, L, n), dtype=dtype, device=device) for n in (D, SHARED)]
+            dk = dv = dk_s = heads = None
+            delta = torch.empty((Z, H, 64 * tables.lines), dtype=torch.float32, device=device)
+            items, n_items, splits, n_splits, slots, partial = None, 0, None, 0, 0, None
+            if need[1] or need[2] or need[4]:
+                dk, dv = [torch.empty((Z, kv, L, D), dtype=dtype, device=device) for _ in range(2)]
+                dk_s, heads = torch.empty((Z, L, SHARED), dtype=dtype, device=device), torch.empty((Z, kv, L, SHARED), dtype=torch.float32, device=device)
+                items, n_items, splits, n_splits, slots = tables.columns(kv, Z)
+                partial = torch.empty((Z, slots, 64, 2 * D + SHARED), dtype=torch.float32, device=device) if slots else None
+            own = _own(Z, kv, L, D)
+            call = _rules.call(q, kv, q_at + k_at + v_at + o_at + do_at + _own(Z, H, L, D) + own + own, tables, scale, softcap, slopes, causal, documents, prefix, ranges, stats, rest)
+            part = _PART.pack(q_s.data_ptr(), k_s.data_ptr(), *qs_at, *ks_at, *_own(Z, H, L, SHARED), L * SHARED, SHARED, dq_s.data_ptr(), _at(dk_s), _at(heads))
+            rc = _lib.load().bsp_attention_shared_bwd(call, part, do.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), dq.data_ptr(), _at(dk), _at(dv), delta.data_ptr(),
+                                                      _at(items), n_items, _at(partial), slots, _at(splits), n_splits, _lib.raw_stream(device))
+            if rc:
+                _lib.check(rc, 'bsp_attention_shared_bwd')
+        return tuple(g if n else None for g, n in zip((dq, dk, dv, dq_s, dk_s), need)) + (None,) * 8
+
+
 class Attention:
     """Attention over a block-sparse layout [heads, blocks, blocks] (block 16, 32, 64 or 128) with score rules.
 
@@ -239,8 +307,10 @@ class Attention:
     causal    row i sees the keys up to i only
     documents None, or [batch, length] int32: a row sees keys of its own document only; negative: padding
     prefix    None, or [batch] int32, with causal: keys before prefix[z] are seen by every row
+    shared    None, or (q_s [batch, heads, length, 64], k_s [batch, length, 64]): scale * (q . k + q_s . k_s) in the place of scale * q . k, with one k_s for all heads, as latent attention
+              has where its keys and values are expanded (`LatentAttention` is its other form)
 
-    Differentiable in q, k and v, once.  Tables are made at the first call on a device (for a backward pass, at the first
+    Differentiable in q, k, v and shared, once.  Tables are made at the first call on a device (for a backward pass, at the first
     one), so a call that is captured into a graph needs one like it before."""
 
     def __init__(self, layout, block):
@@ -286,8 +356,8 @@ class Attention:
             raise ValueError('the rows of a head lie within 4 GiB (got length %d)' % L)
         if H // kv > 127:
             raise ValueError('at most 127 query heads share a key head (got %d)' % (H // kv))
-        if 128 * -(-L // 64) * (H // kv) >= 1 << 30 and torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
-            raise ValueError('the gradient of a key head reads the rows of fewer than 2^29 positions (got %d query heads of %d)' % (H // kv, L))
+        if k.requires_grad or v.requires_grad:
+            self._check_columns(q, k)
         heads, blocks = self.layout.shape[:2]
         if H != heads or -(-L // self.block) != blocks:
             raise ValueError('q %s does not fit a layout of %d heads and %d blocks of %d' % (tuple(q.shape), heads, blocks, self.block))
@@ -300,11 +370,36 @@ class Attention:
         if slopes is not None and slopes.requires_grad and torch.is_grad_enabled():
             raise ValueError('slopes are constants: they get no gradient')
 
-    def __call__(self, q, k, v, scale=1., softcap=0., slopes=None, causal=False, documents=None, prefix=None):
+    @staticmethod
+    def _check_columns(q, k):
+        G, L = q.size(1) // k.size(1), q.size(2)
+        if 128 * -(-L // 64) * G >= 1 << 30 and torch.is_grad_enabled():
+            raise ValueError('the gradient of a key head reads the rows of fewer than 2^29 positions (got %d query heads of %d)' % (G, L))
+
+    @staticmethod
+    def _check_shared(q, k, shared):
+        if not isinstance(shared, (tuple, list)) or len(shared) != 2:
+            raise ValueError('shared must be a pair of tensors, of the queries and of the keys')
+        q_s, k_s = shared
+        for t in shared:
+            _lib.require_gpu_tensor(t, 'a shared part')
+            if t.dtype != q.dtype or t.device != q.device:
+                raise ValueError('shared must be of the type of q, k and v, and on their device')
+        Z, H, L = q.shape[:3]
+        if tuple(q_s.shape) != (Z, H, L, SHARED) or tuple(k_s.shape) != (Z, L, SHARED):
+            raise ValueError('shared must be %s and %s (got %s and %s)' % ([Z, H, L, SHARED], [Z, L, SHARED], list(q_s.shape), list(k_s.shape)))
+        if Z > 65535:
+            raise ValueError('at most 65535 sequences share key parts in a call (got %d)' % Z)
+
+    def __call__(self, q, k, v, scale=1., softcap=0., slopes=None, causal=False, documents=None, prefix=None, shared=None):
         scale, softcap = float(scale), float(softcap or 0.)
         self._check(q, k, v, softcap, scale, slopes, causal, documents, prefix)
+        if shared is not None:
+            self._check_shared(q, k, shared)
+            if shared[1].requires_grad and not (k.requires_grad or v.requires_grad):
+                self._check_columns(q, k)
         if q.numel() == 0:
-            return torch.empty_like(q) + 0 * (q.sum() + k.sum() + v.sum())
+            return torch.empty_like(q) + 0 * (q.sum() + k.sum() + v.sum() + (shared[0].sum() + shared[1].sum() if shared is not None else 0))
         if slopes is not None:
             slopes = slopes.contiguous()
         if prefix is not None:
@@ -312,4 +407,6 @@ class Attention:
         if documents is not None and documents.size(1) > 1 and documents.stride(1) != 1:
             documents = documents.contiguous()
         with _lib.on_device(q.device):
+            if shared is not None:
+                return _shared_rules.apply(q, k, v, *shared, self._tables_for_a_launch(q.device), scale, softcap, slopes, bool(causal), documents, prefix, torch.is_grad_enabled())
             return _rules.apply(q, k, v, self._tables_for_a_launch(q.device), scale, softcap, slopes, bool(causal), documents, prefix, torch.is_grad_enabled())
