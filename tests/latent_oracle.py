@@ -2,7 +2,8 @@
 
 With u half a step of the type, K = latent + 64 and n the positions of a sequence: the operands are exact and a score is summed in fp32, so it is off by (K + 8) 2^-24 of the sum of its terms' sizes, by
 softcap * 2^-22 with a cap and by 4 * 2^-24 of the distance's part; a share (an exponential over a sum of n of them) by twice the largest of that and (n + 16) 2^-24 relative to itself. A share goes into
-the product in two terms: u^2 of it, in fp16 not less than 2^-25 for shares that are relative to a maximum of 1 or less. The product is summed in fp32 (n 2^-24 of the terms), the result rounded once."""
+the product in two terms: u^2 of it, in fp16 not less than 2^-25 for shares that are relative to a maximum of 1 or less.  With more than 32 heads a workgroup (of at most 64, as evenly as can be) it goes
+in one, rounded by u of itself, and the sum is that of the rounded ones: p_j (1 + d_j) / sum_k p_k (1 + d_k) with all |d| <= u is off by u sum_j p_j |c_j| in the one and by u |o| in the other. The product is summed in fp32 (n 2^-24 of the terms), the result rounded once."""
 import math
 
 import torch
@@ -44,7 +45,8 @@ def attention(q, q_r, c, r, table, lengths, block, layout=None, scale=1., softca
         p = p / torch.where(total == 0, 1., total)
         off = 2 * torch.where(seen, off, 0.).amax(1, keepdim=True) + (2 * n + 24) * 2. ** -24 + u * u
         value[b] = p @ cb
-        bound[b] = u * value[b].abs() + off * (1 + u) * (p @ cb.abs()) + tiny * (1 + seen.double() @ cb.abs())
+        one_term = u if -(-H // -(-H // 64)) > 32 else 0.
+        bound[b] = one_term * (p @ cb.abs() + value[b].abs()) * (1 + 2 * u) + u * value[b].abs() + off * (1 + u) * (p @ cb.abs()) + tiny * (1 + seen.double() @ cb.abs())
     return value, bound
 
 

@@ -28,7 +28,7 @@ struct LatentArgs {
   int n_rows;
   const float *slopes;
   float scale, cap;
-  float *partial;                  // two slots a workgroup, [heads a unit][latent + 2]: maximum, sum, sums
+  float *partial;                  // two slots a workgroup: [heads a unit][latent] sums; behind all of them [heads a unit][2] maxima and sums of shares
   int32_t *meta;                   // per item (sequence and unit) three ints: the workgroup that begins it, how many have a part (0, 1: nothing to join), the first part's slot
   int B, H, block, shift;          // shift: log2 of the groups of sixteen positions a block
   int units, per, pieces;          // workgroups' heads a sequence: units of `per`; pieces of the work
@@ -36,30 +36,28 @@ struct LatentArgs {
 
 namespace {
 
-template <typename T> struct Latent16;
-template <> struct Latent16<f16> {
+template <typename T> struct LatentMma;
+template <> struct LatentMma<f16> {
   typedef f16x8 frag8; typedef f16x4 frag4;
   static __device__ __forceinline__ f32x4 run(frag8 a, frag8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
   static __device__ __forceinline__ f32x4 run(frag4 a, frag4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ f32x16 run(frag8 a, frag8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
-template <> struct Latent16<bf16> {
+template <> struct LatentMma<bf16> {
   typedef bf16x8 frag8; typedef bf16x4 frag4;
   static __device__ __forceinline__ f32x4 run(frag8 a, frag8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
   static __device__ __forceinline__ f32x4 run(frag4 a, frag4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0); }
+  static __device__ __forceinline__ f32x16 run(frag8 a, frag8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
 
 template <int LAT> struct LatentGeo {
   static constexpr int ROW = 2 * (LAT + kRope), LROW = 2 * LAT;               // bytes of a position, of its latent vector
   static constexpr int GROUP = 16 * ROW, STAGE = 4 * GROUP, RING = 2 * STAGE;   // sixteen positions: their latent vectors, then their shared parts
   static constexpr int JOIN = LAT + 4;                                         // floats of a head's sums when wavefronts are joined
-  static constexpr int LDS = RING + 64 * 2 * 4;
-  static_assert(64 * JOIN * 4 <= RING, "");
+  static constexpr int CPR = LROW / 16, RPI = 64 / CPR, LOADS = 16 / RPI + 2;   // 16-byte chunks of a latent vector, rows of a load, loads of a group
+  static constexpr int STATS = RING, SHARES = RING + 1024, LDS = SHARES + 4 * 2048;   // behind the stages: heads' maxima and sums; a wavefront's shares (Heads32)
+  static_assert(64 * JOIN * 4 <= RING && LDS <= 160 * 1024, "");
 };
-
-// where 16-byte chunk `chunk` of row r of a group lies: latent vectors with the chunks of 256 bytes exchanged by r, so that sixteen rows' reads of a chunk take sixteen places of
-// the 64 banks, and so do transposing reads of eight rows' pairs of chunks; shared parts, of which two rows fill 256 bytes, by r / 2
-__device__ __forceinline__ uint32_t latent_chunk(uint32_t chunk, uint32_t r) { return chunk ^ r; }
-__device__ __forceinline__ uint32_t rope_chunk(uint32_t chunk, uint32_t r) { return chunk ^ (r >> 1); }
 
 typedef int i32x4b __attribute__((ext_vector_type(4)));
 // 16 bytes a lane from `rows` (a buffer: zeros from behind its end) to 1 KB of LDS
@@ -67,10 +65,453 @@ __device__ __forceinline__ void rows_to_lds(const i32x4b &rows, uint32_t off, ui
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rows), "s"(dst) : "m0", "memory");
 }
 template <typename V> __device__ __forceinline__ V latent_read(uint32_t at) { return *(const V __attribute__((address_space(3))) *)(uintptr_t)at; }
+template <typename V> __device__ __forceinline__ void latent_put(uint32_t at, const V &v) { *(V __attribute__((address_space(3))) *)(uintptr_t)at = v; }
 __device__ __forceinline__ s16x4 latent_read_tr(uint32_t at) {
   typedef s16x4 __attribute__((address_space(3))) * lds_ptr;
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(uintptr_t)at);
 }
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ s16x8 latent_read_tr2(uint32_t at, uint32_t then) { return __builtin_shufflevector(latent_read_tr(at), latent_read_tr(then), 0, 1, 2, 3, 4, 5, 6, 7); }
+// a value that the compiler does not look into
+__device__ __forceinline__ uint32_t own(uint32_t v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+// sums times f, left where the matrix units have them (all at once in the other registers, they would take the place of what the loop keeps there)
+template <typename V> __device__ __forceinline__ V scaled_by(V v, float f) {
+  v *= f;
+  asm volatile("" : "+a"(v));
+  return v;
+}
+// shared parts in LDS: two rows fill the 256 bytes of the 64 banks
+__device__ __forceinline__ uint32_t rope_chunk(uint32_t chunk, uint32_t r) { return chunk ^ (r >> 1); }
+
+// sixteen positions as a step sees them: the first one's number in the sequence, how many count, the heads (bits, the wavefront's own) that see them
+struct LatentGroup { int pos, n, mask; };
+// what a score is made of
+struct LatentScores { float factor, cap; bool capped, sloped; int last; };   // last: the new position
+// N logits, in the log2 domain, less `minus`: one multiply-add each where there is neither a cap nor a bias.  pos(i): the position of score i
+template <int N, class S, class P> __device__ __forceinline__ void latent_logits(float (&y)[N], S &&score, const LatentScores &c, float slope, float minus, P &&pos) {
+  if (!c.capped && !c.sloped) {
+#pragma unroll
+    for (int i = 0; i < N; i++) y[i] = fmaf(score(i), c.factor, -minus);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; i++) y[i] = score(i) * c.factor;
+  if (c.capped)
+#pragma unroll
+    for (int i = 0; i < N; i++) y[i] = c.cap * fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y[i]) + 1.f), 1.f);
+#pragma unroll
+  for (int i = 0; i < N; i++) y[i] = fmaf(-slope, (float)(c.last - pos(i)), y[i]) - minus;
+}
+// the lowest n of four bits, n any number
+__device__ __forceinline__ uint32_t first_of_four(int n) { return (1u << (n < 0 ? 0 : n > 4 ? 4 : n)) - 1u; }
+__device__ __forceinline__ void barrier_of_all() {        // everybody's LDS operations are done
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// The operands of both products come from LDS a batch of four reads at a time while the products of batches before are taken; left alone, the compiler reads one and waits for it, to save registers.  Every
+// batch also issues its part of the next step's loads (load(k)): all at once they would hold up the wavefront for the time that a compute unit takes for them, 64 bytes a clock.
+//
+// Sixteen heads a wavefront (at most 32 a workgroup), each wavefront HW of a step's groups.  Shares in two terms: what they are rounded to and what that leaves out.  The chunks of a latent vector in LDS: every row
+// begins in the first bank, so pairs of chunks of 256 bytes are exchanged by the row's number, which serves both reads without a conflict: a transposing read takes a pair from each of
+// eight rows at a time, a read along the rows a chunk of eight rows and its neighbour of the eight others.
+template <typename T, int LAT, int HW> struct Heads16 {
+  typedef LatentGeo<LAT> G;
+  typedef LatentMma<T> M;
+  typedef typename M::frag8 frag8;
+  typedef typename std::conditional<HW == 1, typename M::frag4, frag8>::type frag;
+  static constexpr int GROUPS = HW, SOURCES = 4 / HW, NS = LAT / 32, NR = kRope / 32, NT = LAT / 16;
+  static constexpr bool BARRIER = HW > 1, OWN_SUMS = true;   // OWN_SUMS: each source has sums of its own
+  static __device__ __forceinline__ uint32_t chunk(uint32_t c, uint32_t r, uint32_t group) { return c ^ (r & 7) << 1; }
+  static __device__ __forceinline__ int first_group(int wave) { return wave / HW * HW; }
+  static __device__ __forceinline__ int head_of(int wave, int lane) { return 16 * (wave % HW) + (lane & 15); }
+  static __device__ __forceinline__ int mask(int wave, int lo, int hi) { return lo >> (16 * (wave % HW)); }
+  // the rows that have what wavefronts found of head h, and where a row's head begins in the sums
+  static __device__ __forceinline__ int source(int h, int p) { return 16 * (p * HW + h / 16) + h % 16; }
+  static __device__ __forceinline__ int sums(int h, int p) { return source(h, p); }
+
+  frag8 q[NS + NR];
+  f32x4 o[NT];
+  float m, l, slope, scaled;
+  uint32_t row_at, rope_at, tr_at;                      // in a group: the lane's row (positions across the matrix rows), and of the transposing reads
+  int key, c;
+  bool here;
+
+  __device__ __forceinline__ void init(const T *pq, const T *pr, bool here_, float slope_, int wave, int lane, uint32_t) {
+    key = lane & 15; c = lane >> 4; here = here_; slope = slope_;
+#pragma unroll
+    for (int s = 0; s < NS + NR; s++) {
+      const T *from = s < NS ? pq + 32 * s : pr + 32 * (s - NS);
+      q[s] = __builtin_bit_cast(frag8, here ? *reinterpret_cast<const u32x4 *>(from + 8 * c) : u32x4{0, 0, 0, 0});
+    }
+    row_at = key * G::LROW + (chunk(c, key, 0) << 4);
+    rope_at = 16 * G::LROW + key * (2 * kRope) + (rope_chunk(c, key) << 4);
+    const uint32_t r = 4 * c + (key >> 2);
+    tr_at = r * G::LROW + (chunk((key & 3) >> 1, r, 0) << 4) + 8 * (key & 1);
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int n = 0; n < NT; n++) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // the queries are here (looked at in the loop, the compiler would wait there for all loads of the next step)
+  __device__ __forceinline__ void arrived() {
+#pragma unroll
+    for (int s = 0; s < NS + NR; s++) asm volatile("" : "+v"(q[s]));
+  }
+
+  // false: the sums are to be scaled first, then the step taken again
+  template <class F> __device__ __forceinline__ bool step(uint32_t stage_of_all, const LatentGroup (&now)[GROUPS], const LatentScores &scores, bool again, bool, int wave, F &&load) {
+    // the step's addresses; all others are constants away (as values of their own, or the compiler keeps hundreds of sums with those constants)
+    const uint32_t stage = stage_of_all + first_group(wave) * G::GROUP;
+    uint32_t at_row[4], at_rope[NR], at_col[8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) at_row[i] = own(stage + (own(row_at) ^ (i << 6)));
+#pragma unroll
+    for (int i = 0; i < NR; i++) at_rope[i] = own(stage + (own(rope_at) ^ (i << 6)));
+    // scores: value 4 k + i is that of position 4 c + i of group k
+    constexpr int ALL = NS + NR, TB = 4 / HW, BATCHES = (ALL + TB - 1) / TB, AHEAD = 3;
+    constexpr int CHAINS = 4 / HW;                        // four products that do not wait for each other
+    f32x4 acc[HW][CHAINS];
+#pragma unroll
+    for (int k = 0; k < HW; k++)
+#pragma unroll
+      for (int x = 0; x < CHAINS; x++) acc[k][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+    frag8 rows[AHEAD + 1][4];
+    auto read_rows = [&](int b) {
+#pragma unroll
+      for (int j = 0; j < TB; j++)
+#pragma unroll
+        for (int k = 0; k < HW; k++) {
+          const int t = b * TB + j;
+          if (t < ALL) rows[b % (AHEAD + 1)][j * HW + k] = latent_read<frag8>((t < NS ? at_row[t & 3] + (t >> 2) * 256 : at_rope[t < NS ? 0 : t - NS]) + k * G::GROUP);
+        }
+    };
+#pragma unroll
+    for (int b = 0; b < AHEAD; b++) read_rows(b);
+#pragma unroll
+    for (int b = 0; b < BATCHES; b++) {
+      if (b + AHEAD < BATCHES) read_rows(b + AHEAD);
+#pragma unroll
+      for (int k = b * G::LOADS / BATCHES; k < (b + 1) * G::LOADS / BATCHES; k++) load(k);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < TB; j++)
+#pragma unroll
+        for (int k = 0; k < HW; k++) {
+          const int t = b * TB + j;
+          if (t < ALL) acc[k][t % CHAINS] = M::run(rows[b % (AHEAD + 1)][j * HW + k], q[t], acc[k][t % CHAINS]);
+        }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    constexpr int PAIRS = HW == 1 ? 1 : HW / 2, NB = NT / 4, PER = HW == 1 ? 4 : 8;
+    frag cols[3][4];
+#pragma unroll
+    for (int i = 0; i < 8; i++) at_col[i] = own(stage + (own(tr_at) ^ (i << 5)));
+    auto read_cols = [&](int b) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int n = b % NB * 4 + j;
+        const uint32_t from = at_col[n & 7] + b / NB * 2 * G::GROUP + (n >> 3) * 256;
+        if constexpr (HW == 1) cols[b % 3][j] = __builtin_bit_cast(frag, latent_read_tr(from));
+        else cols[b % 3][j] = __builtin_bit_cast(frag, latent_read_tr2(from, from + G::GROUP));
+      }
+    };
+    read_cols(0);
+    read_cols(1);
+    __builtin_amdgcn_sched_barrier(0);
+    uint32_t seen = (1u << (4 * HW)) - 1u;
+    bool all = true;
+#pragma unroll
+    for (int k = 0; k < HW; k++) all = all && now[k].n == 16 && (now[k].mask & 0xffff) == 0xffff;
+    if (!all) {
+      seen = 0;
+#pragma unroll
+      for (int k = 0; k < HW; k++) seen |= (here && (now[k].mask >> key & 1) ? first_of_four(now[k].n - 4 * c) : 0u) << (4 * k);
+    }
+    float sc[4 * HW];
+#pragma unroll
+    for (int i = 0; i < 4 * HW; i++) sc[i] = HW == 1 ? (acc[i >> 2][0][i & 3] + acc[i >> 2][1][i & 3]) + (acc[i >> 2][2 % CHAINS][i & 3] + acc[i >> 2][3 % CHAINS][i & 3]) : acc[i >> 2][0][i & 3] + acc[i >> 2][1][i & 3];
+    auto logits = [&](float (&y)[4 * HW], float minus) {
+      latent_logits(y, [&](int i) { return sc[i]; }, scores, slope, minus, [&](int i) { return now[i >> 2].pos + 4 * c + (i & 3); });
+    };
+    // shares relative to the running maximum, which moves when they grow past 8192
+    float e[4 * HW], sum;
+    auto exponentials = [&]() {
+      logits(e, m == -INFINITY ? 0.f : m);
+#pragma unroll
+      for (int i = 0; i < 4 * HW; i++) e[i] = __builtin_amdgcn_exp2f(e[i]);
+      if (!all)
+#pragma unroll
+        for (int i = 0; i < 4 * HW; i++) e[i] = seen >> i & 1 ? e[i] : 0.f;
+      sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4 * HW; i++) sum += e[i];
+    };
+    exponentials();
+    auto top_of = [&]() {
+      float y[4 * HW], top = -INFINITY;
+      logits(y, 0.f);
+#pragma unroll
+      for (int i = 0; i < 4 * HW; i++) top = fmaxf(top, seen >> i & 1 ? y[i] : -INFINITY);
+      top = fmaxf(top, __shfl_xor(top, 16));
+      return fmaxf(top, __shfl_xor(top, 32));
+    };
+    if (__builtin_amdgcn_ballot_w64(m == -INFINITY && seen != 0)) {            // the first that a head sees: its sums are zeros
+      const float top = top_of();
+      m = m == -INFINITY ? top : m;
+      exponentials();
+    }
+    if (!again && __builtin_amdgcn_ballot_w64(sum > 8192.f)) {
+      const float mn = fmaxf(m, top_of());
+      scaled = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+      l *= scaled;
+      m = mn;
+      return false;
+    }
+    l += sum;
+    frag most[PAIRS], rest[PAIRS];
+#pragma unroll
+    for (int i = 0; i < 4 * HW; i++) {
+      most[i / PER][i % PER] = from_float<T>(e[i]);
+      rest[i / PER][i % PER] = from_float<T>(e[i] - to_float(most[i / PER][i % PER]));
+    }
+#pragma unroll
+    for (int b = 0; b < PAIRS * NB; b++) {
+      if (b + 2 < PAIRS * NB) read_cols(b + 2);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < 4; j++) o[b % NB * 4 + j] = M::run(cols[b % 3][j], most[b / NB], o[b % NB * 4 + j]);
+#pragma unroll
+      for (int j = 0; j < 4; j++) o[b % NB * 4 + j] = M::run(cols[b % 3][j], rest[b / NB], o[b % NB * 4 + j]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    return true;
+  }
+  __device__ __forceinline__ void scale() {
+#pragma unroll
+    for (int n = 0; n < NT; n++) o[n] = scaled_by(o[n], scaled);
+  }
+  // maximum, sum and sums to their row
+  __device__ __forceinline__ void put(float *join, float *stats, int wave) {
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    const int r = 16 * wave + key;
+    if (c == 0) stats[2 * r] = m, stats[2 * r + 1] = l;
+#pragma unroll
+    for (int n = 0; n < NT; n++) *reinterpret_cast<f32x4 *>(join + r * G::JOIN + 16 * n + 4 * c) = o[n];
+  }
+};
+
+// 32 heads a wavefront, two wavefronts for the same heads (64 a workgroup): each has the scores of half of a step's positions and, with the other's shares through LDS, the sums of half of the elements, on
+// 32 x 32 x 16 products.  That is half of the reads from LDS of Heads16 for so many heads, and what bounds those.  Shares in one term, which takes a sum's error from that of the result's rounding to 1.4
+// times that: a second one is half again the products (latent_long: 126 us with it, 103 without, both in Heads16).  Pairs of chunks in LDS by two bits of the row's number and the third, as a
+// transposing read takes four chunks of four rows; the lowest bit by the group, as a read along the rows takes a chunk of eight rows of each of two groups.
+template <typename T, int LAT> struct Heads32 {
+  typedef LatentGeo<LAT> G;
+  typedef LatentMma<T> M;
+  typedef typename M::frag8 frag8;
+  static constexpr int GROUPS = 2, SOURCES = 2, NS = LAT / 16, NR = kRope / 16, NT = LAT / 64, HELD = NS < 22 ? NS : 22;   // NT: the wavefront's tiles of 32 elements
+  static constexpr bool BARRIER = true, OWN_SUMS = false;
+  static __device__ __forceinline__ uint32_t chunk(uint32_t c, uint32_t r, uint32_t group) { return c ^ ((r & 3) << 2 | (r >> 1 & 2) | (group & 1)); }
+  static __device__ __forceinline__ int first_group(int wave) { return 2 * (wave & 1); }
+  static __device__ __forceinline__ int head_of(int wave, int lane) { return 32 * (wave >> 1) + (lane & 31); }
+  static __device__ __forceinline__ int mask(int wave, int lo, int hi) { return wave & 2 ? hi : lo; }
+  static __device__ __forceinline__ int source(int h, int p) { return 64 * (h / 32) + 32 * p + h % 32; }   // (of a maximum and sum; the sums are whole)
+  static __device__ __forceinline__ int sums(int h, int) { return h; }
+
+  frag8 q[NS + NR];
+  f32x16 o[NT];
+  float m, l, slope, scaled;
+  uint32_t row_at, rope_at, tr_at, tr_at2, shares, tops;
+  int key, half;
+  bool here;
+
+  __device__ __forceinline__ void init(const T *pq, const T *pr, bool here_, float slope_, int wave, int lane, uint32_t lds) {
+    key = lane & 31; half = lane >> 5; here = here_; slope = slope_;
+#pragma unroll
+    for (int s = 0; s < NS + NR; s++) {
+      const T *from = s < NS ? pq + 16 * s : pr + 16 * (s - NS);
+      q[s] = __builtin_bit_cast(frag8, here ? *reinterpret_cast<const u32x4 *>(from + 8 * half) : u32x4{0, 0, 0, 0});
+    }
+    const uint32_t r = key & 15, group = key >> 4;
+    row_at = group * G::GROUP + r * G::LROW + (chunk(half, r, group) << 4);
+    rope_at = group * G::GROUP + 16 * G::LROW + r * (2 * kRope) + (rope_chunk(half, r) << 4);
+    // transposed: rows 4 half + 0 .. 3 of a group, and those eight further on, whose chunks are exchanged alike
+    const uint32_t i = lane & 15, tr = 4 * half + (i >> 2), col = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+    const uint32_t half_of = (wave & 1) * (LAT / 16);     // (the wavefront's half of the elements, in chunks)
+    tr_at = tr * G::LROW + (chunk(half_of + col, tr, 0) << 4) + 8 * (i & 1);
+    tr_at2 = tr * G::LROW + (chunk(half_of + col, tr, 1) << 4) + 8 * (i & 1);
+    shares = lds + G::SHARES + wave * 2048 + lane * 16;
+    tops = lds + G::STATS + wave * 128 + key * 4;
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int x = 0; x < 16; x++) o[n][x] = 0.f;
+  }
+
+  __device__ __forceinline__ void arrived() {
+#pragma unroll
+    for (int s = 0; s < HELD; s++) asm volatile("" : "+a"(q[s]));   // (beside sums and scores, which fills those registers with LAT = 512)
+#pragma unroll
+    for (int s = HELD; s < NS + NR; s++) asm volatile("" : "+v"(q[s]));
+  }
+
+  template <class F> __device__ __forceinline__ bool step(uint32_t stage, const LatentGroup (&now)[GROUPS], const LatentScores &scores, bool again, bool first, int wave, F &&load) {
+    uint32_t at_row[8], at_rope[NR], at_col[2][4];
+    const uint32_t own_groups = stage + first_group(wave) * G::GROUP;
+#pragma unroll
+    for (int i = 0; i < 8; i++) at_row[i] = own(own_groups + (own(row_at) ^ (i << 5)));
+#pragma unroll
+    for (int i = 0; i < NR; i++) at_rope[i] = own(own_groups + (own(rope_at) ^ (i << 5)));
+    // scores: value i is that of position 8 (i / 4) % 16 + 4 half + i % 4 of group i / 8
+    constexpr int ALL = NS + NR, AHEAD = 6, RING = AHEAD + 2;
+    constexpr int CHAINS = 2;
+    f32x16 acc[CHAINS];
+#pragma unroll
+    for (int x = 0; x < CHAINS; x++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) acc[x][i] = 0.f;
+    frag8 rows[RING];
+    auto read_row = [&](int t) { rows[t % RING] = latent_read<frag8>(t < NS ? at_row[t & 7] + (t >> 3) * 256 : at_rope[t < NS ? 0 : t - NS]); };
+#pragma unroll
+    for (int t = 0; t < AHEAD; t++) read_row(t);
+#pragma unroll
+    for (int t = 0; t < ALL; t += 2) {
+      if (t + AHEAD < ALL) read_row(t + AHEAD), read_row(t + AHEAD + 1);
+#pragma unroll
+      for (int k = t * G::LOADS / ALL; k < (t + 2) * G::LOADS / ALL; k++) load(k);
+      __builtin_amdgcn_sched_barrier(0);
+      acc[t % CHAINS] = M::run(rows[t % RING], q[t], acc[t % CHAINS]);
+      acc[(t + 1) % CHAINS] = M::run(rows[(t + 1) % RING], q[t + 1], acc[(t + 1) % CHAINS]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // (what the second product begins with on its way)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      at_col[0][i] = own(stage + (own(tr_at) ^ (i << 6)));
+      at_col[1][i] = own(stage + (own(tr_at2) ^ (i << 6)));
+    }
+    // a batch: four products, of a group's sixteen positions or, where the wavefront has two tiles, of two groups'
+    frag8 cols[3][4];
+    constexpr int NB = NT;                                // batches
+    auto at = [&](int b, int j, int &n, int &g) { n = (b * 4 + j) % NT; g = (b * 4 + j) / NT; };
+    auto read_cols = [&](int b) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        int n, g;
+        at(b, j, n, g);
+        const uint32_t from = at_col[g & 1][n & 3] + g * G::GROUP + (n >> 2) * 256;
+        cols[b % 3][j] = __builtin_bit_cast(frag8, latent_read_tr2(from, from + 8 * G::LROW));
+      }
+    };
+    read_cols(0);
+    if (NB > 1) read_cols(1);
+    __builtin_amdgcn_sched_barrier(0);
+    float sc[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) sc[i] = acc[0][i] + acc[1][i];
+    uint32_t seen = 0xffffu;
+    const bool all = now[0].n == 16 && now[1].n == 16 && (now[0].mask & now[1].mask) == -1;
+    if (!all) {
+      seen = 0;
+#pragma unroll
+      for (int g = 0; g < 2; g++)
+        if (here && (now[g].mask >> key & 1)) seen |= (first_of_four(now[g].n - 4 * half) | first_of_four(now[g].n - 8 - 4 * half) << 4) << (8 * g);
+    }
+    auto logits = [&](float (&y)[16], float minus) {
+      latent_logits(y, [&](int i) { return sc[i]; }, scores, slope, minus, [&](int i) { return now[i >> 3].pos + 8 * (i >> 2 & 1) + 4 * half + (i & 3); });
+    };
+    // shares relative to the running maximum, the same in both wavefronts of a head
+    frag8 p[2];
+    float sum;
+    auto exponentials = [&]() {
+      float e[16];
+      logits(e, m == -INFINITY ? 0.f : m);
+#pragma unroll
+      for (int i = 0; i < 16; i++) e[i] = __builtin_amdgcn_exp2f(e[i]);
+      if (!all)
+#pragma unroll
+        for (int i = 0; i < 16; i++) e[i] = seen >> i & 1 ? e[i] : 0.f;
+      float part[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) part[i] = (e[i] + e[4 + i]) + (e[8 + i] + e[12 + i]);
+      sum = (part[0] + part[1]) + (part[2] + part[3]);
+#pragma unroll
+      for (int i = 0; i < 16; i++) p[i >> 3][i & 7] = from_float<T>(e[i]);
+    };
+    frag8 their[2];
+    const uint32_t flags = shares - (uint32_t)((threadIdx.x & 63) * 16 + wave * 2048) - 256;     // (between the maxima and the shares)
+    auto exchange = [&](int word) {                       // the shares to the other wavefront, a word to all; returns whether any wavefront's is not zero
+#pragma unroll
+      for (int g = 0; g < 2; g++) latent_put(shares + 1024 * g, __builtin_bit_cast(u32x4, p[g]));
+      if ((threadIdx.x & 63) == 0) latent_put(flags + 4 * wave, word);
+      barrier_of_all();
+      const i32x4b f = latent_read<i32x4b>(flags);
+#pragma unroll
+      for (int g = 0; g < 2; g++) their[g] = latent_read<frag8>((shares ^ 2048) + 1024 * g);
+      return __builtin_amdgcn_readfirstlane(f[0] | f[1] | f[2] | f[3]) != 0;
+    };
+    exponentials();
+    const bool move = __builtin_amdgcn_ballot_w64(sum > 8192.f || (m == -INFINITY && seen != 0)) != 0;
+    if (exchange(move && !again)) {                       // (all wavefronts take the same way)
+      float y[16], top = -INFINITY;
+      logits(y, 0.f);
+#pragma unroll
+      for (int i = 0; i < 16; i++) top = fmaxf(top, seen >> i & 1 ? y[i] : -INFINITY);
+      top = fmaxf(top, __shfl_xor(top, 32));
+      if (half == 0) latent_put(tops, top);
+      barrier_of_all();
+      const float mn = fmaxf(m, fmaxf(top, latent_read<float>(tops ^ 128)));
+      scaled = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+      l *= scaled;
+      m = mn;
+      if (!first) return false;
+      exponentials();                                     // (the sums are zeros)
+      exchange(0);
+    }
+    l += sum;
+    frag8 share[4];                                       // by group
+#pragma unroll
+    for (int g = 0; g < 2; g++) {
+      share[g] = wave & 1 ? their[g] : p[g];
+      share[2 + g] = wave & 1 ? p[g] : their[g];
+    }
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      if (b + 2 < NB) read_cols(b + 2);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        int n, g;
+        at(b, j, n, g);
+        o[n] = M::run(cols[b % 3][j], share[g], o[n]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    return true;
+  }
+  __device__ __forceinline__ void scale() {
+#pragma unroll
+    for (int n = 0; n < NT; n++) o[n] = scaled_by(o[n], scaled);
+  }
+  __device__ __forceinline__ void put(float *join, float *stats, int wave) {
+    l += __shfl_xor(l, 32);
+    const int r = 32 * wave + key;
+    if (half == 0) stats[2 * r] = m, stats[2 * r + 1] = l;
+    float *to = join + (32 * (wave >> 1) + key) * G::JOIN + (wave & 1) * (LAT / 2) + 4 * half;
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int g = 0; g < 4; g++) *reinterpret_cast<f32x4 *>(to + 32 * n + 8 * g) = f32x4{o[n][4 * g], o[n][4 * g + 1], o[n][4 * g + 2], o[n][4 * g + 3]};
+  }
+};
 
 // An item is a sequence and a unit of its heads; its groups of sixteen positions
 struct LatentItem {
@@ -95,16 +536,12 @@ struct LatentItem {
   __device__ __forceinline__ int steps() const { return (groups + 3) >> 2; }
 };
 
-template <typename T, int LAT, int HW>
+template <typename T, int LAT, class Heads>
 __global__ void __launch_bounds__(256, 1) k_latent_attention(LatentArgs a) {
   typedef LatentGeo<LAT> G;
-  typedef Latent16<T> M;
-  typedef typename M::frag8 frag8;
-  typedef typename M::frag4 frag4;
-  constexpr int NS = LAT / 32, NR = kRope / 32, NT = LAT / 16;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), key = lane & 15, c = lane >> 4;
-  const int hw = wave % HW, mine = wave / HW * HW;                            // the wavefront's heads 16 hw .. of the unit; the first of the HW groups of a step that it goes through
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int mine = Heads::first_group(wave);            // the first of the step's groups that the wavefront goes through
   const uint32_t items = (uint32_t)(a.B * a.units), ring = (uint32_t)(uintptr_t)BSP_LDS_PTR(smem);
 
   // the workgroup's piece [lo, hi) of all steps, and the item that it begins in
@@ -112,7 +549,7 @@ __global__ void __launch_bounds__(256, 1) k_latent_attention(LatentArgs a) {
   uint32_t item = 0;
   int pieces;
   {
-    int *sums = reinterpret_cast<int *>(smem + G::RING);                      // (where no tile goes)
+    int *sums = reinterpret_cast<int *>(smem + G::STATS);                     // (where no tile goes)
     auto chunk_sum = [&](uint32_t base, int &own, int &before) {               // of 256 items: own steps, those of the items before it in the chunk; returns the chunk's
       const uint32_t i = base + tid;
       own = i < items ? LatentItem(a, i).steps() : 0;
@@ -173,11 +610,11 @@ __global__ void __launch_bounds__(256, 1) k_latent_attention(LatentArgs a) {
     }
   }
 
-  const bool capped = a.cap > 0.f;
-  const float factor = capped ? 2.f * kLog2e * a.scale / a.cap : a.scale * kLog2e, top_of_cap = a.cap * kLog2e;
-  // addresses in a group: of the lane's row (positions across the matrix rows), and of the transposing reads
-  const uint32_t row_at = key * G::LROW + (latent_chunk(c, key) << 4), rope_at = 16 * G::LROW + key * (2 * kRope) + (rope_chunk(c, key) << 4);
-  const uint32_t tr_row = 4 * c + (key >> 2), tr_at = tr_row * G::LROW + (latent_chunk((key & 3) >> 1, tr_row) << 4) + 8 * (key & 1);
+  LatentScores scores;
+  scores.capped = a.cap > 0.f;
+  scores.sloped = a.slopes != nullptr;
+  scores.factor = scores.capped ? 2.f * kLog2e * a.scale / a.cap : a.scale * kLog2e;
+  scores.cap = a.cap * kLog2e;
 
   for (int64_t at = lo; at < hi && item < items; item++) {
     const LatentItem it(a, item);
@@ -187,8 +624,7 @@ __global__ void __launch_bounds__(256, 1) k_latent_attention(LatentArgs a) {
     const int groups = __builtin_amdgcn_readfirstlane(it.groups), entry = __builtin_amdgcn_readfirstlane(it.entry);
     const int s0 = (int)(at - begin), s1 = begin + steps < hi ? steps : (int)(hi - begin);
     const int first = unit * a.per, heads = a.H - first < a.per ? a.H - first : a.per;
-    const int head = 16 * hw + key;                       // the lane's head among the unit's
-    const bool head_here = head < heads;
+    scores.last = len - 1;
 
     // 64 groups at a time, one a lane
     int base = s0, v_page = 0, v_pos = 0, v_n = 0, v_sub = 0, v_lo = 0, v_hi = 0;
@@ -211,181 +647,82 @@ __global__ void __launch_bounds__(256, 1) k_latent_attention(LatentArgs a) {
       v_n = n < 0 ? 0 : n > 16 ? 16 : n;
       v_page = v_n > 0 ? page : 0;
     };
-    struct Group { int pos, n, mask; };
     auto group_of = [&](int i) {
-      const int lo32 = __builtin_amdgcn_readlane(v_lo, i), hi32 = __builtin_amdgcn_readlane(v_hi, i);
-      return Group{__builtin_amdgcn_readlane(v_pos, i), __builtin_amdgcn_readlane(v_n, i), ((hw & 2 ? hi32 : lo32) >> (16 * (hw & 1))) & 0xffff};
+      return LatentGroup{__builtin_amdgcn_readlane(v_pos, i), __builtin_amdgcn_readlane(v_n, i), Heads::mask(wave, __builtin_amdgcn_readlane(v_lo, i), __builtin_amdgcn_readlane(v_hi, i))};
     };
-    // the wavefront's group of step s on its way to its place in stage s % 2
-    auto issue = [&](int s) {
+    // the wavefront's group of a step on its way to its place in one of the stages: load k of the group
+    i32x4b rows;
+    uint32_t dst = 0;
+    auto aim = [&](int s) {
       const int i = 4 * (s - base) + wave;
-      const int page = __builtin_amdgcn_readlane(v_page, i), sub = __builtin_amdgcn_readlane(v_sub, i), n = __builtin_amdgcn_readlane(v_n, i);
+      const int page = __builtin_amdgcn_readlane(v_page, i), sub = __builtin_amdgcn_readlane(v_sub, i), n = s < s1 ? __builtin_amdgcn_readlane(v_n, i) : 0;
       const uint64_t from = reinterpret_cast<uint64_t>(a.pages) + ((int64_t)page * a.block + 16 * sub) * (int64_t)G::ROW;
-      const i32x4b rows = {(int)(uint32_t)from, (int)(uint32_t)(from >> 32) & 0xffff, n * G::ROW, 0x00020000};
-      const uint32_t dst = __builtin_amdgcn_readfirstlane(ring + (s & 1) * G::STAGE + wave * G::GROUP);
-      constexpr int CPR = G::LROW / 16, RPI = 64 / CPR;   // chunks of a row, rows of a load
-#pragma unroll
-      for (int k = 0; k < 16 / RPI; k++) {
-        const uint32_t r = k * RPI + lane / CPR;
-        rows_to_lds(rows, r * G::ROW + (latent_chunk(lane % CPR, r) << 4), dst + k * 1024);
-      }
-#pragma unroll
-      for (int k = 0; k < 2; k++) {
-        const uint32_t r = 8 * k + lane / 8;
-        rows_to_lds(rows, r * G::ROW + G::LROW + (rope_chunk(lane % 8, r) << 4), dst + 16 * G::LROW + k * 1024);
-      }
+      rows = i32x4b{(int)(uint32_t)from, (int)(uint32_t)(from >> 32) & 0xffff, n * G::ROW, 0x00020000};
+      dst = __builtin_amdgcn_readfirstlane(ring + (s & 1) * G::STAGE + wave * G::GROUP);
+    };
+    // (a row's number is that of the load's first and the lane's, in bits of their own, and the exchange of chunks goes by bits)
+    const uint32_t lane_chunk = Heads::chunk(lane % G::CPR, lane / G::CPR, wave) << 4, lane_row = lane / G::CPR * G::ROW;
+    const uint32_t lane_rope = rope_chunk(lane % 8, lane / 8) << 4, lane_rope_row = lane / 8 * G::ROW + G::LROW;
+    auto load = [&](int k) {
+      const int j = k - (G::LOADS - 2);
+      if (j < 0) rows_to_lds(rows, (own(lane_chunk) ^ Heads::chunk(0, k * G::RPI, 0) << 4) + (lane_row + k * G::RPI * G::ROW), dst + k * 1024);
+      else rows_to_lds(rows, (own(lane_rope) ^ rope_chunk(0, 8 * j) << 4) + (lane_rope_row + 8 * j * G::ROW), dst + 16 * G::LROW + j * 1024);
     };
 
     look();
-    issue(s0);
-    Group now[HW], next[HW];
+    aim(s0);
 #pragma unroll
-    for (int k = 0; k < HW; k++) now[k] = group_of(mine + k);
-
-    // queries: the second operand, a head a lane
-    frag8 q[NS], qr[NR];
-    float slope = 0.f;
+    for (int k = 0; k < G::LOADS; k++) load(k);
+    Heads x;
     {
-      const T *pq = reinterpret_cast<const T *>(a.q) + b * a.q_sb + (first + (head_here ? head : 0)) * a.q_sh + 8 * c;
-      const T *pr = reinterpret_cast<const T *>(a.qr) + b * a.qr_sb + (first + (head_here ? head : 0)) * a.qr_sh + 8 * c;
-#pragma unroll
-      for (int s = 0; s < NS; s++) q[s] = __builtin_bit_cast(frag8, head_here ? *reinterpret_cast<const u32x4 *>(pq + 32 * s) : u32x4{0, 0, 0, 0});
-#pragma unroll
-      for (int s = 0; s < NR; s++) qr[s] = __builtin_bit_cast(frag8, head_here ? *reinterpret_cast<const u32x4 *>(pr + 32 * s) : u32x4{0, 0, 0, 0});
-      if (a.slopes && head_here) slope = a.slopes[first + head] * kLog2e;
+      const int head = Heads::head_of(wave, lane);        // the lane's head among the unit's
+      const bool here = head < heads;
+      const int64_t h = first + (here ? head : 0);
+      x.init(reinterpret_cast<const T *>(a.q) + b * a.q_sb + h * a.q_sh, reinterpret_cast<const T *>(a.qr) + b * a.qr_sb + h * a.qr_sh, here,
+             a.slopes ? a.slopes[h] * kLog2e : 0.f, wave, lane, ring);
     }
-    float m = -INFINITY, l = 0.f;
-    f32x4 o[NT];
+    LatentGroup now[Heads::GROUPS], next[Heads::GROUPS];
 #pragma unroll
-    for (int n = 0; n < NT; n++) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < Heads::GROUPS; k++) now[k] = next[k] = group_of(mine + k);
 
-    for (int s = s0; s < s1; s++) {
-      BSP_WAIT_VM(0);
-      asm volatile("" ::: "memory");
-      if constexpr (HW > 1) {
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-      }
-      if (s + 1 < s1) {
-        if (s + 1 - base == 16) {
-          base = s + 1;
-          look();
-        }
-        issue(s + 1);
-#pragma unroll
-        for (int k = 0; k < HW; k++) next[k] = group_of(4 * (s + 1 - base) + mine + k);
-      }
-      const uint32_t stage = ring + (s & 1) * G::STAGE + mine * G::GROUP;
-      // scores: value 4 k + i is that of position 4 c + i of group k
-      float y[4 * HW];
-      uint32_t seen = 0;
-#pragma unroll
-      for (int k = 0; k < HW; k++) {
-        f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-        const uint32_t group = stage + k * G::GROUP;
-#pragma unroll
-        for (int t = 0; t < NS; t++) acc[t & 1] = M::run(latent_read<frag8>((group + (row_at ^ ((t & 3) << 6))) + (t >> 2) * 256), q[t], acc[t & 1]);
-#pragma unroll
-        for (int t = 0; t < NR; t++) acc[t & 1] = M::run(latent_read<frag8>(group + (rope_at ^ (t << 6))), qr[t], acc[t & 1]);
-        const bool sees = head_here && (now[k].mask >> key & 1);
-        const float behind = (float)(len - 1 - now[k].pos - 4 * c);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          float x = (acc[0][i] + acc[1][i]) * factor;
-          if (capped) {
-            asm volatile("");                             // (a branch: not computed where there is no cap)
-            x = top_of_cap * fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x) + 1.f), 1.f);
+    // A step whose shares grow past 8192 leaves the loop for the sums to be scaled and is taken again: with that in it, the compiler moves all sums out of the matrix
+    // units' registers and back in every step.
+    x.arrived();
+    int s = s0;
+    bool again = false;
+    while (true) {
+      for (; s < s1; s++) {
+        if (!again) {
+          BSP_WAIT_VM(0);
+          asm volatile("" ::: "memory");
+          if constexpr (Heads::BARRIER) {
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
           }
-          y[4 * k + i] = fmaf(-slope, behind - (float)i, x);
-          seen |= sees && 4 * c + i < now[k].n ? 1u << (4 * k + i) : 0u;
-        }
-      }
-      // shares relative to the running maximum, which moves when they grow past 8192
-      float e[4 * HW], sum;
-      auto exponentials = [&]() {
-        const float ms = m == -INFINITY ? 0.f : m;
-        sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4 * HW; i++) {
-          e[i] = seen >> i & 1 ? __builtin_amdgcn_exp2f(y[i] - ms) : 0.f;
-          sum += e[i];
-        }
-      };
-      exponentials();
-      if (__builtin_amdgcn_ballot_w64(sum > 8192.f || (m == -INFINITY && seen != 0))) {
-        float top = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 4 * HW; i++) top = fmaxf(top, seen >> i & 1 ? y[i] : -INFINITY);
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
-        l *= f;
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-          for (int i = 0; i < 4; i++) o[n][i] *= f;
-        m = mn;
-        exponentials();
-      }
-      l += sum;
-      // results, the shares in two terms: what they are rounded to and what that leaves out
-      if constexpr (HW == 1) {
-        frag4 most, rest;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          most[i] = from_float<T>(e[i]);
-          rest[i] = from_float<T>(e[i] - to_float(most[i]));
-        }
-#pragma unroll
-        for (int n0 = 0; n0 < NT; n0 += 4) {
-          frag4 v[4];
-#pragma unroll
-          for (int n = 0; n < 4; n++) v[n] = __builtin_bit_cast(frag4, latent_read_tr(stage + (tr_at ^ (((n0 + n) & 7) << 5)) + ((n0 + n) >> 3) * 256));
-#pragma unroll
-          for (int n = 0; n < 4; n++) o[n0 + n] = M::run(v[n], most, o[n0 + n]);
-#pragma unroll
-          for (int n = 0; n < 4; n++) o[n0 + n] = M::run(v[n], rest, o[n0 + n]);
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < HW; k += 2) {
-          frag8 most, rest;
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            most[i] = from_float<T>(e[4 * k + i]);
-            rest[i] = from_float<T>(e[4 * k + i] - to_float(most[i]));
+          if (s + 1 - base == 16 && s + 1 < s1) {
+            base = s + 1;
+            look();
           }
+          aim(s + 1);                                     // (behind the last step: loads of nothing; a step that is taken again loads the same again)
+          if (s + 1 < s1) {
 #pragma unroll
-          for (int n0 = 0; n0 < NT; n0 += 4) {
-            frag8 v[4];
-#pragma unroll
-            for (int n = 0; n < 4; n++) {
-              const uint32_t from = stage + k * G::GROUP + (tr_at ^ (((n0 + n) & 7) << 5)) + ((n0 + n) >> 3) * 256;
-              typedef short s16x8 __attribute__((ext_vector_type(8)));
-              v[n] = __builtin_bit_cast(frag8, (s16x8)__builtin_shufflevector(latent_read_tr(from), latent_read_tr(from + G::GROUP), 0, 1, 2, 3, 4, 5, 6, 7));
-            }
-#pragma unroll
-            for (int n = 0; n < 4; n++) o[n0 + n] = M::run(v[n], most, o[n0 + n]);
-#pragma unroll
-            for (int n = 0; n < 4; n++) o[n0 + n] = M::run(v[n], rest, o[n0 + n]);
+            for (int k = 0; k < Heads::GROUPS; k++) next[k] = group_of(4 * (s + 1 - base) + mine + k);
           }
         }
-      }
+        again = !x.step(ring + (s & 1) * G::STAGE, now, scores, again, s == s0, wave, load);
+        if (again) break;
 #pragma unroll
-      for (int k = 0; k < HW; k++) now[k] = next[k];
+        for (int k = 0; k < Heads::GROUPS; k++) now[k] = next[k];
+      }
+      if (s >= s1) break;
+      x.scale();
     }
 
     // the wavefronts' results: per head the maximum, the sum, LAT sums
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
+    BSP_WAIT_VM(0);
     __syncthreads();
-    float *join = reinterpret_cast<float *>(smem), *stats = reinterpret_cast<float *>(smem + G::RING);
-    {
-      const int r = 16 * wave + key;
-      if (c == 0) stats[2 * r] = m, stats[2 * r + 1] = l;
-#pragma unroll
-      for (int n = 0; n < NT; n++) *reinterpret_cast<f32x4 *>(join + r * G::JOIN + 16 * n + 4 * c) = o[n];
-    }
+    float *join = reinterpret_cast<float *>(smem), *stats = reinterpret_cast<float *>(smem + G::STATS);
+    x.put(join, stats, wave);
     __syncthreads();
     const bool whole = s0 == 0 && s1 == steps;
     const int slot = 2 * blockIdx.x + (at > lo ? 1 : 0);
@@ -398,32 +735,53 @@ __global__ void __launch_bounds__(256, 1) k_latent_attention(LatentArgs a) {
       int32_t *to = a.meta + 3 * (int64_t)item;
       to[0] = blockIdx.x; to[1] = parts; to[2] = slot;
     }
-    for (int i = tid; i < heads * (LAT / 8); i += 256) {
-      const int h = i / (LAT / 8), d = i % (LAT / 8) * 8;
-      constexpr int PW = 4 / HW;
-      float top = -INFINITY, sum = 0.f, x[8] = {};
+    // what each source's sums are multiplied by, a head a thread; then four elements a thread, four of them on their way
+    float *by = reinterpret_cast<float *>(smem + G::SHARES);
+    float *parts_of = a.partial + (int64_t)slot * a.per * LAT, *stats_of = a.partial + (int64_t)2 * a.pieces * a.per * LAT + (int64_t)slot * a.per * 2;
+    if (tid < heads) {
+      float top = -INFINITY, sum = 0.f, f[Heads::SOURCES];
 #pragma unroll
-      for (int p = 0; p < PW; p++) top = fmaxf(top, stats[2 * (16 * (p * HW + h / 16) + h % 16)]);
+      for (int p = 0; p < Heads::SOURCES; p++) top = fmaxf(top, stats[2 * Heads::source(tid, p)]);
 #pragma unroll
-      for (int p = 0; p < PW; p++) {
-        const int r = 16 * (p * HW + h / 16) + h % 16;
-        const float f = stats[2 * r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(stats[2 * r] - top);
-        sum = fmaf(f, stats[2 * r + 1], sum);
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = fmaf(f, join[r * G::JOIN + d + e], x[e]);
+      for (int p = 0; p < Heads::SOURCES; p++) {
+        const int r = Heads::source(tid, p);
+        f[p] = stats[2 * r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(stats[2 * r] - top);
+        sum = fmaf(f[p], stats[2 * r + 1], sum);
       }
-      if (whole) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        union { u32x4 raw; T e[8]; } out;
+      const float last = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-        for (int e = 0; e < 8; e++) out.e[e] = from_float<T>(sum == 0.f ? 0.f : x[e] * inv);
-        *reinterpret_cast<u32x4 *>(reinterpret_cast<T *>(a.o) + b * a.o_sb + (first + h) * a.o_sh + d) = out.raw;
-      } else {
-        float *to = a.partial + ((int64_t)slot * a.per + h) * (LAT + 2);
-        typedef float f32x2 __attribute__((ext_vector_type(2)));
-        if (d == 0) *reinterpret_cast<f32x2 *>(to) = f32x2{top, sum};
+      for (int p = 0; p < Heads::SOURCES; p++) by[64 * p + tid] = f[p] * last;
+      if (!whole) stats_of[2 * tid] = top, stats_of[2 * tid + 1] = sum;
+    }
+    __syncthreads();
+    constexpr int LANES = LAT / 4, U = 4, TERMS = Heads::OWN_SUMS ? Heads::SOURCES : 1;   // LANES: threads of a head
+    const int all = heads * LANES;
+    for (int i0 = tid; i0 < all; i0 += 256 * U) {
+      f32x4 v[U];
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) *reinterpret_cast<f32x2 *>(to + 2 + d + e) = f32x2{x[e], x[e + 1]};
+      for (int u = 0; u < U; u++) {
+        const int i = i0 + 256 * u < all ? i0 + 256 * u : i0, h = i / LANES, d = i % LANES * 4;
+        v[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int p = 0; p < TERMS; p++) {
+          const float f = by[64 * p + h];
+          const f32x4 w = *reinterpret_cast<const f32x4 *>(join + Heads::sums(h, p) * G::JOIN + d);
+#pragma unroll
+          for (int e = 0; e < 4; e++) v[u][e] = f == 0.f ? v[u][e] : fmaf(f, w[e], v[u][e]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int i = i0 + 256 * u, h = i / LANES, d = i % LANES * 4;
+        if (i >= all) continue;
+        if (whole) {
+          union { u32x2 raw; T e[4]; } out;
+#pragma unroll
+          for (int e = 0; e < 4; e++) out.e[e] = from_float<T>(v[u][e]);
+          *reinterpret_cast<u32x2 *>(reinterpret_cast<T *>(a.o) + b * a.o_sb + (first + h) * a.o_sh + d) = out.raw;
+        } else {
+          *reinterpret_cast<f32x4 *>(parts_of + h * LAT + d) = v[u];
+        }
       }
     }
     __syncthreads();
@@ -445,9 +803,10 @@ template <typename T, int LAT> __global__ void __launch_bounds__(256) k_latent_j
   const int parts = meta[1];
   if (parts <= 1) return;
   const int from = meta[0], slot = meta[2];
-  auto part = [&](int p) { return a.partial + ((int64_t)(p == 0 ? slot : 2 * (from + p)) * a.per + r) * (LAT + 2); };
+  const float *stats = a.partial + (int64_t)2 * a.pieces * a.per * LAT;
+  auto part = [&](int p) { return (int64_t)(p == 0 ? slot : 2 * (from + p)) * a.per + r; };
   float top = -INFINITY;
-  for (int p = tid; p < parts; p += 256) top = fmaxf(top, part(p)[0]);
+  for (int p = tid; p < parts; p += 256) top = fmaxf(top, stats[2 * part(p)]);
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
   if (lane == 0) tops[wave] = top;
@@ -460,11 +819,11 @@ template <typename T, int LAT> __global__ void __launch_bounds__(256) k_latent_j
     float v[4][N];
 #pragma unroll
     for (int u = 0; u < 4; u++) {
-      const float *p = part(p0 + 4 * u < parts ? p0 + 4 * u : p0);
-      own[u] = *reinterpret_cast<const f32x2 *>(p);
+      const int64_t p = part(p0 + 4 * u < parts ? p0 + 4 * u : p0);
+      own[u] = *reinterpret_cast<const f32x2 *>(stats + 2 * p);
 #pragma unroll
       for (int e = 0; e < N; e += 2) {
-        const f32x2 w = *reinterpret_cast<const f32x2 *>(p + 2 + 64 * e + 2 * lane);
+        const f32x2 w = *reinterpret_cast<const f32x2 *>(a.partial + p * LAT + 64 * e + 2 * lane);
         v[u][e] = w[0];
         v[u][e + 1] = w[1];
       }
@@ -491,14 +850,15 @@ template <typename T, int LAT> __global__ void __launch_bounds__(256) k_latent_j
   }
 }
 
-template <typename T, int LAT, int HW> int launch_latent(const LatentArgs &a, hipStream_t st) {
+template <typename T, int LAT, class Heads> int launch_latent_heads(const LatentArgs &a, hipStream_t st) {
   static std::atomic<uint64_t> done{0};
-  if (LatentGeo<LAT>::LDS > 65536 && !raise_lds_limit(reinterpret_cast<const void *>(k_latent_attention<T, LAT, HW>), LatentGeo<LAT>::LDS, done)) return BSP_ERR_HIP;
-  hipLaunchKernelGGL((k_latent_attention<T, LAT, HW>), dim3((unsigned)a.pieces), dim3(256), LatentGeo<LAT>::LDS, st, a);
+  if (LatentGeo<LAT>::LDS > 65536 && !raise_lds_limit(reinterpret_cast<const void *>(k_latent_attention<T, LAT, Heads>), LatentGeo<LAT>::LDS, done)) return BSP_ERR_HIP;
+  hipLaunchKernelGGL((k_latent_attention<T, LAT, Heads>), dim3((unsigned)a.pieces), dim3(256), LatentGeo<LAT>::LDS, st, a);
   return BSP_OK;
 }
 template <typename T, int LAT> int launch_latent(const LatentArgs &a, bool joined, hipStream_t st) {
-  const int rc = a.per <= 16 ? launch_latent<T, LAT, 1>(a, st) : a.per <= 32 ? launch_latent<T, LAT, 2>(a, st) : launch_latent<T, LAT, 4>(a, st);
+  const int rc = a.per <= 16 ? launch_latent_heads<T, LAT, Heads16<T, LAT, 1>>(a, st) : a.per <= 32 ? launch_latent_heads<T, LAT, Heads16<T, LAT, 2>>(a, st)
+                                                                                              : launch_latent_heads<T, LAT, Heads32<T, LAT>>(a, st);
   if (rc != BSP_OK) return rc;
   if (joined) hipLaunchKernelGGL((k_latent_join<T, LAT>), dim3((unsigned)((int64_t)a.B * a.H)), dim3(256), 0, st, a);
   BSP_LAUNCH_CHECK();
