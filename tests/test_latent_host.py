@@ -108,6 +108,6 @@ def test_c_entries_refuse():
     for bad in (dict(dtype=2), dict(block=48), dict(width=1 << 20), dict(n=1 << 27), dict(B=1 << 24), dict(rows=at, n_rows=65537)):
         assert attention(**bad) == UNSUPPORTED, bad
     need = lib.bsp_latent_attention_workspace_bytes(3, 65, 512, 64, 10)
-    assert need == -(-3 * 2 * 12 // 16) * 16 + 60 * 2 * 33 * 514 * 4 and lib.bsp_latent_attention_workspace_bytes(3, 65, 512, 64, 1) == 80
+    assert need == -(-3 * 2 * 8 // 16) * 16 + 60 * 2 * 33 * 514 * 4 and lib.bsp_latent_attention_workspace_bytes(3, 65, 512, 64, 1) == 48
     assert attention(ws=None) == attention(ws_bytes=8) == CAPACITY
     assert lib.bsp_latent_attention_workspace_bytes(3, 65, 96, 64, 10) == lib.bsp_latent_attention_workspace_bytes(0, 65, 512, 64, 10) == ERR_ARG

@@ -29,7 +29,7 @@ struct LatentArgs {
   const float *slopes;
   float scale, cap;
   float *partial;                  // two slots a workgroup: [heads a unit][latent] sums; behind all of them [heads a unit][2] maxima and sums of shares
-  int32_t *meta;                   // per item (sequence and unit) three ints: the workgroup that begins it, how many have a part (0, 1: nothing to join), the first part's slot
+  int32_t *meta;                   // per item (sequence and unit) two ints: the workgroup that begins it, how many have a part (0, 1: nothing to join)
   int B, H, block, shift;          // shift: log2 of the groups of sixteen positions a block
   int units, per, pieces;          // workgroups' heads a sequence: units of `per`; pieces of the work
 };
@@ -125,6 +125,7 @@ template <typename T, int LAT, int HW> struct Heads16 {
   typedef typename M::frag8 frag8;
   typedef typename std::conditional<HW == 1, typename M::frag4, frag8>::type frag;
   static constexpr int GROUPS = HW, SOURCES = 4 / HW, NS = LAT / 32, NR = kRope / 32, NT = LAT / 16;
+  static constexpr int EXTRA = 4;                       // steps that going over to another item takes as long as
   static constexpr bool BARRIER = HW > 1, OWN_SUMS = true;   // OWN_SUMS: each source has sums of its own
   static __device__ __forceinline__ uint32_t chunk(uint32_t c, uint32_t r, uint32_t group) { return c ^ (r & 7) << 1; }
   static __device__ __forceinline__ int first_group(int wave) { return wave / HW * HW; }
@@ -316,6 +317,7 @@ template <typename T, int LAT> struct Heads32 {
   typedef LatentMma<T> M;
   typedef typename M::frag8 frag8;
   static constexpr int GROUPS = 2, SOURCES = 2, NS = LAT / 16, NR = kRope / 16, NT = LAT / 64, HELD = NS < 22 ? NS : 22;   // NT: the wavefront's tiles of 32 elements
+  static constexpr int EXTRA = 8;
   static constexpr bool BARRIER = true, OWN_SUMS = false;
   static __device__ __forceinline__ uint32_t chunk(uint32_t c, uint32_t r, uint32_t group) { return c ^ ((r & 3) << 2 | (r >> 1 & 2) | (group & 1)); }
   static __device__ __forceinline__ int first_group(int wave) { return 2 * (wave & 1); }
@@ -516,6 +518,7 @@ template <typename T, int LAT> struct Heads32 {
 // An item is a sequence and a unit of its heads; its groups of sixteen positions
 struct LatentItem {
   int b, unit, len, groups, entry;
+  LatentItem() = default;
   __device__ __forceinline__ LatentItem(const LatentArgs &a, uint32_t item) {
     const Quotient i(item, a.units);
     b = (int)i.q;
@@ -544,39 +547,51 @@ __global__ void __launch_bounds__(256, 1) k_latent_attention(LatentArgs a) {
   const int mine = Heads::first_group(wave);            // the first of the step's groups that the wavefront goes through
   const uint32_t items = (uint32_t)(a.B * a.units), ring = (uint32_t)(uintptr_t)BSP_LDS_PTR(smem);
 
-  // the workgroup's piece [lo, hi) of all steps, and the item that it begins in
+  // The workgroup's piece [lo, hi) of all steps, and the item that it begins in.  Where there are more steps than pieces, an item counts `extra` steps more ahead of its own: what a
+  // workgroup that goes over to another item spends on the queries and on the sums of the last (16 x 128 heads over up to 16384 positions: 131 us without, 117 with; 128 x 128 heads over up to 500:
+  // 112 and 73; with a step or less a piece the extra steps would only leave pieces empty: 4 x 128 heads over up to 300, 32 us with them, 27 without).
   int64_t total = 0, lo, hi, begin = 0;
   uint32_t item = 0;
-  int pieces;
+  LatentItem found{}, looked{};                         // that item; what the thread has looked at last
+  int pieces, extra;
   {
     int *sums = reinterpret_cast<int *>(smem + G::STATS);                     // (where no tile goes)
-    auto chunk_sum = [&](uint32_t base, int &own, int &before) {               // of 256 items: own steps, those of the items before it in the chunk; returns the chunk's
+    // of 256 items: the thread's steps, the steps and (2^40 each) the number of those before it in the chunk that have any; returns the chunk's
+    auto chunk_sum = [&](uint32_t base, int &own, uint64_t &before) {
       const uint32_t i = base + tid;
-      own = i < items ? LatentItem(a, i).steps() : 0;
-      int x = own;
+      own = 0;
+      if (i < items) {
+        looked = LatentItem(a, i);
+        own = looked.steps();
+      }
+      const uint64_t mine_of = (uint64_t)own | (own > 0 ? (uint64_t)1 << 40 : 0);
+      uint64_t x = mine_of;
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) {
-        const int y = __shfl_up(x, d);
+        const uint64_t y = __shfl_up((unsigned long long)x, d);
         if (lane >= d) x += y;
       }
       __syncthreads();
-      if (lane == 63) sums[wave] = x;
+      if (lane == 63) reinterpret_cast<uint64_t *>(sums)[wave] = x;
       __syncthreads();
-      int all = 0;
-      before = x - own;
+      uint64_t all = 0;
+      before = x - mine_of;
 #pragma unroll
       for (int w = 0; w < 4; w++) {
-        before += w < wave ? sums[w] : 0;
-        all += sums[w];
+        const uint64_t y = reinterpret_cast<uint64_t *>(sums)[w];
+        before += w < wave ? y : 0;
+        all += y;
       }
-      return __builtin_amdgcn_readfirstlane(all);
+      return all;
     };
-    int own = 0, before = 0;
+    constexpr uint64_t kSteps = ((uint64_t)1 << 40) - 1;
+    int own = 0;
+    uint64_t before = 0, every = 0;
     for (uint32_t base = 0; base < items; base += 256) {
-      total += chunk_sum(base, own, before);
+      every += chunk_sum(base, own, before);
       const uint32_t i = base + tid;
       if (i < items && own == 0) {                                            // nothing is seen: zeros
-        if (blockIdx.x == 0) a.meta[3 * (int64_t)i + 1] = 0;
+        if (blockIdx.x == 0) a.meta[2 * (int64_t)i + 1] = 0;
       }
       uint64_t none = __builtin_amdgcn_ballot_w64(i < items && own == 0 && i % gridDim.x == blockIdx.x);
       while (none) {
@@ -588,24 +603,41 @@ __global__ void __launch_bounds__(256, 1) k_latent_attention(LatentArgs a) {
           *reinterpret_cast<u32x4 *>(reinterpret_cast<T *>(a.o) + z.q * a.o_sb + (first + k / (LAT / 8)) * a.o_sh + 8 * (k % (LAT / 8))) = u32x4{0, 0, 0, 0};
       }
     }
+    total = (int64_t)(every & kSteps);
     pieces = total < a.pieces ? (int)total : a.pieces;    // (none is empty)
     if ((int)blockIdx.x >= pieces) return;
+    extra = total > a.pieces ? Heads::EXTRA : 0;
+    auto steps_of = [&](uint64_t x) { return (int64_t)(x & kSteps) + extra * (int64_t)(x >> 40); };
+    total = steps_of(every);
     lo = total * blockIdx.x / pieces;
     hi = total * (blockIdx.x + 1) / pieces;
     int64_t done = 0;
     for (uint32_t base = 0; base < items; base += 256) {
       if (items > 256 || base > 0) {
-        const int all = chunk_sum(base, own, before);
+        const int64_t all = steps_of(chunk_sum(base, own, before));
         if (done + all <= lo) {
           done += all;
           continue;
         }
       }
+      const int64_t from = done + steps_of(before);
       __syncthreads();
-      if (own > 0 && done + before <= lo && lo < done + before + own) sums[4] = (int)base + tid, sums[5] = before;
+      if (own > 0 && from <= lo && lo < from + own + extra) {
+        sums[4] = (int)base + tid;
+        sums[5] = (int)(from - done);
+        sums[6] = looked.len;
+        sums[7] = looked.groups;
+        sums[8] = looked.entry;
+      }
       __syncthreads();
       item = (uint32_t)__builtin_amdgcn_readfirstlane(sums[4]);
       begin = done + __builtin_amdgcn_readfirstlane(sums[5]);
+      const Quotient of(item, a.units);
+      found.b = (int)of.q;
+      found.unit = (int)of.r;
+      found.len = sums[6];
+      found.groups = sums[7];
+      found.entry = sums[8];
       break;
     }
   }
@@ -616,13 +648,19 @@ __global__ void __launch_bounds__(256, 1) k_latent_attention(LatentArgs a) {
   scores.factor = scores.capped ? 2.f * kLog2e * a.scale / a.cap : a.scale * kLog2e;
   scores.cap = a.cap * kLog2e;
 
-  for (int64_t at = lo; at < hi && item < items; item++) {
-    const LatentItem it(a, item);
+  bool looked_up = true;
+  for (; begin < hi && item < items; item++) {
+    const LatentItem it = looked_up ? found : LatentItem(a, item);
+    looked_up = false;
     const int steps = __builtin_amdgcn_readfirstlane(it.steps());
     if (steps == 0) continue;
+    // the item's steps that are the workgroup's
+    const int64_t first_step = begin + extra;
+    begin = first_step + steps;
+    const int s0 = lo > first_step ? (int)(lo - first_step) : 0, s1 = begin < hi ? steps : (int)(hi - first_step);
+    if (s1 <= s0) continue;
     const int b = __builtin_amdgcn_readfirstlane(it.b), unit = __builtin_amdgcn_readfirstlane(it.unit), len = __builtin_amdgcn_readfirstlane(it.len);
     const int groups = __builtin_amdgcn_readfirstlane(it.groups), entry = __builtin_amdgcn_readfirstlane(it.entry);
-    const int s0 = (int)(at - begin), s1 = begin + steps < hi ? steps : (int)(hi - begin);
     const int first = unit * a.per, heads = a.H - first < a.per ? a.H - first : a.per;
     scores.last = len - 1;
 
@@ -725,15 +763,16 @@ __global__ void __launch_bounds__(256, 1) k_latent_attention(LatentArgs a) {
     x.put(join, stats, wave);
     __syncthreads();
     const bool whole = s0 == 0 && s1 == steps;
-    const int slot = 2 * blockIdx.x + (at > lo ? 1 : 0);
+    const int slot = 2 * blockIdx.x + (s0 == 0 ? 1 : 0);  // (of a piece's parts one at most begins its item and one at most does not)
     if (tid == 0 && s0 == 0) {
       int parts = 1;
-      if (!whole) {                                       // the piece that the item's last step is in
-        const int64_t last = ((begin + steps) * pieces - 1) / total;
+      if (!whole) {                                       // up to the piece that the item's last step is in
+        const int64_t last = (begin * pieces - 1) / total;
         parts = (int)(last - blockIdx.x) + 1;
       }
-      int32_t *to = a.meta + 3 * (int64_t)item;
-      to[0] = blockIdx.x; to[1] = parts; to[2] = slot;
+      int32_t *to = a.meta + 2 * (int64_t)item;
+      to[0] = blockIdx.x;
+      to[1] = parts;
     }
     // what each source's sums are multiplied by, a head a thread; then four elements a thread, four of them on their way
     float *by = reinterpret_cast<float *>(smem + G::SHARES);
@@ -785,8 +824,6 @@ __global__ void __launch_bounds__(256, 1) k_latent_attention(LatentArgs a) {
       }
     }
     __syncthreads();
-    at = begin + s1;
-    begin += steps;
   }
 }
 
@@ -799,12 +836,12 @@ template <typename T, int LAT> __global__ void __launch_bounds__(256) k_latent_j
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Quotient at(blockIdx.x, a.H);
   const int b = (int)at.q, h = (int)at.r, unit = h / a.per, r = h % a.per;
-  const int32_t *meta = a.meta + 3 * ((int64_t)b * a.units + unit);
+  const int32_t *meta = a.meta + 2 * ((int64_t)b * a.units + unit);
   const int parts = meta[1];
   if (parts <= 1) return;
-  const int from = meta[0], slot = meta[2];
+  const int from = meta[0];
   const float *stats = a.partial + (int64_t)2 * a.pieces * a.per * LAT;
-  auto part = [&](int p) { return (int64_t)(p == 0 ? slot : 2 * (from + p)) * a.per + r; };
+  auto part = [&](int p) { return (int64_t)(2 * (from + p) + (p == 0 ? 1 : 0)) * a.per + r; };
   float top = -INFINITY;
   for (int p = tid; p < parts; p += 256) top = fmaxf(top, stats[2 * part(p)]);
 #pragma unroll
@@ -889,7 +926,7 @@ extern "C" int bsp_latent_attention_heads(int H) {
 
 extern "C" int64_t bsp_latent_attention_workspace_bytes(int B, int H, int latent, int block, int64_t most_blocks) {
   if (B <= 0 || H <= 0 || !latent_ok(latent, block) || most_blocks <= 0) return BSP_ERR_ARG;
-  const int64_t meta = ((int64_t)B * latent_units(H) * 12 + 15) / 16 * 16;
+  const int64_t meta = ((int64_t)B * latent_units(H) * 8 + 15) / 16 * 16;
   return meta + (most_blocks * block <= 64 ? 0 : (int64_t)latent_pieces(B, H, block, most_blocks) * 2 * bsp_latent_attention_heads(H) * (latent + 2) * 4);
 }
 
@@ -915,7 +952,7 @@ extern "C" int bsp_latent_attention(int dtype, const void *q, int64_t q_stride_b
   a.B = B; a.H = H; a.block = block; a.shift = __builtin_ctz(block) - 4;
   a.units = latent_units(H); a.per = bsp_latent_attention_heads(H); a.pieces = latent_pieces(B, H, block, most_blocks);
   a.meta = reinterpret_cast<int32_t *>(workspace);
-  a.partial = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(workspace) + ((int64_t)B * a.units * 12 + 15) / 16 * 16);
+  a.partial = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(workspace) + ((int64_t)B * a.units * 8 + 15) / 16 * 16);
   const bool joined = most_blocks * block > 64;           // (else no sequence has more than one step)
   return dtype == BSP_F16 ? launch_latent<f16>(a, latent, joined, as_stream(stream)) : launch_latent<bf16>(a, latent, joined, as_stream(stream));
 }

@@ -31,11 +31,16 @@ def _fraction_of_a_turn(f):
 def _operand(t):
     """(t, or a copy that the kernel can address; its strides of batch, head and position); t [batch, heads, length, dim] or [tokens, heads, dim]"""
     for again in (False, True):
-        at = (0,) + (t.stride(1), t.stride(0)) if t.dim() == 3 else t.stride()[:3]
-        sizes = (1, t.size(1), t.size(0)) if t.dim() == 3 else t.shape[:3]
-        at = tuple(s if n > 1 else 0 for s, n in zip(at, sizes))
-        if again or (t.stride(-1) == 1 and not (at[0] | at[1] | at[2]) * t.element_size() % 16 and not t.data_ptr() % 16):
-            return t, at
+        stride, shape = t.stride(), t.shape
+        z, h, l = (0, stride[1], stride[0]) if len(stride) == 3 else stride[:3]      # noqa: E741
+        if shape[0] == 1:
+            z, l = 0, l if len(stride) == 4 else 0                                   # noqa: E741
+        if shape[1] == 1:
+            h = 0
+        if len(stride) == 4 and shape[2] == 1:
+            l = 0                                                                    # noqa: E741
+        if again or (stride[-1] == 1 and not (z | h | l) * t.element_size() % 16 and not t.data_ptr() % 16):
+            return t, (z, h, l)
         t = t.clone(memory_format=torch.contiguous_format)
 
 
@@ -56,8 +61,12 @@ class _turn(torch.autograd.Function):
         if not given:
             return (None,) * (3 + len(grads))
         with _lib.on_device(given[0].device):
-            turned = _turn.apply(ctx.rotation, positions, not ctx.back, *given)
-        turned = iter(turned if len(given) > 1 else (turned,))
+            if torch.is_grad_enabled():                   # (the gradient's gradient is wanted)
+                turned = _turn.apply(ctx.rotation, positions, not ctx.back, *given)
+                turned = turned if len(given) > 1 else (turned,)
+            else:
+                turned = ctx.rotation._launch(given, positions, not ctx.back)
+        turned = iter(turned)
         return (None, None, None) + tuple(next(turned) if g is not None else None for g in grads)
 
 
@@ -102,51 +111,62 @@ class Rotation:
             table = torch.tensor([_fraction_of_a_turn(f) for f in self.frequencies.tolist()], dtype=torch.int64, device='cpu').to(device)
             made = self._fractions[device] = (table, _lib.Readers())
             made[1].table(table)
-        made[1].read(device)
+        if _lib.raw_stream(device) not in made[1].streams:
+            made[1].read(device)
         return made[0]
 
     def check_positions(self, positions, shapes, device):
-        if positions is not None and (positions.dtype != torch.int32 or positions.device != device or tuple(positions.shape) not in shapes):
+        if positions is not None and (positions.dtype != torch.int32 or positions.shape not in shapes or positions.device != device):
             raise ValueError('positions must be int32 %s on %s (got %s %s on %s)' % (' or '.join(str(list(s)) for s in shapes), device, positions.dtype, list(positions.shape), positions.device))
 
     def _check(self, tensors, positions):
         if len(tensors) not in (1, 2):
             raise ValueError('a call takes one tensor or two (got %d)' % len(tensors))
         x = tensors[0]
+        shape, device = x.shape, x.device
         for t in tensors:
-            _lib.require_gpu_tensor(t, 'a rotated tensor')
-            if t.dim() not in (3, 4):
-                raise ValueError('rotated tensors have shape [batch, heads, length, dim] or [tokens, heads, dim] (got %s)' % list(t.shape))
-            if t.dtype not in _lib.DTYPES:
-                raise ValueError('Rotation supports float16, bfloat16 and float32 (got %s)' % t.dtype)
-            if t.dtype != x.dtype or t.device != x.device or t.dim() != x.dim() or t.shape[:1] + t.shape[2:] != x.shape[:1] + x.shape[2:]:
-                raise ValueError('the tensors of a call must be alike but for their number of heads (got %s %s and %s %s)' % (x.dtype, list(x.shape), t.dtype, list(t.shape)))
-        D = x.size(-1)
+            if not t.is_cuda:
+                _lib.require_gpu_tensor(t, 'a rotated tensor')
+        if len(shape) not in (3, 4):
+            raise ValueError('rotated tensors have shape [batch, heads, length, dim] or [tokens, heads, dim] (got %s)' % list(shape))
+        if x.dtype not in _lib.DTYPES:
+            raise ValueError('Rotation supports float16, bfloat16 and float32 (got %s)' % x.dtype)
+        if len(tensors) == 2:
+            y = tensors[1]
+            if y.dtype != x.dtype or y.device != device or y.dim() != len(shape) or y.shape[0] != shape[0] or y.shape[2:] != shape[2:]:
+                raise ValueError('the tensors of a call must be alike but for their number of heads (got %s %s and %s %s)' % (x.dtype, list(shape), y.dtype, list(y.shape)))
+        D, L = shape[-1], shape[0] if len(shape) == 3 else shape[2]
         if D % 8 or D < 2 * self.pairs:
             raise ValueError('heads must have a multiple of 8 elements, at least %d for %d pairs (got %d)' % (2 * self.pairs, self.pairs, D))
-        if x.dim() == 3:
-            self.check_positions(positions, ((x.size(0),),), x.device)
-        else:
-            self.check_positions(positions, ((x.size(2),), (x.size(0), x.size(2))), x.device)
-        tokens = x.size(0) if x.dim() == 3 else x.size(0) * x.size(2)
-        if tokens * D >= 1 << 32:
-            raise ValueError('a call takes fewer than 2^32 elements of a head (got %d positions of %d)' % (tokens, D))
+        if positions is not None:
+            self.check_positions(positions, ((L,),) if len(shape) == 3 else ((L,), (shape[0], L)), device)
+        if (L if len(shape) == 3 else shape[0] * L) * D >= 1 << 32:
+            raise ValueError('a call takes fewer than 2^32 elements of a head (got %s)' % list(shape))
 
     def _launch(self, tensors, positions, back):
-        x, device = tensors[0], tensors[0].device
-        Z, L, D = (1, x.size(0), x.size(2)) if x.dim() == 3 else (x.size(0), x.size(2), x.size(3))
-        out, args = [], []
+        x = tensors[0]
+        shape, device = x.shape, x.device
+        Z, L, D = (1, shape[0], shape[2]) if len(shape) == 3 else (shape[0], shape[2], shape[3])
+        out, args, live = [], [], 0
         for t in tensors:
             y = torch.empty(t.shape, dtype=t.dtype, device=device)
-            t, at = _operand(t)
             out.append(y)
-            args.append((t, y, t.size(1), _STRIDES.pack(*at, *_operand(y)[1])))
-        live = [a for a in args if a[0].numel()]
+            if t.numel():
+                H = t.shape[1]
+                t, at = _operand(t)
+                own = (0, D, H * D) if len(shape) == 3 else (H * L * D, L * D, D)
+                args += [t, y, H, _STRIDES.pack(*at, *own)]
+                live += 1
         if live:
-            (x0, y0, H0, s0), (x1, y1, H1, s1) = live[0], live[1] if len(live) > 1 else (None, None, 0, None)
-            p_z, p_l = (0, 0) if positions is None else (positions.stride(0) if positions.dim() == 2 else 0, positions.stride(-1))
-            rc = _lib.load().bsp_rotate(_lib.DTYPES[x.dtype], Z, L, D, self.pairs, self.neighbours, back, self.fractions(device).data_ptr(), positions.data_ptr() if positions is not None else None,
-                                        p_z, p_l, x0.data_ptr(), y0.data_ptr(), H0, s0, x1.data_ptr() if H1 else None, y1.data_ptr() if H1 else None, H1, s1, _lib.raw_stream(device))
+            x0, y0, H0, s0 = args[:4]
+            x1, y1, H1, s1 = args[4:] if live == 2 else (None, None, 0, None)
+            p_z, p_l, p = 0, 0, None
+            if positions is not None:
+                p, p_l = positions.data_ptr(), positions.stride(-1)
+                if positions.dim() == 2:
+                    p_z = positions.stride(0)
+            rc = _lib.load().bsp_rotate(_lib.DTYPES[x.dtype], Z, L, D, self.pairs, self.neighbours, back, self.fractions(device).data_ptr(), p, p_z, p_l, x0.data_ptr(), y0.data_ptr(), H0, s0,
+                                        x1.data_ptr() if H1 else None, y1.data_ptr() if H1 else None, H1, s1, _lib.raw_stream(device))
             if rc:
                 _lib.check(rc, 'bsp_rotate')
         return tuple(out)
