@@ -7,13 +7,15 @@
 //
 // Both kernels move each byte once; the read is bound by that, the write by its vector operations.  A thread has a chunk of eight elements: 16 bytes in 16-bit types, and the four
 // threads of a group agree on its range by two exchanges within the quad.  Tensors outside the cache are streamed past the L2 (non-temporal): nothing reads them
-// soon.  Measured: 16384 positions of 16 heads of 64, fp16, 8 bits (67 MB and 38 MB): written in 33 us (4 of them the launch that says whose a slot is), read back in 27, or
-// in 16 where a cache level still holds them.  One after the other 45 us: 51 without the streaming, 58 before a thread's place was found without divisions and the rounded
-// quotient taken from the low bits of one sum.  The write's vector units are busy for 68 % of its cycles, 85 to 100 % over more positions.
+// soon.  Measured: 16384 positions of 16 heads of 64, fp16, 8 bits (67 MB and 38 MB): written in 30 us (2 to 4 of them the launch that says whose a slot is), read back in 27, or
+// in 16 where a cache level still holds them.  One after the other 46 us: 48 with a division in two forms and keys and values in one wavefront, 54 without the streaming, 61 before a
+// thread's place was found without divisions and the rounded quotient taken from the low bits of one sum.
 // 32749 positions of 8 heads of 128, bf16, 4 bits (176 MB) read in 41 us, 52 without the streaming.
 //
 // With a rotation (rotation.h) the keys are turned first, all of it in 64 bits, as what rounding in between would leave out decides codes: the vector units do fp64 at the
-// rate of fp32.  A workgroup computes its position's sines and cosines once, into LDS, and a thread takes the other chunk of its pairs from the lane that has it.
+// rate of fp32.  A workgroup computes its position's sines and cosines once, into LDS, and a thread takes the other chunk of its pairs from the lane that has it.  Measured: 16384
+// positions of 8 heads of 128, fp16, 8 bits (67 MB read, 38 MB written): 37 us and the slots' owners 4, where the plain write takes 28.  Its vector units have 250 instructions a
+// wavefront, 66 % of its cycles; with 302 it took 42.5.  Taking all eight elements of the other lane before the first is used, and LDS without conflicts, did not change it.
 #include "cache.h"
 #include "rotation.h"
 
@@ -39,19 +41,27 @@ namespace {
 __device__ __forceinline__ float quad1(float v) { return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xf, 0xf, true)); }
 __device__ __forceinline__ float quad2(float v) { return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xf, 0xf, true)); }
 
-__device__ __forceinline__ double quad_f64(double v, int control) {
+// (greater() below hides from the compiler that it wrote v just before: a lane's value is read by another two cycles later at the earliest)
+__device__ __forceinline__ double quad1(double v) {
+  asm volatile("s_nop 1" : "+v"(v));
   const uint64_t b = __builtin_bit_cast(uint64_t, v);
-  const int lo = (int)(uint32_t)b, hi = (int)(uint32_t)(b >> 32);
-  const uint32_t l = control == 1 ? __builtin_amdgcn_update_dpp(0, lo, 0xB1, 0xf, 0xf, true) : __builtin_amdgcn_update_dpp(0, lo, 0x4E, 0xf, 0xf, true);
-  const uint32_t h = control == 1 ? __builtin_amdgcn_update_dpp(0, hi, 0xB1, 0xf, 0xf, true) : __builtin_amdgcn_update_dpp(0, hi, 0x4E, 0xf, 0xf, true);
+  const uint32_t l = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, 0xB1, 0xf, 0xf, true), h = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), 0xB1, 0xf, 0xf, true);
   return __builtin_bit_cast(double, (uint64_t)h << 32 | l);
 }
-__device__ __forceinline__ double quad1(double v) { return quad_f64(v, 1); }
-__device__ __forceinline__ double quad2(double v) { return quad_f64(v, 2); }
-__device__ __forceinline__ float lesser(float a, float b) { return fminf(a, b); }
-__device__ __forceinline__ double lesser(double a, double b) { return fmin(a, b); }
-__device__ __forceinline__ float greater(float a, float b) { return fmaxf(a, b); }
-__device__ __forceinline__ double greater(double a, double b) { return fmax(a, b); }
+__device__ __forceinline__ double quad2(double v) {
+  asm volatile("s_nop 1" : "+v"(v));
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t l = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, 0x4E, 0xf, 0xf, true), h = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), 0x4E, 0xf, 0xf, true);
+  return __builtin_bit_cast(double, (uint64_t)h << 32 | l);
+}
+// the lesser and the greater of two, NaN if one is; the double's leaves NaN out (no operation has it otherwise), and is one instruction where fmax is three, which quiet its operands
+__device__ __forceinline__ float lesser(float a, float b) { return __builtin_elementwise_minimum(a, b); }
+__device__ __forceinline__ float greater(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ __forceinline__ double greater(double a, double b) {
+  double r;
+  asm("v_max_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
 
 template <typename T> __device__ __forceinline__ void load8(float (&x)[8], const T *p) {
   if constexpr (sizeof(T) == 4) {
@@ -81,67 +91,70 @@ __global__ void __launch_bounds__(256) k_cache_owner(CacheArgs a) {
 // The codes of the thread's eight elements (words), least value and step of their group, which the four threads of a quad have.  X: float, or double for what a rotation
 // left (whose least element is rounded to fp32 on its way to fp16)
 template <int BITS, typename X> __device__ __forceinline__ void quantise(const X (&x)[8], uint32_t (&w)[2], f16 &least, f16 &step) {
-    // the group's range, into that of fp16 here: elements outside get the codes of its ends below
-    bool nan = false;
-    X lo = x[0], hi = x[0];
+  constexpr int MOST = (1 << BITS) - 1;
+  // the group's range, into that of fp16 here: elements outside get the codes of its ends below
+  float y[8];
 #pragma unroll
-  for (int e = 0; e < 8; e += 2) {
-    nan |= __builtin_isunordered(x[e], x[e + 1]);
-    lo = lesser(lesser(lo, x[e]), x[e + 1]);
+  for (int e = 0; e < 8; e++) y[e] = (float)x[e];
+  float lo = lesser(y[0], y[1]);                        // (rounding keeps the order)
+  X hi = greater(x[0], x[1]);
+#pragma unroll
+  for (int e = 2; e < 8; e += 2) {
+    lo = lesser(lesser(lo, y[e]), y[e + 1]);
     hi = greater(greater(hi, x[e]), x[e + 1]);
   }
-  float bad = nan ? 1.f : 0.f;
   lo = lesser(lo, quad1(lo));
   hi = greater(hi, quad1(hi));
-  bad = fmaxf(bad, quad1(bad));
   lo = lesser(lo, quad2(lo));
   hi = greater(hi, quad2(hi));
-  bad = fmaxf(bad, quad2(bad));
-  lo = lesser(greater(lo, (X)-65504), (X)65504);
-  hi = lesser(greater(hi, (X)-65504), (X)65504);
-  constexpr int MOST = (1 << BITS) - 1;
-  float lo32 = (float)lo;
-  if constexpr (sizeof(X) == 8) asm("" : "+v"(lo32));   // (or the compiler makes one rounding of the two)
-  least = (f16)lo32;
+  const bool bad = lo != lo;
+  lo = fminf(fmaxf(lo, -65504.f), 65504.f);
+  hi = hi < (X)-65504 ? (X)-65504 : hi > (X)65504 ? (X)65504 : hi;
+  asm("" : "+v"(lo));                                   // (or the compiler makes one rounding of the two)
+  least = (f16)lo;
   {
-    const double range = (double)hi - (double)(float)least;
-    const float r = (float)range;
-    step = (f16)((double)r == range ? r / (float)MOST : (float)(range / (double)MOST));   // (the same number: both quotients are rounded to the nearest)
+    constexpr double inv = 1. / MOST;
+    const double range = (double)hi - (double)(float)least, q = range * inv;
+    float nearest = (float)fma(fma(-(double)MOST, q, range), inv, q);   // (one step from a quotient that is off by its last bit: rounded to the nearest)
+    asm("" : "+v"(nearest));
+    step = (f16)nearest;
   }
-  if (bad != 0.f) least = __builtin_bit_cast(f16, (uint16_t)0x7e00), step = (f16)0.f;
-    const float l32 = (float)least, s32 = (float)step;
-    if (s32 != 0.f) {                                   // (below zero where the least value was rounded up past the greatest one)
-      // the quotient rounded in the low bits of 1.5 * 2^23 + it
-      const float inv = __builtin_amdgcn_rcpf(s32), magic = 12582912.f;
-      uint32_t code[8];
-      float off = 0.f;
-  #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const float d = (float)(x[e] - (X)l32), r = fmaf(d, inv, magic);
-        off = fmaxf(off, fabsf(fmaf(d, inv, magic - r)));
-        code[e] = __builtin_bit_cast(uint32_t, fminf(fmaxf(r, magic), magic + (float)MOST));
-      }
-      // x - least is off by 2^-24 of itself, the reciprocal by 2^-23, so the quotient by 3 * 2^-24 * MOST: decided in 64 bits where the middle is as near
-      if (off > 0.5f - MOST * 0x1p-22f) {
-        const double h = 0.5 * fabs((double)s32);
-  #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const int n0 = (int)(code[e] & 0x1ffu);
-          const double rest = ((double)x[e] - (double)l32) - (double)n0 * (double)s32, rem = s32 < 0.f ? -rest : rest;
-          const bool odd = n0 & 1;
-          const int m = n0 + (rem > h || (rem == h && odd) ? 1 : 0) - (rem < -h || (rem == -h && odd) ? 1 : 0);
-          code[e] = (uint32_t)(m < 0 ? 0 : m > MOST ? MOST : m);
-        }
-      }
-      if constexpr (BITS == 4) {
-  #pragma unroll
-        for (int e = 0; e < 8; e++) w[0] |= (code[e] & 15u) << (4 * (e >> 1) + 16 * (e & 1));
-      } else {
-  #pragma unroll
-        for (int e = 0; e < 2; e++)
-          w[e] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(code[4 * e + 3], code[4 * e + 2], 0x0c0c0400u), __builtin_amdgcn_perm(code[4 * e + 1], code[4 * e], 0x0c0c0400u), 0x05040100u);
-      }
+  if (bad) least = __builtin_bit_cast(f16, (uint16_t)0x7e00), step = (f16)0.f;
+  const float l32 = (float)least, s32 = (float)step;
+  if (s32 == 0.f) return;
+  // (step is below zero where the least value was rounded up past the greatest one)
+  // the quotient rounded in the low bits of 1.5 * 2^23 + it
+  const float inv = __builtin_amdgcn_rcpf(s32), magic = 12582912.f;
+  float n[8], off = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    const float d = y[e] - l32;
+    n[e] = fmaf(d, inv, magic) - magic;
+    off = fmaxf(off, fabsf(fmaf(d, inv, -n[e])));
+  }
+  // x - least is off by 2^-24 of itself, the reciprocal by 2^-23, so the quotient by 3 * 2^-24 * MOST, and by 2^-24 x / step more where x was rounded: decided in 64 bits where
+  // the middle is as near
+  float sure = 0.5f - MOST * 0x1p-22f;
+  if constexpr (sizeof(X) == 8) sure -= fmaxf(fabsf(lo), fabsf((float)hi)) * fabsf(inv) * 0x1p-23f;
+  if (off > sure) {
+    const double h = 0.5 * fabs((double)s32);
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const float n0 = __builtin_amdgcn_fmed3f(n[e], 0.f, (float)MOST);
+      const double rest = ((double)x[e] - (double)l32) - (double)n0 * (double)s32, rem = s32 < 0.f ? -rest : rest;
+      const bool odd = (int)n0 & 1;
+      n[e] = n0 + (rem > h || (rem == h && odd) ? 1.f : 0.f) - (rem < -h || (rem == -h && odd) ? 1.f : 0.f);
     }
+  }
+  if constexpr (BITS == 4) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) n[e] = __builtin_amdgcn_fmed3f(n[e], 0.f, 15.f);
+    const float even = fmaf(fmaf(fmaf(n[6], 16.f, n[4]), 16.f, n[2]), 16.f, n[0]), odd = fmaf(fmaf(fmaf(n[7], 16.f, n[5]), 16.f, n[3]), 16.f, n[1]);
+    w[0] = (uint32_t)even | (uint32_t)odd << 16;
+  } else {                                              // (the conversion keeps to 0 .. 255)
+#pragma unroll
+    for (int e = 0; e < 8; e++) w[e >> 2] = __builtin_amdgcn_cvt_pk_u8_f32(n[e], e & 3, w[e >> 2]);
+  }
 }
 
 // The turned elements of the thread's chunk j
@@ -198,12 +211,17 @@ template <typename T, int BITS, int D, bool SCAN, bool ROTATED> __global__ void 
     if (tid < a.pairs) turns[tid] = turn_of_f64(as_table(a.positions)[t], a.fractions[tid]);
     __syncthreads();
   }
-  const int page = slot >> a.block_shift, at = slot & (a.block - 1);
-  const int j = tid % CHUNKS, g = j >> 2, c = j & 3;
-  for (int m = tid / CHUNKS; m < 2 * a.heads; m += 256 / CHUNKS) {
-    const int value = m >= a.heads, head = value ? m - a.heads : m;
+  // wavefronts 0 and 2 have keys, 1 and 3 values
+  const int page = slot >> a.block_shift, at = slot & (a.block - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, value = wave & 1;
+  const int j = lane % CHUNKS, g = j >> 2, c = j & 3;
+  const T *from = (value ? reinterpret_cast<const T *>(a.v) + t * a.v_st : reinterpret_cast<const T *>(a.k) + t * a.k_st) + 8 * j;
+  const int64_t stride = value ? a.v_sh : a.k_sh, bytes = P::bytes(a.block);
+  unsigned char *codes = a.pages + (int64_t)page * a.heads * bytes + P::codes(a.block, value) + at * P::ROW + P::chunk(c, g);
+  unsigned char *meta = a.pages + (int64_t)page * a.heads * bytes + P::meta(a.block, value) + at * P::META + 4 * g;
+  constexpr int HEADS = 64 / CHUNKS;                    // of a wavefront
+  for (int head = (wave >> 1) * HEADS + lane / CHUNKS; head < a.heads; head += 2 * HEADS) {
     float x[8];
-    load8<T>(x, (value ? reinterpret_cast<const T *>(a.v) + t * a.v_st + head * a.v_sh : reinterpret_cast<const T *>(a.k) + t * a.k_st + head * a.k_sh) + 8 * j);
+    load8<T>(x, from + head * stride);
     uint32_t w[2] = {0u, 0u};
     f16 least, step;
     if (ROTATED && !value) {
@@ -213,13 +231,10 @@ template <typename T, int BITS, int D, bool SCAN, bool ROTATED> __global__ void 
     } else {
       quantise<BITS>(x, w, least, step);
     }
-    unsigned char *base = a.pages + ((int64_t)page * a.heads + head) * P::bytes(a.block);
-    unsigned char *to = base + P::codes(a.block, value) + at * P::ROW + P::chunk(c, g);
+    unsigned char *to = codes + head * bytes;
     if constexpr (BITS == 4) *reinterpret_cast<uint32_t *>(to) = w[0];
     else *reinterpret_cast<u32x2 *>(to) = u32x2{w[0], w[1]};
-    if (c == 0)
-      *reinterpret_cast<uint32_t *>(base + P::meta(a.block, value) + at * P::META + 4 * g) =
-          (uint32_t)__builtin_bit_cast(uint16_t, step) | (uint32_t)__builtin_bit_cast(uint16_t, least) << 16;
+    if (c == 0) *reinterpret_cast<uint32_t *>(meta + head * bytes) = (uint32_t)__builtin_bit_cast(uint16_t, step) | (uint32_t)__builtin_bit_cast(uint16_t, least) << 16;
   }
 }
 
