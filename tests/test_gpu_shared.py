@@ -59,6 +59,14 @@ def test_forward_and_gradients(dtype, Z, H, kv, L, D, block, causal):
         check(tb.Attention(layout, block), inputs(dtype, Z, H, kv, L, D, L), layout, block, scale=(D + 64) ** -0.5, causal=causal)
 
 
+@pytest.mark.parametrize('dtype,D', [(torch.float16, 64), (torch.bfloat16, 128)])
+def test_many_lines(dtype, D):
+    """so many that a line is one pair of wavefronts', with several tiles"""
+    Z, H, L = 9, 16, 500
+    layout = torch.ones(H, 8, 8, dtype=torch.int64)
+    check(tb.Attention(layout, 64), inputs(dtype, Z, H, H, L, D, 11), layout, 64, scale=0.08, causal=True)
+
+
 @pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16, torch.float32])
 @pytest.mark.parametrize('D', [64, 128])
 def test_rules(dtype, D):

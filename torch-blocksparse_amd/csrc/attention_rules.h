@@ -566,9 +566,12 @@ __device__ __forceinline__ void lds_barrier() {
 // 456 -> 318 (578 -> 642), 82 -> 63 (126 -> 104); 2048 of them 693 -> 577 (1130 -> 1261), 124 -> 116 (198 -> 217); twelve heads of 256 lines of BigBird fp16 51 -> 59.
 // Short lines, of 7 tiles (BigBird): fp16 768 lines 18.0 -> 17.3, 1536 29.7 -> 31.9; bf16 of 128 elements 512 lines 22.9 -> 19.2, 1024 30.6 -> 35.6; fp32 512 lines 68.6 -> 43.3, 1024 76.8 ->
 // 78.7, of 128 elements 256 74.3 -> 45.3, 512 80.2 -> 91.6; of one tile: fp16 768 lines 7.1 -> 8.1, bf16 of 128 elements 1024 14.5 -> 19.4, fp32 512 12.6 -> 11.8, of 128 elements 21.8 -> 29.0.
+// With a shared key part (64 elements more a key, rings that leave room for fewer workgroups) half as many in 16-bit types, forward pass and rows with columns, one pair -> two: bf16 of 128 elements 512
+// lines 61 -> 53 and 204 -> 182 us (of 5 tiles 22 -> 26 and 96 -> 98), 1024 lines 126 -> 173 and 426 -> 459; of 64 elements 1024 lines 95 -> 85 and 303 -> 284 (22 -> 26 and 92 -> 69), 2048 lines 139 -> 158 and 464 ->
+// 469. fp32 of 64 elements: 512 lines 285 -> 132 and 598 -> 470, 2048 1042 -> 920 and 2893 -> 2982.
 constexpr int kLdsBytes = 160 * 1024;                     // of a compute unit
-template <typename T, int D> inline bool few_lines(const RuleArgs &a) {
-  return a.R >= 4 && (int64_t)a.Z * a.H * a.R <= (D == 64 ? 2048 : sizeof(T) == 4 ? 512 : 1024);
+template <typename T, int D, int X> inline bool few_lines(const RuleArgs &a) {
+  return a.R >= 4 && (int64_t)a.Z * a.H * a.R <= (D == 64 ? 2048 : sizeof(T) == 4 ? 512 : 1024) / (X && sizeof(T) == 2 ? 2 : 1);
 }
 template <typename K> int rules_launch(K kernel, int64_t n_wg, int threads, int lds, std::atomic<uint64_t> &done, const RuleArgs &a, hipStream_t st) {
   if (lds > 65536 && !raise_lds_limit(reinterpret_cast<const void *>(kernel), lds, done)) return BSP_ERR_HIP;

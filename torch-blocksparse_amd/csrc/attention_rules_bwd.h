@@ -526,7 +526,7 @@ template <typename T, int D, int X, bool CAP, bool BIAS, bool DOCS> int launch_r
     static std::atomic<uint64_t> done{0}, done2{0};
     const int64_t grid = rules_grid((int64_t)a.Z * a.H, a.R);
     if constexpr (2 * pair_lds<T, D, X, 2>() <= kLdsBytes)
-      if (few_lines<T, D>(a)) return rules_launch(k_rules_bwd_rows<T, D, X, CAP, BIAS, DOCS, 2>, grid, 256, 2 * pair_lds<T, D, X, 2>(), done2, a, st);
+      if (few_lines<T, D, X>(a)) return rules_launch(k_rules_bwd_rows<T, D, X, CAP, BIAS, DOCS, 2>, grid, 256, 2 * pair_lds<T, D, X, 2>(), done2, a, st);
     return rules_launch(k_rules_bwd_rows<T, D, X, CAP, BIAS, DOCS, 1>, grid, 128, rules_lds<T, D, X>(), done, a, st);
   }
   static std::atomic<uint64_t> done{0};
