@@ -595,7 +595,8 @@ int bsp_latent_read(int dtype, const void *pages, int n_pages, int block, int la
  * (n - 1 - j) (softcap 0: no cap, else 2^-10 .. 1024), over the positions j < n = lengths[b]; table, lengths, width, n_pages: as in bsp_cache_attention.  q, o: [B, H, latent], q_r: [B, H, 64], all
  * 16-byte aligned with strides that are multiples of 8; B * H < 2^24.  rows: NULL, or what is seen beside that, for units of bsp_latent_attention_heads(H) heads (the last may have fewer): per unit n_rows + 1
  * ints, the number of the first entry of each block-row and the end of the last one's; behind all of them the entries, three ints each: block-column, and 64 bits (low
- * ones first), one for each of the unit's heads that sees it; one more entry behind the last.  The row is (n - 1) / block.  most_blocks: no sequence sees more blocks (width, or the most entries of a row).  workspace:
+ * ones first), one for each of the unit's heads that sees it; one more entry behind the last.  The row is (n - 1) / block.  most_blocks: a sequence sees so many blocks at most, the
+ * first (width, or the most entries of a row, to see all).  workspace:
  * bsp_latent_attention_workspace_bytes bytes, 16-byte aligned, no initialisation; calls that overlap need one each.  No atomics: the same call gives the same bits. */
 int bsp_latent_attention_heads(int H);
 int64_t bsp_latent_attention_workspace_bytes(int B, int H, int latent, int block, int64_t most_blocks);

@@ -8,6 +8,7 @@ import latent_oracle as O
 import rotation_oracle as R
 import torch_blocksparse as tb
 from helpers import random_layout
+from torch_blocksparse import _lib
 
 pytestmark = pytest.mark.gpu
 DEV = 'cuda'
@@ -241,3 +242,45 @@ def test_on_other_streams():
                 got.append(op(q, q_r, cache, table, lengths, scale=0.1))
     torch.cuda.synchronize()
     assert all(torch.equal(want, x) for x in got)
+
+
+def test_offsets_past_32_bits():
+    cache = tb.LatentCache(70000, 64)                         # 5.2 GB
+    table = torch.tensor([[69999, 3, 65536], [1, 69000, 58254]], dtype=torch.int32, device=DEV)
+    lengths = torch.tensor([170, 131], dtype=torch.int32, device=DEV)
+    q, q_r, want = randn((2, 20, 512), torch.bfloat16, 1), randn((2, 20, 64), torch.bfloat16, 2), []
+    for b in range(2):
+        n = int(lengths[b])
+        c, r = randn((n, 512), torch.bfloat16, 3 + b), randn((n, 64), torch.bfloat16, 5 + b)
+        j = torch.arange(n, device=DEV)
+        slots = (table[b, j // 64] * 64 + j % 64).int()
+        cache.write(c, r, slots)
+        got = cache.read(slots)
+        assert torch.equal(got[0], c) and torch.equal(got[1], r)
+        c, r = [torch.nn.functional.pad(t, (0, 0, 0, 192 - n)) for t in (c, r)]       # (the oracle takes whole pages)
+        small = torch.arange(3, dtype=torch.int32, device=DEV)[None]
+        want.append(O.attention(q[b:b + 1], q_r[b:b + 1], c, r, small, lengths[b:b + 1], 64, scale=0.04))
+    o = tb.LatentAttention(64)(q, q_r, cache, table, lengths, scale=0.04)
+    O.check(o, tuple(torch.cat([w[i] for w in want]) for i in range(2)), 'o')
+
+
+@pytest.mark.parametrize('layout', [False, True])
+def test_no_more_blocks_than_the_workspace_is_for(layout):
+    """A C caller's mistake stays in its workspace: the blocks past most_blocks are not seen"""
+    block, most = 16, 4
+    rows = None
+    if layout:
+        # a first block-row of eight entries, and seven of none
+        rows = torch.tensor([0] + [8] * 8 + [x for j in range(8) for x in (j, 1, 0)] + [0] * 3, dtype=torch.int32, device=DEV)
+    cache, q, q_r, table, lengths = setting(torch.float16, 3, 1, 128, block, [128, 100, 128], 1)
+    lib = _lib.load()
+    need = lib.bsp_latent_attention_workspace_bytes(3, 1, 128, block, most)
+    guard = torch.full((need + 4096,), 77, dtype=torch.uint8, device=DEV)
+    o = torch.empty_like(q)
+    ask = lengths if rows is None else torch.full_like(lengths, block)
+    rc = lib.bsp_latent_attention(0, q.data_ptr(), 128, 128, q_r.data_ptr(), 64, 64, o.data_ptr(), 128, 128, 3, 1, cache.data.data_ptr(), cache.pages, block, 128, table.data_ptr(),
+                                  table.stride(0), table.size(1), ask.data_ptr(), None if rows is None else rows.data_ptr(), 8, most, 0.05, 0., None, guard.data_ptr(), need, _lib.raw_stream(q.device))
+    assert rc == 0
+    assert bool((guard[need:] == 77).all())
+    seen = ask.clamp(max=most * block)
+    O.check(o, expected(cache, q, q_r, table, seen, scale=0.05), 'o')

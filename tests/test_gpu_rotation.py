@@ -116,6 +116,14 @@ def test_views_copies_and_empty_tensors():
     assert empty.grad.shape == empty.shape
 
 
+def test_offsets_past_32_bits():
+    held = torch.empty((1 << 32) + (1 << 20), dtype=torch.bfloat16, device=DEV)           # 8.6 GB
+    for shape, stride in (((2, 3, 5, 64), (1 << 32, 64 * 5, 64, 1)), ((1, 2, 5, 64), (0, 1 << 32, 64, 1)), ((1, 1, 3, 64), (0, 0, 1 << 31, 1))):
+        x = held.as_strided(shape, stride)
+        x.copy_(randn(shape, torch.bfloat16, 1))
+        assert torch.equal(tb.Rotation.of_base(64)(x), tb.Rotation.of_base(64)(x.contiguous()))
+
+
 def test_changed_positions_are_noticed():
     op = tb.Rotation.of_base(64)
     x, positions = randn((4, 2, 64), torch.float32, 1).requires_grad_(True), torch.arange(4, dtype=torch.int32, device=DEV)

@@ -31,6 +31,7 @@ struct LatentArgs {
   float *partial;                  // two slots a workgroup: [heads a unit][latent] sums; behind all of them [heads a unit][2] maxima and sums of shares
   int32_t *meta;                   // per item (sequence and unit) two ints: the workgroup that begins it, how many have a part (0, 1: nothing to join)
   int B, H, block, shift;          // shift: log2 of the groups of sixteen positions a block
+  int most_groups;                 // the most groups of 16 positions that a sequence goes through
   int units, per, pieces;          // workgroups' heads a sequence: units of `per`; pieces of the work
 };
 
@@ -534,6 +535,7 @@ struct LatentItem {
         entry = t[0];
         groups = (t[1] - t[0]) << a.shift;
       }
+      groups = groups < a.most_groups ? groups : a.most_groups;   // (or parts would be written past the workspace, where a caller has most_blocks wrong)
     }
   }
   __device__ __forceinline__ int steps() const { return (groups + 3) >> 2; }
@@ -950,6 +952,7 @@ extern "C" int bsp_latent_attention(int dtype, const void *q, int64_t q_stride_b
   a.pages = pages; a.n_pages = n_pages; a.table = table; a.table_sb = table_stride; a.width = width; a.lengths = lengths;
   a.rows = rows; a.n_rows = n_rows; a.slopes = slopes; a.scale = scale; a.cap = softcap;
   a.B = B; a.H = H; a.block = block; a.shift = __builtin_ctz(block) - 4;
+  a.most_groups = (int)(most_blocks < (1 << 24) ? most_blocks << a.shift : 1 << 30);
   a.units = latent_units(H); a.per = bsp_latent_attention_heads(H); a.pieces = latent_pieces(B, H, block, most_blocks);
   a.meta = reinterpret_cast<int32_t *>(workspace);
   a.partial = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(workspace) + ((int64_t)B * a.units * 8 + 15) / 16 * 16);
