@@ -178,10 +178,11 @@ def test_a_layout_of_fewer_blocks_than_the_table():
 
 
 @pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
-def test_scores_that_grow(dtype):
+@pytest.mark.parametrize('H,latent', [(16, 128), (16, 512), (32, 256), (70, 128), (64, 512)])
+def test_scores_that_grow(dtype, H, latent):
     """the running maximum moves again and again, up and far down"""
-    cache, q, q_r, table, lengths = setting(dtype, 2, 16, 128, 16, [1500, 1500], 2)
-    rows = cache.data.view(-1, 192)
+    cache, q, q_r, table, lengths = setting(dtype, 2, H, latent, 16, [1500, 1500], 2)
+    rows = cache.data.view(-1, latent + 64)
     for b, sign in ((0, 1.), (1, -1.)):
         at = (table[b].long().repeat_interleave(16) * 16 + torch.arange(table.size(1) * 16, device=DEV) % 16)[:1500]
         rows[at, :64] = (sign * torch.linspace(-3, 3, 1500, device=DEV)[:, None]).to(dtype)
