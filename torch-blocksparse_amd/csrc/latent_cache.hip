@@ -2,7 +2,7 @@
 // share, in a 16-bit type; row `slot` of the cache starts at element slot * (latent + 64).  With a rotation (rotation.h) those 64 are turned on the way, in fp32, and rounded once.
 //
 // Bound by the bytes.  A workgroup has eight positions: their latent vectors in chunks of 16 bytes, their shared parts a pair of elements a thread, so that no angle is computed
-// twice.
+// twice.  Measured: 20011 positions of 512 + 64 in bf16 with a rotation (46 MB): 12 us (3.8 TB/s), 2.5 more for the launch that says whose a slot is; 16384 x 8 (302 MB) 110 us.
 #include "latent.h"
 #include "rotation.h"
 
@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(256) k_latent_read(LatentCacheArgs a) {
   __builtin_nontemporal_store(x, reinterpret_cast<u32x4 *>(to));
 }
 
-// up to here each workgroup reads the slots behind its own, which costs less than a launch that says whose a slot is
+// Up to here each workgroup reads the slots behind its own, which costs less than a launch that says whose a slot is (64 positions 2.8 and 4.4 us, 512 4.3 and 5.1, 1024 6.1 and 5.2).
 constexpr int kScan = 512;
 
 template <typename T> void launch_latent_write(const LatentCacheArgs &a, hipStream_t st) {
