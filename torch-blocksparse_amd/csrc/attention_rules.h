@@ -1,4 +1,4 @@
-// Shared pieces of the attention kernels with score rules (attention_rules_fwd.hip, attention_rules_bwd.hip): block-sparse
+// Shared pieces of the attention kernels with score rules (attention_rules_fwd.h, attention_rules_bwd.h): block-sparse
 // attention whose logits are
 //     y_ij = cap * tanh(scale * q_i . k_j / cap) - slope_h * |i - j|        (no cap: scale * q_i . k_j - ...)
 // over the keys j that row i sees: block (h, i / block, j / block) is in the layout, both positions carry the same document

@@ -20,6 +20,7 @@
 namespace bsp {
 namespace {
 
+// wavefronts a SIMD that the registers are for (with a shared part one fewer, or they spill)
 template <typename T, int D, int X, bool CAP> constexpr int row_waves() { return sizeof(T) == 4 ? (D == 64 && !X ? 2 : 1) : D == 64 ? (CAP || X ? 2 : 3) : X ? 1 : 2; }
 template <typename T, int D, int X, bool CAP> constexpr int col_waves() { return D == 64 && !(X && sizeof(T) == 4) ? 2 : 1; }
 

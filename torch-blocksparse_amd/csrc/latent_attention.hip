@@ -13,6 +13,14 @@
 //
 // All steps of all sequences are one row of work that is cut into equal pieces, one a workgroup, so that uneven lengths leave no compute unit idle: a workgroup finds its piece by
 // a sum over the lengths.  A sequence that lies in several pieces is joined by a second kernel.
+//
+// Measured, latent vectors of 512, bf16: 16 sequences of up to 16384 positions (151 MB of pages) with 16 heads 52 us (3.8 TB/s; the join among them), 32 59, 64 66, 128 heads 95 and 9.6 for the join (47
+// GFLOP; 480 TFLOP/s).  16 heads are bound by the loads of a workgroup that has one step's on its way.  64 and more: of 200000 cycles a workgroup half of the products' reads from LDS (17.5 MB a compute
+// unit, 137000 cycles at 128 bytes a clock) and products (45000) overlap, the rest is a step's exponentials between them and a piece's ends: queries, sums written (33 MB, read back by the
+// join), the search for the piece.  Shorter: 16 x 16 heads over up to 4096 positions with a layout, fp16, 15 and 4 us; one sequence of 33 positions 10.8.
+//
+// Wavefronts of 32 heads, two for the same heads, on 32 x 32 x 16 products take half of the reads from LDS, but exchange shares and wait for each other in every step: 128 heads 117 us, 64 85 where this
+// takes 98 and 66.
 #include "attention_common.h"
 #include "latent.h"
 
@@ -42,13 +50,11 @@ template <> struct LatentMma<f16> {
   typedef f16x8 frag8; typedef f16x4 frag4;
   static __device__ __forceinline__ f32x4 run(frag8 a, frag8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
   static __device__ __forceinline__ f32x4 run(frag4 a, frag4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
-  static __device__ __forceinline__ f32x16 run(frag8 a, frag8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 template <> struct LatentMma<bf16> {
   typedef bf16x8 frag8; typedef bf16x4 frag4;
   static __device__ __forceinline__ f32x4 run(frag8 a, frag8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
   static __device__ __forceinline__ f32x4 run(frag4 a, frag4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0); }
-  static __device__ __forceinline__ f32x16 run(frag8 a, frag8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
 
 template <int LAT> struct LatentGeo {
@@ -56,7 +62,7 @@ template <int LAT> struct LatentGeo {
   static constexpr int GROUP = 16 * ROW, STAGE = 4 * GROUP, RING = 2 * STAGE;   // sixteen positions: their latent vectors, then their shared parts
   static constexpr int JOIN = LAT + 4;                                         // floats of a head's sums when wavefronts are joined
   static constexpr int CPR = LROW / 16, RPI = 64 / CPR, LOADS = 16 / RPI + 2;   // 16-byte chunks of a latent vector, rows of a load, loads of a group
-  static constexpr int STATS = RING, SHARES = RING + 1024, LDS = SHARES + 4 * 2048;   // behind the stages: heads' maxima and sums; a wavefront's shares (Heads32)
+  static constexpr int STATS = RING, FACTORS = RING + 512, LDS = FACTORS + 1024;   // behind the stages: maxima and sums of 64 rows, and what each's sums are multiplied by
   static_assert(64 * JOIN * 4 <= RING && LDS <= 160 * 1024, "");
 };
 
@@ -108,33 +114,28 @@ template <int N, class S, class P> __device__ __forceinline__ void latent_logits
 }
 // the lowest n of four bits, n any number
 __device__ __forceinline__ uint32_t first_of_four(int n) { return (1u << (n < 0 ? 0 : n > 4 ? 4 : n)) - 1u; }
-__device__ __forceinline__ void barrier_of_all() {        // everybody's LDS operations are done
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
 
 // The operands of both products come from LDS a batch of four reads at a time while the products of batches before are taken; left alone, the compiler reads one and waits for it, to save registers.  Every
 // batch also issues its part of the next step's loads (load(k)): all at once they would hold up the wavefront for the time that a compute unit takes for them, 64 bytes a clock.
 //
-// Sixteen heads a wavefront (at most 32 a workgroup), each wavefront HW of a step's groups.  Shares in two terms: what they are rounded to and what that leaves out.  The chunks of a latent vector in LDS: every row
+// Sixteen heads a wavefront, each wavefront HW of a step's groups.  Shares in two terms up to 32 heads: what they are rounded to and what that leaves out; past that, where products and their operands are what
+// counts, in one, which takes a sum's error from that of the result's rounding to 1.4 times that at most (128 heads 109 us with the second term, 98 without; 64 72 and 66; bf16 errors of 1.7 and 1.9 in 1000). The chunks of a latent vector in LDS: every row
 // begins in the first bank, so pairs of chunks of 256 bytes are exchanged by the row's number, which serves both reads without a conflict: a transposing read takes a pair from each of
 // eight rows at a time, a read along the rows a chunk of eight rows and its neighbour of the eight others.
-template <typename T, int LAT, int HW> struct Heads16 {
+template <typename T, int LAT, int HW> struct Heads {
   typedef LatentGeo<LAT> G;
   typedef LatentMma<T> M;
   typedef typename M::frag8 frag8;
   typedef typename std::conditional<HW == 1, typename M::frag4, frag8>::type frag;
   static constexpr int GROUPS = HW, SOURCES = 4 / HW, NS = LAT / 32, NR = kRope / 32, NT = LAT / 16;
   static constexpr int EXTRA = 4;                       // steps that going over to another item takes as long as
-  static constexpr bool BARRIER = HW > 1, OWN_SUMS = true;   // OWN_SUMS: each source has sums of its own
-  static __device__ __forceinline__ uint32_t chunk(uint32_t c, uint32_t r, uint32_t group) { return c ^ (r & 7) << 1; }
+  static constexpr bool BARRIER = HW > 1, TWO_TERMS = HW < 4;
+  static __device__ __forceinline__ uint32_t chunk(uint32_t c, uint32_t r) { return c ^ (r & 7) << 1; }
   static __device__ __forceinline__ int first_group(int wave) { return wave / HW * HW; }
   static __device__ __forceinline__ int head_of(int wave, int lane) { return 16 * (wave % HW) + (lane & 15); }
-  static __device__ __forceinline__ int mask(int wave, int lo, int hi) { return lo >> (16 * (wave % HW)); }
-  // the rows that have what wavefronts found of head h, and where a row's head begins in the sums
+  static __device__ __forceinline__ int mask(int wave, int lo, int hi) { return (HW == 4 && wave & 2 ? hi : lo) >> (HW > 1 ? 16 * (wave & 1) : 0); }
+  // the rows that have what wavefronts found of head h
   static __device__ __forceinline__ int source(int h, int p) { return 16 * (p * HW + h / 16) + h % 16; }
-  static __device__ __forceinline__ int sums(int h, int p) { return source(h, p); }
 
   frag8 q[NS + NR];
   f32x4 o[NT];
@@ -150,10 +151,10 @@ template <typename T, int LAT, int HW> struct Heads16 {
       const T *from = s < NS ? pq + 32 * s : pr + 32 * (s - NS);
       q[s] = __builtin_bit_cast(frag8, here ? *reinterpret_cast<const u32x4 *>(from + 8 * c) : u32x4{0, 0, 0, 0});
     }
-    row_at = key * G::LROW + (chunk(c, key, 0) << 4);
+    row_at = key * G::LROW + (chunk(c, key) << 4);
     rope_at = 16 * G::LROW + key * (2 * kRope) + (rope_chunk(c, key) << 4);
     const uint32_t r = 4 * c + (key >> 2);
-    tr_at = r * G::LROW + (chunk((key & 3) >> 1, r, 0) << 4) + 8 * (key & 1);
+    tr_at = r * G::LROW + (chunk((key & 3) >> 1, r) << 4) + 8 * (key & 1);
     m = -INFINITY;
     l = 0.f;
 #pragma unroll
@@ -237,7 +238,11 @@ template <typename T, int LAT, int HW> struct Heads16 {
     }
     float sc[4 * HW];
 #pragma unroll
-    for (int i = 0; i < 4 * HW; i++) sc[i] = HW == 1 ? (acc[i >> 2][0][i & 3] + acc[i >> 2][1][i & 3]) + (acc[i >> 2][2 % CHAINS][i & 3] + acc[i >> 2][3 % CHAINS][i & 3]) : acc[i >> 2][0][i & 3] + acc[i >> 2][1][i & 3];
+    for (int i = 0; i < 4 * HW; i++) {
+      sc[i] = acc[i >> 2][0][i & 3];
+#pragma unroll
+      for (int x = 1; x < CHAINS; x++) sc[i] += acc[i >> 2][x][i & 3];
+    }
     auto logits = [&](float (&y)[4 * HW], float minus) {
       latent_logits(y, [&](int i) { return sc[i]; }, scores, slope, minus, [&](int i) { return now[i >> 2].pos + 4 * c + (i & 3); });
     };
@@ -276,11 +281,11 @@ template <typename T, int LAT, int HW> struct Heads16 {
       return false;
     }
     l += sum;
-    frag most[PAIRS], rest[PAIRS];
+    frag most[PAIRS], rest[TWO_TERMS ? PAIRS : 1];
 #pragma unroll
     for (int i = 0; i < 4 * HW; i++) {
       most[i / PER][i % PER] = from_float<T>(e[i]);
-      rest[i / PER][i % PER] = from_float<T>(e[i] - to_float(most[i / PER][i % PER]));
+      if constexpr (TWO_TERMS) rest[i / PER][i % PER] = from_float<T>(e[i] - to_float(most[i / PER][i % PER]));
     }
 #pragma unroll
     for (int b = 0; b < PAIRS * NB; b++) {
@@ -288,8 +293,9 @@ template <typename T, int LAT, int HW> struct Heads16 {
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int j = 0; j < 4; j++) o[b % NB * 4 + j] = M::run(cols[b % 3][j], most[b / NB], o[b % NB * 4 + j]);
+      if constexpr (TWO_TERMS)
 #pragma unroll
-      for (int j = 0; j < 4; j++) o[b % NB * 4 + j] = M::run(cols[b % 3][j], rest[b / NB], o[b % NB * 4 + j]);
+        for (int j = 0; j < 4; j++) o[b % NB * 4 + j] = M::run(cols[b % 3][j], rest[b / NB], o[b % NB * 4 + j]);
       __builtin_amdgcn_sched_barrier(0);
     }
     return true;
@@ -306,213 +312,6 @@ template <typename T, int LAT, int HW> struct Heads16 {
     if (c == 0) stats[2 * r] = m, stats[2 * r + 1] = l;
 #pragma unroll
     for (int n = 0; n < NT; n++) *reinterpret_cast<f32x4 *>(join + r * G::JOIN + 16 * n + 4 * c) = o[n];
-  }
-};
-
-// 32 heads a wavefront, two wavefronts for the same heads (64 a workgroup): each has the scores of half of a step's positions and, with the other's shares through LDS, the sums of half of the elements, on
-// 32 x 32 x 16 products.  That is half of the reads from LDS of Heads16 for so many heads, and what bounds those.  Shares in one term, which takes a sum's error from that of the result's rounding to 1.4
-// times that: a second one is half again the products (latent_long: 126 us with it, 103 without, both in Heads16).  Pairs of chunks in LDS by two bits of the row's number and the third, as a
-// transposing read takes four chunks of four rows; the lowest bit by the group, as a read along the rows takes a chunk of eight rows of each of two groups.
-template <typename T, int LAT> struct Heads32 {
-  typedef LatentGeo<LAT> G;
-  typedef LatentMma<T> M;
-  typedef typename M::frag8 frag8;
-  static constexpr int GROUPS = 2, SOURCES = 2, NS = LAT / 16, NR = kRope / 16, NT = LAT / 64, HELD = NS < 22 ? NS : 22;   // NT: the wavefront's tiles of 32 elements
-  static constexpr int EXTRA = 8;
-  static constexpr bool BARRIER = true, OWN_SUMS = false;
-  static __device__ __forceinline__ uint32_t chunk(uint32_t c, uint32_t r, uint32_t group) { return c ^ ((r & 3) << 2 | (r >> 1 & 2) | (group & 1)); }
-  static __device__ __forceinline__ int first_group(int wave) { return 2 * (wave & 1); }
-  static __device__ __forceinline__ int head_of(int wave, int lane) { return 32 * (wave >> 1) + (lane & 31); }
-  static __device__ __forceinline__ int mask(int wave, int lo, int hi) { return wave & 2 ? hi : lo; }
-  static __device__ __forceinline__ int source(int h, int p) { return 64 * (h / 32) + 32 * p + h % 32; }   // (of a maximum and sum; the sums are whole)
-  static __device__ __forceinline__ int sums(int h, int) { return h; }
-
-  frag8 q[NS + NR];
-  f32x16 o[NT];
-  float m, l, slope, scaled;
-  uint32_t row_at, rope_at, tr_at, tr_at2, shares, tops;
-  int key, half;
-  bool here;
-
-  __device__ __forceinline__ void init(const T *pq, const T *pr, bool here_, float slope_, int wave, int lane, uint32_t lds) {
-    key = lane & 31; half = lane >> 5; here = here_; slope = slope_;
-#pragma unroll
-    for (int s = 0; s < NS + NR; s++) {
-      const T *from = s < NS ? pq + 16 * s : pr + 16 * (s - NS);
-      q[s] = __builtin_bit_cast(frag8, here ? *reinterpret_cast<const u32x4 *>(from + 8 * half) : u32x4{0, 0, 0, 0});
-    }
-    const uint32_t r = key & 15, group = key >> 4;
-    row_at = group * G::GROUP + r * G::LROW + (chunk(half, r, group) << 4);
-    rope_at = group * G::GROUP + 16 * G::LROW + r * (2 * kRope) + (rope_chunk(half, r) << 4);
-    // transposed: rows 4 half + 0 .. 3 of a group, and those eight further on, whose chunks are exchanged alike
-    const uint32_t i = lane & 15, tr = 4 * half + (i >> 2), col = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
-    const uint32_t half_of = (wave & 1) * (LAT / 16);     // (the wavefront's half of the elements, in chunks)
-    tr_at = tr * G::LROW + (chunk(half_of + col, tr, 0) << 4) + 8 * (i & 1);
-    tr_at2 = tr * G::LROW + (chunk(half_of + col, tr, 1) << 4) + 8 * (i & 1);
-    shares = lds + G::SHARES + wave * 2048 + lane * 16;
-    tops = lds + G::STATS + wave * 128 + key * 4;
-    m = -INFINITY;
-    l = 0.f;
-#pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-      for (int x = 0; x < 16; x++) o[n][x] = 0.f;
-  }
-
-  __device__ __forceinline__ void arrived() {
-#pragma unroll
-    for (int s = 0; s < HELD; s++) asm volatile("" : "+a"(q[s]));   // (beside sums and scores, which fills those registers with LAT = 512)
-#pragma unroll
-    for (int s = HELD; s < NS + NR; s++) asm volatile("" : "+v"(q[s]));
-  }
-
-  template <class F> __device__ __forceinline__ bool step(uint32_t stage, const LatentGroup (&now)[GROUPS], const LatentScores &scores, bool again, bool first, int wave, F &&load) {
-    uint32_t at_row[8], at_rope[NR], at_col[2][4];
-    const uint32_t own_groups = stage + first_group(wave) * G::GROUP;
-#pragma unroll
-    for (int i = 0; i < 8; i++) at_row[i] = own(own_groups + (own(row_at) ^ (i << 5)));
-#pragma unroll
-    for (int i = 0; i < NR; i++) at_rope[i] = own(own_groups + (own(rope_at) ^ (i << 5)));
-    // scores: value i is that of position 8 (i / 4) % 16 + 4 half + i % 4 of group i / 8
-    constexpr int ALL = NS + NR, AHEAD = 6, RING = AHEAD + 2;
-    constexpr int CHAINS = 2;
-    f32x16 acc[CHAINS];
-#pragma unroll
-    for (int x = 0; x < CHAINS; x++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) acc[x][i] = 0.f;
-    frag8 rows[RING];
-    auto read_row = [&](int t) { rows[t % RING] = latent_read<frag8>(t < NS ? at_row[t & 7] + (t >> 3) * 256 : at_rope[t < NS ? 0 : t - NS]); };
-#pragma unroll
-    for (int t = 0; t < AHEAD; t++) read_row(t);
-#pragma unroll
-    for (int t = 0; t < ALL; t += 2) {
-      if (t + AHEAD < ALL) read_row(t + AHEAD), read_row(t + AHEAD + 1);
-#pragma unroll
-      for (int k = t * G::LOADS / ALL; k < (t + 2) * G::LOADS / ALL; k++) load(k);
-      __builtin_amdgcn_sched_barrier(0);
-      acc[t % CHAINS] = M::run(rows[t % RING], q[t], acc[t % CHAINS]);
-      acc[(t + 1) % CHAINS] = M::run(rows[(t + 1) % RING], q[t + 1], acc[(t + 1) % CHAINS]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    // (what the second product begins with on its way)
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      at_col[0][i] = own(stage + (own(tr_at) ^ (i << 6)));
-      at_col[1][i] = own(stage + (own(tr_at2) ^ (i << 6)));
-    }
-    // a batch: four products, of a group's sixteen positions or, where the wavefront has two tiles, of two groups'
-    frag8 cols[3][4];
-    constexpr int NB = NT;                                // batches
-    auto at = [&](int b, int j, int &n, int &g) { n = (b * 4 + j) % NT; g = (b * 4 + j) / NT; };
-    auto read_cols = [&](int b) {
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        int n, g;
-        at(b, j, n, g);
-        const uint32_t from = at_col[g & 1][n & 3] + g * G::GROUP + (n >> 2) * 256;
-        cols[b % 3][j] = __builtin_bit_cast(frag8, latent_read_tr2(from, from + 8 * G::LROW));
-      }
-    };
-    read_cols(0);
-    if (NB > 1) read_cols(1);
-    __builtin_amdgcn_sched_barrier(0);
-    float sc[16];
-#pragma unroll
-    for (int i = 0; i < 16; i++) sc[i] = acc[0][i] + acc[1][i];
-    uint32_t seen = 0xffffu;
-    const bool all = now[0].n == 16 && now[1].n == 16 && (now[0].mask & now[1].mask) == -1;
-    if (!all) {
-      seen = 0;
-#pragma unroll
-      for (int g = 0; g < 2; g++)
-        if (here && (now[g].mask >> key & 1)) seen |= (first_of_four(now[g].n - 4 * half) | first_of_four(now[g].n - 8 - 4 * half) << 4) << (8 * g);
-    }
-    auto logits = [&](float (&y)[16], float minus) {
-      latent_logits(y, [&](int i) { return sc[i]; }, scores, slope, minus, [&](int i) { return now[i >> 3].pos + 8 * (i >> 2 & 1) + 4 * half + (i & 3); });
-    };
-    // shares relative to the running maximum, the same in both wavefronts of a head
-    frag8 p[2];
-    float sum;
-    auto exponentials = [&]() {
-      float e[16];
-      logits(e, m == -INFINITY ? 0.f : m);
-#pragma unroll
-      for (int i = 0; i < 16; i++) e[i] = __builtin_amdgcn_exp2f(e[i]);
-      if (!all)
-#pragma unroll
-        for (int i = 0; i < 16; i++) e[i] = seen >> i & 1 ? e[i] : 0.f;
-      float part[4];
-#pragma unroll
-      for (int i = 0; i < 4; i++) part[i] = (e[i] + e[4 + i]) + (e[8 + i] + e[12 + i]);
-      sum = (part[0] + part[1]) + (part[2] + part[3]);
-#pragma unroll
-      for (int i = 0; i < 16; i++) p[i >> 3][i & 7] = from_float<T>(e[i]);
-    };
-    frag8 their[2];
-    const uint32_t flags = shares - (uint32_t)((threadIdx.x & 63) * 16 + wave * 2048) - 256;     // (between the maxima and the shares)
-    auto exchange = [&](int word) {                       // the shares to the other wavefront, a word to all; returns whether any wavefront's is not zero
-#pragma unroll
-      for (int g = 0; g < 2; g++) latent_put(shares + 1024 * g, __builtin_bit_cast(u32x4, p[g]));
-      if ((threadIdx.x & 63) == 0) latent_put(flags + 4 * wave, word);
-      barrier_of_all();
-      const i32x4b f = latent_read<i32x4b>(flags);
-#pragma unroll
-      for (int g = 0; g < 2; g++) their[g] = latent_read<frag8>((shares ^ 2048) + 1024 * g);
-      return __builtin_amdgcn_readfirstlane(f[0] | f[1] | f[2] | f[3]) != 0;
-    };
-    exponentials();
-    const bool move = __builtin_amdgcn_ballot_w64(sum > 8192.f || (m == -INFINITY && seen != 0)) != 0;
-    if (exchange(move && !again)) {                       // (all wavefronts take the same way)
-      float y[16], top = -INFINITY;
-      logits(y, 0.f);
-#pragma unroll
-      for (int i = 0; i < 16; i++) top = fmaxf(top, seen >> i & 1 ? y[i] : -INFINITY);
-      top = fmaxf(top, __shfl_xor(top, 32));
-      if (half == 0) latent_put(tops, top);
-      barrier_of_all();
-      const float mn = fmaxf(m, fmaxf(top, latent_read<float>(tops ^ 128)));
-      scaled = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
-      l *= scaled;
-      m = mn;
-      if (!first) return false;
-      exponentials();                                     // (the sums are zeros)
-      exchange(0);
-    }
-    l += sum;
-    frag8 share[4];                                       // by group
-#pragma unroll
-    for (int g = 0; g < 2; g++) {
-      share[g] = wave & 1 ? their[g] : p[g];
-      share[2 + g] = wave & 1 ? p[g] : their[g];
-    }
-#pragma unroll
-    for (int b = 0; b < NB; b++) {
-      if (b + 2 < NB) read_cols(b + 2);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        int n, g;
-        at(b, j, n, g);
-        o[n] = M::run(cols[b % 3][j], share[g], o[n]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    return true;
-  }
-  __device__ __forceinline__ void scale() {
-#pragma unroll
-    for (int n = 0; n < NT; n++) o[n] = scaled_by(o[n], scaled);
-  }
-  __device__ __forceinline__ void put(float *join, float *stats, int wave) {
-    l += __shfl_xor(l, 32);
-    const int r = 32 * wave + key;
-    if (half == 0) stats[2 * r] = m, stats[2 * r + 1] = l;
-    float *to = join + (32 * (wave >> 1) + key) * G::JOIN + (wave & 1) * (LAT / 2) + 4 * half;
-#pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-      for (int g = 0; g < 4; g++) *reinterpret_cast<f32x4 *>(to + 32 * n + 8 * g) = f32x4{o[n][4 * g], o[n][4 * g + 1], o[n][4 * g + 2], o[n][4 * g + 3]};
   }
 };
 
@@ -541,17 +340,19 @@ struct LatentItem {
   __device__ __forceinline__ int steps() const { return (groups + 3) >> 2; }
 };
 
-template <typename T, int LAT, class Heads>
+template <typename T, int LAT, int HW>
 __global__ void __launch_bounds__(256, 1) k_latent_attention(LatentArgs a) {
   typedef LatentGeo<LAT> G;
+  typedef Heads<T, LAT, HW> H;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int mine = Heads::first_group(wave);            // the first of the step's groups that the wavefront goes through
+  const int mine = H::first_group(wave);            // the first of the step's groups that the wavefront goes through
   const uint32_t items = (uint32_t)(a.B * a.units), ring = (uint32_t)(uintptr_t)BSP_LDS_PTR(smem);
 
   // The workgroup's piece [lo, hi) of all steps, and the item that it begins in.  Where there are more steps than pieces, an item counts `extra` steps more ahead of its own: what a
-  // workgroup that goes over to another item spends on the queries and on the sums of the last (16 x 128 heads over up to 16384 positions: 131 us without, 117 with; 128 x 128 heads over up to 500:
-  // 112 and 73; with a step or less a piece the extra steps would only leave pieces empty: 4 x 128 heads over up to 300, 32 us with them, 27 without).
+  // workgroup that goes over to another item spends on the queries and on the sums of the last (16 x 64 heads over up to 16384 positions: 76 us without, 66 with; 128 x 128 heads over up to 500:
+  // 85 and 62; 300 x 16 over up to 600: 61 and 46; two or eight steps instead of four: 72 and 66, 63 and 59).  With a step or less a piece they would only leave pieces empty: 4 x 128 heads over up to 300,
+  // 24 us with them, 21 without.
   int64_t total = 0, lo, hi, begin = 0;
   uint32_t item = 0;
   LatentItem found{}, looked{};                         // that item; what the thread has looked at last
@@ -608,7 +409,7 @@ __global__ void __launch_bounds__(256, 1) k_latent_attention(LatentArgs a) {
     total = (int64_t)(every & kSteps);
     pieces = total < a.pieces ? (int)total : a.pieces;    // (none is empty)
     if ((int)blockIdx.x >= pieces) return;
-    extra = total > a.pieces ? Heads::EXTRA : 0;
+    extra = total > a.pieces ? H::EXTRA : 0;
     auto steps_of = [&](uint64_t x) { return (int64_t)(x & kSteps) + extra * (int64_t)(x >> 40); };
     total = steps_of(every);
     lo = total * blockIdx.x / pieces;
@@ -688,7 +489,7 @@ __global__ void __launch_bounds__(256, 1) k_latent_attention(LatentArgs a) {
       v_page = v_n > 0 ? page : 0;
     };
     auto group_of = [&](int i) {
-      return LatentGroup{__builtin_amdgcn_readlane(v_pos, i), __builtin_amdgcn_readlane(v_n, i), Heads::mask(wave, __builtin_amdgcn_readlane(v_lo, i), __builtin_amdgcn_readlane(v_hi, i))};
+      return LatentGroup{__builtin_amdgcn_readlane(v_pos, i), __builtin_amdgcn_readlane(v_n, i), H::mask(wave, __builtin_amdgcn_readlane(v_lo, i), __builtin_amdgcn_readlane(v_hi, i))};
     };
     // the wavefront's group of a step on its way to its place in one of the stages: load k of the group
     i32x4b rows;
@@ -701,11 +502,11 @@ __global__ void __launch_bounds__(256, 1) k_latent_attention(LatentArgs a) {
       dst = __builtin_amdgcn_readfirstlane(ring + (s & 1) * G::STAGE + wave * G::GROUP);
     };
     // (a row's number is that of the load's first and the lane's, in bits of their own, and the exchange of chunks goes by bits)
-    const uint32_t lane_chunk = Heads::chunk(lane % G::CPR, lane / G::CPR, wave) << 4, lane_row = lane / G::CPR * G::ROW;
+    const uint32_t lane_chunk = H::chunk(lane % G::CPR, lane / G::CPR) << 4, lane_row = lane / G::CPR * G::ROW;
     const uint32_t lane_rope = rope_chunk(lane % 8, lane / 8) << 4, lane_rope_row = lane / 8 * G::ROW + G::LROW;
     auto load = [&](int k) {
       const int j = k - (G::LOADS - 2);
-      if (j < 0) rows_to_lds(rows, (own(lane_chunk) ^ Heads::chunk(0, k * G::RPI, 0) << 4) + (lane_row + k * G::RPI * G::ROW), dst + k * 1024);
+      if (j < 0) rows_to_lds(rows, (own(lane_chunk) ^ H::chunk(0, k * G::RPI) << 4) + (lane_row + k * G::RPI * G::ROW), dst + k * 1024);
       else rows_to_lds(rows, (own(lane_rope) ^ rope_chunk(0, 8 * j) << 4) + (lane_rope_row + 8 * j * G::ROW), dst + 16 * G::LROW + j * 1024);
     };
 
@@ -713,17 +514,17 @@ __global__ void __launch_bounds__(256, 1) k_latent_attention(LatentArgs a) {
     aim(s0);
 #pragma unroll
     for (int k = 0; k < G::LOADS; k++) load(k);
-    Heads x;
+    H x;
     {
-      const int head = Heads::head_of(wave, lane);        // the lane's head among the unit's
+      const int head = H::head_of(wave, lane);        // the lane's head among the unit's
       const bool here = head < heads;
       const int64_t h = first + (here ? head : 0);
       x.init(reinterpret_cast<const T *>(a.q) + b * a.q_sb + h * a.q_sh, reinterpret_cast<const T *>(a.qr) + b * a.qr_sb + h * a.qr_sh, here,
              a.slopes ? a.slopes[h] * kLog2e : 0.f, wave, lane, ring);
     }
-    LatentGroup now[Heads::GROUPS], next[Heads::GROUPS];
+    LatentGroup now[H::GROUPS], next[H::GROUPS];
 #pragma unroll
-    for (int k = 0; k < Heads::GROUPS; k++) now[k] = next[k] = group_of(mine + k);
+    for (int k = 0; k < H::GROUPS; k++) now[k] = next[k] = group_of(mine + k);
 
     // A step whose shares grow past 8192 leaves the loop for the sums to be scaled and is taken again: with that in it, the compiler moves all sums out of the matrix
     // units' registers and back in every step.
@@ -735,7 +536,7 @@ __global__ void __launch_bounds__(256, 1) k_latent_attention(LatentArgs a) {
         if (!again) {
           BSP_WAIT_VM(0);
           asm volatile("" ::: "memory");
-          if constexpr (Heads::BARRIER) {
+          if constexpr (H::BARRIER) {
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
           }
@@ -746,13 +547,13 @@ __global__ void __launch_bounds__(256, 1) k_latent_attention(LatentArgs a) {
           aim(s + 1);                                     // (behind the last step: loads of nothing; a step that is taken again loads the same again)
           if (s + 1 < s1) {
 #pragma unroll
-            for (int k = 0; k < Heads::GROUPS; k++) next[k] = group_of(4 * (s + 1 - base) + mine + k);
+            for (int k = 0; k < H::GROUPS; k++) next[k] = group_of(4 * (s + 1 - base) + mine + k);
           }
         }
         again = !x.step(ring + (s & 1) * G::STAGE, now, scores, again, s == s0, wave, load);
         if (again) break;
 #pragma unroll
-        for (int k = 0; k < Heads::GROUPS; k++) now[k] = next[k];
+        for (int k = 0; k < H::GROUPS; k++) now[k] = next[k];
       }
       if (s >= s1) break;
       x.scale();
@@ -777,25 +578,25 @@ __global__ void __launch_bounds__(256, 1) k_latent_attention(LatentArgs a) {
       to[1] = parts;
     }
     // what each source's sums are multiplied by, a head a thread; then four elements a thread, four of them on their way
-    float *by = reinterpret_cast<float *>(smem + G::SHARES);
+    float *by = reinterpret_cast<float *>(smem + G::FACTORS);
     float *parts_of = a.partial + (int64_t)slot * a.per * LAT, *stats_of = a.partial + (int64_t)2 * a.pieces * a.per * LAT + (int64_t)slot * a.per * 2;
     if (tid < heads) {
-      float top = -INFINITY, sum = 0.f, f[Heads::SOURCES];
+      float top = -INFINITY, sum = 0.f, f[H::SOURCES];
 #pragma unroll
-      for (int p = 0; p < Heads::SOURCES; p++) top = fmaxf(top, stats[2 * Heads::source(tid, p)]);
+      for (int p = 0; p < H::SOURCES; p++) top = fmaxf(top, stats[2 * H::source(tid, p)]);
 #pragma unroll
-      for (int p = 0; p < Heads::SOURCES; p++) {
-        const int r = Heads::source(tid, p);
+      for (int p = 0; p < H::SOURCES; p++) {
+        const int r = H::source(tid, p);
         f[p] = stats[2 * r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(stats[2 * r] - top);
         sum = fmaf(f[p], stats[2 * r + 1], sum);
       }
       const float last = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-      for (int p = 0; p < Heads::SOURCES; p++) by[64 * p + tid] = f[p] * last;
+      for (int p = 0; p < H::SOURCES; p++) by[64 * p + tid] = f[p] * last;
       if (!whole) stats_of[2 * tid] = top, stats_of[2 * tid + 1] = sum;
     }
     __syncthreads();
-    constexpr int LANES = LAT / 4, U = 4, TERMS = Heads::OWN_SUMS ? Heads::SOURCES : 1;   // LANES: threads of a head
+    constexpr int LANES = LAT / 4, U = 4, TERMS = H::SOURCES;   // LANES: threads of a head
     const int all = heads * LANES;
     for (int i0 = tid; i0 < all; i0 += 256 * U) {
       f32x4 v[U];
@@ -806,7 +607,7 @@ __global__ void __launch_bounds__(256, 1) k_latent_attention(LatentArgs a) {
 #pragma unroll
         for (int p = 0; p < TERMS; p++) {
           const float f = by[64 * p + h];
-          const f32x4 w = *reinterpret_cast<const f32x4 *>(join + Heads::sums(h, p) * G::JOIN + d);
+          const f32x4 w = *reinterpret_cast<const f32x4 *>(join + H::source(h, p) * G::JOIN + d);
 #pragma unroll
           for (int e = 0; e < 4; e++) v[u][e] = f == 0.f ? v[u][e] : fmaf(f, w[e], v[u][e]);
         }
@@ -829,14 +630,15 @@ __global__ void __launch_bounds__(256, 1) k_latent_attention(LatentArgs a) {
   }
 }
 
-// The parts of a sequence's head joined: a workgroup a head, a part's maximum and sum a lane at a time, then the parts among its four wavefronts.  Parts that saw nothing have
+// The parts of a sequence's head joined: a workgroup a head (or SPAN of its elements), a part's maximum and sum a lane at a time, then the parts among its W wavefronts.  Parts that saw nothing have
 // a factor of 0.
-template <typename T, int LAT> __global__ void __launch_bounds__(256) k_latent_join(LatentArgs a) {
-  constexpr int N = LAT / 64;
+template <typename T, int LAT, int SPAN, int W> __global__ void __launch_bounds__(64 * W) k_latent_join(LatentArgs a) {
+  constexpr int N = SPAN / 64;
   typedef float f32x2 __attribute__((ext_vector_type(2)));
-  __shared__ float sums[4][LAT + 2], tops[4];
+  __shared__ float sums[W][SPAN + 2], tops[W];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Quotient at(blockIdx.x, a.H);
+  const int from_element = blockIdx.y * SPAN;
   const int b = (int)at.q, h = (int)at.r, unit = h / a.per, r = h % a.per;
   const int32_t *meta = a.meta + 2 * ((int64_t)b * a.units + unit);
   const int parts = meta[1];
@@ -845,61 +647,67 @@ template <typename T, int LAT> __global__ void __launch_bounds__(256) k_latent_j
   const float *stats = a.partial + (int64_t)2 * a.pieces * a.per * LAT;
   auto part = [&](int p) { return (int64_t)(2 * (from + p) + (p == 0 ? 1 : 0)) * a.per + r; };
   float top = -INFINITY;
-  for (int p = tid; p < parts; p += 256) top = fmaxf(top, stats[2 * part(p)]);
+  for (int p = tid; p < parts; p += 64 * W) top = fmaxf(top, stats[2 * part(p)]);
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
   if (lane == 0) tops[wave] = top;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 4; w++) top = fmaxf(top, tops[w]);
+  for (int w = 0; w < W; w++) top = fmaxf(top, tops[w]);
   float sum = 0.f, x[N] = {};
-  for (int p0 = wave; p0 < parts; p0 += 16) {             // four of the wavefront's parts on their way
+  for (int p0 = wave; p0 < parts; p0 += 4 * W) {             // four of the wavefront's parts on their way
     f32x2 own[4];
     float v[4][N];
 #pragma unroll
     for (int u = 0; u < 4; u++) {
-      const int64_t p = part(p0 + 4 * u < parts ? p0 + 4 * u : p0);
+      const int64_t p = part(p0 + W * u < parts ? p0 + W * u : p0);
       own[u] = *reinterpret_cast<const f32x2 *>(stats + 2 * p);
 #pragma unroll
       for (int e = 0; e < N; e += 2) {
-        const f32x2 w = *reinterpret_cast<const f32x2 *>(a.partial + p * LAT + 64 * e + 2 * lane);
+        const f32x2 w = *reinterpret_cast<const f32x2 *>(a.partial + p * LAT + from_element + 64 * e + 2 * lane);
         v[u][e] = w[0];
         v[u][e + 1] = w[1];
       }
     }
 #pragma unroll
     for (int u = 0; u < 4; u++) {
-      const float f = p0 + 4 * u >= parts || own[u][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(own[u][0] - top);
+      const float f = p0 + W * u >= parts || own[u][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(own[u][0] - top);
       sum = fmaf(f, own[u][1], sum);
 #pragma unroll
       for (int e = 0; e < N; e++) x[e] = fmaf(f, v[u][e], x[e]);
     }
   }
-  if (lane == 0) sums[wave][LAT] = sum;
+  if (lane == 0) sums[wave][SPAN] = sum;
 #pragma unroll
   for (int e = 0; e < N; e += 2) *reinterpret_cast<f32x2 *>(&sums[wave][0] + 64 * e + 2 * lane) = f32x2{x[e], x[e + 1]};
   __syncthreads();
   sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < 4; w++) sum += sums[w][LAT];
+  for (int w = 0; w < W; w++) sum += sums[w][SPAN];
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  for (int d = tid; d < LAT; d += 256) {
-    const float y = (sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d]);
-    reinterpret_cast<T *>(a.o)[b * a.o_sb + h * a.o_sh + d] = from_float<T>(sum == 0.f ? 0.f : y * inv);
+  for (int d = tid; d < SPAN; d += 64 * W) {
+    float y = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; w++) y += sums[w][d];
+    reinterpret_cast<T *>(a.o)[b * a.o_sb + h * a.o_sh + from_element + d] = from_float<T>(sum == 0.f ? 0.f : y * inv);
   }
 }
 
-template <typename T, int LAT, class Heads> int launch_latent_heads(const LatentArgs &a, hipStream_t st) {
+template <typename T, int LAT, int HW> int launch_latent_heads(const LatentArgs &a, hipStream_t st) {
   static std::atomic<uint64_t> done{0};
-  if (LatentGeo<LAT>::LDS > 65536 && !raise_lds_limit(reinterpret_cast<const void *>(k_latent_attention<T, LAT, Heads>), LatentGeo<LAT>::LDS, done)) return BSP_ERR_HIP;
-  hipLaunchKernelGGL((k_latent_attention<T, LAT, Heads>), dim3((unsigned)a.pieces), dim3(256), LatentGeo<LAT>::LDS, st, a);
+  if (LatentGeo<LAT>::LDS > 65536 && !raise_lds_limit(reinterpret_cast<const void *>(k_latent_attention<T, LAT, HW>), LatentGeo<LAT>::LDS, done)) return BSP_ERR_HIP;
+  hipLaunchKernelGGL((k_latent_attention<T, LAT, HW>), dim3((unsigned)a.pieces), dim3(256), LatentGeo<LAT>::LDS, st, a);
   return BSP_OK;
 }
 template <typename T, int LAT> int launch_latent(const LatentArgs &a, bool joined, hipStream_t st) {
-  const int rc = a.per <= 16 ? launch_latent_heads<T, LAT, Heads16<T, LAT, 1>>(a, st) : a.per <= 32 ? launch_latent_heads<T, LAT, Heads16<T, LAT, 2>>(a, st)
-                                                                                              : launch_latent_heads<T, LAT, Heads32<T, LAT>>(a, st);
+  // (as few wavefronts to a group as have heads: the others would read the same from LDS for nothing.  16 sequences of up to 16384 positions, 16 heads: 52.0 us by one and 52.6 by two, with latent
+  // vectors of 128 22.2 and 24.2)
+  const int rc = a.per <= 16 ? launch_latent_heads<T, LAT, 1>(a, st) : a.per <= 32 ? launch_latent_heads<T, LAT, 2>(a, st) : launch_latent_heads<T, LAT, 4>(a, st);
   if (rc != BSP_OK) return rc;
-  if (joined) hipLaunchKernelGGL((k_latent_join<T, LAT>), dim3((unsigned)((int64_t)a.B * a.H)), dim3(256), 0, st, a);
+  // a head's elements among several workgroups, of more wavefronts, where there are few heads: with one a head one sequence of up to 16384 positions takes 11.7 us for 16 heads (256 parts of
+  // each) and 9.2 for 128, like this 6.2 and 8.4; 4 x 32 heads 6.9 and 6.1
+  if (joined && (int64_t)a.B * a.H <= 128) hipLaunchKernelGGL((k_latent_join<T, LAT, 128, 16>), dim3((unsigned)((int64_t)a.B * a.H), LAT / 128), dim3(1024), 0, st, a);
+  else if (joined) hipLaunchKernelGGL((k_latent_join<T, LAT, LAT, 4>), dim3((unsigned)((int64_t)a.B * a.H)), dim3(256), 0, st, a);
   BSP_LAUNCH_CHECK();
   return BSP_OK;
 }
