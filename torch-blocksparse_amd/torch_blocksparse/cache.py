@@ -85,13 +85,13 @@ class KeyValueCache(Pages):
             raise _lib.BlocksparseLibraryError('torch_blocksparse: %s must live on %s (got device %s)' % (name, self.device, t.device))
         if t.dtype not in _lib.DTYPES:
             raise ValueError('KeyValueCache takes float16, bfloat16 and float32 (got %s)' % t.dtype)
-        if tuple(t.shape) != (tokens, self.heads, self.head_dim):
+        if t.shape != (tokens, self.heads, self.head_dim):
             raise ValueError('%s must be %s (got %s)' % (name, [tokens, self.heads, self.head_dim], list(t.shape)))
-        t = t.detach()
-        unit = 16 // t.element_size()
-        if t.stride(2) != 1 or (t.size(0) > 1 and t.stride(0) % unit) or (t.size(1) > 1 and t.stride(1) % unit) or t.data_ptr() % 16:
-            t = t.clone(memory_format=torch.contiguous_format)
-        return t, (t.stride(0) if t.size(0) > 1 else 0), (t.stride(1) if t.size(1) > 1 else 0)
+        unit, (row, head, one) = 16 // t.element_size(), t.stride()
+        if one != 1 or (tokens > 1 and row % unit) or (self.heads > 1 and head % unit) or t.data_ptr() % 16:
+            t = t.detach().clone(memory_format=torch.contiguous_format)
+            row, head, one = t.stride()
+        return t, (row if tokens > 1 else 0), (head if self.heads > 1 else 0)
 
     def write(self, k, v, slots, rotation=None, positions=None):
         """Quantises k and v [tokens, heads, head_dim] (of one type) into positions slots[t] = page * block + offset of the cache.  Tokens with a
@@ -126,7 +126,8 @@ class KeyValueCache(Pages):
         slots = self._check_slots(slots)
         if dtype not in _lib.DTYPES:
             raise ValueError('KeyValueCache gives float16, bfloat16 and float32 (got %s)' % dtype)
-        k, v = [torch.empty((slots.numel(), self.heads, self.head_dim), dtype=dtype, device=self.device) for _ in range(2)]
+        k = torch.empty((slots.numel(), self.heads, self.head_dim), dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
         if slots.numel():
             with _lib.on_device(self.device):
                 stream = _lib.raw_stream(self.device)

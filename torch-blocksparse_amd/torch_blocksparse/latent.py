@@ -45,12 +45,13 @@ class LatentCache(Pages):
     def _operand(self, t, name, tokens, elements):
         if t.device != self.device:
             raise _lib.BlocksparseLibraryError('torch_blocksparse: %s must live on %s (got device %s)' % (name, self.device, t.device))
-        if t.dtype != self.dtype or tuple(t.shape) != (tokens, elements):
+        if t.dtype != self.dtype or t.shape != (tokens, elements):
             raise ValueError('%s must be %s %s (got %s %s)' % (name, self.dtype, [tokens, elements], t.dtype, list(t.shape)))
-        t = t.detach()
-        if t.stride(1) != 1 or (tokens > 1 and t.stride(0) % 8) or t.data_ptr() % 16:
-            t = t.clone(memory_format=torch.contiguous_format)
-        return t, (t.stride(0) if tokens > 1 else 0)
+        row, one = t.stride()
+        if one != 1 or (tokens > 1 and row % 8) or t.data_ptr() % 16:
+            t = t.detach().clone(memory_format=torch.contiguous_format)
+            row = elements
+        return t, (row if tokens > 1 else 0)
 
     def write(self, c, r, slots, rotation=None, positions=None):
         """Puts c [tokens, latent] and r [tokens, 64] (of the cache's type) at positions slots[t] = page * block + offset, int32.  Tokens with a negative slot, or one past the
@@ -150,7 +151,20 @@ class LatentAttention:
             made[2].table(made[0])
         return made
 
-    def _check(self, q, q_r, cache, table, lengths, scale, softcap, slopes):
+    def _fits(self, q, q_r, cache, table, lengths, slopes):
+        """whether _refuse has nothing to say of the operands, in as few steps as it takes"""
+        if not isinstance(cache, LatentCache):
+            return False
+        device, dtype, shape, pages = cache.device, cache.dtype, q.shape, table.shape
+        if len(shape) != 3 or len(pages) != 2:
+            return False
+        B, H, D = shape
+        return (q.device == device and q_r.device == device and table.device == device and lengths.device == device and q.dtype is dtype and q_r.dtype is dtype and
+                table.dtype is torch.int32 and lengths.dtype is torch.int32 and cache.block == self.block and D == cache.latent and q_r.shape == (B, H, SHARED) and 0 < H and B * H < 1 << 24 and
+                (self.layout is None or self.layout.shape[0] == H) and pages[0] == B and 0 < pages[1] * self.block < 1 << 24 and lengths.shape == (B,) and
+                (slopes is None or (slopes.shape == (H,) and slopes.dtype is torch.float32 and slopes.device == device)))
+
+    def _refuse(self, q, q_r, cache, table, lengths, slopes):
         if not isinstance(cache, LatentCache):
             raise ValueError('LatentAttention reads a LatentCache (got %s)' % type(cache).__name__)
         for name, t in (('q', q), ('q_r', q_r)):
@@ -174,44 +188,51 @@ class LatentAttention:
         for name, t, shape, dtype in (('lengths', lengths, (B,), torch.int32), ('slopes', slopes, (H,), torch.float32)):
             if (t is not None or name == 'lengths') and (tuple(t.shape) != shape or t.dtype != dtype or t.device != q.device):
                 raise ValueError('%s must be %s %s on %s (got %s %s on %s)' % (name, dtype, list(shape), q.device, t.dtype, list(t.shape), t.device))
+
+    def _check(self, q, q_r, cache, table, lengths, scale, softcap, slopes):
+        if not self._fits(q, q_r, cache, table, lengths, slopes):
+            self._refuse(q, q_r, cache, table, lengths, slopes)
         check_scores(scale, softcap)
 
     @staticmethod
     def _operand(t):
-        B, H = t.shape[:2]
-        if t.stride(2) != 1 or (B > 1 and t.stride(0) % 8) or (H > 1 and t.stride(1) % 8) or t.data_ptr() % 16:
-            t = t.clone(memory_format=torch.contiguous_format)
-        return t, (t.stride(0) if B > 1 else 0), (t.stride(1) if H > 1 else 0)
+        (B, H, _), (b, h, one) = t.shape, t.stride()
+        if one != 1 or (B > 1 and b % 8) or (H > 1 and h % 8) or t.data_ptr() % 16:
+            t = t.detach().clone(memory_format=torch.contiguous_format)
+            b, h, one = t.stride()
+        return t, (b if B > 1 else 0), (h if H > 1 else 0)
 
     def __call__(self, q, q_r, cache, table, lengths, scale=1., softcap=0., slopes=None):
         scale, softcap = float(scale), float(softcap or 0.)
         self._check(q, q_r, cache, table, lengths, scale, softcap, slopes)
         B, H, D = q.shape
-        q, q_r = q.detach(), q_r.detach()
-        o = torch.empty((B, H, D), dtype=q.dtype, device=q.device)
+        device = cache.device
+        o = torch.empty_like(q, memory_format=torch.contiguous_format)
         if B == 0:
             return o
         (q, q_sb, q_sh), (q_r, r_sb, r_sh) = self._operand(q), self._operand(q_r)
-        if table.size(1) > 1 and table.stride(1) != 1:
+        width, (next_row, one) = table.shape[1], table.stride()
+        if width > 1 and one != 1:
             table = table.contiguous()
+            next_row = width
         lengths = lengths.contiguous()
         slopes = slopes.detach().contiguous() if slopes is not None else None
         lib = _lib.load()
-        with _lib.on_device(q.device):
-            stream = _lib.raw_stream(q.device)
+        with _lib.on_device(device):
+            stream = _lib.raw_stream(device)
             if stream not in cache._users.streams:
-                cache._users.read(q.device)
-            rows, blocks, n_rows = None, table.size(1), 0
+                cache._users.read(device)
+            rows, blocks, n_rows = None, width, 0
             if self.layout is not None:
-                rows, longest, readers = self._table(q.device)
+                rows, longest, readers = self._table(device)
                 if stream not in readers.streams:
-                    readers.read(q.device)
-                n_rows = self.layout.size(1)
+                    readers.read(device)
+                n_rows = self.layout.shape[1]
                 blocks = max(1, longest[min(blocks, n_rows) - 1])
             need = lib.bsp_latent_attention_workspace_bytes(B, H, D, self.block, blocks)
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
             rc = lib.bsp_latent_attention(_lib.DTYPES[q.dtype], q.data_ptr(), q_sb, q_sh, q_r.data_ptr(), r_sb, r_sh, o.data_ptr(), H * D, D, B, H, cache.data.data_ptr(), cache.pages,
-                                          self.block, D, table.data_ptr(), table.stride(0) if B > 1 else 0, table.size(1), lengths.data_ptr(), rows.data_ptr() if rows is not None else None,
+                                          self.block, D, table.data_ptr(), next_row if B > 1 else 0, width, lengths.data_ptr(), rows.data_ptr() if rows is not None else None,
                                           n_rows, blocks, scale, softcap, slopes.data_ptr() if slopes is not None else None, workspace.data_ptr(), need, stream)
         _lib.check(rc, 'bsp_latent_attention')
         return o

@@ -149,7 +149,7 @@ class Rotation:
         Z, L, D = (1, shape[0], shape[2]) if len(shape) == 3 else (shape[0], shape[2], shape[3])
         out, args, live = [], [], 0
         for t in tensors:
-            y = torch.empty(t.shape, dtype=t.dtype, device=device)
+            y = torch.empty_like(t, memory_format=torch.contiguous_format)
             out.append(y)
             if t.numel():
                 H = t.shape[1]

@@ -178,9 +178,9 @@ class _rules(torch.autograd.Function):
         kv, device = k.size(1), q.device
         (q, q_at), (k, k_at), (v, v_at) = _operand(q, Z, H, L, D), _operand(k, Z, kv, L, D), _operand(v, Z, kv, L, D)
         keep = grad_enabled and any(ctx.needs_input_grad[:3])
-        o = torch.empty((Z, H, L, D), dtype=q.dtype, device=device)
+        o = torch.empty_like(q, memory_format=torch.contiguous_format)
         stats = torch.empty((Z, H, 2, 64 * tables.lines), dtype=torch.float32, device=device) if keep else None
-        rest = torch.empty((Z, H, L, D), dtype=q.dtype, device=device) if keep and q.element_size() == 2 else None
+        rest = torch.empty_like(q, memory_format=torch.contiguous_format) if keep and q.element_size() == 2 else None
         ranges = torch.empty((Z, (L + 15) // 16, 2), dtype=torch.int32, device=device) if documents is not None else None
         call = _rules.call(q, kv, q_at + k_at + v_at + _own(Z, H, L, D) + (0,) * 12, tables, scale, softcap, slopes, causal, documents, prefix, ranges, stats, rest)
         rc = _lib.load().bsp_attention_rules_fwd(call, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _lib.raw_stream(device))
@@ -210,11 +210,11 @@ class _rules(torch.autograd.Function):
             # (what was saved may have been elsewhere in between and have come back in other strides)
             (q, q_at), (k, k_at), (v, v_at) = _operand(q, Z, H, L, D), _operand(k, Z, kv, L, D), _operand(v, Z, kv, L, D)
             (o, o_at), (do, do_at) = _operand(o, Z, H, L, D), _operand(do, Z, H, L, D)
-            dq, dk, dv = torch.empty((Z, H, L, D), dtype=dtype, device=device), None, None
+            dq, dk, dv = torch.empty_like(q, memory_format=torch.contiguous_format), None, None
             delta = torch.empty((Z, H, 64 * tables.lines), dtype=torch.float32, device=device)
             items, n_items, splits, n_splits, slots, partial = None, 0, None, 0, 0, None
             if need_k or need_v:
-                dk, dv = torch.empty((Z, kv, L, D), dtype=dtype, device=device), torch.empty((Z, kv, L, D), dtype=dtype, device=device)
+                dk, dv = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in (k, v)]
                 items, n_items, splits, n_splits, slots = tables.columns(kv, Z)
                 partial = torch.empty((Z, slots, 2, 64, D), dtype=torch.float32, device=device) if slots else None
             own = _own(Z, kv, L, D)
@@ -248,9 +248,9 @@ class _shared_rules(torch.autograd.Function):
         own_k_s = k_s
         q_s, qs_at, k_s, ks_at = _shared_rules._parts(q_s, k_s)
         keep = grad_enabled and any(ctx.needs_input_grad[:5])
-        o = torch.empty((Z, H, L, D), dtype=q.dtype, device=device)
+        o = torch.empty_like(q, memory_format=torch.contiguous_format)
         stats = torch.empty((Z, H, 2, 64 * tables.lines), dtype=torch.float32, device=device) if keep else None
-        rest = torch.empty((Z, H, L, D), dtype=q.dtype, device=device) if keep and q.element_size() == 2 else None
+        rest = torch.empty_like(q, memory_format=torch.contiguous_format) if keep and q.element_size() == 2 else None
         ranges = torch.empty((Z, (L + 15) // 16, 2), dtype=torch.int32, device=device) if documents is not None else None
         call = _rules.call(q, kv, q_at + k_at + v_at + _own(Z, H, L, D) + (0,) * 12, tables, scale, softcap, slopes, causal, documents, prefix, ranges, stats, rest)
         part = _PART.pack(q_s.data_ptr(), k_s.data_ptr(), *qs_at, *ks_at, 0, 0, 0, 0, 0, 0, 0, 0)
@@ -275,12 +275,12 @@ class _shared_rules(torch.autograd.Function):
             (q, q_at), (k, k_at), (v, v_at) = _operand(q, Z, H, L, D), _operand(k, Z, kv, L, D), _operand(v, Z, kv, L, D)
             (o, o_at), (do, do_at) = _operand(o, Z, H, L, D), _operand(do, Z, H, L, D)
             q_s, qs_at, k_s, ks_at = _shared_rules._parts(q_s, k_s)
-            dq, dq_s = [torch.empty((Z, H, L, n), dtype=dtype, device=device) for n in (D, SHARED)]
+            dq, dq_s = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, q_s)]
             dk = dv = dk_s = heads = None
             delta = torch.empty((Z, H, 64 * tables.lines), dtype=torch.float32, device=device)
             items, n_items, splits, n_splits, slots, partial = None, 0, None, 0, 0, None
             if need[1] or need[2] or need[4]:
-                dk, dv = [torch.empty((Z, kv, L, D), dtype=dtype, device=device) for _ in range(2)]
+                dk, dv = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in (k, v)]
                 dk_s, heads = torch.empty((Z, L, SHARED), dtype=dtype, device=device), torch.empty((Z, kv, L, SHARED), dtype=torch.float32, device=device)
                 items, n_items, splits, n_splits, slots = tables.columns(kv, Z)
                 partial = torch.empty((Z, slots, 64, 2 * D + SHARED), dtype=torch.float32, device=device) if slots else None
