@@ -248,6 +248,35 @@ __device__ __forceinline__ void columns_times_exact(f32x16 (&acc)[D / 32], const
   }
 }
 
+// Products whose operands are read A ahead of the one that is taken.  Left alone, the compiler reads one or two and waits for them, to save registers.  begin: the first reads, which may go well ahead
+// of run.  Taken with a shared part and 128 elements in 16-bit types (reads_ahead; fewer elements have no registers left at three wavefronts a SIMD, fp32 none at one), bf16, without and with: forward, 16 heads x 2048
+// causal 51.8 and 47.1 us, x 8192 409 and 406, documents 2 x 16 x 4001 80.9 and 76.8; rows of the backward pass, documents, 210 and 201.
+template <typename T, int D, int X> constexpr bool reads_ahead() { return X && D == 128 && sizeof(T) == 2; }
+template <typename F, int N, int A> struct Ahead {
+  F f[A + 1];
+  template <class R> __device__ __forceinline__ void begin(R &&read) {
+#pragma unroll
+    for (int i = 0; i < A && i < N; i++) f[i] = read(i);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  template <class R, class P> __device__ __forceinline__ void run(R &&read, P &&product) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      if (i + A < N) f[(i + A) % (A + 1)] = read(i + A);
+      __builtin_amdgcn_sched_barrier(0);
+      product(i, f[i % (A + 1)]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+};
+// Fragment i of a piece transposed, for 32 columns and half of the rows each: all columns of the first half of the rows, then of the other
+template <typename T, int D, int OFF, bool LEAN> __device__ __forceinline__ typename RuleOperand<T>::type column_fragment(const PieceReads<T, D, LEAN> &reads, int i) {
+  uint32_t lo[D / 32], hi[D / 32];
+  reads.tr.get(lo, hi);
+  const int mt = i % (D / 32), ks = i / (D / 32);
+  return tr_fragment<T>(lo[mt] + OFF + ks * (16 * 2 * D), hi[mt] + OFF + (LEAN ? 4 * 2 * D : 0) + ks * (16 * 2 * D));
+}
+
 // Capped scores.  With x = scale * s / cap, tanh(x) = 1 - 2 r and 1 - tanh(x)^2 = 4 (r - r^2), r = 1 / (exp(2 x) + 1): the kernels for 16-bit
 // types keep r, whose error of 2^-24 cap * log2 e takes to the logit: little beside what the operands' rounding leaves of it.  In fp32 they keep
 // the tanh, from its series where x is small (in trained models nearly everywhere) with its relative precision: up to x = 0.45 the

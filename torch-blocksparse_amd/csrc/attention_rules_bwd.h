@@ -145,9 +145,32 @@ __global__ void __launch_bounds__(128 * PAIRS, (row_waves<T, D, X, CAP>())) k_ru
         whole = __builtin_amdgcn_ballot_w64(seen != 0xffffu) == 0;
       }
       if (some) {
-        f32x16 s = rows_times<T, D, S * Ring::STAGE, false>(reads, xq, zeros16());
-        if constexpr (X) s = rows_times<T, SX, S * Ring::STAGE + Ring::THIRD, false>(readsx, xqx, s);
-        const f32x16 dp = rows_times<T, D, S * Ring::STAGE + Q::PIECE, false>(reads, xo, zeros16());
+        constexpr bool AHEAD = reads_ahead<T, D, X>();
+        constexpr int NF = Q::NF, NX = X ? Geo<T, SX>::NF : 0, K0 = S * Ring::STAGE, V0 = K0 + Q::PIECE, X0 = K0 + Ring::THIRD;
+        typedef typename RuleOperand<T>::type frag;
+        f32x16 s = zeros16(), dp = zeros16();
+        Ahead<frag, 2 * (MT + XT), 6> columns;
+        auto column = [&](int i) {
+          if constexpr (AHEAD) return i < 2 * MT ? column_fragment<T, D, K0, false>(reads, i) : column_fragment<T, SX, X0, false>(readsx, i - 2 * MT);
+          else return frag();
+        };
+        if constexpr (AHEAD) {
+          Ahead<frag, 2 * NF + NX, 6> rows;
+          auto fragment = [&](int i) {
+            return i < NF ? row_fragment<T, D, K0, false>(reads, i) : i < NF + NX ? row_fragment<T, SX, X0, false>(readsx, i - NF) : row_fragment<T, D, V0, false>(reads, i - NF - NX);
+          };
+          rows.begin(fragment);
+          rows.run(fragment, [&](int i, const frag &f) {
+            if (i < NF) s = fragment_times<T>(f, xq[i], s);
+            else if (i < NF + NX) s = fragment_times<T>(f, xqx[i - NF], s);
+            else dp = fragment_times<T>(f, xo[i - NF - NX], dp);
+          });
+          columns.begin(column);
+        } else {
+          s = rows_times<T, D, K0, false>(reads, xq, s);
+          if constexpr (X) s = rows_times<T, SX, X0, false>(readsx, xqx, s);
+          dp = rows_times<T, D, V0, false>(reads, xo, dp);
+        }
         const Logits<BIAS> logits(row - cur.lo - 8 * half, row - cur.hi - 8 * half, slope);
         if constexpr (CAP)
 #pragma unroll
@@ -174,13 +197,22 @@ __global__ void __launch_bounds__(128 * PAIRS, (row_waves<T, D, X, CAP>())) k_ru
         if constexpr (FINE) {
           Shares<T> most, rest;
           two_terms<T>(e, most, rest);
-          columns_times_exact<T, D, S * Ring::STAGE, false>(dq, reads, most, rest);
-          if constexpr (X) columns_times_exact<T, SX, S * Ring::STAGE + Ring::THIRD, false>(dqx, readsx, most, rest);
+          if constexpr (AHEAD) {
+            columns.run(column, [&](int i, const frag &f) {
+              const int ks = i < 2 * MT ? i / MT : (i - 2 * MT) / XT;
+              f32x16 &to = i < 2 * MT ? dq[i % MT] : dqx[(i - 2 * MT) % XT];
+              to = Mma<T, 32>::run(f, most.f[ks], to);
+              to = Mma<T, 32>::run(f, rest.f[ks], to);
+            });
+          } else {
+            columns_times_exact<T, D, K0, false>(dq, reads, most, rest);
+            if constexpr (X) columns_times_exact<T, SX, X0, false>(dqx, readsx, most, rest);
+          }
         } else {
           Shares<T> ds;
           ds.set(e);
-          columns_times<T, D, S * Ring::STAGE, false>(dq, reads, ds);
-          if constexpr (X) columns_times<T, SX, S * Ring::STAGE + Ring::THIRD, false>(dqx, readsx, ds);
+          columns_times<T, D, K0, false>(dq, reads, ds);
+          if constexpr (X) columns_times<T, SX, X0, false>(dqx, readsx, ds);
         }
       }
       halves = nxt;

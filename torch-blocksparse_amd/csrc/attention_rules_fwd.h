@@ -112,8 +112,25 @@ __global__ void __launch_bounds__(128 * PAIRS, (fwd_waves<T, D, X, BIAS, DOCS>()
         whole = __builtin_amdgcn_ballot_w64(seen != 0xffffu) == 0;
       }
       if (some) {
-        f32x16 s = rows_times<T, D, S * Ring::STAGE, false>(reads, xq, zeros16());
-        if constexpr (X) s = rows_times<T, SX, S * Ring::STAGE + Ring::THIRD, false>(readsx, xqx, s);
+        constexpr int NF = Q::NF, NX = X ? Geo<T, SX>::NF : 0, K0 = S * Ring::STAGE, V0 = K0 + Q::PIECE, X0 = K0 + Ring::THIRD;
+        constexpr bool AHEAD = reads_ahead<T, D, X>();
+        typedef typename RuleOperand<T>::type frag;
+        f32x16 s = zeros16();
+        Ahead<frag, 2 * MT, 3> columns;
+        auto column = [&](int i) {
+          if constexpr (AHEAD) return column_fragment<T, D, V0, false>(reads, i);
+          else return frag();
+        };
+        if constexpr (AHEAD) {
+          Ahead<frag, NF + NX, 5> rows;
+          auto fragment = [&](int i) { return i < NF ? row_fragment<T, D, K0, false>(reads, i) : row_fragment<T, SX, X0, false>(readsx, i - NF); };
+          rows.begin(fragment);
+          rows.run(fragment, [&](int i, const frag &f) { s = fragment_times<T>(f, i < NF ? xq[i] : xqx[i - NF], s); });
+          columns.begin(column);
+        } else {
+          s = rows_times<T, D, K0, false>(reads, xq, s);
+          if constexpr (X) s = rows_times<T, SX, X0, false>(readsx, xqx, s);
+        }
         if constexpr (CAP)
 #pragma unroll
           for (int i = 0; i < 16; i++) s[i] = cap_score<T>(s[i], in);
@@ -146,7 +163,8 @@ __global__ void __launch_bounds__(128 * PAIRS, (fwd_waves<T, D, X, BIAS, DOCS>()
         l += sum;
         Shares<T> p;
         p.set(e);
-        columns_times<T, D, S * Ring::STAGE + Q::PIECE, false>(o, reads, p);
+        if constexpr (AHEAD) columns.run(column, [&](int i, const frag &f) { o[i % MT] = Mma<T, 32>::run(f, p.f[i / MT], o[i % MT]); });
+        else columns_times<T, D, V0, false>(o, reads, p);
       }
       halves = nxt;
       return halves.more;
