@@ -250,7 +250,7 @@ __device__ __forceinline__ void columns_times_exact(f32x16 (&acc)[D / 32], const
 
 // Products whose operands are read A ahead of the one that is taken.  Left alone, the compiler reads one or two and waits for them, to save registers.  begin: the first reads, which may go well ahead
 // of run.  Taken with a shared part and 128 elements in 16-bit types (reads_ahead; fewer elements have no registers left at three wavefronts a SIMD, fp32 none at one), bf16, without and with: forward, 16 heads x 2048
-// causal 51.8 and 47.1 us, x 8192 409 and 406, documents 2 x 16 x 4001 80.9 and 76.8; rows of the backward pass, documents, 210 and 201.
+// causal 51.8 and 47.1 us, x 8192 409 and 406, documents 2 x 16 x 4001 80.9 and 76.8; backward pass, 2 x 16 x 4001 in five documents, rows 210 and 201, columns 217 and 208.
 template <typename T, int D, int X> constexpr bool reads_ahead() { return X && D == 128 && sizeof(T) == 2; }
 template <typename F, int N, int A> struct Ahead {
   F f[A + 1];

@@ -424,8 +424,31 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, X, CAP>())) k_rules_bwd_
       }
       if (some) {
         const bool factors = __builtin_amdgcn_ballot_w64(stat[32 + l32] != 1.f) != 0;
-        f32x16 s = rows_times<T, D, Q0, LEAN>(reads, xk, zeros16());
-        if constexpr (X) s = rows_times<T, SX, X0, LEAN>(readsx, xkx, s);
+        constexpr bool AHEAD = reads_ahead<T, D, X>();
+        constexpr int NF = Q::NF, NX = X ? Geo<T, SX>::NF : 0;
+        typedef typename RuleOperand<T>::type frag;
+        f32x16 s = zeros16();
+        // of the products p^T . do and do . v^T, then of e^T . q
+        Ahead<frag, 2 * MT + NF, 6> of_do;
+        Ahead<frag, 2 * (MT + XT), 6> of_q;
+        auto do_fragment = [&](int i) {
+          if constexpr (AHEAD) return i < 2 * MT ? column_fragment<T, D, O0, LEAN>(reads, i) : row_fragment<T, D, O0, LEAN>(reads, i - 2 * MT);
+          else return frag();
+        };
+        auto q_fragment = [&](int i) {
+          if constexpr (AHEAD) return i < 2 * MT ? column_fragment<T, D, Q0, LEAN>(reads, i) : column_fragment<T, SX, X0, LEAN>(readsx, i - 2 * MT);
+          else return frag();
+        };
+        if constexpr (AHEAD) {
+          Ahead<frag, NF + NX, 6> rows;
+          auto fragment = [&](int i) { return i < NF ? row_fragment<T, D, Q0, LEAN>(reads, i) : row_fragment<T, SX, X0, LEAN>(readsx, i - NF); };
+          rows.begin(fragment);
+          rows.run(fragment, [&](int i, const frag &f) { s = fragment_times<T>(f, i < NF ? xk[i] : xkx[i - NF], s); });
+          of_do.begin(do_fragment);
+        } else {
+          s = rows_times<T, D, Q0, LEAN>(reads, xk, s);
+          if constexpr (X) s = rows_times<T, SX, X0, LEAN>(readsx, xkx, s);
+        }
         float slope_lo = 0.f, slope_hi = 0.f;
         if constexpr (BIAS) {
           slope_lo = as_floats(slopes)[cur.lo >> kHeadShift] * kLog2e;
@@ -457,7 +480,7 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, X, CAP>())) k_rules_bwd_
           for_16<0>([&](auto ic) { p[decltype(ic)::value] = keep(p[decltype(ic)::value], bit_mask<decltype(ic)::value>(seen)); });
         Shares<T> share;
         share.set(p);
-        columns_times<T, D, O0, LEAN>(dv, reads, share);
+        if constexpr (!AHEAD) columns_times<T, D, O0, LEAN>(dv, reads, share);
         f32x16 dp;
 #pragma unroll
         for (int g = 0; g < 4; g++) {
@@ -465,7 +488,15 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, X, CAP>())) k_rules_bwd_
 #pragma unroll
           for (int j = 0; j < 4; j++) dp[4 * g + j] = nd[j];
         }
-        dp = rows_times<T, D, O0, LEAN>(reads, xv, dp);
+        if constexpr (AHEAD) {
+          of_do.run(do_fragment, [&](int i, const frag &f) {
+            if (i < 2 * MT) dv[i % MT] = Mma<T, 32>::run(f, share.f[i / MT], dv[i % MT]);
+            else dp = fragment_times<T>(f, xv[i - 2 * MT], dp);
+          });
+          of_q.begin(q_fragment);
+        } else {
+          dp = rows_times<T, D, O0, LEAN>(reads, xv, dp);
+        }
 #pragma unroll
         for (int i = 0; i < 16; i++) {
           e[i] = p[i] * dp[i];
@@ -474,8 +505,15 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, X, CAP>())) k_rules_bwd_
         if (!whole)
           for_16<0>([&](auto ic) { e[decltype(ic)::value] = keep(e[decltype(ic)::value], bit_mask<decltype(ic)::value>(seen)); });
         share.set(e);
-        columns_times<T, D, Q0, LEAN>(dk, reads, share);
-        if constexpr (X) columns_times<T, SX, X0, LEAN>(dkx, readsx, share);
+        if constexpr (AHEAD) {
+          of_q.run(q_fragment, [&](int i, const frag &f) {
+            f32x16 &to = i < 2 * MT ? dk[i % MT] : dkx[(i - 2 * MT) % XT];
+            to = Mma<T, 32>::run(f, share.f[i < 2 * MT ? i / MT : (i - 2 * MT) / XT], to);
+          });
+        } else {
+          columns_times<T, D, Q0, LEAN>(dk, reads, share);
+          if constexpr (X) columns_times<T, SX, X0, LEAN>(dkx, readsx, share);
+        }
       }
       cur = nxt;
       return cur.n >= 0;
