@@ -14,13 +14,13 @@
 // All steps of all sequences are one row of work that is cut into equal pieces, one a workgroup, so that uneven lengths leave no compute unit idle: a workgroup finds its piece by
 // a sum over the lengths.  A sequence that lies in several pieces is joined by a second kernel.
 //
-// Measured, latent vectors of 512, bf16: 16 sequences of up to 16384 positions (151 MB of pages) with 16 heads 52 us (3.8 TB/s; the join among them), 32 59, 64 66, 128 heads 95 and 9.6 for the join (47
-// GFLOP; 480 TFLOP/s).  16 heads are bound by the loads of a workgroup that has one step's on its way.  64 and more: of 200000 cycles a workgroup half of the products' reads from LDS (17.5 MB a compute
-// unit, 137000 cycles at 128 bytes a clock) and products (45000) overlap, the rest is a step's exponentials between them and a piece's ends: queries, sums written (33 MB, read back by the
+// Measured, latent vectors of 512, bf16: 16 sequences of up to 16384 positions (151 MB of pages) with 16 heads 52 us (3.8 TB/s; the join among them), 32 59, 64 72, 128 heads 109, 9.6 of them the join (47
+// GFLOP; 435 TFLOP/s).  16 heads are bound by the loads of a workgroup that has one step's on its way.  64 and more: of 240000 cycles a workgroup the products' reads from LDS (17.5 MB a compute
+// unit, 137000 cycles at 128 bytes a clock) and products (66000) overlap in part, the rest is a step's exponentials between them and a piece's ends: queries, sums written (33 MB, read back by the
 // join), the search for the piece.  Shorter: 16 x 16 heads over up to 4096 positions with a layout, fp16, 15 and 4 us; one sequence of 33 positions 10.8.
 //
 // Wavefronts of 32 heads, two for the same heads, on 32 x 32 x 16 products take half of the reads from LDS, but exchange shares and wait for each other in every step: 128 heads 117 us, 64 85 where this
-// takes 98 and 66.
+// takes 98 and 66, all of it with shares in one term.
 #include "attention_common.h"
 #include "latent.h"
 
@@ -118,8 +118,9 @@ __device__ __forceinline__ uint32_t first_of_four(int n) { return (1u << (n < 0 
 // The operands of both products come from LDS a batch of four reads at a time while the products of batches before are taken; left alone, the compiler reads one and waits for it, to save registers.  Every
 // batch also issues its part of the next step's loads (load(k)): all at once they would hold up the wavefront for the time that a compute unit takes for them, 64 bytes a clock.
 //
-// Sixteen heads a wavefront, each wavefront HW of a step's groups.  Shares in two terms up to 32 heads: what they are rounded to and what that leaves out; past that, where products and their operands are what
-// counts, in one, which takes a sum's error from that of the result's rounding to 1.4 times that at most (128 heads 109 us with the second term, 98 without; 64 72 and 66; bf16 errors of 1.7 and 1.9 in 1000). The chunks of a latent vector in LDS: every row
+// Sixteen heads a wavefront, each wavefront HW of a step's groups.  Shares go into the product in two terms, what they are rounded to and what that leaves out: with the first alone a sum is off by half a step
+// of the type times the sum of its terms' sizes, which nothing bounds where latent vectors cancel (128 heads 98 us with the first alone, 109 with both, 64 65 and 72; errors against 64 bits 1.94 and 1.65 in 1000 in bf16, 2.3 and 2.1 in 10000 in fp16, where
+// rounding the results alone is the second).  The chunks of a latent vector in LDS: every row
 // begins in the first bank, so pairs of chunks of 256 bytes are exchanged by the row's number, which serves both reads without a conflict: a transposing read takes a pair from each of
 // eight rows at a time, a read along the rows a chunk of eight rows and its neighbour of the eight others.
 template <typename T, int LAT, int HW> struct Heads {
@@ -129,7 +130,7 @@ template <typename T, int LAT, int HW> struct Heads {
   typedef typename std::conditional<HW == 1, typename M::frag4, frag8>::type frag;
   static constexpr int GROUPS = HW, SOURCES = 4 / HW, NS = LAT / 32, NR = kRope / 32, NT = LAT / 16;
   static constexpr int EXTRA = 4;                       // steps that going over to another item takes as long as
-  static constexpr bool BARRIER = HW > 1, TWO_TERMS = HW < 4;
+  static constexpr bool BARRIER = HW > 1;
   static __device__ __forceinline__ uint32_t chunk(uint32_t c, uint32_t r) { return c ^ (r & 7) << 1; }
   static __device__ __forceinline__ int first_group(int wave) { return wave / HW * HW; }
   static __device__ __forceinline__ int head_of(int wave, int lane) { return 16 * (wave % HW) + (lane & 15); }
@@ -281,11 +282,11 @@ template <typename T, int LAT, int HW> struct Heads {
       return false;
     }
     l += sum;
-    frag most[PAIRS], rest[TWO_TERMS ? PAIRS : 1];
+    frag most[PAIRS], rest[PAIRS];
 #pragma unroll
     for (int i = 0; i < 4 * HW; i++) {
       most[i / PER][i % PER] = from_float<T>(e[i]);
-      if constexpr (TWO_TERMS) rest[i / PER][i % PER] = from_float<T>(e[i] - to_float(most[i / PER][i % PER]));
+      rest[i / PER][i % PER] = from_float<T>(e[i] - to_float(most[i / PER][i % PER]));
     }
 #pragma unroll
     for (int b = 0; b < PAIRS * NB; b++) {
@@ -293,9 +294,8 @@ template <typename T, int LAT, int HW> struct Heads {
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int j = 0; j < 4; j++) o[b % NB * 4 + j] = M::run(cols[b % 3][j], most[b / NB], o[b % NB * 4 + j]);
-      if constexpr (TWO_TERMS)
 #pragma unroll
-        for (int j = 0; j < 4; j++) o[b % NB * 4 + j] = M::run(cols[b % 3][j], rest[b / NB], o[b % NB * 4 + j]);
+      for (int j = 0; j < 4; j++) o[b % NB * 4 + j] = M::run(cols[b % 3][j], rest[b / NB], o[b % NB * 4 + j]);
       __builtin_amdgcn_sched_barrier(0);
     }
     return true;
@@ -350,9 +350,9 @@ __global__ void __launch_bounds__(256, 1) k_latent_attention(LatentArgs a) {
   const uint32_t items = (uint32_t)(a.B * a.units), ring = (uint32_t)(uintptr_t)BSP_LDS_PTR(smem);
 
   // The workgroup's piece [lo, hi) of all steps, and the item that it begins in.  Where there are more steps than pieces, an item counts `extra` steps more ahead of its own: what a
-  // workgroup that goes over to another item spends on the queries and on the sums of the last (16 x 64 heads over up to 16384 positions: 76 us without, 66 with; 128 x 128 heads over up to 500:
-  // 85 and 62; 300 x 16 over up to 600: 61 and 46; two or eight steps instead of four: 72 and 66, 63 and 59).  With a step or less a piece they would only leave pieces empty: 4 x 128 heads over up to 300,
-  // 24 us with them, 21 without.
+  // workgroup that goes over to another item spends on the queries and on the sums of the last (16 x 64 heads over up to 16384 positions: 81 us without, 72 with; 128 x 128 heads over up to 500:
+  // 87 and 65; 300 x 16 over up to 600: 61 and 46; two or eight steps instead of four: 76 and 72, 67 and 62).  With a step or less a piece they would only leave pieces empty: 4 x 128 heads over up to 300,
+  // 25 us with them, 21 without.
   int64_t total = 0, lo, hi, begin = 0;
   uint32_t item = 0;
   LatentItem found{}, looked{};                         // that item; what the thread has looked at last

@@ -126,7 +126,7 @@ class LatentAttention:
     over j < n = lengths[b], with a layout those in blocks that row (n - 1) // block of head h has.  A page number outside the cache (-1, say) stands for a page that is not
     held: its positions are not seen.  A sequence of length 0, or one that sees nothing, gets zeros.  Lengths count as at most width * block and as at most the
     layout's positions.  A NaN or an infinity in a latent vector that one head sees can reach the others of its sequence.  Sums and shares are fp32; a share is an operand of a product in two
-    terms of the cache's type, past 32 heads in one.  No gradient.
+    terms of the cache's type.  No gradient.
 
     With a layout a table is made at the first call on a device, so a call that is captured into a graph needs one like it before."""
 
