@@ -188,7 +188,7 @@ __device__ __forceinline__ f32x16 zeros16() {
 }
 
 // Sixteen values a lane, one per row of a piece as rows_times deals them, as the operand of columns_times: rounded to the
-// operands' type (the products take no other; the two-term form that loses nothing is twice the products), in fp32 as they are.  The forward pass has its shares
+// operands' type (the products take no other; the two-term form that loses nothing is twice the products: in_two_terms), in fp32 as they are.  The forward pass has its shares
 // relative to the running maximum, the backward pass normalised ones: in fp16 those below 2^-14 are off by up to 2^-25, as every fp16 number.
 template <typename T> struct Shares {
   typename Mma<T, 32>::frag_t f[2];
@@ -248,9 +248,14 @@ __device__ __forceinline__ void columns_times_exact(f32x16 (&acc)[D / 32], const
   }
 }
 
+// With a shared part every operand that a kernel rounds itself goes into its product in two terms (16-bit types), so that results are as exact as of products in fp32, rounded once.  In one term (with which the
+// kernels without a shared part take the shares of o and dv and the score gradients of dk) errors against 64 bits are, bf16 of 128 elements, 2.1 to 2.3 in 1000 of o, 2.3 of dk, dv and the shared
+// part's, in two 1.65 of each; fp16 2.3 to 3.0 and 2.05 in 10000.  It costs, 16 heads x 8192 causal forward 405 -> 505 us, 2 x 16 x 4001 in five documents forward 121 -> 135, columns 208 -> 252.
+template <typename T, int X> constexpr bool in_two_terms() { return X && sizeof(T) == 2; }
+
 // Products whose operands are read A ahead of the one that is taken.  Left alone, the compiler reads one or two and waits for them, to save registers.  begin: the first reads, which may go well ahead
 // of run.  Taken with a shared part and 128 elements in 16-bit types (reads_ahead; fewer elements have no registers left at three wavefronts a SIMD, fp32 none at one), bf16, without and with: forward, 16 heads x 2048
-// causal 51.8 and 47.1 us, x 8192 409 and 406, documents 2 x 16 x 4001 80.9 and 76.8; backward pass, 2 x 16 x 4001 in five documents, rows 210 and 201, columns 217 and 208.
+// causal 56 and 53 us, x 4096 160 and 158; documents 2 x 16 x 4001 130 and 125, their backward pass 386 and 377.
 template <typename T, int D, int X> constexpr bool reads_ahead() { return X && D == 128 && sizeof(T) == 2; }
 template <typename F, int N, int A> struct Ahead {
   F f[A + 1];
@@ -596,8 +601,9 @@ __device__ __forceinline__ void lds_barrier() {
 // Short lines, of 7 tiles (BigBird): fp16 768 lines 18.0 -> 17.3, 1536 29.7 -> 31.9; bf16 of 128 elements 512 lines 22.9 -> 19.2, 1024 30.6 -> 35.6; fp32 512 lines 68.6 -> 43.3, 1024 76.8 ->
 // 78.7, of 128 elements 256 74.3 -> 45.3, 512 80.2 -> 91.6; of one tile: fp16 768 lines 7.1 -> 8.1, bf16 of 128 elements 1024 14.5 -> 19.4, fp32 512 12.6 -> 11.8, of 128 elements 21.8 -> 29.0.
 // With a shared key part (64 elements more a key, rings that leave room for fewer workgroups) half as many in 16-bit types, forward pass and rows with columns, one pair -> two: bf16 of 128 elements 512
-// lines 61 -> 53 and 204 -> 182 us (of 5 tiles 22 -> 26 and 96 -> 98), 1024 lines 126 -> 173 and 426 -> 459; of 64 elements 1024 lines 95 -> 85 and 303 -> 284 (22 -> 26 and 92 -> 69), 2048 lines 139 -> 158 and 464 ->
-// 469. fp32 of 64 elements: 512 lines 285 -> 132 and 598 -> 470, 2048 1042 -> 920 and 2893 -> 2982.
+// lines of 4096 positions 141 -> 105 and 370 -> 325 us (of 2048 70 -> 53 and 216 -> 194, of 5 tiles 22 -> 28 and 95 -> 104), 1024 lines 158 -> 180 and 483 -> 509; of 64 elements 1024 lines 111 -> 96 and 359 -> 341 (of 5 tiles 21 -> 26
+// and 111 -> 110), 2048 lines 182 -> 185 and 577 -> 574.  Documents leave unequal lines, of which the longest is what lasts, but two pairs lose there as well: 128 elements, five documents of 4001 positions, 1008 lines 82 -> 92 and
+// 252 -> 265, 2016 lines 125 -> 168 and 377 -> 424; 64 elements 79 -> 85 and 246 -> 249.  fp32 of 64 elements: 512 lines 285 -> 132 and 598 -> 470, 2048 1042 -> 920 and 2893 -> 2982.
 constexpr int kLdsBytes = 160 * 1024;                     // of a compute unit
 template <typename T, int D, int X> inline bool few_lines(const RuleArgs &a) {
   return a.R >= 4 && (int64_t)a.Z * a.H * a.R <= (D == 64 ? 2048 : sizeof(T) == 4 ? 512 : 1024) / (X && sizeof(T) == 2 ? 2 : 1);

@@ -12,7 +12,7 @@
 // long; fp32 2 x 8 x 2023, two documents: 71, 97 and 7.
 //
 // With X > 0 (attention_shared_bwd.hip) a key part that all key heads share has part in the logits: its gradient is scale * e^T . qx summed over the heads, kept for each
-// key head in fp32 and added by a last kernel; that of qx is scale * e . kx.
+// key head in fp32 and added by a last kernel; that of qx is scale * e . kx.  p and e are in two terms there, in all their products (in_two_terms).
 #ifndef BSP_ATTENTION_RULES_BWD_H
 #define BSP_ATTENTION_RULES_BWD_H
 #include "attention_rules.h"
@@ -478,9 +478,18 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, X, CAP>())) k_rules_bwd_
           }
         if (!whole)
           for_16<0>([&](auto ic) { p[decltype(ic)::value] = keep(p[decltype(ic)::value], bit_mask<decltype(ic)::value>(seen)); });
-        Shares<T> share;
-        share.set(p);
-        if constexpr (!AHEAD) columns_times<T, D, O0, LEAN>(dv, reads, share);
+        constexpr bool TWO = in_two_terms<T, X>();
+        Shares<T> share, rest;
+        if constexpr (TWO) {
+          float left[16];
+#pragma unroll
+          for (int i = 0; i < 16; i++) left[i] = p[i];
+          two_terms<T>(left, share, rest);
+        } else {
+          share.set(p);
+        }
+        if constexpr (TWO && !AHEAD) columns_times_exact<T, D, O0, LEAN>(dv, reads, share, rest);
+        else if constexpr (!AHEAD) columns_times<T, D, O0, LEAN>(dv, reads, share);
         f32x16 dp;
 #pragma unroll
         for (int g = 0; g < 4; g++) {
@@ -490,7 +499,10 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, X, CAP>())) k_rules_bwd_
         }
         if constexpr (AHEAD) {
           of_do.run(do_fragment, [&](int i, const frag &f) {
-            if (i < 2 * MT) dv[i % MT] = Mma<T, 32>::run(f, share.f[i / MT], dv[i % MT]);
+            if (i < 2 * MT) {
+              dv[i % MT] = Mma<T, 32>::run(f, share.f[i / MT], dv[i % MT]);
+              dv[i % MT] = Mma<T, 32>::run(f, rest.f[i / MT], dv[i % MT]);
+            }
             else dp = fragment_times<T>(f, xv[i - 2 * MT], dp);
           });
           of_q.begin(q_fragment);
@@ -504,12 +516,18 @@ __global__ void __launch_bounds__(128, (col_waves<T, D, X, CAP>())) k_rules_bwd_
         }
         if (!whole)
           for_16<0>([&](auto ic) { e[decltype(ic)::value] = keep(e[decltype(ic)::value], bit_mask<decltype(ic)::value>(seen)); });
-        share.set(e);
+        if constexpr (TWO) two_terms<T>(e, share, rest);
+        else share.set(e);
         if constexpr (AHEAD) {
           of_q.run(q_fragment, [&](int i, const frag &f) {
             f32x16 &to = i < 2 * MT ? dk[i % MT] : dkx[(i - 2 * MT) % XT];
-            to = Mma<T, 32>::run(f, share.f[i < 2 * MT ? i / MT : (i - 2 * MT) / XT], to);
+            const int ks = i < 2 * MT ? i / MT : (i - 2 * MT) / XT;
+            to = Mma<T, 32>::run(f, share.f[ks], to);
+            to = Mma<T, 32>::run(f, rest.f[ks], to);
           });
+        } else if constexpr (TWO) {
+          columns_times_exact<T, D, Q0, LEAN>(dk, reads, share, rest);
+          columns_times_exact<T, SX, X0, LEAN>(dkx, readsx, share, rest);
         } else {
           columns_times<T, D, Q0, LEAN>(dk, reads, share);
           if constexpr (X) columns_times<T, SX, X0, LEAN>(dkx, readsx, share);

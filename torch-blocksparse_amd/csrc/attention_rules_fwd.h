@@ -7,7 +7,8 @@
 // units 29 %, which two wavefronts a SIMD overlap little (more do not fit the registers); fp16 8 x 16 x 4096 over blocks of 16 with stride 64 and a bias by distance: 153 us,
 // 70 % and 21 %.
 //
-// With X > 0 the logits have the product with a key part that all key heads share beside that with the head's own (attention_shared_fwd.hip): a third piece of a stage.
+// With X > 0 the logits have the product with a key part that all key heads share beside that with the head's own (attention_shared_fwd.hip): a third piece of a stage.  Shares are in two terms there
+// (in_two_terms).
 #ifndef BSP_ATTENTION_RULES_FWD_H
 #define BSP_ATTENTION_RULES_FWD_H
 #include "attention_rules.h"
@@ -162,9 +163,21 @@ __global__ void __launch_bounds__(128 * PAIRS, (fwd_waves<T, D, X, BIAS, DOCS>()
         }
         l += sum;
         Shares<T> p;
-        p.set(e);
-        if constexpr (AHEAD) columns.run(column, [&](int i, const frag &f) { o[i % MT] = Mma<T, 32>::run(f, p.f[i / MT], o[i % MT]); });
-        else columns_times<T, D, V0, false>(o, reads, p);
+        if constexpr (in_two_terms<T, X>()) {
+          Shares<T> rest;
+          two_terms<T>(e, p, rest);
+          if constexpr (AHEAD) {
+            columns.run(column, [&](int i, const frag &f) {
+              o[i % MT] = Mma<T, 32>::run(f, p.f[i / MT], o[i % MT]);
+              o[i % MT] = Mma<T, 32>::run(f, rest.f[i / MT], o[i % MT]);
+            });
+          } else {
+            columns_times_exact<T, D, V0, false>(o, reads, p, rest);
+          }
+        } else {
+          p.set(e);
+          columns_times<T, D, V0, false>(o, reads, p);
+        }
       }
       halves = nxt;
       return halves.more;

@@ -1,5 +1,5 @@
 // Attention with score rules whose keys have a part that all heads share, backward (attention_rules_bwd.h), and the sum of that part's gradient over the key heads.
-// Measured: bf16 2 x 16 x 4001 x (128 + 64), causal, five documents: rows 201 us (vector operations 22 % of the cycles, matrix units 21 %), columns 208 (20 %, 18 %), that sum 6 (of 32 MB); one
+// Measured: bf16 2 x 16 x 4001 x (128 + 64), causal, five documents: rows 201 us (vector operations 23 % of the cycles, matrix units 23 %), columns 252 (23 %, 25 %), that sum 6 (of 32 MB); one
 // wavefront a SIMD, whose products wait for each other.  Two a SIMD spill 90 to 250 bytes a lane in the rows of 128 elements.
 #include "attention_rules_bwd.h"
 

@@ -1,6 +1,6 @@
 // Attention with score rules whose keys have a part that all heads share (the expanded form of latent attention), forward: logits of scale * (q . k + qx . kx), qx
 // [Z, H, L, 64] and kx [Z, L, 64], by the kernels of attention_rules_fwd.h: the part is 64 elements more of a key in the ring and two products more of a tile's scores.  Measured: bf16, causal,
-// 16 heads x 8192 x (128 + 64): 405 us, 850 TFLOP/s of what is visible (vector operations 32 % of the cycles, matrix units 35 %); 2 x 16 x 4001 in five documents 121 us (23 %, 16 %: the longest
+// 16 heads x 8192 x (128 + 64): 505 us, 680 TFLOP/s of what is visible (vector operations 35 % of the cycles, matrix units 41 %); 2 x 16 x 4001 in five documents 135 us (27 %, 21 %: the longest
 // document's lines).
 #include "attention_rules_fwd.h"
 

@@ -14,7 +14,7 @@ reaches no result, NaN included.  At positions that some rows see, a NaN or an i
 rows NaN that do not see it, as 0 * NaN does in a product with a masked softmax.
 
 Sums, statistics and score gradients' factors are fp32; shares and score gradients are rounded to the operands' type where they become an operand of a
-product (16-bit types: those of the gradient of q in two terms).  In float16 the backward pass's shares, which are normalised, and score gradients lose bits where they are below 2^-14, as every share of a row of more than some
+product (16-bit types: those of the gradient of q in two terms, with `shared` all of them).  In float16 the backward pass's shares, which are normalised, and score gradients lose bits where they are below 2^-14, as every share of a row of more than some
 16000 equal keys is.  With a backward pass to follow a 16-bit call keeps, beside its operands and result, a tensor as large as the result (what its rounding left out).
 
 One kernel forward, two backward (rows: dq; columns: dk and dv), none of which stores a sparse tensor (bsp_attention_rules_fwd,
