@@ -140,8 +140,10 @@ template <int BITS, typename X> __device__ __forceinline__ void quantise(const X
     const double h = 0.5 * fabs((double)s32);
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-      const float n0 = __builtin_amdgcn_fmed3f(n[e], 0.f, (float)MOST);
-      const double rest = ((double)x[e] - (double)l32) - (double)n0 * (double)s32, rem = s32 < 0.f ? -rest : rest;
+      const double d = (double)x[e] - (double)l32;
+      // (turned elements that fp32 does not tell apart may be many codes from n: their quotient in 64 bits, by the same reciprocal, is less than one off)
+      const float n0 = __builtin_amdgcn_fmed3f(sizeof(X) == 8 ? (float)__builtin_rint(d * (double)inv) : n[e], 0.f, (float)MOST);
+      const double rest = d - (double)n0 * (double)s32, rem = s32 < 0.f ? -rest : rest;
       const bool odd = (int)n0 & 1;
       n[e] = n0 + (rem > h || (rem == h && odd) ? 1.f : 0.f) - (rem < -h || (rem == -h && odd) ? 1.f : 0.f);
     }
