@@ -15,6 +15,7 @@ import struct
 from fractions import Fraction
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -49,7 +50,8 @@ class _turn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rotation, positions, back, *tensors):
         ctx.save_for_backward(positions)
-        ctx.rotation, ctx.back = rotation, back
+        ctx.save_for_forward(positions)
+        ctx.rotation, ctx.back, ctx.shapes = rotation, back, [t.shape for t in tensors]
         ctx.set_materialize_grads(False)
         out = rotation._launch(tensors, positions, back)
         return out if len(out) > 1 else out[0]
@@ -60,14 +62,16 @@ class _turn(torch.autograd.Function):
         given = [g for g in grads if g is not None]
         if not given:
             return (None,) * (3 + len(grads))
-        with _lib.on_device(given[0].device):
-            if torch.is_grad_enabled():                   # (the gradient's gradient is wanted)
-                turned = _turn.apply(ctx.rotation, positions, not ctx.back, *given)
-                turned = turned if len(given) > 1 else (turned,)
-            else:
-                turned = ctx.rotation._launch(given, positions, not ctx.back)
-        turned = iter(turned)
+        turned = iter(ctx.rotation._turned(given, positions, not ctx.back))
         return (None, None, None) + tuple(next(turned) if g is not None else None for g in grads)
+
+    @staticmethod
+    def jvp(ctx, _, __, ___, *tangents):                  # the turn is linear: the same of the tangents
+        positions, = ctx.saved_tensors
+        given = [t for t in tangents if t is not None]
+        turned = iter(ctx.rotation._turned(given, positions, ctx.back))
+        turned = tuple(next(turned) if t is not None else given[0].new_zeros(shape) for t, shape in zip(tangents, ctx.shapes))     # (an output has to have one)
+        return turned if len(turned) > 1 else turned[0]
 
 
 class Rotation:
@@ -79,7 +83,7 @@ class Rotation:
     Called with one or two tensors (queries and keys: of one type, float16, bfloat16 or float32, and alike but for their number of heads) of shape [batch,
     heads, length, dim] with positions [length] or [batch, length], or [tokens, heads, dim] with positions [tokens]: int32, on the tensors'
     device; without positions they are 0 .. length - 1.  dim is a multiple of 8, 2 * pairs at least.  Returns the turned tensors (one: not in a tuple), contiguous; differentiable
-    in them, any number of times.
+    in them, any number of times, backward and in forward mode.
 
     A copy of the frequencies is made at the first call on a device, so a call that is captured into a graph needs one on its device before."""
 
@@ -171,10 +175,15 @@ class Rotation:
                 _lib.check(rc, 'bsp_rotate')
         return tuple(out)
 
+    def _turned(self, tensors, positions, back):
+        """the turned tensors; through autograd where a derivative may be wanted: a tensor that requires a gradient, or a forward-mode level that is open (whose tensors do not require one)"""
+        with _lib.on_device(tensors[0].device):
+            if (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)) or forward_ad._current_level >= 0:
+                out = _turn.apply(self, positions, back, *tensors)
+                return out if len(tensors) > 1 else (out,)
+            return self._launch(tensors, positions, back)
+
     def __call__(self, *tensors, positions=None):
         self._check(tensors, positions)
-        with _lib.on_device(tensors[0].device):
-            if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-                return _turn.apply(self, positions, False, *tensors)
-            out = self._launch(tensors, positions, False)
+        out = self._turned(tensors, positions, False)
         return out if len(out) > 1 else out[0]
