@@ -97,6 +97,10 @@ class Rotation:
             raise ValueError('frequencies must be finite numbers below 2^64')
         self.frequencies, self.pairs, self.neighbours = torch.tensor(f, dtype=torch.float64, device='cpu'), len(f), bool(neighbours)
         self._fractions = dict()
+        self._turns = self._as_turns()
+
+    def _as_turns(self):
+        return torch.tensor([_fraction_of_a_turn(f) for f in self.frequencies.tolist()], dtype=torch.int64, device='cpu')
 
     @classmethod
     def of_base(cls, dim, base=10000., neighbours=False):
@@ -106,13 +110,19 @@ class Rotation:
         return cls([float(base) ** (-2. * p / dim) for p in range(dim // 2)], neighbours)
 
     def __getstate__(self):
-        return dict(self.__dict__, _fractions=dict())
+        state = dict(self.__dict__, _fractions=dict())
+        state.pop('_turns', None)
+        return state
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._turns = self._as_turns()
 
     def fractions(self, device):
         """the frequencies as the kernels read them, noted as read by the current stream"""
         made = self._fractions.get(device)
         if made is None:
-            table = torch.tensor([_fraction_of_a_turn(f) for f in self.frequencies.tolist()], dtype=torch.int64, device='cpu').to(device)
+            table = self._turns.to(device)
             made = self._fractions[device] = (table, _lib.Readers())
             made[1].table(table)
         if _lib.raw_stream(device) not in made[1].streams:
