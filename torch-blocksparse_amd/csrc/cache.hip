@@ -18,6 +18,7 @@
 // wavefront, 66 % of its cycles; with 302 it took 42.5.  Taking all eight elements of the other lane before the first is used, and LDS without conflicts, did not change it.
 #include "cache.h"
 #include "rotation.h"
+#include "slots.h"
 
 namespace bsp {
 
@@ -77,15 +78,6 @@ template <typename T> __device__ __forceinline__ void load8(float (&x)[8], const
 #pragma unroll
     for (int i = 0; i < 8; i++) x[i] = to_float(u.e[i]);
   }
-}
-
-// Which of the positions of a slot that is given twice is written: the last.  owner[slot] (zero between calls) becomes the
-// greatest number t + 1 among them.
-__global__ void __launch_bounds__(256) k_cache_owner(CacheArgs a) {
-  const int t = blockIdx.x * 256 + threadIdx.x;
-  if (t >= a.T) return;
-  const int slot = a.slots[t];
-  if (slot >= 0 && slot < a.capacity) atomicMax(a.owner + slot, t + 1);
 }
 
 // The codes of the thread's eight elements (words), least value and step of their group, which the four threads of a quad have.  X: float, or double for what a rotation
@@ -287,7 +279,7 @@ template <typename T, int BITS, int D, bool ROTATED> void launch_cache_write(con
   if (a.T <= kScan) {
     hipLaunchKernelGGL((k_cache_write<T, BITS, D, true, ROTATED>), dim3((unsigned)a.T), dim3(256), 0, st, a);
   } else {
-    hipLaunchKernelGGL(k_cache_owner, dim3((unsigned)cdiv(a.T, 256)), dim3(256), 0, st, a);
+    launch_slot_owners(a.slots, a.T, a.capacity, a.owner, st);
     hipLaunchKernelGGL((k_cache_write<T, BITS, D, false, ROTATED>), dim3((unsigned)a.T), dim3(256), 0, st, a);
   }
 }

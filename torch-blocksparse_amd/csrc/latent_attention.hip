@@ -3,8 +3,8 @@
 //     y_j = cap * tanh(scale * (q . c_j + q_r . r_j) / cap) - slope_h * (n - 1 - j),   o = sum_j softmax_j(y) c_j        (no cap: scale * (q . c_j + q_r . r_j) - ...)
 // over the positions j < n whose page the sequence holds and, with a layout, whose block is in row (n - 1) / block of head h.
 //
-// Each byte of the pages is read once for all heads of a workgroup (up to 64) and is key and value at once, so it goes to LDS, straight from global memory. A wavefront has
-// sixteen heads.  Both products are taken transposed on the matrix units (16 x 16 x 32): scores as positions x heads, results as elements x heads.  A lane then has one head, so
+// Each byte of the pages is read once for all heads of a workgroup (up to 64; more are several workgroups', which read the pages again) and is key and value at once, so it goes to LDS, straight
+// from global memory. A wavefront has sixteen heads.  Both products are taken transposed on the matrix units (16 x 16 x 32): scores as positions x heads, results as elements x heads.  A lane then has one head, so
 // maximum, sum and rescaling are single registers, and the shares a lane has computed are the operand of the second product as they are: its other operand, positions across, comes from
 // LDS by transposing reads in the same order of positions.
 //
@@ -72,7 +72,6 @@ __device__ __forceinline__ void rows_to_lds(const i32x4b &rows, uint32_t off, ui
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(rows), "s"(dst) : "m0", "memory");
 }
 template <typename V> __device__ __forceinline__ V latent_read(uint32_t at) { return *(const V __attribute__((address_space(3))) *)(uintptr_t)at; }
-template <typename V> __device__ __forceinline__ void latent_put(uint32_t at, const V &v) { *(V __attribute__((address_space(3))) *)(uintptr_t)at = v; }
 __device__ __forceinline__ s16x4 latent_read_tr(uint32_t at) {
   typedef s16x4 __attribute__((address_space(3))) * lds_ptr;
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(uintptr_t)at);
@@ -145,7 +144,7 @@ template <typename T, int LAT, int HW> struct Heads {
   int key, c;
   bool here;
 
-  __device__ __forceinline__ void init(const T *pq, const T *pr, bool here_, float slope_, int wave, int lane, uint32_t) {
+  __device__ __forceinline__ void init(const T *pq, const T *pr, bool here_, float slope_, int lane) {
     key = lane & 15; c = lane >> 4; here = here_; slope = slope_;
 #pragma unroll
     for (int s = 0; s < NS + NR; s++) {
@@ -169,7 +168,7 @@ template <typename T, int LAT, int HW> struct Heads {
   }
 
   // false: the sums are to be scaled first, then the step taken again
-  template <class F> __device__ __forceinline__ bool step(uint32_t stage_of_all, const LatentGroup (&now)[GROUPS], const LatentScores &scores, bool again, bool, int wave, F &&load) {
+  template <class F> __device__ __forceinline__ bool step(uint32_t stage_of_all, const LatentGroup (&now)[GROUPS], const LatentScores &scores, bool again, int wave, F &&load) {
     // the step's addresses; all others are constants away (as values of their own, or the compiler keeps hundreds of sums with those constants)
     const uint32_t stage = stage_of_all + first_group(wave) * G::GROUP;
     uint32_t at_row[4], at_rope[NR], at_col[8];
@@ -520,7 +519,7 @@ __global__ void __launch_bounds__(256, 1) k_latent_attention(LatentArgs a) {
       const bool here = head < heads;
       const int64_t h = first + (here ? head : 0);
       x.init(reinterpret_cast<const T *>(a.q) + b * a.q_sb + h * a.q_sh, reinterpret_cast<const T *>(a.qr) + b * a.qr_sb + h * a.qr_sh, here,
-             a.slopes ? a.slopes[h] * kLog2e : 0.f, wave, lane, ring);
+             a.slopes ? a.slopes[h] * kLog2e : 0.f, lane);
     }
     LatentGroup now[H::GROUPS], next[H::GROUPS];
 #pragma unroll
@@ -550,7 +549,7 @@ __global__ void __launch_bounds__(256, 1) k_latent_attention(LatentArgs a) {
             for (int k = 0; k < H::GROUPS; k++) next[k] = group_of(4 * (s + 1 - base) + mine + k);
           }
         }
-        again = !x.step(ring + (s & 1) * G::STAGE, now, scores, again, s == s0, wave, load);
+        again = !x.step(ring + (s & 1) * G::STAGE, now, scores, again, wave, load);
         if (again) break;
 #pragma unroll
         for (int k = 0; k < H::GROUPS; k++) now[k] = next[k];

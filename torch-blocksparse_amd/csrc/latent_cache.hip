@@ -5,6 +5,7 @@
 // twice.  Measured: 20011 positions of 512 + 64 in bf16 with a rotation (46 MB): 12 us (3.8 TB/s), 2.5 more for the launch that says whose a slot is; 16384 x 8 (302 MB) 110 us.
 #include "latent.h"
 #include "rotation.h"
+#include "slots.h"
 
 namespace bsp {
 
@@ -23,14 +24,6 @@ struct LatentCacheArgs {
 };
 
 namespace {
-
-// as in cache.hip: owner[slot] becomes the greatest number t + 1 among the positions that are given the slot
-__global__ void __launch_bounds__(256) k_latent_owner(LatentCacheArgs a) {
-  const int t = blockIdx.x * 256 + threadIdx.x;
-  if (t >= a.T) return;
-  const int slot = a.slots[t];
-  if (slot >= 0 && slot < a.capacity) atomicMax(a.owner + slot, t + 1);
-}
 
 constexpr int kTogether = 8;       // positions of a workgroup
 
@@ -102,7 +95,7 @@ template <typename T> void launch_latent_write(const LatentCacheArgs &a, hipStre
   if (a.T <= kScan) {
     hipLaunchKernelGGL((k_latent_write<T, true>), grid, dim3(256), 0, st, a);
   } else {
-    hipLaunchKernelGGL(k_latent_owner, dim3((unsigned)cdiv(a.T, 256)), dim3(256), 0, st, a);
+    launch_slot_owners(a.slots, a.T, a.capacity, a.owner, st);
     hipLaunchKernelGGL((k_latent_write<T, false>), grid, dim3(256), 0, st, a);
   }
 }
