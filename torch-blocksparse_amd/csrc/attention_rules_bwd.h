@@ -20,7 +20,8 @@
 namespace bsp {
 namespace {
 
-// wavefronts a SIMD that the registers are for (with a shared part one fewer, or they spill)
+// wavefronts a SIMD that the registers are for (with a shared part one fewer, or they spill: the rows of 16-bit types and 128 elements 90 to 250 bytes a lane.  What does so with a shared part as it is: the columns of fp32 and 128
+// elements, at one wavefront a SIMD, 16 to 24 bytes, with a cap or documents 88 to 172; those of 16-bit types and 64 elements with all rules 12)
 template <typename T, int D, int X, bool CAP> constexpr int row_waves() { return sizeof(T) == 4 ? (D == 64 && !X ? 2 : 1) : D == 64 ? (CAP || X ? 2 : 3) : X ? 1 : 2; }
 template <typename T, int D, int X, bool CAP> constexpr int col_waves() { return D == 64 && !(X && sizeof(T) == 4) ? 2 : 1; }
 

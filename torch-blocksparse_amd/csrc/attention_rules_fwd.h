@@ -16,7 +16,7 @@
 namespace bsp {
 namespace {
 
-// (four wavefronts a SIMD leave 128 registers, which a bias or documents overrun)
+// (four wavefronts a SIMD leave 128 registers, which a bias or documents overrun; with a shared part, 16-bit types, a bias and documents 8 to 36 bytes a lane are in scratch memory all the same)
 template <typename T, int D, int X, bool BIAS, bool DOCS> constexpr int fwd_waves() { return sizeof(T) == 4 ? (D == 64 ? 2 : 1) : D == 64 ? (BIAS || DOCS || X ? 3 : 4) : 2; }
 
 template <typename T, int D, int X, bool CAP, bool BIAS, bool DOCS, int PAIRS>

@@ -19,6 +19,8 @@
 // unit, 137000 cycles at 128 bytes a clock) and products (66000) overlap in part, the rest is a step's exponentials between them and a piece's ends: queries, sums written (33 MB, read back by the
 // join), the search for the piece.  Shorter: 16 x 16 heads over up to 4096 positions with a layout, fp16, 15 and 4 us; one sequence of 33 positions 10.8.
 //
+// Latent vectors of 512 take all of a wavefront's 512 registers, and 16 to 48 bytes a lane are in scratch memory (smaller ones none).
+//
 // Wavefronts of 32 heads, two for the same heads, on 32 x 32 x 16 products take half of the reads from LDS, but exchange shares and wait for each other in every step: 128 heads 117 us, 64 85 where this
 // takes 98 and 66, all of it with shares in one term.
 #include "attention_common.h"

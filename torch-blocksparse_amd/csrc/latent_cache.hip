@@ -2,7 +2,8 @@
 // share, in a 16-bit type; row `slot` of the cache starts at element slot * (latent + 64).  With a rotation (rotation.h) those 64 are turned on the way, in fp32, and rounded once.
 //
 // Bound by the bytes.  A workgroup has eight positions: their latent vectors in chunks of 16 bytes, their shared parts a pair of elements a thread, so that no angle is computed
-// twice.  Measured: 20011 positions of 512 + 64 in bf16 with a rotation (46 MB): 12 us (3.8 TB/s), 2.5 more for the launch that says whose a slot is; 16384 x 8 (302 MB) 110 us.
+// twice.  Measured: 20011 positions of 512 + 64 in bf16 with a rotation (46 MB): 12 us (3.8 TB/s), 2.5 more for the launch that says whose a slot is; 131072 of them (302 MB) 58 us with
+// it (5.2 TB/s), 262144 120.  Read back: 9.4, 51 and 103 us (4.9 and 5.9 TB/s).
 #include "latent.h"
 #include "rotation.h"
 #include "slots.h"
