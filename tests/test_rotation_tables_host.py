@@ -27,3 +27,22 @@ def test_states_without_them():
     op = tb.Rotation.__new__(tb.Rotation)
     op.__setstate__(state)
     assert op._turns.tolist() == tb.Rotation.of_base(32)._turns.tolist()
+
+
+def test_two_threads_make_one_table(monkeypatch):
+    """a table that was given to a call stays: nothing else holds it until the launch"""
+    op, device, inner = tb.Rotation.of_base(64), torch.device('cpu', 0), []
+    monkeypatch.setattr(_lib, 'raw_stream', lambda device: 0)
+    monkeypatch.setattr(_lib.Readers, 'read', lambda self, device: None)
+    turns = op._turns
+
+    class Turns:
+        def to(self, device):                              # (the other thread's call, while this one copies its table)
+            if not inner:
+                inner.append(None)
+                inner[0] = op.fractions(device)
+            return turns.clone()
+
+    op._turns = Turns()
+    outer = op.fractions(device)
+    assert outer is inner[0] and op.fractions(device) is outer

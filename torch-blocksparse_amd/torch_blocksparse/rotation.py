@@ -122,9 +122,9 @@ class Rotation:
         """the frequencies as the kernels read them, noted as read by the current stream"""
         made = self._fractions.get(device)
         if made is None:
-            table = self._turns.to(device)
-            made = self._fractions[device] = (table, _lib.Readers())
-            made[1].table(table)
+            made = (self._turns.to(device), _lib.Readers())
+            made[1].table(made[0])
+            made = self._fractions.setdefault(device, made)      # (another thread's, which a call may be on its way to read, stays)
         if _lib.raw_stream(device) not in made[1].streams:
             made[1].read(device)
         return made[0]
